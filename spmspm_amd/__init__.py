@@ -35,3 +35,12 @@ from .api import (  # noqa: F401
     library_path,
     load_weight_files,
 )
+
+
+def __getattr__(name):
+    # the decode operators need torch, which the host encoder and the C ABI do without: imported when first asked for
+    if name in ("KV4Cache", "kv4_append", "kv4_gather", "kv4_attention", "W4Linear", "quantize_w4", "w4_pack"):
+        from . import decode
+        value = globals()[name] = getattr(decode, name)
+        return value
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

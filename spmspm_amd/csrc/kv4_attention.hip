@@ -1,0 +1,659 @@
+// Attention over the paged 4-bit key/value cache: KV4_Attention (decode_api.h holds the format).
+//
+// Mathematics.  With a key's scale s and zero point z and the integer codes k,
+//   q.K = s * (sum_d q_d k_d - z * sum_d q_d):
+// the matrix cores multiply the codes themselves.  A code masked out of its dword in place is as an fp16 number the subnormal
+// k * 2^-24 (k * 2^-20 for the second nibble of a half, whose q is 1/16 of the other's), which v_mfma_f32_16x16x32_f16
+// multiplies as it is: one AND per two codes and a shift per four.  Its sums lose a few bits to that (it aligns by exponent
+// fields): scores were measured within 6e-6 of float64.
+// For the values v - z goes into the product, an exact small integer in fp16: the code is put into the mantissa of 1024 (of
+// 64, where it is the second nibble) and 1024 + z (64 + z) is taken off, two codes at a time.  Their scale goes into the
+// probabilities, p'_t = p_t s_t.  p' must fit fp16 whatever the scales are, so their exponents go into the softmax: with
+// s_t = f_t 2^e_t, f_t in [1/2, 1), the running reference m follows the maximum of x_t = log2(p_t) + e_t, p'_t = 2^(x_t - m) f_t, and
+// the sum of probabilities is the sum of 2^(x_t - m) 2^-e_t.
+//
+// Layout.  One wave works on 32 keys at a time and RT tiles of 16 query rows (the heads that share a key/value head, for
+// each new token).  Scores are computed transposed, S^T = K Q^T, so that a lane owns one query row (its column) and keys
+// 8h..8h+7 of the 32 (h = lane / 16): these are exactly the k indices that it has to supply for O^T = V^T P^T, so
+// probabilities go from one product to the next in registers, and maxima, sums and rescaling need no exchange but the
+// one between the four lanes of a row, only when the maximum rises by more than 2^8.  V^T is built from rows of V: a lane
+// loads 4 bytes of each of its 8 keys and pairs their halves (v_perm); LDS is not used until the waves' results are joined.
+#include "decode_common.hiph"
+
+#include <algorithm>
+
+namespace decode {
+
+constexpr int   kTile   = 32;    // keys per step of a wave
+constexpr int   kWaves  = 4;     // waves of a workgroup, each with every fourth tile of the workgroup's keys
+constexpr float kNone   = -1e30f; // m before any key
+// The reference m of the exponentials starts 7 below the first maximum and follows when a score passes it by more than 15:
+// p' stays below 2^15 and uses fp16's range down to 2^-32 of the largest.
+constexpr float kBelow = 7.f, kSlack = 15.f;
+
+struct AttentionArgs {
+    const uint8_t * k_codes, *v_codes;
+    const int32_t * k_words, *v_words;
+    const int *     table, *lens, *cu;
+    const uint16_t* q;
+    int64_t         q_token, q_head;
+    uint16_t*       out;
+    float*          lse;
+    float*          part_o; // [split][row][D], row = token * q_heads + head
+    float*          part_ml; // [split][row][2]
+    float           scale_log2;
+    int             num_pages, page_log2, kv_heads, q_heads, share, batch, width, stride, tokens, window, splits, bf16;
+};
+
+template <int D>
+struct Shape {
+    static constexpr int kSteps  = D / 32;              // MFMA steps of a score
+    static constexpr int kDwords = D / 32;              // dwords of key codes per lane: D/4 elements of one key
+    static constexpr int kVal    = D == 96 ? 8 : D / 16; // value elements of one key per lane (96: lanes 12..15 have none)
+    static constexpr int kValBytes = kVal / 2;
+    static constexpr int waves(int rt) { return D == 256 || rt == 2 ? 2 : 3; } // waves per SIMD
+};
+
+template <int D>
+struct Keys {
+    unsigned k[2][Shape<D>::kDwords]; // key codes of the two 16-key tiles
+    unsigned v[8][(Shape<D>::kValBytes + 3) / 4];
+    uintx4   kw[2], vw[2];            // words of keys 8h .. 8h+7
+};
+
+template <int N>
+__device__ __forceinline__ void load_dwords(unsigned (&dst)[N], const uint8_t* p)
+{
+    if constexpr (N == 2) {
+        const uintx2 t = *reinterpret_cast<const uintx2*>(p);
+        dst[0] = t[0], dst[1] = t[1];
+    } else if constexpr (N == 3) {
+        __builtin_memcpy(dst, __builtin_assume_aligned(p, 4), 12);
+    } else if constexpr (N == 4) {
+        const uintx4 t = *reinterpret_cast<const uintx4*>(p);
+        dst[0] = t[0], dst[1] = t[1], dst[2] = t[2], dst[3] = t[3];
+    } else {
+        const uintx4 t = *reinterpret_cast<const uintx4*>(p), u = *reinterpret_cast<const uintx4*>(p + 16);
+        dst[0] = t[0], dst[1] = t[1], dst[2] = t[2], dst[3] = t[3];
+        dst[4] = u[0], dst[5] = u[1], dst[6] = u[2], dst[7] = u[3];
+    }
+}
+
+// The page that holds key `pos` of the sequence, or -1.
+__device__ __forceinline__ int page_at(const AttentionArgs& a, const int* row, int pos)
+{
+    const int idx = pos >> a.page_log2;
+    if (idx >= a.width)
+        return -1;
+    const int page = row[idx];
+    return page >= 0 && page < a.num_pages ? page : -1;
+}
+
+// Loads of the 32 keys from `tile` on (a multiple of 32); p0 and p1 are the pages of its two halves of 16.
+template <int D>
+__device__ __forceinline__ void load_keys(Keys<D>& t, const AttentionArgs& a, int head, int tile, int p0, int p1, int c, int h)
+{
+    const int P = 1 << a.page_log2;
+    // key r of tile T is key 8 (r / 4) + 4 T + r % 4 of the 32: half 0 for r < 8
+    const int      kr  = 8 * (c >> 2) + (c & 3);
+    const int      kp  = max(c < 8 ? p0 : p1, 0);
+    const int64_t  kat = (((int64_t)kp * a.kv_heads + head) << a.page_log2) + ((tile + kr) & (P - 1));
+    const uint8_t* kc  = a.k_codes + kat * (D / 2) + h * (D / 8);
+    load_dwords(t.k[0], kc);
+    load_dwords(t.k[1], kc + 4 * (D / 2));
+}
+
+__device__ __forceinline__ int64_t word_index(const AttentionArgs& a, int head, int tile, int p0, int p1, int h)
+{
+    const int mine = h < 2 ? p0 : p1;
+    return (((int64_t)max(mine, 0) * a.kv_heads + head) << a.page_log2) + ((tile + 8 * h) & ((1 << a.page_log2) - 1));
+}
+
+template <int D>
+__device__ __forceinline__ void load_key_words(Keys<D>& t, const AttentionArgs& a, int head, int tile, int p0, int p1, int h)
+{
+    const uintx4* kw = reinterpret_cast<const uintx4*>(a.k_words + word_index(a, head, tile, p0, p1, h));
+    t.kw[0] = kw[0], t.kw[1] = kw[1];
+}
+
+template <int D>
+__device__ __forceinline__ void load_values(Keys<D>& t, const AttentionArgs& a, int head, int tile, int p0, int p1, int c, int h)
+{
+    const int64_t  vat = word_index(a, head, tile, p0, p1, h);
+    const uintx4*  vw  = reinterpret_cast<const uintx4*>(a.v_words + vat);
+    const int      vc  = D == 96 && c >= 12 ? 0 : c;
+    const uint8_t* vb  = a.v_codes + vat * (D / 2) + vc * Shape<D>::kValBytes;
+    t.vw[0] = vw[0], t.vw[1] = vw[1];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if constexpr (Shape<D>::kValBytes == 2)
+            t.v[j][0] = *reinterpret_cast<const uint16_t*>(vb + j * (D / 2));
+        else if constexpr (Shape<D>::kValBytes == 4)
+            t.v[j][0] = *reinterpret_cast<const unsigned*>(vb + j * (D / 2));
+        else {
+            const uintx2 w = *reinterpret_cast<const uintx2*>(vb + j * (D / 2));
+            t.v[j][0] = w[0], t.v[j][1] = w[1];
+        }
+    }
+}
+
+template <int D, int RT>
+struct Rows {
+    half8  q[RT][Shape<D>::kSteps];
+    float  qsum[RT];          // sum of the row's q, in the scores' units
+    int    first[RT], last[RT]; // visible keys, last < first where there is none
+    float  m[RT], l[RT];
+    floatx4 o[RT][Shape<D>::kVal];
+};
+
+// Scores, softmax and product with the values for 32 keys.  The loads of the wave's next 32 are issued where the
+// registers that they fill become free: the codes of the keys behind the scores, their words behind the exponents, the
+// values at the end.  `edge`: some key of the tile is hidden from some row; `gone`: the lane's page is not in the cache.
+template <int D, int RT, typename LoadKeys, typename LoadWords, typename LoadValues>
+__device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool edge, bool gone, float qscale, int h,
+                                     LoadKeys load_k, LoadWords load_kw, LoadValues load_v)
+{
+    constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+    constexpr int      NV   = Shape<D>::kVal;
+    floatx4 sc[2][RT];
+#pragma unroll
+    for (int T = 0; T < 2; ++T) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+            sc[T][r] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < Shape<D>::kSteps; ++j) {
+            const unsigned w = t.k[T][j], w8 = w >> 8;
+            const uintx4   raw{w & kLow, w & kHigh, w8 & kLow, w8 & kHigh};
+            const half8    kk = __builtin_bit_cast(half8, raw);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                sc[T][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, s.q[r][j], sc[T][r], 0, 0, 0);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_k();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const unsigned kw = t.kw[i >> 2][i & 3], vw = t.vw[i >> 2][i & 3];
+        const float    zk = (float)(kw & 15u), ev = (float)(vw >> 23);
+        const float    u  = __uint_as_float(kw) * qscale; // the zero point in the lowest bits is part of the scale
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+            sc[i >> 2][r][i & 3] = __builtin_fmaf(__builtin_fmaf(-zk, s.qsum[r], sc[i >> 2][r][i & 3]), u, ev);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_kw();
+    __builtin_amdgcn_sched_barrier(0);
+    float f[8], il[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const unsigned vw = t.vw[i >> 2][i & 3];
+        f[i]  = __builtin_amdgcn_frexp_mantf(__uint_as_float(vw));
+        il[i] = __uint_as_float(0x7f000000u - (vw & 0x7f800000u)); // 2^(127 - e)
+    }
+    half8 pp[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int from = s.first[r] - tile - 8 * h, to = s.last[r] - tile - 8 * h;
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (gone || i < from || i > to)
+                    sc[i >> 2][r][i & 3] = -__builtin_inff();
+        }
+        float mx = kNone;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            mx = fmaxf(mx, sc[i >> 2][r][i & 3]);
+        if (__any(mx > s.m[r] + kSlack)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float m2 = fmaxf(mx - kBelow, s.m[r]), alpha = __builtin_amdgcn_exp2f(s.m[r] - m2);
+            s.m[r] = m2;
+            s.l[r] *= alpha;
+#pragma unroll
+            for (int e = 0; e < NV; ++e)
+                s.o[r][e] *= alpha;
+        }
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            p[i] = __builtin_amdgcn_exp2f(sc[i >> 2][r][i & 3] - s.m[r]);
+        if (edge) { // the words of a hidden key may be anything
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool hidden = gone || i < from || i > to;
+                s.l[r] += hidden ? 0.f : p[i] * il[i];
+                p[i] = hidden ? 0.f : p[i] * f[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s.l[r] = __builtin_fmaf(p[i], il[i], s.l[r]);
+                p[i] *= f[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) // rounded to 11 bits, as the output is: errors of either sign that average over the keys
+            pp[r][i] = (_Float16)p[i];
+    }
+    // -(1024 + z) and -(64 + z) of pairs of keys
+    half2 below[4], above[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned z = __builtin_amdgcn_perm(t.vw[i >> 1][2 * (i & 1) + 1], t.vw[i >> 1][2 * (i & 1)], 0x05040100u) & kLow;
+        below[i] = __builtin_bit_cast(half2, z | 0xe400e400u);
+        above[i] = __builtin_bit_cast(half2, z << 4 | 0xd400d400u);
+    }
+#pragma unroll
+    for (int g = 0; g < (NV + 3) / 4; ++g) { // four elements of every key: one half of a dword
+        uintx4 a0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            a0[i] = __builtin_amdgcn_perm(t.v[2 * i + 1][g >> 1], t.v[2 * i][g >> 1], (g & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uintx4 raw;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned w = e >= 2 ? a0[i] >> 8 : a0[i];
+                const half2    v = (e & 1) ? __builtin_bit_cast(half2, (w & kHigh) | 0x54005400u) + above[i]
+                                           : __builtin_bit_cast(half2, (w & kLow) | 0x64006400u) + below[i];
+                raw[i] = __builtin_bit_cast(unsigned, v);
+            }
+            const half8 va = __builtin_bit_cast(half8, raw);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                s.o[r][4 * g + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pp[r], s.o[r][4 * g + e], 0, 0, 0);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_v();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Rows of a block of 16 RT: the heads that share a key/value head for one token, then for the next.  Where sequences have
+// different numbers of rows, a sequence's blocks begin at floor(first token * share / rows of a block) + its number, which leaves room for all of every sequence's.
+__device__ __forceinline__ int block_base(const AttentionArgs& a, int b, int rows)
+{
+    if (a.cu == nullptr)
+        return b * ((a.share + rows - 1) / rows);
+    return (int)((int64_t)a.cu[b] * a.share / rows) + b;
+}
+
+template <int D, int RT>
+__global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attention(AttentionArgs a)
+{
+    constexpr int NV = Shape<D>::kVal, kRows = 16 * RT;
+    __shared__ float join[kWaves][16][D + 4];
+    __shared__ float join_m[kWaves][kRows], join_l[kWaves][kRows];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, h = lane >> 4;
+    const int head = blockIdx.y, split = blockIdx.z;
+
+    if (a.cu != nullptr && a.splits == 1) { // rows of no sequence (otherwise kv4_attention_join writes them)
+        const int before = min(max(a.cu[0], 0), a.tokens), behind = min(max(a.cu[a.batch], 0), a.tokens);
+        const int idle = before + a.tokens - behind;
+        for (int i = blockIdx.x; i < idle; i += gridDim.x) {
+            const int64_t at = (int64_t)(i < before ? i : behind + i - before) * a.q_heads + head * a.share;
+            for (int e = threadIdx.x; e < a.share * (D / 8); e += kWave * kWaves)
+                *reinterpret_cast<uintx4*>(a.out + at * D + e * 8) = uintx4{0, 0, 0, 0};
+            if (a.lse != nullptr)
+                for (int e = threadIdx.x; e < a.share; e += kWave * kWaves)
+                    a.lse[at + e] = -__builtin_inff();
+        }
+    }
+
+    // which sequence, which of its blocks
+    int b = 0;
+    for (int hi = a.batch; hi - b > 1;) {
+        const int mid = (b + hi) >> 1;
+        if (block_base(a, mid, kRows) <= (int)blockIdx.x)
+            b = mid;
+        else
+            hi = mid;
+    }
+    const int first = a.cu ? a.cu[b] : b, count = a.cu ? min(a.cu[b + 1], a.tokens) - first : 1;
+    const int row0 = ((int)blockIdx.x - block_base(a, b, kRows)) * kRows;
+    if (first < 0 || row0 < 0 || (int64_t)row0 >= (int64_t)count * a.share)
+        return;
+    const int rows   = min(kRows, count * a.share - row0);
+    const int len    = min(a.lens[b], a.width << a.page_log2);
+    const int* table = a.table + (int64_t)b * a.stride;
+    const int place0 = a.lens[b] - (a.cu ? a.cu[b + 1] - first : 1); // place of the sequence's first row's token
+
+    // the block's queries, scaled by a power of two that brings the largest to 2^13: fp16 then holds them exactly down to
+    // 2^-27 of it, with a factor 1/16 on those that meet the second nibble of a half
+    Rows<D, RT> s;
+    int lo = 0x7fffffff, hi = -1, lo_top = 0, hi_low = 0x7fffffff; // visible keys: of any row, of all rows
+    float qmax = 0.f;
+    const uint16_t* qrow[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int  row  = r * 16 + c;
+        const bool live = row < rows;
+        const int  tok = (row0 + (live ? row : 0)) / a.share, sub = (row0 + (live ? row : 0)) % a.share;
+        qrow[r] = a.q + (int64_t)(first + tok) * a.q_token + (int64_t)(head * a.share + sub) * a.q_head + h * (D / 4);
+#pragma unroll
+        for (int j = 0; j < Shape<D>::kSteps; ++j) {
+            const uintx4 raw = *reinterpret_cast<const uintx4*>(qrow[r] + 8 * j);
+            uint16_t     e[8];
+            __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float mag = fabsf(from16(e[i], a.bf16));
+                if (mag < 3.4e38f) // an infinity or NaN spoils its own row only
+                    qmax = fmaxf(qmax, mag);
+            }
+        }
+        const int place = place0 + tok;
+        s.first[r] = a.window > 0 ? max(0, place - a.window + 1) : 0;
+        s.last[r]  = min(place, len - 1);
+        if (place < 0 || place >= a.width << a.page_log2)
+            s.last[r] = -1;
+        if (!live)
+            s.first[r] = 0x7fffffff, s.last[r] = -1;
+        if (live && s.first[r] <= s.last[r]) {
+            lo = min(lo, s.first[r]);
+            hi = max(hi, s.last[r]);
+        }
+        if (live) { // a row that sees nothing makes every tile one with hidden keys
+            lo_top = max(lo_top, s.first[r]);
+            hi_low = min(hi_low, s.last[r]);
+        }
+        s.m[r] = kNone;
+        s.l[r] = 0.f;
+#pragma unroll
+        for (int e = 0; e < NV; ++e)
+            s.o[r][e] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        lo     = min(lo, __shfl_xor(lo, m));
+        hi     = max(hi, __shfl_xor(hi, m));
+        lo_top = max(lo_top, __shfl_xor(lo_top, m));
+        hi_low = min(hi_low, __shfl_xor(hi_low, m));
+        qmax   = fmaxf(qmax, __shfl_xor(qmax, m));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+    lo_top = __builtin_amdgcn_readfirstlane(lo_top), hi_low = __builtin_amdgcn_readfirstlane(hi_low);
+    int qexp = 13 - (int)__builtin_amdgcn_frexp_expf(qmax); // frexp: qmax < 2^exp
+    if (!(qmax > 0.f))
+        qexp = 0;
+    qexp = __builtin_amdgcn_readfirstlane(min(max(qexp, -110), 110));
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < Shape<D>::kSteps; ++j) {
+            half8        v;
+            const uintx4 raw = *reinterpret_cast<const uintx4*>(qrow[r] + 8 * j); // again: cheaper than the registers
+            uint16_t     e[8];
+            __builtin_memcpy(e, &raw, 16);
+            constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7}; // element of each half of the unpacked dword
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float  full = ldexpf(from16(e[kOrder[i]], a.bf16), qexp);
+                v[i]              = (_Float16)((i >> 1) & 1 ? full * 0.0625f : full);
+                sum += (float)(_Float16)full;
+            }
+            s.q[r][j] = v;
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        s.qsum[r] = sum * 0x1p-24f;
+    }
+    const float qscale = ldexpf(a.scale_log2, 24 - qexp);
+
+    // the workgroup's share of the block's keys, in tiles of 32; wave w takes every fourth
+    if (hi >= 0 && lo <= hi) {
+        const int t_lo = lo / kTile, t_all = hi / kTile + 1 - t_lo;
+        const int per = (t_all + a.splits - 1) / a.splits;
+        const int t0 = t_lo + split * per, t1 = min(t_lo + t_all, t0 + per);
+        int t = t0 + wave;
+        if (t < t1) {
+            Keys<D> keys;
+            int     p0 = page_at(a, table, t * kTile), p1 = page_at(a, table, t * kTile + 16);
+            load_keys<D>(keys, a, head, t * kTile, p0, p1, c, h);
+            load_key_words<D>(keys, a, head, t * kTile, p0, p1, h);
+            load_values<D>(keys, a, head, t * kTile, p0, p1, c, h);
+            int tn = min(t + kWaves, t1 - 1); // the wave's last tile is loaded once more and not used
+            int n0 = page_at(a, table, tn * kTile), n1 = page_at(a, table, tn * kTile + 16);
+            for (; t < t1; t += kWaves) {
+                const int  tile = t * kTile, next = tn * kTile, q0 = n0, q1 = n1;
+                const bool whole = p0 >= 0 && p1 >= 0 && tile >= lo_top && tile + kTile - 1 <= hi_low;
+                tn = min(tn + kWaves, t1 - 1);
+                n0 = page_at(a, table, tn * kTile), n1 = page_at(a, table, tn * kTile + 16);
+                step<D, RT>(
+                    s, keys, tile, !whole, (h < 2 ? p0 : p1) < 0, qscale, h,
+                    [&] { load_keys<D>(keys, a, head, next, q0, q1, c, h); },
+                    [&] { load_key_words<D>(keys, a, head, next, q0, q1, h); },
+                    [&] { load_values<D>(keys, a, head, next, q0, q1, c, h); });
+                p0 = q0, p1 = q1;
+            }
+        }
+    }
+
+    // join the waves
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        s.l[r] += __shfl_xor(s.l[r], 16);
+        s.l[r] += __shfl_xor(s.l[r], 32);
+        if (h == 0) {
+            join_m[wave][r * 16 + c] = s.m[r];
+            join_l[wave][r * 16 + c] = s.l[r];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        float m = kNone;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+            m = fmaxf(m, join_m[w][r * 16 + c]);
+        const float alpha = __builtin_amdgcn_exp2f(s.m[r] - m);
+        if (r > 0)
+            __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < NV; ++e) {
+                const int d = NV * (4 * h + i) + e;
+                if (D != 96 || d < D) {
+                    join[wave][c][d] = s.o[r][e][i] * alpha * 2.f; // f is half of the mantissa
+                }
+            }
+        __syncthreads();
+        for (int at = threadIdx.x; at < 16 * (D / 8); at += kWave * kWaves) {
+            const int row = at / (D / 8), d0 = at % (D / 8) * 8;
+            if (r * 16 + row >= rows)
+                break;
+            float mm = kNone, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            for (int w = 0; w < kWaves; ++w)
+                mm = fmaxf(mm, join_m[w][r * 16 + row]);
+            for (int w = 0; w < kWaves; ++w) {
+                l += join_l[w][r * 16 + row] * __builtin_amdgcn_exp2f(join_m[w][r * 16 + row] - mm);
+                for (int i = 0; i < 8; ++i)
+                    o[i] += join[w][row][d0 + i];
+            }
+            const int     g   = row0 + r * 16 + row;
+            const int64_t idx = (int64_t)(first + g / a.share) * a.q_heads + head * a.share + g % a.share;
+            if (a.splits > 1) {
+                float* dst = a.part_o + ((int64_t)split * a.tokens * a.q_heads + idx) * D + d0;
+                *reinterpret_cast<floatx4*>(dst)     = floatx4{o[0], o[1], o[2], o[3]};
+                *reinterpret_cast<floatx4*>(dst + 4) = floatx4{o[4], o[5], o[6], o[7]};
+                if (d0 == 0) {
+                    float* ml = a.part_ml + ((int64_t)split * a.tokens * a.q_heads + idx) * 2;
+                    ml[0] = mm, ml[1] = l;
+                }
+                continue;
+            }
+            const bool  none = l == 0.f; // no key seen (a sum of probabilities is never 0 otherwise)
+            const float inv  = none ? 0.f : 1.f / l;
+            uint16_t    e[8];
+            for (int i = 0; i < 8; ++i)
+                e[i] = to16(none ? 0.f : o[i] * inv, a.bf16);
+            uintx4 v;
+            __builtin_memcpy(&v, e, 16);
+            *reinterpret_cast<uintx4*>(a.out + idx * D + d0) = v;
+            if (a.lse != nullptr && d0 == 0) // l is 2^127 times the sum relative to m
+                a.lse[idx] = none ? -__builtin_inff() : (__log2f(l) + (mm - 127.f)) * 0.69314718055994531f;
+        }
+    }
+}
+
+// Joins the splits: one thread per 8 elements of a row.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_attention_join(AttentionArgs a)
+{
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)a.tokens * a.q_heads;
+    const int64_t idx = at / (D / 8);
+    const int     d0 = (int)(at % (D / 8)) * 8;
+    if (idx >= all)
+        return;
+    float mm = kNone, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    // a token of no sequence has no partial results: its row is 0
+    int       first, count;
+    const int t = (int)(idx / a.q_heads);
+    if (sequence_of(t, a.cu, a.batch, first, count) >= 0) {
+        for (int s = 0; s < a.splits; ++s)
+            mm = fmaxf(mm, a.part_ml[(s * all + idx) * 2]);
+        for (int s = 0; s < a.splits; ++s) {
+            const float w = __builtin_amdgcn_exp2f(a.part_ml[(s * all + idx) * 2] - mm);
+            l += w * a.part_ml[(s * all + idx) * 2 + 1];
+            const float* src = a.part_o + (s * all + idx) * D + d0;
+            for (int i = 0; i < 8; ++i)
+                o[i] += w * src[i];
+        }
+    }
+    const bool  none = l == 0.f;
+    const float inv  = none ? 0.f : 1.f / l;
+    uint16_t    e[8];
+    for (int i = 0; i < 8; ++i)
+        e[i] = to16(none ? 0.f : o[i] * inv, a.bf16);
+    uintx4 v;
+    __builtin_memcpy(&v, e, 16);
+    *reinterpret_cast<uintx4*>(a.out + idx * D + d0) = v;
+    if (a.lse != nullptr && d0 == 0)
+        a.lse[idx] = none ? -__builtin_inff() : (__log2f(l) + (mm - 127.f)) * 0.69314718055994531f;
+}
+
+namespace {
+
+struct Plan {
+    int row_tiles, blocks, splits;
+};
+
+// Row tiles per wave: as many as the average sequence fills, up to two.  Splits of the keys: enough workgroups for every
+// CU to hold two, no split below four tiles per wave.
+Plan plan_of(const KV4_Cache& c, const KV4_Batch& b, int q_heads, int window, int max_len)
+{
+    Plan          p;
+    const int     share = q_heads / c.kv_heads;
+    const int64_t rows  = (int64_t)b.total_tokens * share, each = (rows + b.batch - 1) / b.batch;
+    p.row_tiles = each <= 16 || c.head_dim == 256 ? 1 : 2;
+    const int64_t per = 16 * p.row_tiles;
+    p.blocks          = (int)(b.cu_tokens == nullptr ? b.batch * ((share + per - 1) / per) : rows / per + b.batch);
+    const int64_t capacity = (int64_t)b.table_width * c.page_size;
+    int64_t       len      = max_len > 0 ? std::min<int64_t>(max_len, capacity) : capacity;
+    if (window > 0) // what a block's rows see of it
+        len = std::min<int64_t>(len, (int64_t)window + (per + share - 1) / share + kTile);
+    const int64_t tiles = (len + kTile - 1) / kTile, groups = (int64_t)p.blocks * c.kv_heads;
+    int64_t       want  = (512 + groups - 1) / groups;
+    want                = std::min<int64_t>(want, (tiles + 4 * kWaves - 1) / (4 * kWaves));
+    p.splits            = (int)std::max<int64_t>(1, std::min<int64_t>(want, 128));
+    return p;
+}
+
+size_t workspace_of(const KV4_Cache& c, const KV4_Batch& b, int q_heads, const Plan& p)
+{
+    if (p.splits <= 1)
+        return 0;
+    const size_t rows = (size_t)p.splits * b.total_tokens * q_heads;
+    return rows * (c.head_dim + 2) * sizeof(float);
+}
+
+int check_heads(const KV4_Cache* c, int q_heads)
+{
+    if (q_heads < 1 || q_heads % c->kv_heads != 0)
+        return refuse("%d query heads over %d key/value heads", q_heads, c->kv_heads);
+    return 0;
+}
+
+template <int D>
+int run(hipStream_t stream, const Plan& p, const AttentionArgs& a)
+{
+    const dim3 grid((unsigned)p.blocks, (unsigned)a.kv_heads, (unsigned)p.splits), block(kWave * kWaves, 1, 1);
+    int        err;
+    if (p.row_tiles == 1)
+        err = launch(kv4_attention<D, 1>, grid, block, stream, a);
+    else if constexpr (D < 256)
+        err = launch(kv4_attention<D, 2>, grid, block, stream, a);
+    else
+        return (int)hipErrorInvalidValue; // plan_of gives heads of 256 one row tile: two would not fit the registers
+    if (err != 0 || p.splits == 1)
+        return err;
+    const int64_t threads = (int64_t)a.tokens * a.q_heads * (D / 8);
+    return launch(kv4_attention_join<D>, dim3((unsigned)((threads + 255) / 256), 1, 1), dim3(256, 1, 1), stream, a);
+}
+
+} // namespace
+} // namespace decode
+
+using namespace decode;
+
+extern "C" size_t KV4_AttentionWorkspaceBytes(const KV4_Cache* cache, const KV4_Batch* batch, int q_heads, int window,
+                                              int max_len)
+{
+    if (cache == nullptr || batch == nullptr || cache->kv_heads < 1 || q_heads < 1 || q_heads % cache->kv_heads != 0 ||
+        batch->batch < 1 || batch->total_tokens < 1)
+        return 0;
+    return workspace_of(*cache, *batch, q_heads, plan_of(*cache, *batch, q_heads, window, max_len));
+}
+
+extern "C" int KV4_Attention(hipStream_t stream, const KV4_Cache* cache, const KV4_Batch* batch, KV4_Rows q, int q_heads,
+                             void* out, float* lse, float scale, int window, int max_len, void* workspace,
+                             size_t workspace_bytes, int dtype)
+{
+    if (int e = check_cache(cache))
+        return e;
+    if (int e = check_batch(batch, cache))
+        return e;
+    if (int e = check_heads(cache, q_heads))
+        return e;
+    if (dtype != DECODE_FP16 && dtype != DECODE_BF16)
+        return refuse("unknown element type %d", dtype);
+    if (window < 0 || max_len < 0 || !(scale == scale))
+        return refuse("window %d, max_len %d, scale %f", window, max_len, (double)scale);
+    if (batch->total_tokens == 0)
+        return 0;
+    if (bad_pointer(q.data, 16) || bad_pointer(out, 16) || (lse != nullptr && bad_pointer(lse, 4)) ||
+        q.token_stride % 8 != 0 || q.head_stride % 8 != 0)
+        return refuse("a null or misaligned q, out or lse (16 bytes, strides multiples of 8 elements)");
+    const Plan   p    = plan_of(*cache, *batch, q_heads, window, max_len);
+    const size_t need = workspace_of(*cache, *batch, q_heads, p);
+    if (need > 0 && (bad_pointer(workspace, 16) || workspace_bytes < need))
+        return refuse("workspace of %zu bytes (16-byte aligned), %zu needed", workspace == nullptr ? (size_t)0 : workspace_bytes, need);
+    AttentionArgs a{};
+    a.k_codes = static_cast<const uint8_t*>(cache->k_codes), a.v_codes = static_cast<const uint8_t*>(cache->v_codes);
+    a.k_words = cache->k_words, a.v_words = cache->v_words;
+    a.table = batch->block_table, a.lens = batch->seq_lens, a.cu = batch->cu_tokens;
+    a.q = static_cast<const uint16_t*>(q.data), a.q_token = q.token_stride, a.q_head = q.head_stride;
+    a.out = static_cast<uint16_t*>(out), a.lse = lse;
+    a.part_o     = static_cast<float*>(workspace);
+    a.part_ml    = a.part_o + (size_t)p.splits * batch->total_tokens * q_heads * cache->head_dim;
+    a.scale_log2 = scale * 1.44269504088896341f;
+    a.num_pages = cache->num_pages, a.page_log2 = __builtin_ctz((unsigned)cache->page_size);
+    a.kv_heads = cache->kv_heads, a.q_heads = q_heads, a.share = q_heads / cache->kv_heads;
+    a.batch = batch->batch, a.width = batch->table_width, a.stride = batch->table_stride, a.tokens = batch->total_tokens;
+    a.window = window, a.splits = p.splits, a.bf16 = dtype == DECODE_BF16;
+    switch (cache->head_dim) {
+    case 64: return run<64>(stream, p, a);
+    case 96: return run<96>(stream, p, a);
+    case 128: return run<128>(stream, p, a);
+    default: return run<256>(stream, p, a);
+    }
+}
