@@ -1,37 +1,45 @@
 // Linear with 4-bit weights: W4_Pack, W4_Linear (decode_api.h).
 //
 // Mathematics.  Within a group of K a row's scale s and zero point z are constant, so
-//   sum_k x_k s (w_k - z) = s * (sum_k x_k w_k - z * sum_k x_k):
-// the matrix cores multiply activations by the codes themselves, the sums of x come from a product with ones, and scale and
-// zero point are applied to a group's sums in float32.
-// For fp16 a code masked out of its dword in place is the subnormal w * 2^-22 (bits 2..5 of a half) or w * 2^-18 (bits
-// 6..9): one AND per two codes, one rotation per eight.  v_mfma_f32_16x16x32_f16 multiplies subnormals as they are, but
-// aligns its sums by exponent fields, so that a code's distance from the top of the mantissa costs precision: hence bits
-// 2..9 and not 0..7, and ones for the sums of x that are normal numbers.  The two kinds go into products of their own,
-// since x itself may not be scaled by 1/16 without loss.  bf16 has no mantissa to spare for that: there a code is put
-// into the mantissa of 16 (16 + w is exact) and 16 sum x is taken off with the zero point.
+//   sum_k x_k s (w_k - z) = s * (sum_k x_k (16 + w_k) - (16 + z) * sum_k x_k):
+// the matrix cores multiply activations by the codes themselves, put into the mantissa of 16 (16 + w is exact in fp16 and
+// in bf16; an OR with a mask and, for three codes of four, a rotation), the sums of x come from a product with ones, and
+// scale and zero point are applied to a group's sums in float32.
 #include "decode_common.hiph"
 
 namespace decode {
 
 constexpr int kBlockK = 128; // columns of W in a block: 16 rows x 128 columns, 16 bytes a lane
 
-// Packed weights: codes [row tile of 16][block of 128 columns][lane][4 dwords], then words [row tile][group][16 rows], the
-// bits of a float32 scale (the 16-bit types' values fit its upper 20 bits) with the zero point in its four lowest.
-// Lane r + 16 h of a block holds, of row r, for each half p of 64 columns the dwords A = 2p, B = 2p + 1:
+// Packed weights: codes [row tile of 16][block of 128 columns][lane][4 dwords], scales [row tile][group][16 rows] in 16
+// bits, zero points [row tile][block][h][group of the block][rows 4 h .. 4 h + 3] in 4.  Lane r + 16 h of a block holds, of row r, for each half p of 64 columns
+// the dwords A = 2p, B = 2p + 1:
 //   columns 64 p + 8 h + 0..7        nibbles 0 4 2 6 of A, then of B
 //   columns 64 p + 32 + 8 h + 0..7   nibbles 1 5 3 7 of A, then of B
-// and the dwords are rotated left by 2 bits (fp16) or 3 (bf16), to where the kernel masks them out.
-__host__ __device__ inline int64_t code_bytes(int M, int K)
+// and the dwords are rotated left to where the kernel masks the first nibbles out: by 6 bits for fp16, 3 for bf16.
+struct Layout {
+    int     tiles, blocks, groups;
+    int64_t scales, zeros, bytes; // offsets, size
+};
+
+__host__ __device__ inline Layout layout_of(int M, int K, int group)
 {
-    return (int64_t)((M + 15) / 16) * ((K + kBlockK - 1) / kBlockK) * 1024;
+    Layout l;
+    l.tiles  = (M + 15) / 16;
+    l.blocks = (K + kBlockK - 1) / kBlockK;
+    l.groups = K / group;
+    l.scales = (int64_t)l.tiles * l.blocks * 1024;
+    l.zeros  = l.scales + (int64_t)l.tiles * l.groups * 32;
+    l.bytes  = (l.zeros + (int64_t)l.tiles * l.blocks * (kBlockK / group) * 8 + 15) / 16 * 16;
+    return l;
 }
 
 __global__ __launch_bounds__(64) void w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int M,
                                               int K, int group, int bf16, uint8_t* packed)
 {
-    const int lane = threadIdx.x, r = lane & 15, h = lane >> 4, blocks = (K + kBlockK - 1) / kBlockK, groups = K / group;
-    const int tile = blockIdx.y, kb = blockIdx.x, row = tile * 16 + r;
+    const int    lane = threadIdx.x, r = lane & 15, h = lane >> 4;
+    const Layout l = layout_of(M, K, group);
+    const int    tile = blockIdx.y, kb = blockIdx.x, row = tile * 16 + r, turn = bf16 ? 3 : 6;
     constexpr int kNibble[8] = {0, 4, 2, 6, 0, 4, 2, 6};
     uintx4        out{0, 0, 0, 0};
     for (int p = 0; p < 2; ++p)
@@ -41,16 +49,20 @@ __global__ __launch_bounds__(64) void w4_pack(const uint8_t* codes, const uint16
                 if (row < M && k < K)
                     out[2 * p + (x >> 2)] |= (codes[(int64_t)row * K + k] & 15u) << (4 * (kNibble[x] + q));
             }
-    const int turn = bf16 ? 3 : 2;
     for (int i = 0; i < 4; ++i)
         out[i] = out[i] << turn | out[i] >> (32 - turn);
-    reinterpret_cast<uintx4*>(packed)[((int64_t)tile * blocks + kb) * 64 + lane] = out;
-    unsigned* words = reinterpret_cast<unsigned*>(packed + code_bytes(M, K));
-    for (int g = kb * kBlockK / group + h; g < groups && g < (kb + 1) * kBlockK / group; g += 4) {
-        unsigned w = 0;
-        if (row < M)
-            w = (__float_as_uint(from16(scales[(int64_t)row * groups + g], bf16)) & ~15u) | (zeros[(int64_t)row * groups + g] & 15u);
-        words[((int64_t)tile * groups + g) * 16 + r] = w;
+    reinterpret_cast<uintx4*>(packed)[((int64_t)tile * l.blocks + kb) * 64 + lane] = out;
+    const int per = kBlockK / group;
+    for (int g = h; g < per; g += 4) {
+        const int     gk   = kb * per + g;
+        const bool    live = row < M && gk < l.groups;
+        const int64_t src  = (int64_t)row * l.groups + gk;
+        if (gk < l.groups)
+            reinterpret_cast<uint16_t*>(packed + l.scales)[((int64_t)tile * l.groups + gk) * 16 + r] = live ? scales[src] : (uint16_t)0;
+        if ((r & 1) == 0) { // rows r and r + 1 of rows 4 (r / 4) ..
+            const unsigned z0 = live ? zeros[src] & 15u : 0u, z1 = live && row + 1 < M ? zeros[src + l.groups] & 15u : 0u;
+            packed[l.zeros + ((((int64_t)tile * l.blocks + kb) * 4 + (r >> 2)) * per + g) * 2 + (r >> 1 & 1)] = (uint8_t)(z0 | z1 << 4);
+        }
     }
 }
 
@@ -60,7 +72,7 @@ struct LinearArgs {
     int64_t         x_stride;
     uint16_t*       y;
     const uint16_t* bias;
-    int             M, N, K, groups, act;
+    int             M, N, K, act;
 };
 
 template <bool BF16>
@@ -68,6 +80,7 @@ struct Types;
 template <>
 struct Types<false> {
     using vec = half8;
+    static constexpr unsigned kMask = 0x03c003c0u, k16 = 0x4c004c00u, kOne = 0x3c003c00u;
     static __device__ __forceinline__ floatx4 mfma(vec a, vec b, floatx4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -76,6 +89,7 @@ struct Types<false> {
 template <>
 struct Types<true> {
     using vec = bf8;
+    static constexpr unsigned kMask = 0x00780078u, k16 = 0x41804180u, kOne = 0x3f803f80u;
     static __device__ __forceinline__ floatx4 mfma(vec a, vec b, floatx4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -85,7 +99,7 @@ struct Types<true> {
 __device__ __forceinline__ float activate(float y, int act)
 {
     if (act == 1)
-        return fmaxf(y, 0.f) + (y != y ? y : 0.f); // a NaN stays one
+        return y < 0.f ? 0.f : y; // a NaN stays one
     if (act == 2) { // y * sigmoid(2u) = y/2 (1 + tanh u); large |u| ends at 0 and y
         const float u = 0.7978845608028654f * (y + 0.044715f * y * y * y);
         return y / (1.f + __expf(-2.f * u));
@@ -93,114 +107,105 @@ __device__ __forceinline__ float activate(float y, int act)
     return y;
 }
 
-// One workgroup: R row tiles of 16 rows and NT column tiles of 16 columns, the blocks of K dealt to its waves in turn; the
-// waves' sums are joined through LDS.  G: group size.
+// One workgroup: R row tiles of 16 rows and NT column tiles of 16 columns, the blocks of K dealt to its WAVES waves in turn;
+// the waves' sums are joined through LDS.  G: group size.
 template <int NT, int R, int G, bool BF16, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void w4_linear(LinearArgs a)
 {
     using T   = Types<BF16>;
     using vec = typename T::vec;
-    constexpr int      kGroups = kBlockK / G; // groups of a block
-    constexpr unsigned kLow = 0x003c003cu, kHigh = 0x03c003c0u, kBf16 = 0x00780078u, k16 = 0x41804180u;
+    constexpr int kGroups = kBlockK / G; // groups of a block
     __shared__ float join[WAVES][R * 16 * NT * 16];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
-    const int tiles = (a.M + 15) / 16, blocks = (a.K + kBlockK - 1) / kBlockK;
-    const int tile0 = blockIdx.x * R, n0 = blockIdx.y * 16 * NT;
+    const int    lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
+    const Layout l = layout_of(a.M, a.K, G);
+    const int    tile0 = blockIdx.x * R, n0 = blockIdx.y * 16 * NT;
 
-    const uintx4* codes[R];
-    const unsigned* words[R];
+    const uintx4*   codes[R];
+    const uint16_t* scales[R];
+    const uint8_t*  zeros[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int tile = min(tile0 + r, tiles - 1); // a tile past the end is computed again and not stored
-        codes[r]       = reinterpret_cast<const uintx4*>(a.packed) + (int64_t)tile * blocks * 64 + lane;
-        words[r]       = reinterpret_cast<const unsigned*>(a.packed + code_bytes(a.M, a.K)) + (int64_t)tile * a.groups * 16 + 4 * h;
+        const int64_t tile = min(tile0 + r, l.tiles - 1); // a tile past the end is computed again and not stored
+        codes[r]  = reinterpret_cast<const uintx4*>(a.packed) + tile * l.blocks * 64 + lane;
+        scales[r] = reinterpret_cast<const uint16_t*>(a.packed + l.scales) + tile * l.groups * 16 + 4 * h;
+        zeros[r]  = a.packed + l.zeros + (tile * l.blocks * 4 + h) * kGroups * 2;
     }
     const uint16_t* x[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
         x[n] = a.x + (int64_t)min(n0 + 16 * n + c, a.N - 1) * a.x_stride + 8 * h;
 
-    floatx4 y[R][NT];
+    const floatx4 zero{0.f, 0.f, 0.f, 0.f};
+    floatx4       y[R][NT];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-            y[r][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-    const unsigned one = BF16 ? 0x3f803f80u : 0x04000400u; // 1, or the smallest normal number 2^-14
-    const vec      ones = __builtin_bit_cast(vec, uintx4{one, one, one, one});
+            y[r][n] = zero;
+    const vec ones = __builtin_bit_cast(vec, uintx4{T::kOne, T::kOne, T::kOne, T::kOne});
 
-    uintx4 wn[R], sn[R][kGroups];
-    auto   fetch = [&](int kb) {
+    // two sets of registers: the loads of a wave's next block are in flight while it works on one
+    struct Block {
+        uintx4   w[R];
+        uintx2   s[R][kGroups];
+        unsigned z[R][(kGroups + 1) / 2];
+        vec      x[4][NT];
+    } set[2];
+    auto fetch = [&](Block& b, int kb) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            wn[r] = __builtin_nontemporal_load(codes[r] + (int64_t)kb * 64);
+            b.w[r] = __builtin_nontemporal_load(codes[r] + (int64_t)kb * 64);
 #pragma unroll
             for (int g = 0; g < kGroups; ++g)
-                sn[r][g] = *reinterpret_cast<const uintx4*>(words[r] + min(kb * kGroups + g, a.groups - 1) * 16);
+                b.s[r][g] = *reinterpret_cast<const uintx2*>(scales[r] + min(kb * kGroups + g, l.groups - 1) * 16);
+            const uint8_t* z = zeros[r] + (int64_t)kb * 8 * kGroups;
+            if constexpr (kGroups == 1)
+                b.z[r][0] = *reinterpret_cast<const uint16_t*>(z);
+            else
+#pragma unroll
+                for (int g = 0; g < kGroups / 2; ++g)
+                    b.z[r][g] = reinterpret_cast<const unsigned*>(z)[g];
         }
-    };
-    int kb = wave;
-    if (kb < blocks)
-        fetch(kb);
-    for (; kb < blocks; kb += WAVES) {
-        uintx4 w[R], sw[R][kGroups];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            w[r] = wn[r];
-#pragma unroll
-            for (int g = 0; g < kGroups; ++g)
-                sw[r][g] = sn[r][g];
-        }
-        vec xv[4][NT]; // columns 32 j + 8 h + 0..7 of the block
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 4; ++j) { // columns past the end as zeros (K is a multiple of 32)
             const int  k      = kb * kBlockK + 32 * j;
-            const bool inside = k < a.K; // K is a multiple of 32
+            const bool inside = k < a.K;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 uintx4 raw = *reinterpret_cast<const uintx4*>(x[n] + (inside ? k : 0));
                 if (!inside)
                     raw = uintx4{0, 0, 0, 0};
-                xv[j][n] = __builtin_bit_cast(vec, raw);
+                b.x[j][n] = __builtin_bit_cast(vec, raw);
             }
         }
-        fetch(min(kb + WAVES, blocks - 1));
-        floatx4 lo[R][NT], up[R][NT], xs[NT];
-        const floatx4 zero{0.f, 0.f, 0.f, 0.f};
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto work = [&](const Block& b) {
+        floatx4 acc[R][NT], xs[NT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { // 32 columns: lower nibbles for even j, upper ones for odd
+        for (int j = 0; j < 4; ++j) { // 32 columns: nibbles 0 4 2 6 of two dwords, or 1 5 3 7
             constexpr int kSteps = G / 32;
-            const bool    first  = j % kSteps == 0;
-            if (first) {
+            if (j % kSteps == 0) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     xs[n] = zero;
 #pragma unroll
                     for (int r = 0; r < R; ++r)
-                        lo[r][n] = up[r][n] = zero;
+                        acc[r][n] = zero;
                 }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                xs[n] = T::mfma(ones, xv[j][n], xs[n]);
+                xs[n] = T::mfma(ones, b.x[j][n], xs[n]);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const unsigned A = w[r][j & 2], B = w[r][(j & 2) + 1];
-                uintx4         raw;
-                if constexpr (BF16) {
-                    auto part = [](unsigned v, int n) { return (__builtin_amdgcn_alignbit(v, v, n) & kBf16) | k16; };
-                    const int n = (j & 1) * 4;
-                    raw = uintx4{part(A, n), part(A, n + 8), part(B, n), part(B, n + 8)};
-                } else {
-                    const unsigned m = (j & 1) ? kHigh : kLow;
-                    raw = uintx4{A & m, __builtin_amdgcn_alignbit(A, A, 8) & m, B & m, __builtin_amdgcn_alignbit(B, B, 8) & m};
-                }
-                const vec wv = __builtin_bit_cast(vec, raw);
+                const unsigned A = b.w[r][j & 2], B = b.w[r][(j & 2) + 1];
+                const int      n0 = 4 * (j & 1);
+                auto part = [](unsigned v, int n) { return (__builtin_amdgcn_alignbit(v, v, n) & T::kMask) | T::k16; };
+                const vec wv = __builtin_bit_cast(vec, uintx4{part(A, n0), part(A, n0 + 8), part(B, n0), part(B, n0 + 8)});
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    floatx4& acc = !BF16 && (j & 1) ? up[r][n] : lo[r][n];
-                    acc          = T::mfma(wv, xv[j][n], acc);
-                }
+                for (int n = 0; n < NT; ++n)
+                    acc[r][n] = T::mfma(wv, b.x[j][n], acc[r][n]);
             }
             if (j % kSteps == kSteps - 1) {
                 const int g = j / kSteps;
@@ -208,23 +213,28 @@ __global__ __launch_bounds__(64 * WAVES) void w4_linear(LinearArgs a)
                 for (int r = 0; r < R; ++r)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const unsigned word = sw[r][g][i];
-                        // the zero point's bits change the scale by less than 2^-19 of it, a 256th of the output's rounding
-                        const float s = __uint_as_float(word) * (BF16 ? 1.f : 0x1p22f);
-                        const float z = BF16 ? (float)(word & 15u) + 16.f : (float)(word & 15u) * 0x1p-8f;
+                        const float sc = from16((uint16_t)(b.s[r][g][i >> 1] >> (16 * (i & 1))), BF16);
+                        const float zp = (float)((b.z[r][g >> 1] >> (16 * (g & 1) + 4 * i)) & 15u) + 16.f;
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float t = lo[r][n][i];
-                            if constexpr (!BF16) {
-                                if (G == 32)
-                                    t = (j & 1) ? up[r][n][i] * 0.0625f : t;
-                                else
-                                    t = __builtin_fmaf(up[r][n][i], 0.0625f, t);
-                            }
-                            y[r][n][i] = __builtin_fmaf(__builtin_fmaf(-z, xs[n][i], t), s, y[r][n][i]);
-                        }
+                        for (int n = 0; n < NT; ++n)
+                            y[r][n][i] = __builtin_fmaf(__builtin_fmaf(-zp, xs[n][i], acc[r][n][i]), sc, y[r][n][i]);
                     }
             }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (wave < l.blocks) {
+        int kb = wave;
+        fetch(set[0], kb);
+        while (true) {
+            fetch(set[1], min(kb + WAVES, l.blocks - 1)); // the last one is fetched again and not used
+            work(set[0]);
+            if ((kb += WAVES) >= l.blocks)
+                break;
+            fetch(set[0], min(kb + WAVES, l.blocks - 1));
+            work(set[1]);
+            if ((kb += WAVES) >= l.blocks)
+                break;
         }
     }
 
@@ -285,7 +295,7 @@ extern "C" size_t W4_PackedBytes(int M, int K, int group)
 {
     if ((group != 32 && group != 64 && group != 128) || M < 1 || M > 16 * 65535 || K < group || K % group != 0)
         return 0;
-    return (size_t)code_bytes(M, K) + (size_t)((M + 15) / 16) * (K / group) * 64;
+    return (size_t)layout_of(M, K, group).bytes;
 }
 
 extern "C" int W4_Pack(hipStream_t stream, const uint8_t* codes, const void* scales, const uint8_t* zeros, int M, int K,
@@ -315,7 +325,7 @@ extern "C" int W4_Linear(hipStream_t stream, const void* packed, const void* X, 
         (N > 1 && x_stride < K) || x_stride % 8 != 0)
         return refuse("a null or misaligned weight, X (16 bytes, rows too), Y or bias (2)");
     const LinearArgs a{static_cast<const uint8_t*>(packed), static_cast<const uint16_t*>(X), x_stride,
-                       static_cast<uint16_t*>(Y),           static_cast<const uint16_t*>(bias), M, N, K, K / group, activation};
+                       static_cast<uint16_t*>(Y),           static_cast<const uint16_t*>(bias), M, N, K, activation};
     const bool       bf16 = dtype == DECODE_BF16;
     if (N <= 16)
         return run_linear<1, 1, 8>(stream, a, group, bf16);
