@@ -7,9 +7,13 @@
 // scale and zero point are applied to a group's sums in float32.
 #include "decode_common.hiph"
 
+#include <algorithm>
+
 namespace decode {
 
-constexpr int kBlockK = 128; // columns of W in a block: 16 rows x 128 columns, 16 bytes a lane
+constexpr int kBlockK     = 128;        // columns of W in a block: 16 rows x 128 columns, 16 bytes a lane
+constexpr int kWaves      = 8;          // waves of a workgroup of w4_linear
+constexpr int kMaxColumns = 16 * 65535; // column tiles are the y dimension of the grid
 
 // Packed weights: codes [row tile of 16][block of 128 columns][lane][4 dwords], scales [row tile][group][16 rows] in 16
 // bits, zero points [row tile][block][h][group of the block][rows 4 h .. 4 h + 3] in 4.  Lane r + 16 h of a block holds, of row r, for each half p of 64 columns
@@ -72,7 +76,8 @@ struct LinearArgs {
     int64_t         x_stride;
     uint16_t*       y;
     const uint16_t* bias;
-    int             M, N, K, act;
+    float*          part;
+    int             M, N, K, act, splits;
 };
 
 template <bool BF16>
@@ -107,57 +112,46 @@ __device__ __forceinline__ float activate(float y, int act)
     return y;
 }
 
-// One workgroup: R row tiles of 16 rows and NT column tiles of 16 columns, the blocks of K dealt to its WAVES waves in turn;
-// the waves' sums are joined through LDS.  G: group size.
-template <int NT, int R, int G, bool BF16, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void w4_linear(LinearArgs a)
-{
-    using T   = Types<BF16>;
-    using vec = typename T::vec;
-    constexpr int kGroups = kBlockK / G; // groups of a block
-    __shared__ float join[WAVES][R * 16 * NT * 16];
-    const int    lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
-    const Layout l = layout_of(a.M, a.K, G);
-    const int    tile0 = blockIdx.x * R, n0 = blockIdx.y * 16 * NT;
+// What a lane loads of one block of R row tiles.
+template <int R, int G>
+struct Weights {
+    static constexpr int kGroups = kBlockK / G; // groups of a block
+    uintx4   w[R];
+    uintx2   s[R][kGroups];
+    unsigned z[R][(kGroups + 1) / 2];
+};
 
+template <int R, int G>
+struct Source {
     const uintx4*   codes[R];
     const uint16_t* scales[R];
     const uint8_t*  zeros[R];
+    int             groups;
+
+    // Row tiles from tile0 on; one past the end is the last one again (it is computed and not stored).
+    __device__ __forceinline__ Source(const LinearArgs& a, const Layout& l, int tile0, int lane)
+    {
+        constexpr int kGroups = kBlockK / G;
+        const int     h       = lane >> 4;
+        groups                = l.groups;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t tile = min(tile0 + r, l.tiles - 1); // a tile past the end is computed again and not stored
-        codes[r]  = reinterpret_cast<const uintx4*>(a.packed) + tile * l.blocks * 64 + lane;
-        scales[r] = reinterpret_cast<const uint16_t*>(a.packed + l.scales) + tile * l.groups * 16 + 4 * h;
-        zeros[r]  = a.packed + l.zeros + (tile * l.blocks * 4 + h) * kGroups * 2;
+        for (int r = 0; r < R; ++r) {
+            const int64_t tile = min(tile0 + r, l.tiles - 1);
+            codes[r]  = reinterpret_cast<const uintx4*>(a.packed) + tile * l.blocks * 64 + lane;
+            scales[r] = reinterpret_cast<const uint16_t*>(a.packed + l.scales) + tile * l.groups * 16 + 4 * h;
+            zeros[r]  = a.packed + l.zeros + (tile * l.blocks * 4 + h) * kGroups * 2;
+        }
     }
-    const uint16_t* x[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-        x[n] = a.x + (int64_t)min(n0 + 16 * n + c, a.N - 1) * a.x_stride + 8 * h;
 
-    const floatx4 zero{0.f, 0.f, 0.f, 0.f};
-    floatx4       y[R][NT];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            y[r][n] = zero;
-    const vec ones = __builtin_bit_cast(vec, uintx4{T::kOne, T::kOne, T::kOne, T::kOne});
-
-    // two sets of registers: the loads of a wave's next block are in flight while it works on one
-    struct Block {
-        uintx4   w[R];
-        uintx2   s[R][kGroups];
-        unsigned z[R][(kGroups + 1) / 2];
-        vec      x[4][NT];
-    } set[2];
-    auto fetch = [&](Block& b, int kb) {
+    __device__ __forceinline__ void fetch(Weights<R, G>& b, int kb) const
+    {
+        constexpr int kGroups = kBlockK / G;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             b.w[r] = __builtin_nontemporal_load(codes[r] + (int64_t)kb * 64);
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g)
-                b.s[r][g] = *reinterpret_cast<const uintx2*>(scales[r] + min(kb * kGroups + g, l.groups - 1) * 16);
+            for (int g = 0; g < kGroups; ++g) // a group past the end meets zeros of X
+                b.s[r][g] = *reinterpret_cast<const uintx2*>(scales[r] + min(kb * kGroups + g, groups - 1) * 16);
             const uint8_t* z = zeros[r] + (int64_t)kb * 8 * kGroups;
             if constexpr (kGroups == 1)
                 b.z[r][0] = *reinterpret_cast<const uint16_t*>(z);
@@ -166,91 +160,129 @@ __global__ __launch_bounds__(64 * WAVES) void w4_linear(LinearArgs a)
                 for (int g = 0; g < kGroups / 2; ++g)
                     b.z[r][g] = reinterpret_cast<const unsigned*>(z)[g];
         }
+    }
+};
+
+// y += W X of one block; x(j, n) gives the lane's operand for columns 32 j .. 32 j + 31 of column tile n.
+template <int NT, int R, int G, bool BF16, typename X>
+__device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G>& b, X x)
+{
+    using T   = Types<BF16>;
+    using vec = typename T::vec;
+    constexpr int kSteps = G / 32;
+    const floatx4 zero{0.f, 0.f, 0.f, 0.f};
+    const vec     ones = __builtin_bit_cast(vec, uintx4{T::kOne, T::kOne, T::kOne, T::kOne});
+    floatx4       acc[R][NT], xs[NT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { // 32 columns: nibbles 0 4 2 6 of two dwords, or 1 5 3 7
+        if (j % kSteps == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                xs[n] = zero;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    acc[r][n] = zero;
+            }
+        }
+        vec xv[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            xv[n] = x(j, n);
+            xs[n] = T::mfma(ones, xv[n], xs[n]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const unsigned A = b.w[r][j & 2], B = b.w[r][(j & 2) + 1];
+            const int      n0 = 4 * (j & 1);
+            auto part = [](unsigned v, int n) { return (__builtin_amdgcn_alignbit(v, v, n) & T::kMask) | T::k16; };
+            const vec wv = __builtin_bit_cast(vec, uintx4{part(A, n0), part(A, n0 + 8), part(B, n0), part(B, n0 + 8)});
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                acc[r][n] = T::mfma(wv, xv[n], acc[r][n]);
+        }
+        if (j % kSteps == kSteps - 1) {
+            const int g = j / kSteps;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float sc = from16((uint16_t)(b.s[r][g][i >> 1] >> (16 * (i & 1))), BF16);
+                    const float zp = (float)((b.z[r][g >> 1] >> (16 * (g & 1) + 4 * i)) & 15u) + 16.f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        y[r][n][i] = __builtin_fmaf(__builtin_fmaf(-zp, xs[n][i], acc[r][n][i]), sc, y[r][n][i]);
+                }
+        }
+    }
+}
+
+// Few columns.  One workgroup: R row tiles of 16 rows and 16 columns, the blocks of K dealt to its waves in turn; the waves'
+// sums are joined through LDS.  G: group size.  Bound by memory where it has one workgroup for every CU: 28672x7168, N = 16,
+// groups of 128, in 26.7 us is 4.0 TB/s of weights (a large copy moves 4.9).  What it took: two sets of registers, so that no
+// wait for X includes the weights behind it; X from the cache as rarely as the registers allow (R tiles per read of it).
+template <int R, int G, bool BF16>
+__global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
+{
+    using vec = typename Types<BF16>::vec;
+    __shared__ float join[kWaves][R * 256];
+    const int    lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
+    const Layout l = layout_of(a.M, a.K, G);
+    const int    tile0 = blockIdx.x * R, n0 = blockIdx.y * 16;
+    const Source<R, G> source(a, l, tile0, lane);
+    const uint16_t*    x = a.x + (int64_t)min(n0 + c, a.N - 1) * a.x_stride + 8 * h;
+
+    floatx4 y[R][1];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        y[r][0] = floatx4{0.f, 0.f, 0.f, 0.f};
+    // two sets of registers: the loads of a wave's next block are in flight while it works on one
+    struct Block {
+        Weights<R, G> w;
+        vec           x[4];
+    } set[2];
+    auto fetch = [&](Block& b, int kb) {
+        source.fetch(b.w, kb);
 #pragma unroll
         for (int j = 0; j < 4; ++j) { // columns past the end as zeros (K is a multiple of 32)
             const int  k      = kb * kBlockK + 32 * j;
             const bool inside = k < a.K;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                uintx4 raw = *reinterpret_cast<const uintx4*>(x[n] + (inside ? k : 0));
-                if (!inside)
-                    raw = uintx4{0, 0, 0, 0};
-                b.x[j][n] = __builtin_bit_cast(vec, raw);
-            }
+            uintx4     raw    = *reinterpret_cast<const uintx4*>(x + (inside ? k : 0));
+            if (!inside)
+                raw = uintx4{0, 0, 0, 0};
+            b.x[j] = __builtin_bit_cast(vec, raw);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
     auto work = [&](const Block& b) {
-        floatx4 acc[R][NT], xs[NT];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { // 32 columns: nibbles 0 4 2 6 of two dwords, or 1 5 3 7
-            constexpr int kSteps = G / 32;
-            if (j % kSteps == 0) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    xs[n] = zero;
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        acc[r][n] = zero;
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-                xs[n] = T::mfma(ones, b.x[j][n], xs[n]);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const unsigned A = b.w[r][j & 2], B = b.w[r][(j & 2) + 1];
-                const int      n0 = 4 * (j & 1);
-                auto part = [](unsigned v, int n) { return (__builtin_amdgcn_alignbit(v, v, n) & T::kMask) | T::k16; };
-                const vec wv = __builtin_bit_cast(vec, uintx4{part(A, n0), part(A, n0 + 8), part(B, n0), part(B, n0 + 8)});
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    acc[r][n] = T::mfma(wv, b.x[j][n], acc[r][n]);
-            }
-            if (j % kSteps == kSteps - 1) {
-                const int g = j / kSteps;
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float sc = from16((uint16_t)(b.s[r][g][i >> 1] >> (16 * (i & 1))), BF16);
-                        const float zp = (float)((b.z[r][g >> 1] >> (16 * (g & 1) + 4 * i)) & 15u) + 16.f;
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            y[r][n][i] = __builtin_fmaf(__builtin_fmaf(-zp, xs[n][i], acc[r][n][i]), sc, y[r][n][i]);
-                    }
-            }
-        }
+        multiply<1, R, G, BF16>(y, b.w, [&](int j, int) { return b.x[j]; });
         __builtin_amdgcn_sched_barrier(0);
     };
     if (wave < l.blocks) {
         int kb = wave;
         fetch(set[0], kb);
         while (true) {
-            fetch(set[1], min(kb + WAVES, l.blocks - 1)); // the last one is fetched again and not used
+            fetch(set[1], min(kb + kWaves, l.blocks - 1)); // the last one is fetched again and not used
             work(set[0]);
-            if ((kb += WAVES) >= l.blocks)
+            if ((kb += kWaves) >= l.blocks)
                 break;
-            fetch(set[0], min(kb + WAVES, l.blocks - 1));
+            fetch(set[0], min(kb + kWaves, l.blocks - 1));
             work(set[1]);
-            if ((kb += WAVES) >= l.blocks)
+            if ((kb += kWaves) >= l.blocks)
                 break;
         }
     }
 
 #pragma unroll
     for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<floatx4*>(&join[wave][((n * 16 + c) * R + r) * 16 + 4 * h]) = y[r][n];
+        *reinterpret_cast<floatx4*>(&join[wave][(c * R + r) * 16 + 4 * h]) = y[r][0];
     __syncthreads();
-    for (int at = threadIdx.x; at < R * 16 * NT * 16; at += 64 * WAVES) {
+    for (int at = threadIdx.x; at < R * 256; at += 64 * kWaves) {
         const int m = tile0 * 16 + at % (R * 16), n = n0 + at / (R * 16);
         if (m >= a.M || n >= a.N)
             continue;
         float sum = 0.f;
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v)
+        for (int v = 0; v < kWaves; ++v)
             sum += join[v][at];
         if (a.bias != nullptr)
             sum += from16(a.bias[m], BF16);
@@ -258,21 +290,211 @@ __global__ __launch_bounds__(64 * WAVES) void w4_linear(LinearArgs a)
     }
 }
 
+// Many columns.  One workgroup: WAVES waves of R row tiles each and NT column tiles, over a share of K's blocks; the X of a
+// block goes through LDS, once for all waves.  Partial sums of a split K go to `part` [split][column][row].  9216x36864, N = 64,
+// bf16, groups of 64, seven shares: 91.5 us, 2.1 TB/s of weights; bound by the SIMDs' issue of matrix products (a third of
+// them sums of X) and of the scales' multiplications, which two waves a SIMD do not overlap.  w4_linear, which reads X from
+// the cache for every wave, takes 190 to 240 there.
+template <int NT, int R, int G, bool BF16, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void w4_linear_wide(LinearArgs a)
+{
+    using vec = typename Types<BF16>::vec;
+    constexpr int kThreads = 64 * WAVES, kChunks = NT * 16 * 16 / kThreads; // 16-byte chunks of X a thread moves per block
+    static_assert(kChunks * kThreads == NT * 256, "");
+    __shared__ uintx4 slab[2][4 * NT * 64];
+    const int    lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, h = lane >> 4;
+    const Layout l = layout_of(a.M, a.K, G);
+    const int    tile0 = (blockIdx.x * WAVES + wave) * R, n0 = blockIdx.y * 16 * NT;
+    const int    per = (l.blocks + a.splits - 1) / a.splits, first = blockIdx.z * per, last = min(first + per, l.blocks);
+    const Source<R, G> source(a, l, tile0, lane);
+
+    floatx4 y[R][NT];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            y[r][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+    // chunk q of a thread: 8 columns k0 .. of row `row` of the slab; sixteen threads read a row's 256 bytes.  In LDS an operand's
+    // sixteen rows are permuted by its place in the block, which spreads the sixteen chunks of a row over the banks.
+    const int       ch = threadIdx.x & 15, k0 = 8 * ch;
+    const uint16_t* xsrc[kChunks];
+    int             xdst[kChunks];
+#pragma unroll
+    for (int q = 0; q < kChunks; ++q) {
+        const int row = (threadIdx.x >> 4) + q * (kThreads / 16);
+        xsrc[q] = a.x + (int64_t)min(n0 + row, a.N - 1) * a.x_stride + k0;
+        xdst[q] = ((ch >> 2) * NT + (row >> 4)) * 64 + (ch & 3) * 16 + ((row & 15) ^ ch);
+    }
+    uintx4 xr[kChunks];
+    auto   fetch_x = [&](int kb) {
+        const bool inside = kb * kBlockK + k0 < a.K;
+#pragma unroll
+        for (int q = 0; q < kChunks; ++q) {
+            xr[q] = *reinterpret_cast<const uintx4*>(xsrc[q] + (inside ? kb * kBlockK : -k0));
+            if (!inside)
+                xr[q] = uintx4{0, 0, 0, 0};
+        }
+    };
+    auto store_x = [&](int buf) {
+#pragma unroll
+        for (int q = 0; q < kChunks; ++q)
+            slab[buf][xdst[q]] = xr[q];
+    };
+    Weights<R, G> set[2];
+    auto          work = [&](const Weights<R, G>& w, int buf) {
+        multiply<NT, R, G, BF16>(y, w, [&](int j, int n) {
+            return __builtin_bit_cast(vec, slab[buf][(j * NT + n) * 64 + h * 16 + (c ^ (4 * j + h))]);
+        });
+    };
+    if (first < last) {
+        int kb = first;
+        fetch_x(kb);
+        source.fetch(set[0], kb);
+        store_x(0);
+        fetch_x(min(kb + 1, last - 1));
+        __syncthreads();
+        while (true) {
+            // block kb is in slab 0 and set 0, X of the next in registers
+            source.fetch(set[1], min(kb + 1, last - 1));
+            store_x(1);
+            fetch_x(min(kb + 2, last - 1));
+            __builtin_amdgcn_sched_barrier(0);
+            work(set[0], 0);
+            __syncthreads();
+            if (++kb >= last)
+                break;
+            source.fetch(set[0], min(kb + 1, last - 1));
+            store_x(0);
+            fetch_x(min(kb + 2, last - 1));
+            __builtin_amdgcn_sched_barrier(0);
+            work(set[1], 1);
+            __syncthreads();
+            if (++kb >= last)
+                break;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int col = n0 + n * 16 + c;
+        if (col >= a.N)
+            continue;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int m = (tile0 + r) * 16 + 4 * h;
+            if (a.splits > 1) { // the slabs' rows are padded to whole tiles
+                if (tile0 + r < l.tiles)
+                    *reinterpret_cast<floatx4*>(a.part + ((int64_t)blockIdx.z * a.N + col) * (l.tiles * 16) + m) = y[r][n];
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (m + i < a.M) {
+                    const float sum = y[r][n][i] + (a.bias != nullptr ? from16(a.bias[m + i], BF16) : 0.f);
+                    a.y[(int64_t)col * a.M + m + i] = to16(activate(sum, a.act), BF16);
+                }
+        }
+    }
+}
+
+// Sums the slabs of a split K: four rows of a column per thread.
+__global__ __launch_bounds__(256) void w4_join(LinearArgs a, int bf16)
+{
+    const int quads = (a.M + 15) / 16 * 4;
+    const int at    = blockIdx.x * 256 + threadIdx.x;
+    const int col = at / quads, m = at % quads * 4;
+    if (col >= a.N || m >= a.M)
+        return;
+    floatx4 sum{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s)
+        sum += *reinterpret_cast<const floatx4*>(a.part + ((int64_t)s * a.N + col) * (quads * 4) + m);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (m + i < a.M)
+            a.y[(int64_t)col * a.M + m + i] =
+                to16(activate(sum[i] + (a.bias != nullptr ? from16(a.bias[m + i], bf16) : 0.f), a.act), bf16);
+}
+
 namespace {
 
-template <int NT, int R, int WAVES>
-int run_linear(hipStream_t stream, const LinearArgs& a, int group, bool bf16)
+// How a call runs: w4_linear with `row_tiles` tiles a workgroup, or w4_linear_wide with `column_tiles` tiles a workgroup and
+// the blocks of K in `splits` shares.
+struct Plan {
+    int row_tiles;    // of w4_linear; 0: w4_linear_wide
+    int column_tiles; // of w4_linear_wide, 2 or 4
+    int splits;
+};
+
+constexpr int kWideTiles = 2; // row tiles of a wave of the wide kernel
+constexpr int wide_waves(int column_tiles) { return column_tiles == 2 ? 4 : 8; }
+
+// The most row tiles w4_linear's registers hold (finer groups have more scales).
+constexpr int most_tiles(int group) { return group == 128 ? 7 : (group == 64 ? 6 : 4); }
+
+// The cheapest by a model of a call's time in microseconds, fitted to calls of 512x1024 to 28672x7168 and 9216x36864 with 1 to
+// 64 columns.  One workgroup of w4_linear runs on a CU at a time; a step, a block of K for each of its 8 waves, takes
+// 0.4 for a row tile and 0.6 for X: 28672x7168, N = 16, fp16, groups of 128, with 7 / 4 / 2 / 1 row tiles 26.7 / 33.9 /
+// 40.7 / 59.5 us.  Columns past 16 are workgroups of their own.  The wide kernel takes a block of K in 1.13 with two column
+// tiles (two workgroups a CU) and 1.75 with four (one), and 8 for launch, ends and the sum of the shares: N = 32 on that
+// matrix 38.8 (w4_linear 50.7), N = 64 53.6 (103), 5120x5120 with N = 32 13.5 (13.5), 512x1024 with N = 64 8.6 (4.0).
+Plan plan_of(int M, int N, int K, int group)
 {
-    const int  tiles = (a.M + 15) / 16;
-    const dim3 grid((unsigned)((tiles + R - 1) / R), (unsigned)((a.N + 16 * NT - 1) / (16 * NT)), 1), block(64 * WAVES, 1, 1);
-    if (group == 32)
-        return bf16 ? launch(w4_linear<NT, R, 32, true, WAVES>, grid, block, stream, a)
-                    : launch(w4_linear<NT, R, 32, false, WAVES>, grid, block, stream, a);
-    if (group == 64)
-        return bf16 ? launch(w4_linear<NT, R, 64, true, WAVES>, grid, block, stream, a)
-                    : launch(w4_linear<NT, R, 64, false, WAVES>, grid, block, stream, a);
-    return bf16 ? launch(w4_linear<NT, R, 128, true, WAVES>, grid, block, stream, a)
-                : launch(w4_linear<NT, R, 128, false, WAVES>, grid, block, stream, a);
+    const int64_t tiles = (M + 15) / 16, blocks = (K + kBlockK - 1) / kBlockK;
+    auto          up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    Plan          p{1, 0, 1};
+    double        best = 1e30;
+    for (int r = 1; r <= most_tiles(group); ++r) {
+        const double us = 3.0 + (double)(up(up(tiles, r) * up(N, 16), 256) * up(blocks, 8)) * (0.4 * r + 0.6);
+        if (us < best)
+            best = us, p.row_tiles = r;
+    }
+    if (N <= 16)
+        return p;
+    const int     nt = N <= 32 ? 2 : 4, slots = nt == 2 ? 512 : 256;
+    const int64_t groups = up(tiles, kWideTiles * wide_waves(nt)) * up(N, 16 * nt);
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(slots / groups, blocks / 2));
+    if (8.0 + (double)(up(groups * splits, slots) * up(blocks, splits)) * (nt == 2 ? 1.13 : 1.75) < best)
+        p = Plan{0, nt, (int)splits};
+    return p;
+}
+
+size_t workspace_of(int M, int N, const Plan& p)
+{
+    return p.splits > 1 ? (size_t)p.splits * N * ((M + 15) / 16 * 16) * sizeof(float) : 0;
+}
+
+template <int R, int G, bool BF16>
+int run_narrow(hipStream_t stream, int row_tiles, const LinearArgs& a)
+{
+    if constexpr (R > 1)
+        if (row_tiles < R)
+            return run_narrow<R - 1, G, BF16>(stream, row_tiles, a);
+    const unsigned tiles = (unsigned)(a.M + 15) / 16;
+    return launch(w4_linear<R, G, BF16>, dim3((tiles + R - 1) / R, (unsigned)(a.N + 15) / 16, 1), dim3(64 * kWaves, 1, 1),
+                  stream, a);
+}
+
+template <int NT, int G, bool BF16>
+int run_wide(hipStream_t stream, const LinearArgs& a)
+{
+    constexpr int      W = wide_waves(NT);
+    constexpr unsigned kRows = W * kWideTiles;
+    const unsigned     tiles = (unsigned)(a.M + 15) / 16;
+    const int          err   = launch(w4_linear_wide<NT, kWideTiles, G, BF16, W>,
+                                      dim3((tiles + kRows - 1) / kRows, (unsigned)(a.N + 16 * NT - 1) / (16 * NT), (unsigned)a.splits),
+                                      dim3(64 * W, 1, 1), stream, a);
+    if (err != 0 || a.splits == 1)
+        return err;
+    const int64_t quads = (int64_t)tiles * 4 * a.N;
+    return launch(w4_join, dim3((unsigned)((quads + 255) / 256), 1, 1), dim3(256, 1, 1), stream, a, (int)BF16);
+}
+
+template <int G, bool BF16>
+int run_linear(hipStream_t stream, const Plan& p, const LinearArgs& a)
+{
+    if (p.row_tiles > 0)
+        return run_narrow<most_tiles(G), G, BF16>(stream, p.row_tiles, a);
+    return p.column_tiles == 2 ? run_wide<2, G, BF16>(stream, a) : run_wide<4, G, BF16>(stream, a);
 }
 
 int check_weights(int M, int K, int group, int dtype)
@@ -310,13 +532,21 @@ extern "C" int W4_Pack(hipStream_t stream, const uint8_t* codes, const void* sca
                   dtype == DECODE_BF16, static_cast<uint8_t*>(packed));
 }
 
+extern "C" size_t W4_WorkspaceBytes(int M, int N, int K)
+{
+    if (M < 1 || M > 16 * 65535 || N < 1 || N > kMaxColumns || K < 32)
+        return 0;
+    return workspace_of(M, N, plan_of(M, N, K, 128)); // the split does not depend on the group
+}
+
 extern "C" int W4_Linear(hipStream_t stream, const void* packed, const void* X, int64_t x_stride, void* Y, int M, int N,
-                         int K, int group, const void* bias, int activation, int dtype)
+                         int K, int group, const void* bias, int activation, void* workspace, size_t workspace_bytes,
+                         int dtype)
 {
     if (int e = check_weights(M, K, group, dtype))
         return e;
-    if (N < 0 || N > 65535 * 64)
-        return refuse("%d columns (0 to 64 * 65535)", N);
+    if (N < 0 || N > kMaxColumns)
+        return refuse("%d columns of X (0 to %d)", N, kMaxColumns);
     if (activation < 0 || activation > 2)
         return refuse("unknown activation %d (0 none, 1 ReLU, 2 GELU)", activation);
     if (N == 0)
@@ -324,12 +554,18 @@ extern "C" int W4_Linear(hipStream_t stream, const void* packed, const void* X, 
     if (bad_pointer(packed, 16) || bad_pointer(X, 16) || bad_pointer(Y, 2) || (bias != nullptr && bad_pointer(bias, 2)) ||
         (N > 1 && x_stride < K) || x_stride % 8 != 0)
         return refuse("a null or misaligned weight, X (16 bytes, rows too), Y or bias (2)");
-    const LinearArgs a{static_cast<const uint8_t*>(packed), static_cast<const uint16_t*>(X), x_stride,
-                       static_cast<uint16_t*>(Y),           static_cast<const uint16_t*>(bias), M, N, K, activation};
-    const bool       bf16 = dtype == DECODE_BF16;
-    if (N <= 16)
-        return run_linear<1, 1, 8>(stream, a, group, bf16);
-    if (N <= 32)
-        return run_linear<2, 1, 8>(stream, a, group, bf16);
-    return run_linear<4, 1, 8>(stream, a, group, bf16);
+    const Plan   p    = plan_of(M, N, K, group);
+    const size_t need = workspace_of(M, N, p);
+    if (need > 0 && (bad_pointer(workspace, 16) || workspace_bytes < need))
+        return refuse("workspace of %zu bytes (16-byte aligned), %zu needed", workspace == nullptr ? (size_t)0 : workspace_bytes, need);
+    LinearArgs a{};
+    a.packed = static_cast<const uint8_t*>(packed), a.x = static_cast<const uint16_t*>(X), a.x_stride = x_stride;
+    a.y = static_cast<uint16_t*>(Y), a.bias = static_cast<const uint16_t*>(bias), a.part = static_cast<float*>(workspace);
+    a.M = M, a.N = N, a.K = K, a.act = activation, a.splits = p.splits;
+    const bool bf16 = dtype == DECODE_BF16;
+    if (group == 32)
+        return bf16 ? run_linear<32, true>(stream, p, a) : run_linear<32, false>(stream, p, a);
+    if (group == 64)
+        return bf16 ? run_linear<64, true>(stream, p, a) : run_linear<64, false>(stream, p, a);
+    return bf16 ? run_linear<128, true>(stream, p, a) : run_linear<128, false>(stream, p, a);
 }

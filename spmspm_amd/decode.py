@@ -67,7 +67,9 @@ def _library():
         L.W4_Pack.argtypes = [C.c_void_p] * 4 + [C.c_int] * 4 + [C.c_void_p]
         L.W4_Linear.restype = C.c_int
         L.W4_Linear.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p] + [C.c_int] * 4 + [
-            C.c_void_p, C.c_int, C.c_int]
+            C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_int]
+        L.W4_WorkspaceBytes.restype = C.c_size_t
+        L.W4_WorkspaceBytes.argtypes = [C.c_int] * 3
         _lib = L
     return _lib
 
@@ -369,9 +371,12 @@ class W4Linear:
         def call(handle):
             y = torch.empty((N, self.M), dtype=self.dtype, device=self.device) if out is None else out
             if N:
-                err = _library().W4_Linear(handle, self.packed.data_ptr(), x.data_ptr(), stride, y.data_ptr(), self.M, N,
-                                           self.K, self.group, None if self.bias is None else self.bias.data_ptr(),
-                                           self.activation, _TYPES[self.dtype])
+                L = _library()
+                need = L.W4_WorkspaceBytes(self.M, N, self.K)
+                ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+                err = L.W4_Linear(handle, self.packed.data_ptr(), x.data_ptr(), stride, y.data_ptr(), self.M, N, self.K,
+                                  self.group, None if self.bias is None else self.bias.data_ptr(), self.activation,
+                                  None if ws is None else ws.data_ptr(), need, _TYPES[self.dtype])
                 _raise(err, "W4Linear")
             return y
 

@@ -23,7 +23,7 @@ def _declared():
 def test_every_declared_function_is_exported():
     names = _declared()
     assert names == ["KV4_Append", "KV4_Attention", "KV4_AttentionWorkspaceBytes", "KV4_Gather", "W4_Linear", "W4_Pack",
-                     "W4_PackedBytes"]
+                     "W4_PackedBytes", "W4_WorkspaceBytes"]
     for n in names:
         assert hasattr(S.library(), n)
     for n in M.__all__:
@@ -132,7 +132,7 @@ def test_linear_sizes_and_refusals(capfd):
     for bad in ((0, 128, 64), (16, 0, 64), (16, 100, 32), (16, 128, 16), (16, 128, 256), (16 * 65535 + 1, 128, 64)):
         assert L.W4_PackedBytes(*bad) == 0
         assert L.W4_Pack(None, X, X, X, *bad, 0, X) == 1
-        assert L.W4_Linear(None, X, X, 4096, X, bad[0], 1, bad[1], bad[2], None, 0, 0) == 1
+        assert L.W4_Linear(None, X, X, 4096, X, bad[0], 1, bad[1], bad[2], None, 0, None, 0, 0) == 1
     for codes, scales, zeros, packed in ((None, X, X, X), (X, X + 1, X, X), (X, X, None, X), (X, X, X, X + 8)):
         assert L.W4_Pack(None, codes, scales, zeros, 16, 128, 64, 0, packed) == 1
     ok = dict(packed=X, x=X, stride=128, y=X, M=16, N=4, K=128, G=64, bias=None, act=0, dtype=0)
@@ -140,8 +140,13 @@ def test_linear_sizes_and_refusals(capfd):
                dict(stride=129), dict(bias=X + 1), dict(act=3), dict(act=-1), dict(dtype=2), dict(N=-1)):
         a = dict(ok, **kw)
         assert L.W4_Linear(None, a["packed"], a["x"], a["stride"], a["y"], a["M"], a["N"], a["K"], a["G"], a["bias"],
-                           a["act"], a["dtype"]) == 1, kw
-    assert L.W4_Linear(None, X, X, 128, X, 16, 0, 128, 64, None, 0, 0) == 0
+                           a["act"], None, 0, a["dtype"]) == 1, kw
+    assert L.W4_Linear(None, X, X, 128, X, 16, 0, 128, 64, None, 0, None, 0, 0) == 0
+    # a split K needs its workspace
+    need = L.W4_WorkspaceBytes(9216, 64, 36864)
+    assert need > 0 and need % (4 * 9216 * 64) == 0 and L.W4_WorkspaceBytes(9216, 16, 36864) == 0
+    for ws, size in ((None, need), (X, need - 1), (X + 8, need)):
+        assert L.W4_Linear(None, X, X, 36864, X, 9216, 64, 36864, 64, None, 0, ws, size, 0) == 1
 
 
 def test_cache_encoding_is_within_half_a_step_and_holds_zero_exactly():
