@@ -88,8 +88,9 @@ def _context(device, stream):
 
 def _run(device, stream, call):
     """`call(handle)` with `device` current and torch's allocations on the call's stream."""
-    if stream is None and torch.cuda.current_device() == device.index:
-        return call(torch.cuda.current_stream(device).cuda_stream)
+    # the two calls behind torch.cuda.current_device() and current_stream(): 2 us less of a call's 10
+    if stream is None and torch._C._cuda_getDevice() == device.index:
+        return call(torch._C._cuda_getCurrentRawStream(device.index))
     with _context(device, stream) as handle:
         return call(handle)
 
@@ -155,12 +156,13 @@ class KV4Cache:
 
 
 def _batch(cache, block_table, seq_lens, cu_tokens, tokens):
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1 or seq_lens.dim() != 1 \
-            or seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous() or block_table.shape[0] != seq_lens.shape[0]:
+    shape, strides = block_table.shape, block_table.stride()
+    if len(shape) != 2 or block_table.dtype != torch.int32 or strides[1] != 1 or seq_lens.dtype != torch.int32 \
+            or not seq_lens.is_contiguous() or seq_lens.shape != shape[:1]:
         raise ValueError("block_table must be int32 [batch][pages], seq_lens int32 [batch]")
-    n = seq_lens.shape[0]
-    if block_table.device != cache.device or seq_lens.device != cache.device:
-        raise ValueError(f"block_table and seq_lens must be on the cache's device {cache.device}")
+    n, device = seq_lens.shape[0], cache.device
+    if block_table.device != device or seq_lens.device != device:
+        raise ValueError(f"block_table and seq_lens must be on the cache's device {device}")
     if cu_tokens is None:
         if tokens != n:
             raise ValueError(f"{tokens} tokens of {n} sequences: cu_tokens must say whose they are")
@@ -170,18 +172,19 @@ def _batch(cache, block_table, seq_lens, cu_tokens, tokens):
                 or cu_tokens.device != cache.device:
             raise ValueError("cu_tokens must be int32 [batch + 1] on the cache's device")
         cu = cu_tokens.data_ptr()
-    stride = block_table.stride(0) if n > 1 else max(block_table.shape[1], 1)
-    return _Batch(block_table.data_ptr(), seq_lens.data_ptr(), cu, n, block_table.shape[1], stride, tokens)
+    width = shape[1]
+    return _Batch(block_table.data_ptr(), seq_lens.data_ptr(), cu, n, width, strides[0] if n > 1 else max(width, 1), tokens)
 
 
 def _rows(name, t, cache, heads, dtype, tokens):
-    if t.dim() != 3 or t.dtype != dtype or t.shape[0] != tokens or t.shape[2] != cache.head_dim \
-            or (heads is not None and t.shape[1] != heads) or (t.numel() and t.stride(2) != 1):
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or t.dtype != dtype or shape[0] != tokens or shape[2] != cache.head_dim \
+            or (heads is not None and shape[1] != heads) or strides[2] != 1:
         raise ValueError(f"{name} must be {dtype} [{tokens}][{'heads' if heads is None else heads}][{cache.head_dim}] with "
                          "its last dimension contiguous")
     if t.device != cache.device:
         raise ValueError(f"{name} is on {t.device}, the cache on {cache.device}")
-    return _Rows(t.data_ptr(), t.stride(0), t.stride(1))
+    return _Rows(t.data_ptr(), strides[0], strides[1])
 
 
 def _type(t):
@@ -231,7 +234,7 @@ def kv4_append(cache, k, v, block_table, seq_lens, cu_tokens=None, q=None, rotat
     def call(handle):
         out = q_out
         if q is not None and out is None:
-            out = torch.empty((tokens, heads, cache.head_dim), dtype=k.dtype, device=cache.device)
+            out = k.new_empty((tokens, heads, cache.head_dim))
         err = _library().KV4_Append(handle, cache._desc, batch, kr, vr, qr, heads, None if out is None else out.data_ptr(),
                                     rot, dtype)
         _raise(err, "kv4_append")
@@ -282,12 +285,12 @@ def kv4_attention(q, cache, block_table, seq_lens, cu_tokens=None, scale=None, w
         _check("out", out, cache.device, q.dtype, (tokens, heads, cache.head_dim))
 
     def call(handle):
-        y = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=cache.device) if out is None else out
+        y = q.new_empty((tokens, heads, cache.head_dim)) if out is None else out
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=cache.device) if return_lse else None
         if tokens:
             L = _library()
             need = L.KV4_AttentionWorkspaceBytes(cache._desc, batch, heads, window, max_len)
-            ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+            ws = cache.k_codes.new_empty(need) if need else None
             err = L.KV4_Attention(handle, cache._desc, batch, rows, heads, y.data_ptr(),
                                   None if lse is None else lse.data_ptr(),
                                   cache.head_dim ** -0.5 if scale is None else float(scale), window, max_len,
@@ -369,11 +372,11 @@ class W4Linear:
             _check("out", out, self.device, self.dtype, (N, self.M))
 
         def call(handle):
-            y = torch.empty((N, self.M), dtype=self.dtype, device=self.device) if out is None else out
+            y = x.new_empty((N, self.M)) if out is None else out
             if N:
                 L = _library()
                 need = L.W4_WorkspaceBytes(self.M, N, self.K)
-                ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+                ws = self.packed.new_empty(need) if need else None
                 err = L.W4_Linear(handle, self.packed.data_ptr(), x.data_ptr(), stride, y.data_ptr(), self.M, N, self.K,
                                   self.group, None if self.bias is None else self.bias.data_ptr(), self.activation,
                                   None if ws is None else ws.data_ptr(), need, _TYPES[self.dtype])
