@@ -79,14 +79,20 @@ __device__ __forceinline__ void load_dwords(unsigned (&dst)[N], const uint8_t* p
     }
 }
 
-// The page that holds key `pos` of the sequence, or -1.
-__device__ __forceinline__ int page_at(const AttentionArgs& a, const int* row, int pos)
+// A uniform int from memory that no kernel writes: a scalar load, which the waits for keys and values do not include.
+__device__ __forceinline__ int uniform_load(const int* p)
 {
-    const int idx = pos >> a.page_log2;
-    if (idx >= a.width)
-        return -1;
-    const int page = row[idx];
-    return page >= 0 && page < a.num_pages ? page : -1;
+    return *reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p));
+}
+
+// The entry of the block table for key `pos` of the sequence, and the page that it names, or -1.
+__device__ __forceinline__ int entry_at(const AttentionArgs& a, const int* row, int pos)
+{
+    return uniform_load(row + min(pos >> a.page_log2, a.width - 1));
+}
+__device__ __forceinline__ int page_of(const AttentionArgs& a, int entry, int pos)
+{
+    return pos >> a.page_log2 < a.width && entry >= 0 && entry < a.num_pages ? entry : -1;
 }
 
 // Loads of the 32 keys from `tile` on (a multiple of 32); p0 and p1 are the pages of its two halves of 16.
@@ -416,17 +422,19 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
         int t = t0 + wave;
         if (t < t1) {
             Keys<D> keys;
-            int     p0 = page_at(a, table, t * kTile), p1 = page_at(a, table, t * kTile + 16);
+            int     p0 = page_of(a, entry_at(a, table, t * kTile), t * kTile);
+            int     p1 = page_of(a, entry_at(a, table, t * kTile + 16), t * kTile + 16);
             load_keys<D>(keys, a, head, t * kTile, p0, p1, c, h);
             load_key_words<D>(keys, a, head, t * kTile, p0, p1, h);
             load_values<D>(keys, a, head, t * kTile, p0, p1, c, h);
             int tn = min(t + kWaves, t1 - 1); // the wave's last tile is loaded once more and not used
-            int n0 = page_at(a, table, tn * kTile), n1 = page_at(a, table, tn * kTile + 16);
+            int n0 = entry_at(a, table, tn * kTile), n1 = entry_at(a, table, tn * kTile + 16);
             for (; t < t1; t += kWaves) {
-                const int  tile = t * kTile, next = tn * kTile, q0 = n0, q1 = n1;
+                const int  tile = t * kTile, next = tn * kTile;
+                const int  q0 = page_of(a, n0, next), q1 = page_of(a, n1, next + 16);
                 const bool whole = p0 >= 0 && p1 >= 0 && tile >= lo_top && tile + kTile - 1 <= hi_low;
                 tn = min(tn + kWaves, t1 - 1);
-                n0 = page_at(a, table, tn * kTile), n1 = page_at(a, table, tn * kTile + 16);
+                n0 = entry_at(a, table, tn * kTile), n1 = entry_at(a, table, tn * kTile + 16);
                 step<D, RT>(
                     s, keys, tile, !whole, (h < 2 ? p0 : p1) < 0, qscale, h,
                     [&] { load_keys<D>(keys, a, head, next, q0, q1, c, h); },
