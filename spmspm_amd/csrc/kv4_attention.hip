@@ -147,6 +147,7 @@ template <int D, int RT>
 struct Rows {
     half8  q[RT][Shape<D>::kSteps];
     float  qsum[RT];          // sum of the row's q, in the scores' units
+    float  unit[RT];          // what a score's unit is worth, in powers of two of a probability
     int    first[RT], last[RT]; // visible keys, last < first where there is none
     float  m[RT], l[RT];
     floatx4 o[RT][Shape<D>::kVal];
@@ -156,7 +157,7 @@ struct Rows {
 // registers that they fill become free: the codes of the keys behind the scores, their words behind the exponents, the
 // values at the end.  `edge`: some key of the tile is hidden from some row; `gone`: the lane's page is not in the cache.
 template <int D, int RT, typename LoadKeys, typename LoadWords, typename LoadValues>
-__device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool edge, bool gone, float qscale, int h,
+__device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool edge, bool gone, int h,
                                      LoadKeys load_k, LoadWords load_kw, LoadValues load_v)
 {
     constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u;
@@ -184,10 +185,10 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
     for (int i = 0; i < 8; ++i) {
         const unsigned kw = t.kw[i >> 2][i & 3], vw = t.vw[i >> 2][i & 3];
         const float    zk = (float)(kw & 15u), ev = (float)(vw >> 23);
-        const float    u  = __uint_as_float(kw) * qscale; // the zero point in the lowest bits is part of the scale
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-            sc[i >> 2][r][i & 3] = __builtin_fmaf(__builtin_fmaf(-zk, s.qsum[r], sc[i >> 2][r][i & 3]), u, ev);
+        for (int r = 0; r < RT; ++r) // the zero point in the scale's lowest bits is part of it
+            sc[i >> 2][r][i & 3] = __builtin_fmaf(__builtin_fmaf(-zk, s.qsum[r], sc[i >> 2][r][i & 3]),
+                                                  __uint_as_float(kw) * s.unit[r], ev);
     }
     __builtin_amdgcn_sched_barrier(0);
     load_kw();
@@ -315,95 +316,85 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
 
     // which sequence, which of its blocks
     int b = 0;
-    for (int hi = a.batch; hi - b > 1;) {
-        const int mid = (b + hi) >> 1;
-        if (block_base(a, mid, kRows) <= (int)blockIdx.x)
-            b = mid;
-        else
-            hi = mid;
+    if (a.cu == nullptr) {
+        b = (int)blockIdx.x / ((a.share + kRows - 1) / kRows);
+    } else {
+        for (int top = a.batch; top - b > 1;) {
+            const int mid = (b + top) >> 1;
+            if (block_base(a, mid, kRows) <= (int)blockIdx.x)
+                b = mid;
+            else
+                top = mid;
+        }
     }
-    const int first = a.cu ? a.cu[b] : b, count = a.cu ? min(a.cu[b + 1], a.tokens) - first : 1;
-    const int row0 = ((int)blockIdx.x - block_base(a, b, kRows)) * kRows;
+    const int len    = uniform_load(a.lens + b);
+    const int first  = a.cu ? uniform_load(a.cu + b) : b, behind = a.cu ? uniform_load(a.cu + b + 1) : b + 1;
+    const int count  = min(behind, a.tokens) - first;
+    const int row0   = ((int)blockIdx.x - block_base(a, b, kRows)) * kRows;
     if (first < 0 || row0 < 0 || (int64_t)row0 >= (int64_t)count * a.share)
         return;
-    const int rows   = min(kRows, count * a.share - row0);
-    const int len    = min(a.lens[b], a.width << a.page_log2);
-    const int* table = a.table + (int64_t)b * a.stride;
-    const int place0 = a.lens[b] - (a.cu ? a.cu[b + 1] - first : 1); // place of the sequence's first row's token
+    const int  rows   = min(kRows, count * a.share - row0);
+    const int  cap    = a.width << a.page_log2;
+    const int* table  = a.table + (int64_t)b * a.stride;
+    const int  place0 = len - (behind - first); // place of the sequence's first row's token, below 0 where it has none
 
-    // the block's queries, scaled by a power of two that brings the largest to 2^13: fp16 then holds them exactly down to
-    // 2^-27 of it, with a factor 1/16 on those that meet the second nibble of a half
+    // keys that some row of the block sees, lo .. hi, and those that all rows see, lo_all .. hi_all
+    const int  p_first = place0 + row0 / a.share, p_last = place0 + (row0 + rows - 1) / a.share;
+    const int  hi = min(p_last, cap - 1), hi_all = p_first < 0 || p_last >= cap ? -1 : p_first;
+    const int  lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0, lo_all = a.window > 0 ? max(0, p_last - a.window + 1) : 0;
+    // the workgroup's share of them in tiles of 32; wave w takes every fourth
+    const int  t_lo = lo / kTile, t_all = hi < lo ? 0 : hi / kTile + 1 - t_lo, per = (t_all + a.splits - 1) / a.splits;
+    const int  t0 = t_lo + split * per, t1 = min(t_lo + t_all, t0 + per);
+    int        t = t0 + wave;
+    const bool any = t < t1;
+
+    // the first tile's loads go ahead of the queries'
+    Keys<D> keys;
+    int     p0 = -1, p1 = -1, n0 = -1, n1 = -1, tn = t;
+    if (any) {
+        p0 = page_of(a, entry_at(a, table, t * kTile), t * kTile);
+        p1 = page_of(a, entry_at(a, table, t * kTile + 16), t * kTile + 16);
+        tn = min(t + kWaves, t1 - 1); // the wave's last tile is loaded once more and not used
+        n0 = entry_at(a, table, tn * kTile), n1 = entry_at(a, table, tn * kTile + 16);
+        load_keys<D>(keys, a, head, t * kTile, p0, p1, c, h);
+        load_key_words<D>(keys, a, head, t * kTile, p0, p1, h);
+        load_values<D>(keys, a, head, t * kTile, p0, p1, c, h);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    // the block's queries, each row scaled by a power of two that brings its largest element to 2^13: fp16 then holds them
+    // exactly down to 2^-27 of that, with a factor 1/16 on those that meet the second nibble of a half
     Rows<D, RT> s;
-    int lo = 0x7fffffff, hi = -1, lo_top = 0, hi_low = 0x7fffffff; // visible keys: of any row, of all rows
-    float qmax = 0.f;
-    const uint16_t* qrow[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int  row  = r * 16 + c;
         const bool live = row < rows;
         const int  tok = (row0 + (live ? row : 0)) / a.share, sub = (row0 + (live ? row : 0)) % a.share;
-        qrow[r] = a.q + (int64_t)(first + tok) * a.q_token + (int64_t)(head * a.share + sub) * a.q_head + h * (D / 4);
+        const uint16_t* q = a.q + (int64_t)(first + tok) * a.q_token + (int64_t)(head * a.share + sub) * a.q_head + h * (D / 4);
+        uintx4 raw[Shape<D>::kSteps];
+#pragma unroll
+        for (int j = 0; j < Shape<D>::kSteps; ++j)
+            raw[j] = *reinterpret_cast<const uintx4*>(q + 8 * j);
+        float qmax = 0.f;
+#pragma unroll
+        for (int j = 0; j < Shape<D>::kSteps; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                qmax = fmaxf(qmax, fabsf(from16((uint16_t)(raw[j][i >> 1] >> (16 * (i & 1))), a.bf16)));
+        qmax = fmaxf(qmax, __shfl_xor(qmax, 16));
+        qmax = fmaxf(qmax, __shfl_xor(qmax, 32));
+        // an infinity spoils the row whatever the scale; frexp: qmax < 2^exp
+        const int qexp = qmax > 0.f && qmax < 3.4e38f ? min(13 - (int)__builtin_amdgcn_frexp_expf(qmax), 110) : 0;
+        float     sum  = 0.f;
 #pragma unroll
         for (int j = 0; j < Shape<D>::kSteps; ++j) {
-            const uintx4 raw = *reinterpret_cast<const uintx4*>(qrow[r] + 8 * j);
-            uint16_t     e[8];
-            __builtin_memcpy(e, &raw, 16);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float mag = fabsf(from16(e[i], a.bf16));
-                if (mag < 3.4e38f) // an infinity or NaN spoils its own row only
-                    qmax = fmaxf(qmax, mag);
-            }
-        }
-        const int place = place0 + tok;
-        s.first[r] = a.window > 0 ? max(0, place - a.window + 1) : 0;
-        s.last[r]  = min(place, len - 1);
-        if (place < 0 || place >= a.width << a.page_log2)
-            s.last[r] = -1;
-        if (!live)
-            s.first[r] = 0x7fffffff, s.last[r] = -1;
-        if (live && s.first[r] <= s.last[r]) {
-            lo = min(lo, s.first[r]);
-            hi = max(hi, s.last[r]);
-        }
-        if (live) { // a row that sees nothing makes every tile one with hidden keys
-            lo_top = max(lo_top, s.first[r]);
-            hi_low = min(hi_low, s.last[r]);
-        }
-        s.m[r] = kNone;
-        s.l[r] = 0.f;
-#pragma unroll
-        for (int e = 0; e < NV; ++e)
-            s.o[r][e] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        lo     = min(lo, __shfl_xor(lo, m));
-        hi     = max(hi, __shfl_xor(hi, m));
-        lo_top = max(lo_top, __shfl_xor(lo_top, m));
-        hi_low = min(hi_low, __shfl_xor(hi_low, m));
-        qmax   = fmaxf(qmax, __shfl_xor(qmax, m));
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
-    lo_top = __builtin_amdgcn_readfirstlane(lo_top), hi_low = __builtin_amdgcn_readfirstlane(hi_low);
-    int qexp = 13 - (int)__builtin_amdgcn_frexp_expf(qmax); // frexp: qmax < 2^exp
-    if (!(qmax > 0.f))
-        qexp = 0;
-    qexp = __builtin_amdgcn_readfirstlane(min(max(qexp, -110), 110));
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < Shape<D>::kSteps; ++j) {
-            half8        v;
-            const uintx4 raw = *reinterpret_cast<const uintx4*>(qrow[r] + 8 * j); // again: cheaper than the registers
-            uint16_t     e[8];
-            __builtin_memcpy(e, &raw, 16);
+            half8         v;
             constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7}; // element of each half of the unpacked dword
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float  full = ldexpf(from16(e[kOrder[i]], a.bf16), qexp);
-                v[i]              = (_Float16)((i >> 1) & 1 ? full * 0.0625f : full);
+                const int   e    = kOrder[i];
+                const float full = ldexpf(from16((uint16_t)(raw[j][e >> 1] >> (16 * (e & 1))), a.bf16), qexp);
+                v[i]             = (_Float16)((i >> 1) & 1 ? full * 0.0625f : full);
                 sum += (float)(_Float16)full;
             }
             s.q[r][j] = v;
@@ -411,37 +402,30 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         s.qsum[r] = sum * 0x1p-24f;
+        s.unit[r] = ldexpf(a.scale_log2, 24 - qexp);
+        const int place = place0 + tok;
+        s.first[r] = live && a.window > 0 ? max(0, place - a.window + 1) : 0;
+        s.last[r]  = live && place < cap ? place : -1;
+        s.m[r] = kNone;
+        s.l[r] = 0.f;
+#pragma unroll
+        for (int e = 0; e < NV; ++e)
+            s.o[r][e] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
-    const float qscale = ldexpf(a.scale_log2, 24 - qexp);
 
-    // the workgroup's share of the block's keys, in tiles of 32; wave w takes every fourth
-    if (hi >= 0 && lo <= hi) {
-        const int t_lo = lo / kTile, t_all = hi / kTile + 1 - t_lo;
-        const int per = (t_all + a.splits - 1) / a.splits;
-        const int t0 = t_lo + split * per, t1 = min(t_lo + t_all, t0 + per);
-        int t = t0 + wave;
-        if (t < t1) {
-            Keys<D> keys;
-            int     p0 = page_of(a, entry_at(a, table, t * kTile), t * kTile);
-            int     p1 = page_of(a, entry_at(a, table, t * kTile + 16), t * kTile + 16);
-            load_keys<D>(keys, a, head, t * kTile, p0, p1, c, h);
-            load_key_words<D>(keys, a, head, t * kTile, p0, p1, h);
-            load_values<D>(keys, a, head, t * kTile, p0, p1, c, h);
-            int tn = min(t + kWaves, t1 - 1); // the wave's last tile is loaded once more and not used
-            int n0 = entry_at(a, table, tn * kTile), n1 = entry_at(a, table, tn * kTile + 16);
-            for (; t < t1; t += kWaves) {
-                const int  tile = t * kTile, next = tn * kTile;
-                const int  q0 = page_of(a, n0, next), q1 = page_of(a, n1, next + 16);
-                const bool whole = p0 >= 0 && p1 >= 0 && tile >= lo_top && tile + kTile - 1 <= hi_low;
-                tn = min(tn + kWaves, t1 - 1);
-                n0 = entry_at(a, table, tn * kTile), n1 = entry_at(a, table, tn * kTile + 16);
-                step<D, RT>(
-                    s, keys, tile, !whole, (h < 2 ? p0 : p1) < 0, qscale, h,
-                    [&] { load_keys<D>(keys, a, head, next, q0, q1, c, h); },
-                    [&] { load_key_words<D>(keys, a, head, next, q0, q1, h); },
-                    [&] { load_values<D>(keys, a, head, next, q0, q1, c, h); });
-                p0 = q0, p1 = q1;
-            }
+    if (any) {
+        for (; t < t1; t += kWaves) {
+            const int  tile = t * kTile, next = tn * kTile;
+            const int  q0 = page_of(a, n0, next), q1 = page_of(a, n1, next + 16);
+            const bool whole = p0 >= 0 && p1 >= 0 && tile >= lo_all && tile + kTile - 1 <= hi_all;
+            tn = min(tn + kWaves, t1 - 1);
+            n0 = entry_at(a, table, tn * kTile), n1 = entry_at(a, table, tn * kTile + 16);
+            step<D, RT>(
+                s, keys, tile, !whole, (h < 2 ? p0 : p1) < 0, h,
+                [&] { load_keys<D>(keys, a, head, next, q0, q1, c, h); },
+                [&] { load_key_words<D>(keys, a, head, next, q0, q1, h); },
+                [&] { load_values<D>(keys, a, head, next, q0, q1, c, h); });
+            p0 = q0, p1 = q1;
         }
     }
 
@@ -513,29 +497,59 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
     }
 }
 
-// Joins the splits: one thread per 8 elements of a row.
+// Joins the splits of a row: threads of one row take 8 elements each, in `lanes` groups that deal the splits among them and
+// meet in LDS.
 template <int D>
-__global__ __launch_bounds__(256) void kv4_attention_join(AttentionArgs a)
+__global__ __launch_bounds__(256) void kv4_attention_join(AttentionArgs a, int lanes)
 {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)a.tokens * a.q_heads;
-    const int64_t idx = at / (D / 8);
-    const int     d0 = (int)(at % (D / 8)) * 8;
-    if (idx >= all)
-        return;
-    float mm = kNone, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    constexpr int kChunks = D / 8;
+    __shared__ float part[256][11];
+    const int     width = kChunks * lanes, rows = 256 / width; // threads of a row, rows of a workgroup
+    const int     in = threadIdx.x % width, chunk = in % kChunks, lane = in / kChunks;
+    const int64_t all = (int64_t)a.tokens * a.q_heads, idx = (int64_t)blockIdx.x * rows + threadIdx.x / width;
+    const bool    live = (int)threadIdx.x < rows * width && idx < all;
+    float         mm = kNone, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     // a token of no sequence has no partial results: its row is 0
-    int       first, count;
-    const int t = (int)(idx / a.q_heads);
-    if (sequence_of(t, a.cu, a.batch, first, count) >= 0) {
-        for (int s = 0; s < a.splits; ++s)
+    int first, count;
+    if (live && sequence_of((int)(idx / a.q_heads), a.cu, a.batch, first, count) >= 0) {
+        for (int s = lane; s < a.splits; s += lanes)
             mm = fmaxf(mm, a.part_ml[(s * all + idx) * 2]);
-        for (int s = 0; s < a.splits; ++s) {
-            const float w = __builtin_amdgcn_exp2f(a.part_ml[(s * all + idx) * 2] - mm);
+        for (int s = lane; s < a.splits; s += lanes) {
+            const float  w   = __builtin_amdgcn_exp2f(a.part_ml[(s * all + idx) * 2] - mm);
+            const float* src = a.part_o + (s * all + idx) * D + chunk * 8;
+            const floatx4 u = *reinterpret_cast<const floatx4*>(src), v = *reinterpret_cast<const floatx4*>(src + 4);
             l += w * a.part_ml[(s * all + idx) * 2 + 1];
-            const float* src = a.part_o + (s * all + idx) * D + d0;
-            for (int i = 0; i < 8; ++i)
-                o[i] += w * src[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[i] += w * u[i];
+                o[4 + i] += w * v[i];
+            }
         }
+    }
+    if (lanes > 1) {
+        float* mine = part[threadIdx.x];
+        mine[8] = mm, mine[9] = l;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            mine[i] = o[i];
+        __syncthreads();
+        if (!live || lane != 0)
+            return;
+        for (int g = 1; g < lanes; ++g)
+            mm = fmaxf(mm, part[threadIdx.x + g * kChunks][8]);
+        l = 0.f;
+        for (int i = 0; i < 8; ++i)
+            o[i] = 0.f;
+        for (int g = 0; g < lanes; ++g) {
+            const float* p = part[threadIdx.x + g * kChunks];
+            const float  w = __builtin_amdgcn_exp2f(p[8] - mm);
+            l += w * p[9];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                o[i] += w * p[i];
+        }
+    } else if (!live) {
+        return;
     }
     const bool  none = l == 0.f;
     const float inv  = none ? 0.f : 1.f / l;
@@ -544,8 +558,8 @@ __global__ __launch_bounds__(256) void kv4_attention_join(AttentionArgs a)
         e[i] = to16(none ? 0.f : o[i] * inv, a.bf16);
     uintx4 v;
     __builtin_memcpy(&v, e, 16);
-    *reinterpret_cast<uintx4*>(a.out + idx * D + d0) = v;
-    if (a.lse != nullptr && d0 == 0)
+    *reinterpret_cast<uintx4*>(a.out + idx * D + chunk * 8) = v;
+    if (a.lse != nullptr && chunk == 0)
         a.lse[idx] = none ? -__builtin_inff() : (__log2f(l) + (mm - 127.f)) * 0.69314718055994531f;
 }
 
@@ -604,8 +618,11 @@ int run(hipStream_t stream, const Plan& p, const AttentionArgs& a)
         return (int)hipErrorInvalidValue; // plan_of gives heads of 256 one row tile: two would not fit the registers
     if (err != 0 || p.splits == 1)
         return err;
-    const int64_t threads = (int64_t)a.tokens * a.q_heads * (D / 8);
-    return launch(kv4_attention_join<D>, dim3((unsigned)((threads + 255) / 256), 1, 1), dim3(256, 1, 1), stream, a);
+    int lanes = 1;
+    while (lanes < a.splits && 2 * lanes * (D / 8) <= 256)
+        lanes *= 2;
+    const int64_t per = 256 / (lanes * (D / 8)), all = (int64_t)a.tokens * a.q_heads;
+    return launch(kv4_attention_join<D>, dim3((unsigned)((all + per - 1) / per), 1, 1), dim3(256, 1, 1), stream, a, lanes);
 }
 
 } // namespace
