@@ -299,12 +299,14 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, h = lane >> 4;
-    const int head = blockIdx.y, split = blockIdx.z;
+    // heads are dealt first: workgroups go to the eight dies in turn, and so do a sequence's heads, whatever its length, while
+    // all of a head's blocks of rows find its keys in one L2 wherever the number of heads is a multiple of eight
+    const int head = blockIdx.x % a.kv_heads, block = blockIdx.x / a.kv_heads, split = blockIdx.y;
 
     if (a.cu != nullptr && a.splits == 1) { // rows of no sequence (otherwise kv4_attention_join writes them)
         const int before = min(max(a.cu[0], 0), a.tokens), behind = min(max(a.cu[a.batch], 0), a.tokens);
         const int idle = before + a.tokens - behind;
-        for (int i = blockIdx.x; i < idle; i += gridDim.x) {
+        for (int i = block; i < idle; i += (int)(gridDim.x / a.kv_heads)) {
             const int64_t at = (int64_t)(i < before ? i : behind + i - before) * a.q_heads + head * a.share;
             for (int e = threadIdx.x; e < a.share * (D / 8); e += kWave * kWaves)
                 *reinterpret_cast<uintx4*>(a.out + at * D + e * 8) = uintx4{0, 0, 0, 0};
@@ -317,11 +319,11 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
     // which sequence, which of its blocks
     int b = 0;
     if (a.cu == nullptr) {
-        b = (int)blockIdx.x / ((a.share + kRows - 1) / kRows);
+        b = block / ((a.share + kRows - 1) / kRows);
     } else {
         for (int top = a.batch; top - b > 1;) {
             const int mid = (b + top) >> 1;
-            if (block_base(a, mid, kRows) <= (int)blockIdx.x)
+            if (block_base(a, mid, kRows) <= block)
                 b = mid;
             else
                 top = mid;
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
     const int len    = uniform_load(a.lens + b);
     const int first  = a.cu ? uniform_load(a.cu + b) : b, behind = a.cu ? uniform_load(a.cu + b + 1) : b + 1;
     const int count  = min(behind, a.tokens) - first;
-    const int row0   = ((int)blockIdx.x - block_base(a, b, kRows)) * kRows;
+    const int row0   = (block - block_base(a, b, kRows)) * kRows;
     if (first < 0 || row0 < 0 || (int64_t)row0 >= (int64_t)count * a.share)
         return;
     const int  rows   = min(kRows, count * a.share - row0);
@@ -566,7 +568,8 @@ __global__ __launch_bounds__(256) void kv4_attention_join(AttentionArgs a, int l
 namespace {
 
 struct Plan {
-    int row_tiles, blocks, splits;
+    int     row_tiles, splits;
+    int64_t blocks;
 };
 
 // Row tiles per wave: as many as the average sequence fills, up to two.  Splits of the keys: enough workgroups for every
@@ -578,7 +581,7 @@ Plan plan_of(const KV4_Cache& c, const KV4_Batch& b, int q_heads, int window, in
     const int64_t rows  = (int64_t)b.total_tokens * share, each = (rows + b.batch - 1) / b.batch;
     p.row_tiles = each <= 16 || c.head_dim == 256 ? 1 : 2;
     const int64_t per = 16 * p.row_tiles;
-    p.blocks          = (int)(b.cu_tokens == nullptr ? b.batch * ((share + per - 1) / per) : rows / per + b.batch);
+    p.blocks          = (b.cu_tokens == nullptr ? b.batch * ((share + per - 1) / per) : rows / per + b.batch);
     const int64_t capacity = (int64_t)b.table_width * c.page_size;
     int64_t       len      = max_len > 0 ? std::min<int64_t>(max_len, capacity) : capacity;
     if (window > 0) // what a block's rows see of it
@@ -608,7 +611,7 @@ int check_heads(const KV4_Cache* c, int q_heads)
 template <int D>
 int run(hipStream_t stream, const Plan& p, const AttentionArgs& a)
 {
-    const dim3 grid((unsigned)p.blocks, (unsigned)a.kv_heads, (unsigned)p.splits), block(kWave * kWaves, 1, 1);
+    const dim3 grid((unsigned)p.blocks * a.kv_heads, (unsigned)p.splits, 1), block(kWave * kWaves, 1, 1);
     int        err;
     if (p.row_tiles == 1)
         err = launch(kv4_attention<D, 1>, grid, block, stream, a);
@@ -658,7 +661,9 @@ extern "C" int KV4_Attention(hipStream_t stream, const KV4_Cache* cache, const K
     if (bad_pointer(q.data, 16) || bad_pointer(out, 16) || (lse != nullptr && bad_pointer(lse, 4)) ||
         q.token_stride % 8 != 0 || q.head_stride % 8 != 0)
         return refuse("a null or misaligned q, out or lse (16 bytes, strides multiples of 8 elements)");
-    const Plan   p    = plan_of(*cache, *batch, q_heads, window, max_len);
+    const Plan p = plan_of(*cache, *batch, q_heads, window, max_len);
+    if (p.blocks * cache->kv_heads > 0x7fffffff || (int64_t)batch->total_tokens * q_heads > 0x7fffffff)
+        return refuse("%d tokens of %d heads: the grid is too large", batch->total_tokens, q_heads);
     const size_t need = workspace_of(*cache, *batch, q_heads, p);
     if (need > 0 && (bad_pointer(workspace, 16) || workspace_bytes < need))
         return refuse("workspace of %zu bytes (16-byte aligned), %zu needed", workspace == nullptr ? (size_t)0 : workspace_bytes, need);
