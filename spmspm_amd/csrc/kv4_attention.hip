@@ -79,12 +79,6 @@ __device__ __forceinline__ void load_dwords(unsigned (&dst)[N], const uint8_t* p
     }
 }
 
-// A uniform int from memory that no kernel writes: a scalar load, which the waits for keys and values do not include.
-__device__ __forceinline__ int uniform_load(const int* p)
-{
-    return *reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p));
-}
-
 // The entry of the block table for key `pos` of the sequence, and the page that it names, or -1.
 __device__ __forceinline__ int entry_at(const AttentionArgs& a, const int* row, int pos)
 {
@@ -512,8 +506,8 @@ __global__ __launch_bounds__(256) void kv4_attention_join(AttentionArgs a, int l
     const bool    live = (int)threadIdx.x < rows * width && idx < all;
     float         mm = kNone, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     // a token of no sequence has no partial results: its row is 0
-    int first, count;
-    if (live && sequence_of((int)(idx / a.q_heads), a.cu, a.batch, first, count) >= 0) {
+    const int token = (int)(idx / a.q_heads);
+    if (live && (a.cu == nullptr || (token >= a.cu[0] && token < a.cu[a.batch]))) {
         for (int s = lane; s < a.splits; s += lanes)
             mm = fmaxf(mm, a.part_ml[(s * all + idx) * 2]);
         for (int s = lane; s < a.splits; s += lanes) {

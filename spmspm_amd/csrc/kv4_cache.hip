@@ -1,6 +1,8 @@
 // Writing and reading the paged 4-bit key/value cache: KV4_Append, KV4_Gather (decode_api.h holds the format).
 #include "decode_common.hiph"
 
+#include <algorithm>
+
 // Every product, sum and quotient below is rounded by itself: the codes are then the same wherever they are computed.
 #pragma clang fp contract(off)
 
@@ -9,7 +11,7 @@ namespace decode {
 struct CacheView {
     uint8_t* codes[2]; // keys, values
     int32_t* words[2];
-    int      num_pages, page_size, kv_heads, head_dim;
+    int      num_pages, page_log2, kv_heads, head_dim;
 };
 
 struct BatchView {
@@ -26,10 +28,12 @@ struct AppendArgs {
     const float*    rot;
     const int*      positions;
     int             q_heads, rot_rows, rot_dims, interleaved, bf16;
+    int             rot_quads; // the rotation's rows can be read 16 bytes at a time
     int             wide; // bit s: src[s] can be read 16 bytes at a time
 };
 
-// Place of row t in its sequence: page (or -1) and slot; `place` is the position, negative where there is none.
+// Place of row t in its sequence: page (or -1) and slot; `place` is the position, negative where there is none.  The same for
+// the whole wave.
 __device__ __forceinline__ int locate(const CacheView& c, const BatchView& b, int t, int& slot, int& place)
 {
     int       first, count;
@@ -38,153 +42,193 @@ __device__ __forceinline__ int locate(const CacheView& c, const BatchView& b, in
     slot        = 0;
     if (s < 0)
         return -1;
-    const int pos = b.lens[s] - count + (t - first);
+    const int pos = uniform_load(b.lens + s) - count + (t - first);
     if (pos < 0)
         return -1;
     place         = pos;
-    const int idx = pos / c.page_size; // a power of two, but a division once per vector costs nothing here
+    const int idx = pos >> c.page_log2;
     if (idx >= b.width)
         return -1;
-    const int page = b.table[(int64_t)s * b.stride + idx];
+    const int page = uniform_load(b.table + (int64_t)s * b.stride + idx);
     if (page < 0 || page >= c.num_pages)
         return -1;
-    slot = pos & (c.page_size - 1);
+    slot = pos & ((1 << c.page_log2) - 1);
     return page;
 }
 
-__device__ __forceinline__ void load8(const uint16_t* p, bool wide, bool bf16, float (&x)[8])
+// Eight 16-bit elements, one by one where they are not aligned.
+__device__ __forceinline__ uintx4 load8(const uint16_t* p, bool wide)
 {
+    if (wide)
+        return *reinterpret_cast<const uintx4*>(p);
     uint16_t raw[8];
-    if (wide) {
-        const uintx4 v = *reinterpret_cast<const uintx4*>(p);
-        __builtin_memcpy(raw, &v, 16);
-    } else {
-        for (int i = 0; i < 8; ++i)
-            raw[i] = p[i];
-    }
     for (int i = 0; i < 8; ++i)
-        x[i] = from16(raw[i], bf16);
+        raw[i] = p[i];
+    uintx4 v;
+    __builtin_memcpy(&v, raw, 16);
+    return v;
 }
 
-// Rotates elements d0 .. d0+7 (in x) of the head at `row`.
-__device__ __forceinline__ void rotate8(const AppendArgs& a, const uint16_t* row, bool wide, int d0, int pos, float (&x)[8])
+__device__ __forceinline__ float element(const uintx4& v, int i, bool bf16)
 {
-    const int half = a.rot_dims >> 1;
-    if (d0 >= a.rot_dims)
-        return;
-    const bool   inside = pos >= 0 && pos < a.rot_rows;
-    const float* tab    = a.rot + (int64_t)(inside ? pos : 0) * a.rot_dims;
-    const float  nan    = __uint_as_float(0x7fc00000u);
-    if (a.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            if (d0 + i < a.rot_dims) {
-                const float c = inside ? tab[(d0 + i) >> 1] : nan, s = inside ? tab[half + ((d0 + i) >> 1)] : nan;
-                const float u = x[i], v = x[i + 1];
-                x[i]     = u * c - v * s;
-                x[i + 1] = v * c + u * s;
-            }
-        }
-        return;
-    }
-    float other[8];
-    if ((half & 7) == 0) { // all eight on one side: the partners are eight neighbours too
-        load8(row + (d0 < half ? d0 + half : d0 - half), wide, a.bf16, other);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int d = d0 + i, p = d < half ? d + half : d - half;
-            other[i]    = d < a.rot_dims ? from16(row[p], a.bf16) : 0.f;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = d0 + i;
-        if (d < a.rot_dims) {
-            const bool  low = d < half;
-            const int   j   = low ? d : d - half;
-            const float c = inside ? tab[j] : nan, s = inside ? tab[half + j] : nan;
-            x[i] = low ? x[i] * c - other[i] * s : x[i] * c + other[i] * s;
-        }
-    }
+    return from16((uint16_t)(v[i >> 1] >> (16 * (i & 1))), bf16);
 }
 
-// One group of L lanes (8 elements each; L = 8, 16 or 32) per head vector: keys, values, then queries of a token.  A key or
-// value is read once, rotated and encoded in registers (the extremes pass between the group's lanes) and written as one
-// dword of codes per lane.
+// One token per workgroup row, one group of L lanes (8 elements each; L = 8, 16 or 32) per head vector at a time: keys, values,
+// then queries.  A vector is read once, rotated and encoded in registers (its extremes pass between the group's lanes) and
+// written as one dword of codes per lane; the lane's part of the rotation's row is read once for all of them.  Bound by
+// memory for long prompts, by launch and the chain cu_tokens -> length -> table for single tokens.
 template <int L>
-__global__ __launch_bounds__(256) void kv4_append(AppendArgs a, int heads)
+__global__ __launch_bounds__(256) void kv4_append(AppendArgs a, int heads, int per)
 {
-    const int lane = threadIdx.x & (L - 1), d0 = lane * 8;
-    const int unit = blockIdx.y * (256 / L) + threadIdx.x / L;
-    const int t    = blockIdx.x;
-    if (unit >= heads)
-        return; // whole groups
-    const bool live = d0 < a.cache.head_dim; // heads of 96 leave four lanes of sixteen idle: they exchange zeros below
-    const int side = unit < a.cache.kv_heads ? 0 : (unit < 2 * a.cache.kv_heads ? 1 : 2);
-    const int head = unit - side * a.cache.kv_heads;
+    constexpr int kGroups = 256 / L;
+    const int     lane = threadIdx.x & (L - 1), d0 = lane * 8, t = blockIdx.x, D = a.cache.head_dim;
+    const bool    live = d0 < D; // heads of 96 leave four lanes of sixteen idle: they exchange zeros below
+    const int     first = blockIdx.y * per * kGroups + threadIdx.x / L, last = min(heads, first + per * kGroups);
+    const int     kvh = a.cache.kv_heads, half = a.rot_dims >> 1;
+    const bool    together = (half & 7) == 0; // the partners of eight elements are eight elements in a row
+
+    // a vector's elements, and those `half` away that they are rotated with
+    auto source = [&](int unit) {
+        const int side = unit < kvh ? 0 : (unit < 2 * kvh ? 1 : 2);
+        return a.src[side] + t * a.token_stride[side] + (unit - side * kvh) * a.head_stride[side];
+    };
+    auto is_wide = [&](int unit) { return ((a.wide >> (unit < kvh ? 0 : (unit < 2 * kvh ? 1 : 2))) & 1) != 0; };
+    auto partner = [&](int unit) {
+        return together && !a.interleaved && d0 < a.rot_dims ? load8(source(unit) + (d0 < half ? d0 + half : d0 - half), is_wide(unit))
+                                                             : uintx4{0, 0, 0, 0};
+    };
+    uintx4 raw{0, 0, 0, 0}, beside{0, 0, 0, 0};
+    if (live && first < last) { // on their way before the token's place is known
+        raw    = load8(source(first) + d0, is_wide(first));
+        beside = partner(first);
+    }
     int       slot, place;
     const int page = locate(a.cache, a.batch, t, slot, place);
-    if (side < 2 && page < 0)
-        return;
-    const uint16_t* row  = a.src[side] + t * a.token_stride[side] + head * a.head_stride[side];
-    const bool      wide = (a.wide >> side) & 1;
-    float           x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live)
-        load8(row + d0, wide, a.bf16, x);
-    if (live && side != 1 && a.rot_dims > 0) {
-        if (a.positions != nullptr)
-            rotate8(a, row, wide, d0, a.positions[t], x);
-        else if (place >= 0)
-            rotate8(a, row, wide, d0, place, x);
-    }
-    if (side == 2) {
-        if (!live)
-            return;
-        uint16_t out[8];
-        for (int i = 0; i < 8; ++i)
-            out[i] = to16(x[i], a.bf16);
-        uintx4 v;
-        __builtin_memcpy(&v, out, 16);
-        *reinterpret_cast<uintx4*>(a.q_out + ((int64_t)t * a.q_heads + head) * a.cache.head_dim + d0) = v;
-        return;
-    }
-    float hi = 0.f, lo = 0.f;
-    int   bad = 0;
-    for (int i = 0; i < 8; ++i) {
-        hi = fmaxf(hi, x[i]);
-        lo = fminf(lo, x[i]);
-        bad |= (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u;
-    }
+
+    // what an element is multiplied by, and what its partner is before it is added
+    const int  row  = a.positions != nullptr ? uniform_load(a.positions + t) : place;
+    const bool turn = live && d0 < a.rot_dims && (a.positions != nullptr || place >= 0);
+    float      own[8], other[8];
+    if (turn) {
+        const bool   inside = row >= 0 && row < a.rot_rows;
+        const float* tab    = a.rot + (int64_t)(inside ? row : 0) * a.rot_dims;
+        if (a.rot_quads) {
+            if (a.interleaved) {
+                const floatx4 c = *reinterpret_cast<const floatx4*>(tab + (d0 >> 1)), s = *reinterpret_cast<const floatx4*>(tab + half + (d0 >> 1));
 #pragma unroll
-    for (int m = 1; m < L; m <<= 1) {
-        hi = fmaxf(hi, __shfl_xor(hi, m, L));
-        lo = fminf(lo, __shfl_xor(lo, m, L));
-        bad |= __shfl_xor(bad, m, L);
+                for (int i = 0; i < 8; ++i)
+                    own[i] = c[i >> 1], other[i] = (i & 1) ? s[i >> 1] : -s[i >> 1];
+            } else {
+                const bool   low = d0 < half;
+                const float* at  = tab + (low ? d0 : d0 - half);
+                floatx4      c[2], s[2];
+                c[0] = *reinterpret_cast<const floatx4*>(at), c[1] = *reinterpret_cast<const floatx4*>(at + 4);
+                s[0] = *reinterpret_cast<const floatx4*>(at + half), s[1] = *reinterpret_cast<const floatx4*>(at + half + 4);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    own[i] = c[i >> 2][i & 3], other[i] = low ? -s[i >> 2][i & 3] : s[i >> 2][i & 3]; // a + (-b) is a - b
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int  d = min(d0 + i, a.rot_dims - 1);
+                const bool low = a.interleaved ? (i & 1) == 0 : d < half;
+                const int  j = a.interleaved ? d >> 1 : (low ? d : d - half);
+                own[i]   = tab[j];
+                other[i] = low ? -tab[half + j] : tab[half + j];
+            }
+        }
+        if (!inside) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                own[i] = other[i] = __uint_as_float(0x7fc00000u);
+        }
     }
-    const float fifteenth = 1.0f / 15.0f;
-    const float s         = hi * fifteenth - lo * fifteenth;
-    unsigned    word      = (__float_as_uint(s) + 8u) & ~15u;
-    if (s < 0x1p-100f)
-        word = 0x3f800000u;
-    const float z    = fminf(fmaxf(rintf(-lo * (1.0f / __uint_as_float(word))), 0.f), 15.f);
-    word |= (unsigned)z;
-    const float inv   = 1.0f / __uint_as_float(word);
-    unsigned    codes = 0;
-    for (int i = 0; i < 8; ++i) {
-        const float q = fminf(fmaxf(rintf(x[i] * inv) + z, 0.f), 15.f);
-        codes |= (unsigned)q << (4 * i);
+    for (int unit = first; unit < last; unit += kGroups) {
+        const int    side = unit < kvh ? 0 : (unit < 2 * kvh ? 1 : 2), head = unit - side * kvh;
+        const uintx4 mine = raw, theirs = beside;
+        if (live && unit + kGroups < last) {
+            raw    = load8(source(unit + kGroups) + d0, is_wide(unit + kGroups));
+            beside = partner(unit + kGroups);
+        }
+        if (side < 2 && page < 0)
+            continue; // the whole group
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[i] = element(mine, i, a.bf16);
+        if (turn && side != 1) {
+            float y[8];
+            if (a.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    y[i] = x[i ^ 1];
+            } else if (together) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    y[i] = element(theirs, i, a.bf16);
+            } else {
+                const uint16_t* src = source(unit);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int d = min(d0 + i, a.rot_dims - 1);
+                    y[i]        = from16(src[d < half ? d + half : d - half], a.bf16);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[i] = d0 + i < a.rot_dims ? x[i] * own[i] + y[i] * other[i] : x[i];
+        }
+        if (side == 2) {
+            uint16_t out[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                out[i] = to16(x[i], a.bf16);
+            uintx4 v;
+            __builtin_memcpy(&v, out, 16);
+            if (live)
+                *reinterpret_cast<uintx4*>(a.q_out + ((int64_t)t * a.q_heads + head) * D + d0) = v;
+            continue;
+        }
+        float hi = 0.f, lo = 0.f;
+        int   bad = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            hi = fmaxf(hi, x[i]);
+            lo = fminf(lo, x[i]);
+            bad |= (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u;
+        }
+#pragma unroll
+        for (int m = 1; m < L; m <<= 1) {
+            hi = fmaxf(hi, __shfl_xor(hi, m, L));
+            lo = fminf(lo, __shfl_xor(lo, m, L));
+            bad |= __shfl_xor(bad, m, L);
+        }
+        const float fifteenth = 1.0f / 15.0f;
+        const float s         = hi * fifteenth - lo * fifteenth;
+        unsigned    word      = (__float_as_uint(s) + 8u) & ~15u;
+        if (s < 0x1p-100f)
+            word = 0x3f800000u;
+        const float z = fminf(fmaxf(rintf(-lo * (1.0f / __uint_as_float(word))), 0.f), 15.f);
+        word |= (unsigned)z;
+        const float inv   = 1.0f / __uint_as_float(word);
+        unsigned    codes = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q = fminf(fmaxf(rintf(x[i] * inv) + z, 0.f), 15.f);
+            codes |= (unsigned)q << (4 * i);
+        }
+        if (bad) {
+            word  = 0x7fc00000u;
+            codes = 0;
+        }
+        const int64_t at = ((((int64_t)page * kvh + head)) << a.cache.page_log2) + slot;
+        if (live)
+            *reinterpret_cast<unsigned*>(a.cache.codes[side] + at * (D / 2) + lane * 4) = codes;
+        if (lane == 0)
+            a.cache.words[side][at] = (int)word;
     }
-    if (bad) {
-        word  = 0x7fc00000u;
-        codes = 0;
-    }
-    if (!live)
-        return;
-    const int64_t at = ((int64_t)page * a.cache.kv_heads + head) * a.cache.page_size + slot;
-    *reinterpret_cast<unsigned*>(a.cache.codes[side] + at * (a.cache.head_dim / 2) + lane * 4) = codes;
-    if (lane == 0)
-        a.cache.words[side][at] = (int)word;
 }
 
 struct GatherArgs {
@@ -195,32 +239,33 @@ struct GatherArgs {
 };
 
 template <int L>
-__global__ __launch_bounds__(256) void kv4_gather(GatherArgs a)
+__global__ __launch_bounds__(256) void kv4_gather(GatherArgs a, int per)
 {
-    const int lane = threadIdx.x & (L - 1), d0 = lane * 8;
-    const int unit = blockIdx.y * (256 / L) + threadIdx.x / L;
-    const int t    = blockIdx.x;
-    if (unit >= 2 * a.cache.kv_heads || d0 >= a.cache.head_dim)
-        return;
-    const int side = unit < a.cache.kv_heads ? 0 : 1, head = unit - side * a.cache.kv_heads;
-    if (a.dst[side] == nullptr)
+    constexpr int kGroups = 256 / L;
+    const int     lane = threadIdx.x & (L - 1), d0 = lane * 8, t = blockIdx.x, D = a.cache.head_dim, kvh = a.cache.kv_heads;
+    const int     first = blockIdx.y * per * kGroups + threadIdx.x / L, last = min(2 * kvh, first + per * kGroups);
+    if (d0 >= D)
         return;
     int       slot, place;
     const int page = locate(a.cache, a.batch, t, slot, place);
-    uint16_t  out[8];
-    for (int i = 0; i < 8; ++i)
-        out[i] = 0;
-    if (page >= 0) {
-        const int64_t  at    = ((int64_t)page * a.cache.kv_heads + head) * a.cache.page_size + slot;
-        const unsigned codes = *reinterpret_cast<const unsigned*>(a.cache.codes[side] + at * (a.cache.head_dim / 2) + lane * 4);
-        const unsigned word  = (unsigned)a.cache.words[side][at];
-        const int      z     = word & 15;
-        for (int i = 0; i < 8; ++i)
-            out[i] = to16(__uint_as_float(word) * (float)((int)((codes >> (4 * i)) & 15) - z), a.bf16);
+    for (int unit = first; unit < last; unit += kGroups) {
+        const int side = unit < kvh ? 0 : 1, head = unit - side * kvh;
+        if (a.dst[side] == nullptr)
+            continue;
+        uint16_t out[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (page >= 0) {
+            const int64_t  at    = (((int64_t)page * kvh + head) << a.cache.page_log2) + slot;
+            const unsigned codes = *reinterpret_cast<const unsigned*>(a.cache.codes[side] + at * (D / 2) + lane * 4);
+            const unsigned word  = (unsigned)a.cache.words[side][at];
+            const int      z     = word & 15;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                out[i] = to16(__uint_as_float(word) * (float)((int)((codes >> (4 * i)) & 15) - z), a.bf16);
+        }
+        uintx4 v;
+        __builtin_memcpy(&v, out, 16);
+        *reinterpret_cast<uintx4*>(a.dst[side] + ((int64_t)t * kvh + head) * D + d0) = v;
     }
-    uintx4 v;
-    __builtin_memcpy(&v, out, 16);
-    *reinterpret_cast<uintx4*>(a.dst[side] + ((int64_t)t * a.cache.kv_heads + head) * a.cache.head_dim + d0) = v;
 }
 
 namespace {
@@ -230,7 +275,7 @@ CacheView view(const KV4_Cache& c)
     return {{static_cast<uint8_t*>(c.k_codes), static_cast<uint8_t*>(c.v_codes)},
             {c.k_words, c.v_words},
             c.num_pages,
-            c.page_size,
+            __builtin_ctz((unsigned)c.page_size),
             c.kv_heads,
             c.head_dim};
 }
@@ -243,6 +288,14 @@ BatchView view(const KV4_Batch& b)
 int lanes_of(int head_dim)
 {
     return head_dim == 64 ? 8 : (head_dim == 256 ? 32 : 16);
+}
+
+// Head vectors a group of lanes takes one after the other: all of a token's where there are many tokens, so that its place and
+// its row of the rotation are looked up once, one where they are few and the chain of loads is what counts.
+int vectors_per_group(int heads, int groups, int tokens)
+{
+    const int all = (heads + groups - 1) / groups;
+    return std::max(1, std::min<int>(all, (int)((int64_t)all * tokens / 2048)));
 }
 
 int check_dtype(int dtype)
@@ -278,6 +331,7 @@ extern "C" int KV4_Append(hipStream_t stream, const KV4_Cache* cache, const KV4_
         a.rot_rows    = rotary->table_rows;
         a.rot_dims    = rotary->dims;
         a.interleaved = rotary->interleaved != 0;
+        a.rot_quads   = rotary->dims % 16 == 0 && !bad_pointer(rotary->table, 16);
     }
     if (q.data != nullptr && rotary == nullptr)
         return refuse("queries are given and no rotation");
@@ -302,9 +356,10 @@ extern "C" int KV4_Append(hipStream_t stream, const KV4_Cache* cache, const KV4_
     a.bf16          = dtype == DECODE_BF16;
     const int heads = 2 * cache->kv_heads + (q.data != nullptr ? q_heads : 0);
     const int L     = lanes_of(cache->head_dim), per = 256 / L;
-    dim3      grid((unsigned)batch->total_tokens, (unsigned)((heads + per - 1) / per), 1);
+    const int each = vectors_per_group(heads, per, batch->total_tokens);
+    dim3      grid((unsigned)batch->total_tokens, (unsigned)((heads + per * each - 1) / (per * each)), 1);
     auto      kernel = L == 8 ? kv4_append<8> : (L == 16 ? kv4_append<16> : kv4_append<32>);
-    return launch(kernel, grid, dim3(256, 1, 1), stream, a, heads);
+    return launch(kernel, grid, dim3(256, 1, 1), stream, a, heads, each);
 }
 
 extern "C" int KV4_Gather(hipStream_t stream, const KV4_Cache* cache, const KV4_Batch* batch, void* k, void* v, int dtype)
@@ -321,7 +376,8 @@ extern "C" int KV4_Gather(hipStream_t stream, const KV4_Cache* cache, const KV4_
         return 0;
     GatherArgs a{view(*cache), view(*batch), {static_cast<uint16_t*>(k), static_cast<uint16_t*>(v)}, dtype == DECODE_BF16};
     const int  L = lanes_of(cache->head_dim), per = 256 / L;
-    dim3       grid((unsigned)batch->total_tokens, (unsigned)((2 * cache->kv_heads + per - 1) / per), 1);
+    const int  each = vectors_per_group(2 * cache->kv_heads, per, batch->total_tokens);
+    dim3       grid((unsigned)batch->total_tokens, (unsigned)((2 * cache->kv_heads + per * each - 1) / (per * each)), 1);
     auto       kernel = L == 8 ? kv4_gather<8> : (L == 16 ? kv4_gather<16> : kv4_gather<32>);
-    return launch(kernel, grid, dim3(256, 1, 1), stream, a);
+    return launch(kernel, grid, dim3(256, 1, 1), stream, a, each);
 }
