@@ -19,6 +19,25 @@ struct BatchView {
     int        batch, width, stride, tokens;
 };
 
+// The largest of L lanes' values (at least 0), in all of them.
+template <int PATTERN>
+__device__ __forceinline__ float across(float v)
+{
+    return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), PATTERN, 0xf, 0xf, true));
+}
+template <int L>
+__device__ __forceinline__ float group_max(float v)
+{
+    v = fmaxf(v, across<0xb1>(v));  // neighbours
+    v = fmaxf(v, across<0x4e>(v));  // pairs of a quad
+    v = fmaxf(v, across<0x141>(v)); // quads of eight, mirrored
+    if constexpr (L >= 16)
+        v = fmaxf(v, across<0x140>(v)); // eights of sixteen, mirrored
+    if constexpr (L == 32)
+        v = fmaxf(v, __shfl_xor(v, 16, 32));
+    return v;
+}
+
 struct AppendArgs {
     CacheView       cache;
     BatchView       batch;
@@ -32,8 +51,7 @@ struct AppendArgs {
     int             wide; // bit s: src[s] can be read 16 bytes at a time
 };
 
-// Place of row t in its sequence: page (or -1) and slot; `place` is the position, negative where there is none.  The same for
-// the whole wave.
+// Place of row t in its sequence: page (or -1) and slot; `place` is the position, negative where there is none.
 __device__ __forceinline__ int locate(const CacheView& c, const BatchView& b, int t, int& slot, int& place)
 {
     int       first, count;
@@ -42,14 +60,14 @@ __device__ __forceinline__ int locate(const CacheView& c, const BatchView& b, in
     slot        = 0;
     if (s < 0)
         return -1;
-    const int pos = uniform_load(b.lens + s) - count + (t - first);
+    const int pos = b.lens[s] - count + (t - first);
     if (pos < 0)
         return -1;
     place         = pos;
     const int idx = pos >> c.page_log2;
     if (idx >= b.width)
         return -1;
-    const int page = uniform_load(b.table + (int64_t)s * b.stride + idx);
+    const int page = b.table[(int64_t)s * b.stride + idx];
     if (page < 0 || page >= c.num_pages)
         return -1;
     slot = pos & ((1 << c.page_log2) - 1);
@@ -74,19 +92,24 @@ __device__ __forceinline__ float element(const uintx4& v, int i, bool bf16)
     return from16((uint16_t)(v[i >> 1] >> (16 * (i & 1))), bf16);
 }
 
-// One token per workgroup row, one group of L lanes (8 elements each; L = 8, 16 or 32) per head vector at a time: keys, values,
-// then queries.  A vector is read once, rotated and encoded in registers (its extremes pass between the group's lanes) and
-// written as one dword of codes per lane; the lane's part of the rotation's row is read once for all of them.  Bound by
-// memory for long prompts, by launch and the chain cu_tokens -> length -> table for single tokens.
+// A group of L lanes (8 elements each; L = 8, 16 or 32) works for one token, the groups of a workgroup for tokens in a row,
+// and takes `per` of its vectors one after the other: keys, values, then queries.  A vector is read once, rotated and encoded
+// in registers (its extremes pass between the group's lanes) and written as one dword of codes per lane.  Tokens in a row lie
+// side by side in a page, so that a workgroup writes whole lines of codes and words; with a workgroup for each token, codes
+// and above all single words went to memory as parts of lines (12k tokens, 8 key/value and 32 query heads of 128: 105 us).
+// The lane's part of the rotation's row is read once for all of the token's vectors.
 template <int L>
 __global__ __launch_bounds__(256) void kv4_append(AppendArgs a, int heads, int per)
 {
     constexpr int kGroups = 256 / L;
-    const int     lane = threadIdx.x & (L - 1), d0 = lane * 8, t = blockIdx.x, D = a.cache.head_dim;
+    const int     lane = threadIdx.x & (L - 1), d0 = lane * 8, D = a.cache.head_dim;
+    const int     t    = blockIdx.x * kGroups + threadIdx.x / L;
     const bool    live = d0 < D; // heads of 96 leave four lanes of sixteen idle: they exchange zeros below
-    const int     first = blockIdx.y * per * kGroups + threadIdx.x / L, last = min(heads, first + per * kGroups);
+    const int     first = blockIdx.y * per, last = min(heads, first + per);
     const int     kvh = a.cache.kv_heads, half = a.rot_dims >> 1;
     const bool    together = (half & 7) == 0; // the partners of eight elements are eight elements in a row
+    if (t >= a.batch.tokens)
+        return; // whole groups
 
     // a vector's elements, and those `half` away that they are rotated with
     auto source = [&](int unit) {
@@ -107,7 +130,7 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a, int heads, int p
     const int page = locate(a.cache, a.batch, t, slot, place);
 
     // what an element is multiplied by, and what its partner is before it is added
-    const int  row  = a.positions != nullptr ? uniform_load(a.positions + t) : place;
+    const int  row  = a.positions != nullptr ? a.positions[t] : place;
     const bool turn = live && d0 < a.rot_dims && (a.positions != nullptr || place >= 0);
     float      own[8], other[8];
     if (turn) {
@@ -145,12 +168,12 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a, int heads, int p
                 own[i] = other[i] = __uint_as_float(0x7fc00000u);
         }
     }
-    for (int unit = first; unit < last; unit += kGroups) {
+    for (int unit = first; unit < last; ++unit) {
         const int    side = unit < kvh ? 0 : (unit < 2 * kvh ? 1 : 2), head = unit - side * kvh;
         const uintx4 mine = raw, theirs = beside;
-        if (live && unit + kGroups < last) {
-            raw    = load8(source(unit + kGroups) + d0, is_wide(unit + kGroups));
-            beside = partner(unit + kGroups);
+        if (live && unit + 1 < last) {
+            raw    = load8(source(unit + 1) + d0, is_wide(unit + 1));
+            beside = partner(unit + 1);
         }
         if (side < 2 && page < 0)
             continue; // the whole group
@@ -191,20 +214,17 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a, int heads, int p
                 *reinterpret_cast<uintx4*>(a.q_out + ((int64_t)t * a.q_heads + head) * D + d0) = v;
             continue;
         }
-        float hi = 0.f, lo = 0.f;
-        int   bad = 0;
+        float hi = 0.f, lo = 0.f, none = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            hi = fmaxf(hi, x[i]);
-            lo = fminf(lo, x[i]);
-            bad |= (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u;
+            hi = __builtin_fmaxf(hi, x[i]);
+            lo = __builtin_fminf(lo, x[i]);
+            none = __builtin_fmaf(x[i], 0.f, none); // NaN with an infinity or a NaN
         }
-#pragma unroll
-        for (int m = 1; m < L; m <<= 1) {
-            hi = fmaxf(hi, __shfl_xor(hi, m, L));
-            lo = fminf(lo, __shfl_xor(lo, m, L));
-            bad |= __shfl_xor(bad, m, L);
-        }
+        hi = none == 0.f ? hi : __builtin_inff();
+        hi = group_max<L>(hi);
+        lo = -group_max<L>(-lo);
+        const bool  bad       = !(hi < __builtin_inff());
         const float fifteenth = 1.0f / 15.0f;
         const float s         = hi * fifteenth - lo * fifteenth;
         unsigned    word      = (__float_as_uint(s) + 8u) & ~15u;
@@ -216,7 +236,7 @@ __global__ __launch_bounds__(256) void kv4_append(AppendArgs a, int heads, int p
         unsigned    codes = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float q = fminf(fmaxf(rintf(x[i] * inv) + z, 0.f), 15.f);
+            const float q = __builtin_amdgcn_fmed3f(rintf(x[i] * inv) + z, 0.f, 15.f);
             codes |= (unsigned)q << (4 * i);
         }
         if (bad) {
@@ -242,13 +262,14 @@ template <int L>
 __global__ __launch_bounds__(256) void kv4_gather(GatherArgs a, int per)
 {
     constexpr int kGroups = 256 / L;
-    const int     lane = threadIdx.x & (L - 1), d0 = lane * 8, t = blockIdx.x, D = a.cache.head_dim, kvh = a.cache.kv_heads;
-    const int     first = blockIdx.y * per * kGroups + threadIdx.x / L, last = min(2 * kvh, first + per * kGroups);
-    if (d0 >= D)
+    const int     lane = threadIdx.x & (L - 1), d0 = lane * 8, D = a.cache.head_dim, kvh = a.cache.kv_heads;
+    const int     t    = blockIdx.x * kGroups + threadIdx.x / L;
+    const int     first = blockIdx.y * per, last = min(2 * kvh, first + per);
+    if (t >= a.batch.tokens || d0 >= D)
         return;
     int       slot, place;
     const int page = locate(a.cache, a.batch, t, slot, place);
-    for (int unit = first; unit < last; unit += kGroups) {
+    for (int unit = first; unit < last; ++unit) {
         const int side = unit < kvh ? 0 : 1, head = unit - side * kvh;
         if (a.dst[side] == nullptr)
             continue;
@@ -290,12 +311,11 @@ int lanes_of(int head_dim)
     return head_dim == 64 ? 8 : (head_dim == 256 ? 32 : 16);
 }
 
-// Head vectors a group of lanes takes one after the other: all of a token's where there are many tokens, so that its place and
-// its row of the rotation are looked up once, one where they are few and the chain of loads is what counts.
-int vectors_per_group(int heads, int groups, int tokens)
+// Head vectors a group of lanes takes one after the other: more than one, so that a token's place and its row of the rotation
+// are looked up less often, once that leaves 2048 workgroups.
+int vectors_per_group(int heads, int64_t blocks)
 {
-    const int all = (heads + groups - 1) / groups;
-    return std::max(1, std::min<int>(all, (int)((int64_t)all * tokens / 2048)));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(heads, heads * blocks / 2048));
 }
 
 int check_dtype(int dtype)
@@ -335,7 +355,7 @@ extern "C" int KV4_Append(hipStream_t stream, const KV4_Cache* cache, const KV4_
     }
     if (q.data != nullptr && rotary == nullptr)
         return refuse("queries are given and no rotation");
-    if (q.data != nullptr && (q_heads < 1 || q_heads > 65536 || bad_pointer(q_out, 16)))
+    if (q.data != nullptr && (q_heads < 1 || q_heads > 32768 || bad_pointer(q_out, 16)))
         return refuse("%d query heads, or a null or misaligned q_out (16 bytes)", q_heads);
     if (batch->total_tokens == 0)
         return 0;
@@ -356,8 +376,9 @@ extern "C" int KV4_Append(hipStream_t stream, const KV4_Cache* cache, const KV4_
     a.bf16          = dtype == DECODE_BF16;
     const int heads = 2 * cache->kv_heads + (q.data != nullptr ? q_heads : 0);
     const int L     = lanes_of(cache->head_dim), per = 256 / L;
-    const int each = vectors_per_group(heads, per, batch->total_tokens);
-    dim3      grid((unsigned)batch->total_tokens, (unsigned)((heads + per * each - 1) / (per * each)), 1);
+    const unsigned blocks = (unsigned)((batch->total_tokens + per - 1) / per);
+    const int      each   = vectors_per_group(heads, blocks);
+    dim3      grid(blocks, (unsigned)((heads + each - 1) / each), 1);
     auto      kernel = L == 8 ? kv4_append<8> : (L == 16 ? kv4_append<16> : kv4_append<32>);
     return launch(kernel, grid, dim3(256, 1, 1), stream, a, heads, each);
 }
@@ -376,8 +397,9 @@ extern "C" int KV4_Gather(hipStream_t stream, const KV4_Cache* cache, const KV4_
         return 0;
     GatherArgs a{view(*cache), view(*batch), {static_cast<uint16_t*>(k), static_cast<uint16_t*>(v)}, dtype == DECODE_BF16};
     const int  L = lanes_of(cache->head_dim), per = 256 / L;
-    const int  each = vectors_per_group(2 * cache->kv_heads, per, batch->total_tokens);
-    dim3       grid((unsigned)batch->total_tokens, (unsigned)((2 * cache->kv_heads + per * each - 1) / (per * each)), 1);
+    const unsigned blocks = (unsigned)((batch->total_tokens + per - 1) / per);
+    const int      each   = vectors_per_group(2 * cache->kv_heads, blocks);
+    dim3       grid(blocks, (unsigned)((2 * cache->kv_heads + each - 1) / each), 1);
     auto       kernel = L == 8 ? kv4_gather<8> : (L == 16 ? kv4_gather<16> : kv4_gather<32>);
     return launch(kernel, grid, dim3(256, 1, 1), stream, a, each);
 }
