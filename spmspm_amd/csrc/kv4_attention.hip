@@ -284,6 +284,74 @@ __device__ __forceinline__ int block_base(const AttentionArgs& a, int b, int row
     return (int)((int64_t)a.cu[b] * a.share / rows) + b;
 }
 
+// Where a block of rows stands: its sequence b, the sequence's first row, the place of that row's token (below 0 where it has
+// none), the block's first row among the sequence's and how many it has (0: there is no such block).
+struct Place {
+    int b, first, place0, row0, rows, share;
+
+    // Keys that some of rows `from` .. `from + count - 1` of the block see, lo .. hi, and those that all see, lo_all .. hi_all.
+    __device__ __forceinline__ int top(int row) const { return place0 + (row0 + row) / share; }
+    __device__ __forceinline__ int lo(const AttentionArgs& a, int from, int) const
+    {
+        return a.window > 0 ? max(0, top(from) - a.window + 1) : 0;
+    }
+    __device__ __forceinline__ int hi(const AttentionArgs&, int cap, int from, int count) const
+    {
+        return min(top(from + count - 1), cap - 1);
+    }
+    __device__ __forceinline__ int lo_all(const AttentionArgs& a, int from, int count) const
+    {
+        return a.window > 0 ? max(0, top(from + count - 1) - a.window + 1) : 0;
+    }
+    __device__ __forceinline__ int hi_all(int cap, int from, int count) const
+    {
+        return top(from) < 0 || top(from + count - 1) >= cap ? -1 : top(from);
+    }
+};
+
+__device__ __forceinline__ Place place_of(const AttentionArgs& a, int block, int rows)
+{
+    Place p;
+    p.b = 0, p.share = a.share, p.rows = 0;
+    if (a.cu == nullptr) {
+        p.b = block / ((a.share + rows - 1) / rows);
+    } else {
+        for (int top = a.batch; top - p.b > 1;) {
+            const int mid = (p.b + top) >> 1;
+            if (block_base(a, mid, rows) <= block)
+                p.b = mid;
+            else
+                top = mid;
+        }
+    }
+    const int behind = a.cu ? uniform_load(a.cu + p.b + 1) : p.b + 1;
+    p.first          = a.cu ? uniform_load(a.cu + p.b) : p.b;
+    p.place0         = uniform_load(a.lens + p.b) - (behind - p.first);
+    p.row0           = (block - block_base(a, p.b, rows)) * rows;
+    const int64_t left = (int64_t)(min(behind, a.tokens) - p.first) * a.share - p.row0;
+    if (p.first >= 0 && p.row0 >= 0)
+        p.rows = (int)min<int64_t>(rows, max<int64_t>(left, 0));
+    return p;
+}
+
+// Rows of no sequence are 0 (with splits kv4_attention_join writes them): dealt to the blocks.
+template <int D>
+__device__ __forceinline__ void zero_idle(const AttentionArgs& a, int head, int block, int blocks)
+{
+    if (a.cu == nullptr || a.splits != 1)
+        return;
+    const int before = min(max(uniform_load(a.cu), 0), a.tokens), behind = min(max(uniform_load(a.cu + a.batch), 0), a.tokens);
+    const int idle = before + a.tokens - behind;
+    for (int i = block; i < idle; i += blocks) {
+        const int64_t at = (int64_t)(i < before ? i : behind + i - before) * a.q_heads + head * a.share;
+        for (int e = threadIdx.x; e < a.share * (D / 8); e += kWave * kWaves)
+            *reinterpret_cast<uintx4*>(a.out + at * D + e * 8) = uintx4{0, 0, 0, 0};
+        if (a.lse != nullptr)
+            for (int e = threadIdx.x; e < a.share; e += kWave * kWaves)
+                a.lse[at + e] = -__builtin_inff();
+    }
+}
+
 template <int D, int RT>
 __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attention(AttentionArgs a)
 {
@@ -297,47 +365,15 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
     // all of a head's blocks of rows find its keys in one L2 wherever the number of heads is a multiple of eight
     const int head = blockIdx.x % a.kv_heads, block = blockIdx.x / a.kv_heads, split = blockIdx.y;
 
-    if (a.cu != nullptr && a.splits == 1) { // rows of no sequence (otherwise kv4_attention_join writes them)
-        const int before = min(max(a.cu[0], 0), a.tokens), behind = min(max(a.cu[a.batch], 0), a.tokens);
-        const int idle = before + a.tokens - behind;
-        for (int i = block; i < idle; i += (int)(gridDim.x / a.kv_heads)) {
-            const int64_t at = (int64_t)(i < before ? i : behind + i - before) * a.q_heads + head * a.share;
-            for (int e = threadIdx.x; e < a.share * (D / 8); e += kWave * kWaves)
-                *reinterpret_cast<uintx4*>(a.out + at * D + e * 8) = uintx4{0, 0, 0, 0};
-            if (a.lse != nullptr)
-                for (int e = threadIdx.x; e < a.share; e += kWave * kWaves)
-                    a.lse[at + e] = -__builtin_inff();
-        }
-    }
+    zero_idle<D>(a, head, block, (int)(gridDim.x / a.kv_heads));
 
-    // which sequence, which of its blocks
-    int b = 0;
-    if (a.cu == nullptr) {
-        b = block / ((a.share + kRows - 1) / kRows);
-    } else {
-        for (int top = a.batch; top - b > 1;) {
-            const int mid = (b + top) >> 1;
-            if (block_base(a, mid, kRows) <= block)
-                b = mid;
-            else
-                top = mid;
-        }
-    }
-    const int len    = uniform_load(a.lens + b);
-    const int first  = a.cu ? uniform_load(a.cu + b) : b, behind = a.cu ? uniform_load(a.cu + b + 1) : b + 1;
-    const int count  = min(behind, a.tokens) - first;
-    const int row0   = (block - block_base(a, b, kRows)) * kRows;
-    if (first < 0 || row0 < 0 || (int64_t)row0 >= (int64_t)count * a.share)
+    const Place p = place_of(a, block, kRows);
+    if (p.rows <= 0)
         return;
-    const int  rows   = min(kRows, count * a.share - row0);
-    const int  cap    = a.width << a.page_log2;
-    const int* table  = a.table + (int64_t)b * a.stride;
-    const int  place0 = len - (behind - first); // place of the sequence's first row's token, below 0 where it has none
-
-    // keys that some row of the block sees, lo .. hi, and those that all rows see, lo_all .. hi_all
-    const int  p_first = place0 + row0 / a.share, p_last = place0 + (row0 + rows - 1) / a.share;
-    const int  hi = min(p_last, cap - 1), hi_all = p_first < 0 || p_last >= cap ? -1 : p_first;
-    const int  lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0, lo_all = a.window > 0 ? max(0, p_last - a.window + 1) : 0;
+    const int  first = p.first, row0 = p.row0, rows = p.rows, place0 = p.place0;
+    const int  cap   = a.width << a.page_log2;
+    const int* table = a.table + (int64_t)p.b * a.stride;
+    const int  lo = p.lo(a, 0, rows), hi = p.hi(a, cap, 0, rows), lo_all = p.lo_all(a, 0, rows), hi_all = p.hi_all(cap, 0, rows);
     // the workgroup's share of them in tiles of 32; wave w takes every fourth
     const int  t_lo = lo / kTile, t_all = hi < lo ? 0 : hi / kTile + 1 - t_lo, per = (t_all + a.splits - 1) / a.splits;
     const int  t0 = t_lo + split * per, t1 = min(t_lo + t_all, t0 + per);
@@ -493,6 +529,359 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
     }
 }
 
+// Many rows per sequence (prompts and chunks of them): four waves of two row tiles each share the keys, which go unpacked
+// through LDS, 64 at a time: two waves unpack the keys' codes, two the values', as operands of the products, and the words
+// as what a score is multiplied by (u), what is added to it (ev), what its probability is multiplied by (f) and what it
+// counts in the sum (il).  Here z is taken off the keys' codes too, and all rows of the block share the queries' scale.
+template <int D>
+struct Slab {
+    uintx4 k[4][D / 32][kWave];
+    uintx4 v[2][Shape<D>::kVal][kWave];
+    float  u[64], ev[64], f[64], il[64];
+};
+
+// What a wave loads of a slab: 32 keys' codes or values.
+struct Raw {
+    unsigned d[8];
+    uintx4   w[2];
+    unsigned own;
+};
+
+template <int D>
+__device__ __forceinline__ void load_raw(Raw& t, const AttentionArgs& a, int head, int base, int p0, int p1, bool values,
+                                         int lane)
+{
+    const int     c = lane & 15, h = lane >> 4, P = 1 << a.page_log2, key = lane & 31;
+    const int64_t at0 = ((int64_t)max(key < 16 ? p0 : p1, 0) * a.kv_heads + head) << a.page_log2;
+    const int64_t at  = at0 + ((base + key) & (P - 1));
+    if (values) {
+        const int64_t  vat = word_index(a, head, base, p0, p1, h);
+        const uint8_t* vb  = a.v_codes + vat * (D / 2) + (D == 96 && c >= 12 ? 0 : c) * Shape<D>::kValBytes;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (Shape<D>::kValBytes == 2)
+                t.d[j] = *reinterpret_cast<const uint16_t*>(vb + j * (D / 2));
+            else
+                t.d[j] = *reinterpret_cast<const unsigned*>(vb + j * (D / 2));
+        }
+        const uintx4* vw = reinterpret_cast<const uintx4*>(a.v_words + vat);
+        t.w[0] = vw[0], t.w[1] = vw[1];
+        t.own  = (unsigned)a.v_words[at];
+    } else {
+        constexpr int  N   = D / 32;
+        const int      kr  = 8 * (c >> 2) + (c & 3);
+        const int64_t  kat = (((int64_t)max(c < 8 ? p0 : p1, 0) * a.kv_heads + head) << a.page_log2) + ((base + kr) & (P - 1));
+        const uint8_t* kc  = a.k_codes + kat * (D / 2) + h * (D / 8);
+        unsigned       x[2][N];
+        load_dwords(x[0], kc);
+        load_dwords(x[1], kc + 4 * (D / 2));
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            t.d[j] = x[0][j], t.d[N + j] = x[1][j];
+        t.w[0][0] = (unsigned)a.k_words[kat], t.w[0][1] = (unsigned)a.k_words[kat + 4];
+        t.own     = (unsigned)a.k_words[at];
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void unpack(Slab<D>& slab, const Raw& t, int g, bool values, float unit, int lane)
+{
+    constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+    auto code = [](unsigned w, bool high, unsigned below, unsigned above) {
+        const half2 v = high ? __builtin_bit_cast(half2, (w & kHigh) | 0x54005400u) + __builtin_bit_cast(half2, above)
+                             : __builtin_bit_cast(half2, (w & kLow) | 0x64006400u) + __builtin_bit_cast(half2, below);
+        return __builtin_bit_cast(unsigned, v);
+    };
+    if (values) {
+        unsigned below[4], above[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned z = __builtin_amdgcn_perm(t.w[i >> 1][2 * (i & 1) + 1], t.w[i >> 1][2 * (i & 1)], 0x05040100u) & kLow;
+            below[i] = z | 0xe400e400u;
+            above[i] = z << 4 | 0xd400d400u;
+        }
+#pragma unroll
+        for (int q = 0; q < Shape<D>::kVal / 4; ++q) {
+            uintx4 a0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                a0[i] = __builtin_amdgcn_perm(t.d[2 * i + 1], t.d[2 * i], (q & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uintx4 out;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    out[i] = code(e >= 2 ? a0[i] >> 8 : a0[i], (e & 1) != 0, below[i], above[i]);
+                slab.v[g][4 * q + e][lane] = out;
+            }
+        }
+        if (lane < 32) { // a scale that is no number: NaN where it is seen, 0 where it is hidden
+            const bool none = (t.own & 0x7f800000u) == 0x7f800000u;
+            slab.ev[32 * g + lane] = none ? __uint_as_float(0x7fc00000u) : (float)(t.own >> 23);
+            slab.f[32 * g + lane]  = none ? 0.f : __builtin_amdgcn_frexp_mantf(__uint_as_float(t.own));
+            slab.il[32 * g + lane] = none ? 0.f : __uint_as_float(0x7f000000u - (t.own & 0x7f800000u));
+        }
+    } else {
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+            const unsigned z = (t.w[0][T] & 15u) * 0x00010001u, below = z | 0xe400e400u, above = z << 4 | 0xd400d400u;
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                const unsigned w = t.d[T * (D / 32) + j], w8 = w >> 8;
+                slab.k[2 * g + T][j][lane] = uintx4{code(w, false, below, above), code(w, true, below, above),
+                                                    code(w8, false, below, above), code(w8, true, below, above)};
+            }
+        }
+        if (lane < 32)
+            slab.u[32 * g + lane] = __uint_as_float(t.own) * unit;
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(kWave* kWaves, 2) void kv4_attention_rows(AttentionArgs a)
+{
+    constexpr int NV = Shape<D>::kVal, kSteps = Shape<D>::kSteps, RT = 2, kRows = 16 * RT * kWaves;
+    __shared__ Slab<D> slab[2];
+    __shared__ float   tops[kWaves];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, h = lane >> 4;
+    // the last blocks of rows, which see the most keys, go first
+    const int head = blockIdx.x % a.kv_heads, blocks = gridDim.x / a.kv_heads, block = blocks - 1 - (int)blockIdx.x / a.kv_heads;
+    const int split = blockIdx.y;
+    zero_idle<D>(a, head, block, blocks);
+
+    const Place p = place_of(a, block, kRows);
+    if (p.rows <= 0)
+        return;
+    const int  cap = a.width << a.page_log2;
+    const int* table = a.table + (int64_t)p.b * a.stride;
+    const int  lo = p.lo(a, 0, p.rows), hi = p.hi(a, cap, 0, p.rows);
+    const int  t_lo = lo / 64, t_all = hi < lo ? 0 : hi / 64 + 1 - t_lo, per = (t_all + a.splits - 1) / a.splits;
+    const int  t0 = t_lo + split * per, t1 = min(t_lo + t_all, t0 + per);
+    // this wave's rows, and the keys that some, and that all of them see
+    const int  w0 = wave * 16 * RT, w_rows = max(0, min(16 * RT, p.rows - w0));
+    const int  w_lo = w_rows > 0 ? p.lo(a, w0, w_rows) : 0, w_hi = w_rows > 0 ? p.hi(a, cap, w0, w_rows) : -1;
+    const int  all_lo = w_rows > 0 ? p.lo_all(a, w0, w_rows) : 0, all_hi = w_rows > 0 ? p.hi_all(cap, w0, w_rows) : -1;
+
+    const int  g = wave & 1;
+    const bool values = wave >= 2;
+    Raw        raw;
+    int        e[4], n[4]; // entries of the block table for the slab worked on and for the one loaded
+    auto       entries = [&](int (&dst)[4], int t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            dst[i] = page_of(a, entry_at(a, table, t * 64 + 16 * i), t * 64 + 16 * i);
+    };
+    auto load = [&](const int (&pg)[4], int t) {
+        load_raw<D>(raw, a, head, t * 64 + 32 * g, g ? pg[2] : pg[0], g ? pg[3] : pg[1], values, lane);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (t0 < t1) {
+        entries(e, t0);
+        load(e, t0);
+    }
+
+    // queries
+    half8 q[RT][kSteps];
+    int   first[RT], last[RT];
+    float m[RT], l[RT];
+    floatx4 o[RT][NV];
+    uintx4  qraw[RT][kSteps];
+    float   top = 0.f;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int  row  = w0 + r * 16 + c;
+        const bool live = row < p.rows;
+        const int  at = p.row0 + (live ? row : 0), tok = at / a.share, sub = at % a.share;
+        const uint16_t* src = a.q + (int64_t)(p.first + tok) * a.q_token + (int64_t)(head * a.share + sub) * a.q_head + h * (D / 4);
+        const int place = p.place0 + tok;
+        first[r] = live && a.window > 0 ? max(0, place - a.window + 1) : 0;
+        last[r]  = live && place < cap ? place : -1;
+        m[r] = kNone, l[r] = 0.f;
+#pragma unroll
+        for (int d = 0; d < NV; ++d)
+            o[r][d] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            qraw[r][j] = *reinterpret_cast<const uintx4*>(src + 8 * j);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float mag = fabsf(from16((uint16_t)(qraw[r][j][i >> 1] >> (16 * (i & 1))), a.bf16));
+                if (last[r] >= 0 && mag < 3.4e38f) // rows that see nothing and infinities do not count
+                    top = fmaxf(top, mag);
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1)
+        top = fmaxf(top, __shfl_xor(top, x));
+    if (lane == 0)
+        tops[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const int   qexp = __builtin_amdgcn_readfirstlane(top > 0.f ? min(13 - (int)__builtin_amdgcn_frexp_expf(top), 110) : 0);
+    const float unit = ldexpf(a.scale_log2, -qexp);
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7}; // element of each half of the unpacked dword
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int x = kOrder[i];
+                q[r][j][i]  = (_Float16)ldexpf(from16((uint16_t)(qraw[r][j][x >> 1] >> (16 * (x & 1))), a.bf16), qexp);
+            }
+        }
+
+    if (t0 < t1) {
+        unpack<D>(slab[0], raw, g, values, unit, lane);
+        entries(n, min(t0 + 1, t1 - 1));
+        load(n, min(t0 + 1, t1 - 1));
+        __syncthreads();
+        for (int t = t0; t < t1; ++t) {
+            const Slab<D>& b    = slab[(t - t0) & 1];
+            const int      tile = t * 64;
+            if (tile <= w_hi && tile + 63 >= w_lo) {
+                const bool edge = !(e[0] >= 0 && e[1] >= 0 && e[2] >= 0 && e[3] >= 0 && tile >= all_lo && tile + 63 <= all_hi);
+                floatx4    sc[4][RT];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+                        sc[k][r] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const half8 kk = __builtin_bit_cast(half8, b.k[k][j][lane]);
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+                            sc[k][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[r][j], sc[k][r], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { // keys 32 (k / 2) + 8 h + 4 (k % 2) + i
+                    const int     at = 32 * (k >> 1) + 8 * h + 4 * (k & 1);
+                    const floatx4 u = *reinterpret_cast<const floatx4*>(&b.u[at]), ev = *reinterpret_cast<const floatx4*>(&b.ev[at]);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            sc[k][r][i] = __builtin_fmaf(sc[k][r][i], u[i], ev[i]);
+                }
+                if (edge) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const bool gone = (h < 2 ? e[2 * (k >> 1)] : e[2 * (k >> 1) + 1]) < 0;
+                        const int  at   = tile + 32 * (k >> 1) + 8 * h + 4 * (k & 1);
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (gone || at + i < first[r] || at + i > last[r])
+                                    sc[k][r][i] = -__builtin_inff();
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    float mx = kNone;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mx = fmaxf(mx, sc[k][r][i]);
+                    if (__any(mx > m[r] + kSlack)) {
+                        mx = fmaxf(mx, __shfl_xor(mx, 16));
+                        mx = fmaxf(mx, __shfl_xor(mx, 32));
+                        const float m2 = fmaxf(mx - kBelow, m[r]), alpha = __builtin_amdgcn_exp2f(m[r] - m2);
+                        m[r] = m2;
+                        l[r] *= alpha;
+#pragma unroll
+                        for (int d = 0; d < NV; ++d)
+                            o[r][d] *= alpha;
+                    }
+                }
+                half8 pp[2][RT];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int     at = 32 * (k >> 1) + 8 * h + 4 * (k & 1);
+                    const floatx4 f = *reinterpret_cast<const floatx4*>(&b.f[at]), il = *reinterpret_cast<const floatx4*>(&b.il[at]);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float ex = __builtin_amdgcn_exp2f(sc[k][r][i] - m[r]);
+                            l[r] = __builtin_fmaf(ex, il[i], l[r]);
+                            pp[k >> 1][r][4 * (k & 1) + i] = (_Float16)(ex * f[i]);
+                        }
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int d = 0; d < NV; ++d) {
+                        const half8 va = __builtin_bit_cast(half8, b.v[k][d][lane]);
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+                            o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pp[k][r], o[r][d], 0, 0, 0);
+                    }
+            }
+            if (t + 1 < t1) { // the other slab was last read before the barrier
+                unpack<D>(slab[(t + 1 - t0) & 1], raw, g, values, unit, lane);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    e[i] = n[i];
+                entries(n, min(t + 2, t1 - 1));
+                load(n, min(t + 2, t1 - 1));
+            }
+            __syncthreads();
+        }
+    }
+
+    // a lane holds 4 NV elements in a row of its row
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        l[r] += __shfl_xor(l[r], 16);
+        l[r] += __shfl_xor(l[r], 32);
+        const int row = w0 + r * 16 + c;
+        if (row >= p.rows || 4 * NV * h >= D)
+            continue;
+        const int     at  = p.row0 + row;
+        const int64_t idx = (int64_t)(p.first + at / a.share) * a.q_heads + head * a.share + at % a.share;
+        if (a.splits > 1) {
+            float* dst = a.part_o + ((int64_t)split * a.tokens * a.q_heads + idx) * D + 4 * NV * h;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d = 0; d < NV; d += 4)
+                    *reinterpret_cast<floatx4*>(dst + NV * i + d) = floatx4{o[r][d][i] * 2.f, o[r][d + 1][i] * 2.f,
+                                                                           o[r][d + 2][i] * 2.f, o[r][d + 3][i] * 2.f};
+            if (h == 0) {
+                float* ml = a.part_ml + ((int64_t)split * a.tokens * a.q_heads + idx) * 2;
+                ml[0] = m[r], ml[1] = l[r];
+            }
+            continue;
+        }
+        const bool  none = l[r] == 0.f;
+        const float inv  = none ? 0.f : 2.f / l[r]; // f is half of the mantissa
+        uint16_t    out[4 * NV];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < NV; ++d)
+                out[NV * i + d] = to16(none ? 0.f : o[r][d][i] * inv, a.bf16);
+        uint16_t* dst = a.out + idx * D + 4 * NV * h;
+#pragma unroll
+        for (int i = 0; i < 4 * NV; i += 8) {
+            uintx4 v;
+            __builtin_memcpy(&v, out + i, 16);
+            *reinterpret_cast<uintx4*>(dst + i) = v;
+        }
+        if (a.lse != nullptr && h == 0)
+            a.lse[idx] = none ? -__builtin_inff() : (__log2f(l[r]) + (m[r] - 127.f)) * 0.69314718055994531f;
+    }
+}
+
 // Joins the splits of a row: threads of one row take 8 elements each, in `lanes` groups that deal the splits among them and
 // meet in LDS.
 template <int D>
@@ -562,9 +951,11 @@ __global__ __launch_bounds__(256) void kv4_attention_join(AttentionArgs a, int l
 namespace {
 
 struct Plan {
-    int     row_tiles, splits;
+    int     row_tiles, splits; // row tiles of a block; 8: kv4_attention_rows
     int64_t blocks;
 };
+
+constexpr int kManyRows = 64; // average rows of a sequence from which its keys go through LDS
 
 // Row tiles per wave: as many as the average sequence fills, up to two.  Splits of the keys: enough workgroups for every
 // CU to hold two, no split below four tiles per wave.
@@ -573,7 +964,7 @@ Plan plan_of(const KV4_Cache& c, const KV4_Batch& b, int q_heads, int window, in
     Plan          p;
     const int     share = q_heads / c.kv_heads;
     const int64_t rows  = (int64_t)b.total_tokens * share, each = (rows + b.batch - 1) / b.batch;
-    p.row_tiles = each <= 16 || c.head_dim == 256 ? 1 : 2;
+    p.row_tiles = each <= 16 || c.head_dim == 256 ? 1 : (each <= kManyRows ? 2 : 8);
     const int64_t per = 16 * p.row_tiles;
     p.blocks          = (b.cu_tokens == nullptr ? b.batch * ((share + per - 1) / per) : rows / per + b.batch);
     const int64_t capacity = (int64_t)b.table_width * c.page_size;
@@ -610,7 +1001,7 @@ int run(hipStream_t stream, const Plan& p, const AttentionArgs& a)
     if (p.row_tiles == 1)
         err = launch(kv4_attention<D, 1>, grid, block, stream, a);
     else if constexpr (D < 256)
-        err = launch(kv4_attention<D, 2>, grid, block, stream, a);
+        err = launch(p.row_tiles == 2 ? kv4_attention<D, 2> : kv4_attention_rows<D>, grid, block, stream, a);
     else
         return (int)hipErrorInvalidValue; // plan_of gives heads of 256 one row tile: two would not fit the registers
     if (err != 0 || p.splits == 1)
