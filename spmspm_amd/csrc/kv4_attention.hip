@@ -529,15 +529,17 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
     }
 }
 
-// Many rows per sequence (prompts and chunks of them): four waves of two row tiles each share the keys, which go unpacked
-// through LDS, 64 at a time: two waves unpack the keys' codes, two the values', as operands of the products, and the words
-// as what a score is multiplied by (u), what is added to it (ev), what its probability is multiplied by (f) and what it
-// counts in the sum (il).  Here z is taken off the keys' codes too, and all rows of the block share the queries' scale.
+// Many rows per sequence (prompts and chunks of them): the waves of a workgroup, two row tiles each, share the keys, which go
+// unpacked through LDS, 16 for every wave at a time: half of the waves unpack the codes of 32 keys each, the others those of
+// values, as operands of the products, and the words as what a score is multiplied by (u), what is added to it (ev) and what
+// its probability counts in the sum (il).  Here z is taken off the keys' codes too, all rows of the block share the queries'
+// scale, and a value's whole scale goes into the exponent, p'_t = 2^(log2 p_t + log2 s_t - m), with il = 2^-6 / s_t:
+// logarithm and reciprocal are taken once for all rows of the block, and save a product for each probability.
 template <int D>
-struct Slab {
+struct Slab { // of 64 keys
     uintx4 k[4][D / 32][kWave];
     uintx4 v[2][Shape<D>::kVal][kWave];
-    float  u[64], ev[64], f[64], il[64];
+    float  u[64], ev[64], il[64];
 };
 
 // What a wave loads of a slab: 32 keys' codes or values.
@@ -547,15 +549,18 @@ struct Raw {
     unsigned own;
 };
 
+// The 32 keys from `base` on; p0 and p1 are the pages of the two halves.
 template <int D>
 __device__ __forceinline__ void load_raw(Raw& t, const AttentionArgs& a, int head, int base, int p0, int p1, bool values,
                                          int lane)
 {
-    const int     c = lane & 15, h = lane >> 4, P = 1 << a.page_log2, key = lane & 31;
-    const int64_t at0 = ((int64_t)max(key < 16 ? p0 : p1, 0) * a.kv_heads + head) << a.page_log2;
-    const int64_t at  = at0 + ((base + key) & (P - 1));
+    // entries of the cache at the halves' beginnings, the same for the whole wave
+    const int     c = lane & 15, h = lane >> 4, mask = (1 << a.page_log2) - 1;
+    const int64_t half0 = (((int64_t)max(p0, 0) * a.kv_heads + head) << a.page_log2) + (base & mask);
+    const int64_t half1 = (((int64_t)max(p1, 0) * a.kv_heads + head) << a.page_log2) + ((base + 16) & mask);
+    const int64_t own   = ((lane & 31) < 16 ? half0 : half1) + (lane & 15);
     if (values) {
-        const int64_t  vat = word_index(a, head, base, p0, p1, h);
+        const int64_t  vat = (h < 2 ? half0 : half1) + 8 * (h & 1);
         const uint8_t* vb  = a.v_codes + vat * (D / 2) + (D == 96 && c >= 12 ? 0 : c) * Shape<D>::kValBytes;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -566,11 +571,10 @@ __device__ __forceinline__ void load_raw(Raw& t, const AttentionArgs& a, int hea
         }
         const uintx4* vw = reinterpret_cast<const uintx4*>(a.v_words + vat);
         t.w[0] = vw[0], t.w[1] = vw[1];
-        t.own  = (unsigned)a.v_words[at];
+        t.own  = (unsigned)a.v_words[own];
     } else {
         constexpr int  N   = D / 32;
-        const int      kr  = 8 * (c >> 2) + (c & 3);
-        const int64_t  kat = (((int64_t)max(c < 8 ? p0 : p1, 0) * a.kv_heads + head) << a.page_log2) + ((base + kr) & (P - 1));
+        const int64_t  kat = (c < 8 ? half0 : half1) + 8 * ((c >> 2) & 1) + (c & 3);
         const uint8_t* kc  = a.k_codes + kat * (D / 2) + h * (D / 8);
         unsigned       x[2][N];
         load_dwords(x[0], kc);
@@ -579,7 +583,7 @@ __device__ __forceinline__ void load_raw(Raw& t, const AttentionArgs& a, int hea
         for (int j = 0; j < N; ++j)
             t.d[j] = x[0][j], t.d[N + j] = x[1][j];
         t.w[0][0] = (unsigned)a.k_words[kat], t.w[0][1] = (unsigned)a.k_words[kat + 4];
-        t.own     = (unsigned)a.k_words[at];
+        t.own     = (unsigned)a.k_words[own];
     }
 }
 
@@ -615,11 +619,11 @@ __device__ __forceinline__ void unpack(Slab<D>& slab, const Raw& t, int g, bool 
                 slab.v[g][4 * q + e][lane] = out;
             }
         }
-        if (lane < 32) { // a scale that is no number: NaN where it is seen, 0 where it is hidden
-            const bool none = (t.own & 0x7f800000u) == 0x7f800000u;
-            slab.ev[32 * g + lane] = none ? __uint_as_float(0x7fc00000u) : (float)(t.own >> 23);
-            slab.f[32 * g + lane]  = none ? 0.f : __builtin_amdgcn_frexp_mantf(__uint_as_float(t.own));
-            slab.il[32 * g + lane] = none ? 0.f : __uint_as_float(0x7f000000u - (t.own & 0x7f800000u));
+        if (lane < 32) { // a scale that is no positive number: NaN where it is seen, 0 where it is hidden
+            const float w    = __uint_as_float(t.own);
+            const bool  fine = w > 0.f && w < __builtin_inff();
+            slab.ev[32 * g + lane] = fine ? __log2f(w) : __uint_as_float(0x7fc00000u);
+            slab.il[32 * g + lane] = fine ? 0x1p-6f / w : 0.f;
         }
     } else {
 #pragma unroll
@@ -637,12 +641,12 @@ __device__ __forceinline__ void unpack(Slab<D>& slab, const Raw& t, int g, bool 
     }
 }
 
-template <int D>
-__global__ __launch_bounds__(kWave* kWaves, 2) void kv4_attention_rows(AttentionArgs a)
+template <int D, int W>
+__global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs a)
 {
-    constexpr int NV = Shape<D>::kVal, kSteps = Shape<D>::kSteps, RT = 2, kRows = 16 * RT * kWaves;
-    __shared__ Slab<D> slab[2];
-    __shared__ float   tops[kWaves];
+    constexpr int NV = Shape<D>::kVal, kSteps = Shape<D>::kSteps, RT = 2, kRows = 16 * RT * W, kStep = 16 * W;
+    __shared__ Slab<D> slab[2][W / 4];
+    __shared__ float   tops[W];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, h = lane >> 4;
@@ -657,30 +661,40 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void kv4_attention_rows(Attention
     const int  cap = a.width << a.page_log2;
     const int* table = a.table + (int64_t)p.b * a.stride;
     const int  lo = p.lo(a, 0, p.rows), hi = p.hi(a, cap, 0, p.rows);
-    const int  t_lo = lo / 64, t_all = hi < lo ? 0 : hi / 64 + 1 - t_lo, per = (t_all + a.splits - 1) / a.splits;
+    const int  t_lo = lo / kStep, t_all = hi < lo ? 0 : hi / kStep + 1 - t_lo, per = (t_all + a.splits - 1) / a.splits;
     const int  t0 = t_lo + split * per, t1 = min(t_lo + t_all, t0 + per);
     // this wave's rows, and the keys that some, and that all of them see
     const int  w0 = wave * 16 * RT, w_rows = max(0, min(16 * RT, p.rows - w0));
     const int  w_lo = w_rows > 0 ? p.lo(a, w0, w_rows) : 0, w_hi = w_rows > 0 ? p.hi(a, cap, w0, w_rows) : -1;
     const int  all_lo = w_rows > 0 ? p.lo_all(a, w0, w_rows) : 0, all_hi = w_rows > 0 ? p.hi_all(cap, w0, w_rows) : -1;
 
-    const int  g = wave & 1;
-    const bool values = wave >= 2;
+    const int  group = wave % (W / 2); // the 32 keys that this wave unpacks
+    const bool values = wave >= W / 2;
     Raw        raw;
-    int        e[4], n[4]; // entries of the block table for the slab worked on and for the one loaded
-    auto       entries = [&](int (&dst)[4], int t) {
+    unsigned   gone = 0, gone_next = 0; // bit i: keys 16 i .. of the step lie in no page of the cache
+    // the pages of a step's keys: their absence as bits, and the two of this wave's keys
+    auto load = [&](unsigned& absent, int t) {
+        absent = 0;
+        int       p0 = -1, p1 = -1;
+        const int each = max(1, (1 << a.page_log2) / 16); // sixteens of a page
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            dst[i] = page_of(a, entry_at(a, table, t * 64 + 16 * i), t * 64 + 16 * i);
-    };
-    auto load = [&](const int (&pg)[4], int t) {
-        load_raw<D>(raw, a, head, t * 64 + 32 * g, g ? pg[2] : pg[0], g ? pg[3] : pg[1], values, lane);
+        for (int i = 0; i < W; ++i) {
+            if (i % each != 0 && i > 0) // uniform; a step begins with a page or lies in one
+                continue;
+            const int pos  = t * kStep + 16 * i;
+            const int page = page_of(a, entry_at(a, table, pos), pos);
+            if (page < 0)
+                absent |= (each >= 32 ? ~0u : (1u << each) - 1) << i;
+            if (2 * group >= i && 2 * group < i + each)
+                p0 = page;
+            if (2 * group + 1 >= i && 2 * group + 1 < i + each)
+                p1 = page;
+        }
+        load_raw<D>(raw, a, head, t * kStep + 32 * group, p0, p1, values, lane);
         __builtin_amdgcn_sched_barrier(0);
     };
-    if (t0 < t1) {
-        entries(e, t0);
-        load(e, t0);
-    }
+    if (t0 < t1)
+        load(gone, t0);
 
     // queries
     half8 q[RT][kSteps];
@@ -719,7 +733,9 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void kv4_attention_rows(Attention
     if (lane == 0)
         tops[wave] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+        top = fmaxf(top, tops[w]);
     const int   qexp = __builtin_amdgcn_readfirstlane(top > 0.f ? min(13 - (int)__builtin_amdgcn_frexp_expf(top), 110) : 0);
     const float unit = ldexpf(a.scale_log2, -qexp);
 #pragma unroll
@@ -734,105 +750,106 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void kv4_attention_rows(Attention
             }
         }
 
-    if (t0 < t1) {
-        unpack<D>(slab[0], raw, g, values, unit, lane);
-        entries(n, min(t0 + 1, t1 - 1));
-        load(n, min(t0 + 1, t1 - 1));
-        __syncthreads();
-        for (int t = t0; t < t1; ++t) {
-            const Slab<D>& b    = slab[(t - t0) & 1];
-            const int      tile = t * 64;
-            if (tile <= w_hi && tile + 63 >= w_lo) {
-                const bool edge = !(e[0] >= 0 && e[1] >= 0 && e[2] >= 0 && e[3] >= 0 && tile >= all_lo && tile + 63 <= all_hi);
-                floatx4    sc[4][RT];
+    // 64 keys; `absent` as above, for them
+    auto work = [&](const Slab<D>& b, int tile, unsigned absent) {
+        if (tile > w_hi || tile + 63 < w_lo)
+            return;
+        const bool edge = (absent & 15u) != 0 || tile < all_lo || tile + 63 > all_hi;
+        floatx4    sc[4][RT];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-                    for (int r = 0; r < RT; ++r)
-                        sc[k][r] = floatx4{0.f, 0.f, 0.f, 0.f};
+            for (int r = 0; r < RT; ++r)
+                sc[k][r] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < kSteps; ++j) {
+        for (int j = 0; j < kSteps; ++j) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const half8 kk = __builtin_bit_cast(half8, b.k[k][j][lane]);
+            for (int k = 0; k < 4; ++k) {
+                const half8 kk = __builtin_bit_cast(half8, b.k[k][j][lane]);
 #pragma unroll
-                        for (int r = 0; r < RT; ++r)
-                            sc[k][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[r][j], sc[k][r], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) { // keys 32 (k / 2) + 8 h + 4 (k % 2) + i
-                    const int     at = 32 * (k >> 1) + 8 * h + 4 * (k & 1);
-                    const floatx4 u = *reinterpret_cast<const floatx4*>(&b.u[at]), ev = *reinterpret_cast<const floatx4*>(&b.ev[at]);
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            sc[k][r][i] = __builtin_fmaf(sc[k][r][i], u[i], ev[i]);
-                }
-                if (edge) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const bool gone = (h < 2 ? e[2 * (k >> 1)] : e[2 * (k >> 1) + 1]) < 0;
-                        const int  at   = tile + 32 * (k >> 1) + 8 * h + 4 * (k & 1);
-#pragma unroll
-                        for (int r = 0; r < RT; ++r)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (gone || at + i < first[r] || at + i > last[r])
-                                    sc[k][r][i] = -__builtin_inff();
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    float mx = kNone;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            mx = fmaxf(mx, sc[k][r][i]);
-                    if (__any(mx > m[r] + kSlack)) {
-                        mx = fmaxf(mx, __shfl_xor(mx, 16));
-                        mx = fmaxf(mx, __shfl_xor(mx, 32));
-                        const float m2 = fmaxf(mx - kBelow, m[r]), alpha = __builtin_amdgcn_exp2f(m[r] - m2);
-                        m[r] = m2;
-                        l[r] *= alpha;
-#pragma unroll
-                        for (int d = 0; d < NV; ++d)
-                            o[r][d] *= alpha;
-                    }
-                }
-                half8 pp[2][RT];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int     at = 32 * (k >> 1) + 8 * h + 4 * (k & 1);
-                    const floatx4 f = *reinterpret_cast<const floatx4*>(&b.f[at]), il = *reinterpret_cast<const floatx4*>(&b.il[at]);
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float ex = __builtin_amdgcn_exp2f(sc[k][r][i] - m[r]);
-                            l[r] = __builtin_fmaf(ex, il[i], l[r]);
-                            pp[k >> 1][r][4 * (k & 1) + i] = (_Float16)(ex * f[i]);
-                        }
-                }
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int d = 0; d < NV; ++d) {
-                        const half8 va = __builtin_bit_cast(half8, b.v[k][d][lane]);
-#pragma unroll
-                        for (int r = 0; r < RT; ++r)
-                            o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pp[k][r], o[r][d], 0, 0, 0);
-                    }
+                for (int r = 0; r < RT; ++r)
+                    sc[k][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[r][j], sc[k][r], 0, 0, 0);
             }
-            if (t + 1 < t1) { // the other slab was last read before the barrier
-                unpack<D>(slab[(t + 1 - t0) & 1], raw, g, values, unit, lane);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { // keys 32 (k / 2) + 8 h + 4 (k % 2) + i
+            const int     at = 32 * (k >> 1) + 8 * h + 4 * (k & 1);
+            const floatx4 u = *reinterpret_cast<const floatx4*>(&b.u[at]), ev = *reinterpret_cast<const floatx4*>(&b.ev[at]);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    e[i] = n[i];
-                entries(n, min(t + 2, t1 - 1));
-                load(n, min(t + 2, t1 - 1));
+                    sc[k][r][i] = __builtin_fmaf(sc[k][r][i], u[i], ev[i]);
+        }
+        if (edge) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool none = ((absent >> (2 * (k >> 1) + (h >> 1))) & 1u) != 0;
+                const int  at   = tile + 32 * (k >> 1) + 8 * h + 4 * (k & 1);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool hidden = (int)none | (int)(at + i < first[r]) | (int)(at + i > last[r]);
+                        sc[k][r][i] = hidden ? -__builtin_inff() : sc[k][r][i];
+                    }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            float mx = kNone;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    mx = fmaxf(mx, sc[k][r][i]);
+            if (__any(mx > m[r] + kSlack)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16));
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                const float m2 = fmaxf(mx - kBelow, m[r]), alpha = __builtin_amdgcn_exp2f(m[r] - m2);
+                m[r] = m2;
+                l[r] *= alpha;
+#pragma unroll
+                for (int d = 0; d < NV; ++d)
+                    o[r][d] *= alpha;
+            }
+        }
+        half8 pp[2][RT];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const floatx4 il = *reinterpret_cast<const floatx4*>(&b.il[32 * (k >> 1) + 8 * h + 4 * (k & 1)]);
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float ex = __builtin_amdgcn_exp2f(sc[k][r][i] - m[r]);
+                    l[r] = __builtin_fmaf(ex, il[i], l[r]);
+                    pp[k >> 1][r][4 * (k & 1) + i] = (_Float16)ex; // rounded to 11 bits, as in kv4_attention
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int d = 0; d < NV; ++d) {
+                const half8 va = __builtin_bit_cast(half8, b.v[k][d][lane]);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                    o[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pp[k][r], o[r][d], 0, 0, 0);
+            }
+    };
+
+    if (t0 < t1) {
+        unpack<D>(slab[0][group >> 1], raw, group & 1, values, unit, lane);
+        load(gone_next, min(t0 + 1, t1 - 1));
+        __syncthreads();
+        for (int t = t0; t < t1; ++t) {
+#pragma unroll
+            for (int x = 0; x < W / 4; ++x)
+                work(slab[(t - t0) & 1][x], t * kStep + 64 * x, gone >> (4 * x));
+            if (t + 1 < t1) { // the other slab was last read before the barrier
+                unpack<D>(slab[(t + 1 - t0) & 1][group >> 1], raw, group & 1, values, unit, lane);
+                gone = gone_next;
+                load(gone_next, min(t + 2, t1 - 1));
             }
             __syncthreads();
         }
@@ -854,16 +871,16 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void kv4_attention_rows(Attention
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int d = 0; d < NV; d += 4)
-                    *reinterpret_cast<floatx4*>(dst + NV * i + d) = floatx4{o[r][d][i] * 2.f, o[r][d + 1][i] * 2.f,
-                                                                           o[r][d + 2][i] * 2.f, o[r][d + 3][i] * 2.f};
+                    *reinterpret_cast<floatx4*>(dst + NV * i + d) = floatx4{o[r][d][i] * 0x1p-6f, o[r][d + 1][i] * 0x1p-6f,
+                                                                           o[r][d + 2][i] * 0x1p-6f, o[r][d + 3][i] * 0x1p-6f};
             if (h == 0) {
                 float* ml = a.part_ml + ((int64_t)split * a.tokens * a.q_heads + idx) * 2;
-                ml[0] = m[r], ml[1] = l[r];
+                ml[0] = m[r] + 133.f, ml[1] = l[r]; // as kv4_attention counts, whose sums are 2^127 times theirs
             }
             continue;
         }
         const bool  none = l[r] == 0.f;
-        const float inv  = none ? 0.f : 2.f / l[r]; // f is half of the mantissa
+        const float inv  = none ? 0.f : 0x1p-6f / l[r]; // as il is
         uint16_t    out[4 * NV];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -878,7 +895,7 @@ __global__ __launch_bounds__(kWave* kWaves, 2) void kv4_attention_rows(Attention
             *reinterpret_cast<uintx4*>(dst + i) = v;
         }
         if (a.lse != nullptr && h == 0)
-            a.lse[idx] = none ? -__builtin_inff() : (__log2f(l[r]) + (m[r] - 127.f)) * 0.69314718055994531f;
+            a.lse[idx] = none ? -__builtin_inff() : (__log2f(l[r]) + (m[r] + 6.f)) * 0.69314718055994531f;
     }
 }
 
@@ -972,7 +989,7 @@ Plan plan_of(const KV4_Cache& c, const KV4_Batch& b, int q_heads, int window, in
     if (window > 0) // what a block's rows see of it
         len = std::min<int64_t>(len, (int64_t)window + (per + share - 1) / share + kTile);
     const int64_t tiles = (len + kTile - 1) / kTile, groups = (int64_t)p.blocks * c.kv_heads;
-    int64_t       want  = (512 + groups - 1) / groups;
+    int64_t       want  = p.row_tiles == 8 && groups >= 384 ? 1 : (512 + groups - 1) / groups;
     want                = std::min<int64_t>(want, (tiles + 4 * kWaves - 1) / (4 * kWaves));
     p.splits            = (int)std::max<int64_t>(1, std::min<int64_t>(want, 128));
     return p;
@@ -1001,7 +1018,7 @@ int run(hipStream_t stream, const Plan& p, const AttentionArgs& a)
     if (p.row_tiles == 1)
         err = launch(kv4_attention<D, 1>, grid, block, stream, a);
     else if constexpr (D < 256)
-        err = launch(p.row_tiles == 2 ? kv4_attention<D, 2> : kv4_attention_rows<D>, grid, block, stream, a);
+        err = launch(p.row_tiles == 2 ? kv4_attention<D, 2> : kv4_attention_rows<D, 4>, grid, block, stream, a);
     else
         return (int)hipErrorInvalidValue; // plan_of gives heads of 256 one row tile: two would not fit the registers
     if (err != 0 || p.splits == 1)
