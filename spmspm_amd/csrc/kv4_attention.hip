@@ -137,6 +137,13 @@ __device__ __forceinline__ void load_values(Keys<D>& t, const AttentionArgs& a, 
     }
 }
 
+// A constant in a register: an instruction takes one literal, and with two a code's AND and OR are two instructions.
+__device__ __forceinline__ unsigned in_register(unsigned v)
+{
+    asm("" : "+v"(v));
+    return v;
+}
+
 template <int D, int RT>
 struct Rows {
     half8  q[RT][Shape<D>::kSteps];
@@ -241,7 +248,8 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
             pp[r][i] = (_Float16)p[i];
     }
     // -(1024 + z) and -(64 + z) of pairs of keys
-    half2 below[4], above[4];
+    const unsigned low = in_register(kLow), up = in_register(kHigh);
+    half2          below[4], above[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const unsigned z = __builtin_amdgcn_perm(t.vw[i >> 1][2 * (i & 1) + 1], t.vw[i >> 1][2 * (i & 1)], 0x05040100u) & kLow;
@@ -260,8 +268,8 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const unsigned w = e >= 2 ? a0[i] >> 8 : a0[i];
-                const half2    v = (e & 1) ? __builtin_bit_cast(half2, (w & kHigh) | 0x54005400u) + above[i]
-                                           : __builtin_bit_cast(half2, (w & kLow) | 0x64006400u) + below[i];
+                const half2    v = (e & 1) ? __builtin_bit_cast(half2, (w & up) | 0x54005400u) + above[i]
+                                           : __builtin_bit_cast(half2, (w & low) | 0x64006400u) + below[i];
                 raw[i] = __builtin_bit_cast(unsigned, v);
             }
             const half8 va = __builtin_bit_cast(half8, raw);
@@ -590,17 +598,17 @@ __device__ __forceinline__ void load_raw(Raw& t, const AttentionArgs& a, int hea
 template <int D>
 __device__ __forceinline__ void unpack(Slab<D>& slab, const Raw& t, int g, bool values, float unit, int lane)
 {
-    constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-    auto code = [](unsigned w, bool high, unsigned below, unsigned above) {
-        const half2 v = high ? __builtin_bit_cast(half2, (w & kHigh) | 0x54005400u) + __builtin_bit_cast(half2, above)
-                             : __builtin_bit_cast(half2, (w & kLow) | 0x64006400u) + __builtin_bit_cast(half2, below);
+    const unsigned low = in_register(0x000f000fu), up = in_register(0x00f000f0u);
+    auto code = [&](unsigned w, bool high, unsigned below, unsigned above) {
+        const half2 v = high ? __builtin_bit_cast(half2, (w & up) | 0x54005400u) + __builtin_bit_cast(half2, above)
+                             : __builtin_bit_cast(half2, (w & low) | 0x64006400u) + __builtin_bit_cast(half2, below);
         return __builtin_bit_cast(unsigned, v);
     };
     if (values) {
         unsigned below[4], above[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const unsigned z = __builtin_amdgcn_perm(t.w[i >> 1][2 * (i & 1) + 1], t.w[i >> 1][2 * (i & 1)], 0x05040100u) & kLow;
+            const unsigned z = __builtin_amdgcn_perm(t.w[i >> 1][2 * (i & 1) + 1], t.w[i >> 1][2 * (i & 1)], 0x05040100u) & low;
             below[i] = z | 0xe400e400u;
             above[i] = z << 4 | 0xd400d400u;
         }
@@ -671,30 +679,21 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
     const int  group = wave % (W / 2); // the 32 keys that this wave unpacks
     const bool values = wave >= W / 2;
     Raw        raw;
-    unsigned   gone = 0, gone_next = 0; // bit i: keys 16 i .. of the step lie in no page of the cache
-    // the pages of a step's keys: their absence as bits, and the two of this wave's keys
-    auto load = [&](unsigned& absent, int t) {
-        absent = 0;
-        int       p0 = -1, p1 = -1;
-        const int each = max(1, (1 << a.page_log2) / 16); // sixteens of a page
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            if (i % each != 0 && i > 0) // uniform; a step begins with a page or lies in one
-                continue;
-            const int pos  = t * kStep + 16 * i;
-            const int page = page_of(a, entry_at(a, table, pos), pos);
-            if (page < 0)
-                absent |= (each >= 32 ? ~0u : (1u << each) - 1) << i;
-            if (2 * group >= i && 2 * group < i + each)
-                p0 = page;
-            if (2 * group + 1 >= i && 2 * group + 1 < i + each)
-                p1 = page;
-        }
+    // Loads this wave's keys of step t, and for lane i the table's entry for keys 16 i .. of the step: which of them lie in no
+    // page of the cache is asked for a step later.
+    int  entry = 0;
+    auto load = [&](int t) {
+        const int pos = t * kStep + 32 * group, mine = t * kStep + 16 * (lane & (W - 1));
+        const int p0 = page_of(a, entry_at(a, table, pos), pos), p1 = page_of(a, entry_at(a, table, pos + 16), pos + 16);
+        entry = table[min(mine >> a.page_log2, a.width - 1)];
         load_raw<D>(raw, a, head, t * kStep + 32 * group, p0, p1, values, lane);
         __builtin_amdgcn_sched_barrier(0);
     };
+    auto absent = [&](int t) { // bit i: keys 16 i .. of step t, the one that was loaded last
+        return (unsigned)__ballot(page_of(a, entry, t * kStep + 16 * (lane & (W - 1))) < 0) & ((1u << W) - 1);
+    };
     if (t0 < t1)
-        load(gone, t0);
+        load(t0);
 
     // queries
     half8 q[RT][kSteps];
@@ -750,11 +749,11 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
             }
         }
 
-    // 64 keys; `absent` as above, for them
-    auto work = [&](const Slab<D>& b, int tile, unsigned absent) {
+    // 64 keys; bit i of `gone`: the i-th sixteen of them lie in no page
+    auto work = [&](const Slab<D>& b, int tile, unsigned gone) {
         if (tile > w_hi || tile + 63 < w_lo)
             return;
-        const bool edge = (absent & 15u) != 0 || tile < all_lo || tile + 63 > all_hi;
+        const bool edge = (gone & 15u) != 0 || tile < all_lo || tile + 63 > all_hi;
         floatx4    sc[4][RT];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -784,14 +783,14 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
         if (edge) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const bool none = ((absent >> (2 * (k >> 1) + (h >> 1))) & 1u) != 0;
+                const int  none = -(int)((gone >> (2 * (k >> 1) + (h >> 1))) & 1u);
                 const int  at   = tile + 32 * (k >> 1) + 8 * h + 4 * (k & 1);
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const bool hidden = (int)none | (int)(at + i < first[r]) | (int)(at + i > last[r]);
-                        sc[k][r][i] = hidden ? -__builtin_inff() : sc[k][r][i];
+                        const int hidden = (at + i - first[r]) | (last[r] - at - i) | none; // below 0 where it is
+                        sc[k][r][i] = hidden < 0 ? -__builtin_inff() : sc[k][r][i];
                     }
             }
         }
@@ -840,7 +839,8 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
 
     if (t0 < t1) {
         unpack<D>(slab[0][group >> 1], raw, group & 1, values, unit, lane);
-        load(gone_next, min(t0 + 1, t1 - 1));
+        unsigned gone = absent(t0);
+        load(min(t0 + 1, t1 - 1));
         __syncthreads();
         for (int t = t0; t < t1; ++t) {
 #pragma unroll
@@ -848,8 +848,8 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
                 work(slab[(t - t0) & 1][x], t * kStep + 64 * x, gone >> (4 * x));
             if (t + 1 < t1) { // the other slab was last read before the barrier
                 unpack<D>(slab[(t + 1 - t0) & 1][group >> 1], raw, group & 1, values, unit, lane);
-                gone = gone_next;
-                load(gone_next, min(t + 2, t1 - 1));
+                gone = absent(t + 1);
+                load(min(t + 2, t1 - 1));
             }
             __syncthreads();
         }

@@ -16,7 +16,7 @@ constexpr int kWaves      = 8;          // waves of a workgroup of w4_linear
 constexpr int kMaxColumns = 16 * 65535; // column tiles are the y dimension of the grid
 
 // Packed weights: codes [row tile of 16][block of 128 columns][lane][4 dwords], scales [row tile][group][16 rows] in 16
-// bits, zero points [row tile][block][h][group of the block][rows 4 h .. 4 h + 3] in 4.  Lane r + 16 h of a block holds, of row r, for each half p of 64 columns
+// bits, zero points plus 16 [row tile][block][h][group of the block][rows 4 h .. 4 h + 3] in 8.  Lane r + 16 h of a block holds, of row r, for each half p of 64 columns
 // the dwords A = 2p, B = 2p + 1:
 //   columns 64 p + 8 h + 0..7        nibbles 0 4 2 6 of A, then of B
 //   columns 64 p + 32 + 8 h + 0..7   nibbles 1 5 3 7 of A, then of B
@@ -34,7 +34,7 @@ __host__ __device__ inline Layout layout_of(int M, int K, int group)
     l.groups = K / group;
     l.scales = (int64_t)l.tiles * l.blocks * 1024;
     l.zeros  = l.scales + (int64_t)l.tiles * l.groups * 32;
-    l.bytes  = (l.zeros + (int64_t)l.tiles * l.blocks * (kBlockK / group) * 8 + 15) / 16 * 16;
+    l.bytes  = (l.zeros + (int64_t)l.tiles * l.blocks * (kBlockK / group) * 16 + 15) / 16 * 16;
     return l;
 }
 
@@ -63,10 +63,8 @@ __global__ __launch_bounds__(64) void w4_pack(const uint8_t* codes, const uint16
         const int64_t src  = (int64_t)row * l.groups + gk;
         if (gk < l.groups)
             reinterpret_cast<uint16_t*>(packed + l.scales)[((int64_t)tile * l.groups + gk) * 16 + r] = live ? scales[src] : (uint16_t)0;
-        if ((r & 1) == 0) { // rows r and r + 1 of rows 4 (r / 4) ..
-            const unsigned z0 = live ? zeros[src] & 15u : 0u, z1 = live && row + 1 < M ? zeros[src + l.groups] & 15u : 0u;
-            packed[l.zeros + ((((int64_t)tile * l.blocks + kb) * 4 + (r >> 2)) * per + g) * 2 + (r >> 1 & 1)] = (uint8_t)(z0 | z1 << 4);
-        }
+        packed[l.zeros + ((((int64_t)tile * l.blocks + kb) * 4 + (r >> 2)) * per + g) * 4 + (r & 3)] =
+            (uint8_t)(16 + (live ? zeros[src] & 15 : 0));
     }
 }
 
@@ -118,7 +116,7 @@ struct Weights {
     static constexpr int kGroups = kBlockK / G; // groups of a block
     uintx4   w[R];
     uintx2   s[R][kGroups];
-    unsigned z[R][(kGroups + 1) / 2];
+    unsigned z[R][kGroups];
 };
 
 template <int R, int G>
@@ -139,7 +137,7 @@ struct Source {
             const int64_t tile = min(tile0 + r, l.tiles - 1);
             codes[r]  = reinterpret_cast<const uintx4*>(a.packed) + tile * l.blocks * 64 + lane;
             scales[r] = reinterpret_cast<const uint16_t*>(a.packed + l.scales) + tile * l.groups * 16 + 4 * h;
-            zeros[r]  = a.packed + l.zeros + (tile * l.blocks * 4 + h) * kGroups * 2;
+            zeros[r]  = a.packed + l.zeros + (tile * l.blocks * 4 + h) * kGroups * 4;
         }
     }
 
@@ -152,13 +150,18 @@ struct Source {
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) // a group past the end meets zeros of X
                 b.s[r][g] = *reinterpret_cast<const uintx2*>(scales[r] + min(kb * kGroups + g, groups - 1) * 16);
-            const uint8_t* z = zeros[r] + (int64_t)kb * 8 * kGroups;
-            if constexpr (kGroups == 1)
-                b.z[r][0] = *reinterpret_cast<const uint16_t*>(z);
-            else
+            const unsigned* z = reinterpret_cast<const unsigned*>(zeros[r] + (int64_t)kb * 16 * kGroups);
+            if constexpr (kGroups == 1) {
+                b.z[r][0] = z[0];
+            } else if constexpr (kGroups == 2) {
+                const uintx2 v = *reinterpret_cast<const uintx2*>(z);
+                b.z[r][0] = v[0], b.z[r][1] = v[1];
+            } else {
+                const uintx4 v = *reinterpret_cast<const uintx4*>(z);
 #pragma unroll
-                for (int g = 0; g < kGroups / 2; ++g)
-                    b.z[r][g] = reinterpret_cast<const unsigned*>(z)[g];
+                for (int g = 0; g < 4; ++g)
+                    b.z[r][g] = v[g];
+            }
         }
     }
 };
@@ -173,6 +176,8 @@ __device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G
     const floatx4 zero{0.f, 0.f, 0.f, 0.f};
     const vec     ones = __builtin_bit_cast(vec, uintx4{T::kOne, T::kOne, T::kOne, T::kOne});
     floatx4       acc[R][NT], xs[NT];
+    unsigned      mask = T::kMask;
+    asm("" : "+v"(mask)); // in a register: an instruction takes one literal, and with two a code's AND and OR are two instructions
 #pragma unroll
     for (int j = 0; j < 4; ++j) { // 32 columns: nibbles 0 4 2 6 of two dwords, or 1 5 3 7
         if (j % kSteps == 0) {
@@ -194,7 +199,7 @@ __device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G
         for (int r = 0; r < R; ++r) {
             const unsigned A = b.w[r][j & 2], B = b.w[r][(j & 2) + 1];
             const int      n0 = 4 * (j & 1);
-            auto part = [](unsigned v, int n) { return (__builtin_amdgcn_alignbit(v, v, n) & T::kMask) | T::k16; };
+            auto part = [&](unsigned v, int n) { return (__builtin_amdgcn_alignbit(v, v, n) & mask) | T::k16; };
             const vec wv = __builtin_bit_cast(vec, uintx4{part(A, n0), part(A, n0 + 8), part(B, n0), part(B, n0 + 8)});
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -207,7 +212,7 @@ __device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float sc = from16((uint16_t)(b.s[r][g][i >> 1] >> (16 * (i & 1))), BF16);
-                    const float zp = (float)((b.z[r][g >> 1] >> (16 * (g & 1) + 4 * i)) & 15u) + 16.f;
+                    const float zp = (float)((b.z[r][g] >> (8 * i)) & 255u);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
                         y[r][n][i] = __builtin_fmaf(__builtin_fmaf(-zp, xs[n][i], acc[r][n][i]), sc, y[r][n][i]);
@@ -429,7 +434,7 @@ constexpr int kWideTiles = 2; // row tiles of a wave of the wide kernel
 constexpr int wide_waves(int column_tiles) { return column_tiles == 2 ? 4 : 8; }
 
 // The most row tiles w4_linear's registers hold (finer groups have more scales).
-constexpr int most_tiles(int group) { return group == 128 ? 7 : (group == 64 ? 6 : 4); }
+constexpr int most_tiles(int group) { return group == 128 ? 7 : (group == 64 ? 5 : 4); }
 
 // The cheapest by a model of a call's time in microseconds, fitted to calls of 512x1024 to 28672x7168 and 9216x36864 with 1 to
 // 64 columns.  One workgroup of w4_linear runs on a CU at a time; a step, a block of K for each of its 8 waves, takes

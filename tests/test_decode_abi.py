@@ -124,11 +124,11 @@ def test_attention_refusals(capfd):
 
 def test_linear_sizes_and_refusals(capfd):
     L = M._library()
-    # codes of 16 rows x 128 columns are 1024 bytes, scales of 16 rows 32 bytes a group, zero points 8 for each of
+    # codes of 16 rows x 128 columns are 1024 bytes, scales of 16 rows 32 bytes a group, zero points 16 for each of
     # the blocks' groups; a multiple of 16
-    assert L.W4_PackedBytes(16, 128, 128) == 1024 + 40 + 8
-    assert L.W4_PackedBytes(17, 160, 32) == 2 * 2 * 1024 + 2 * 5 * 32 + 2 * 8 * 8
-    assert L.W4_PackedBytes(1048560, 65536, 64) == 65535 * (512 * 1024 + 1024 * 40)
+    assert L.W4_PackedBytes(16, 128, 128) == 1024 + 32 + 16
+    assert L.W4_PackedBytes(17, 160, 32) == 2 * 2 * 1024 + 2 * 5 * 32 + 2 * 8 * 16
+    assert L.W4_PackedBytes(1048560, 65536, 64) == 65535 * (512 * 1024 + 1024 * 48)
     for bad in ((0, 128, 64), (16, 0, 64), (16, 100, 32), (16, 128, 16), (16, 128, 256), (16 * 65535 + 1, 128, 64)):
         assert L.W4_PackedBytes(*bad) == 0
         assert L.W4_Pack(None, X, X, X, *bad, 0, X) == 1
