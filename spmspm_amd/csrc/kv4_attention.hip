@@ -974,8 +974,14 @@ struct Plan {
 
 constexpr int kManyRows = 64; // average rows of a sequence from which its keys go through LDS
 
-// Row tiles per wave: as many as the average sequence fills, up to two.  Splits of the keys: enough workgroups for every
-// CU to hold two, no split below four tiles per wave.
+// Row tiles: as many as the average sequence fills.  Splits of the keys: two workgroups for every CU (three quarters of that
+// is as good where they are long), none of less than 16 tiles of 32 keys (4 where all waves share them), and none at all
+// below 32 tiles: the second launch costs 3 us.  Measured in us with 1 / 2 / 4 / 8 / 16 splits: one sequence of 2048 keys,
+// 40 heads 19.5 / 16.4 / 13.5 / 13.9 / 13.9 (4 here); 131071 keys, 8 key/value heads 1020 / 518 / 265 / 139 / 76, then 46 / 39 /
+// 44 with 32 / 64 / 128 (64 here); 4 sequences of 1000 keys, 8 heads 11.9 / 12.8 / 12.9 / 12.7 / 12.8 (1 here); 30 new tokens of
+// 2 sequences of 1000 keys, 16 heads over 4 34.7 / 26.2 / 20.5 / 18.9 / 20.1 (8 here); 1024 new tokens over 8192 keys, 456
+// workgroups 313 / 328 / 317 / 367 / 498 (1 here); 256 new tokens of 4 sequences over 8192, 288 workgroups 332 / 195 / 210 / 248 /
+// 317 (2 here).
 Plan plan_of(const KV4_Cache& c, const KV4_Batch& b, int q_heads, int window, int max_len)
 {
     Plan          p;
@@ -990,7 +996,8 @@ Plan plan_of(const KV4_Cache& c, const KV4_Batch& b, int q_heads, int window, in
         len = std::min<int64_t>(len, (int64_t)window + (per + share - 1) / share + kTile);
     const int64_t tiles = (len + kTile - 1) / kTile, groups = (int64_t)p.blocks * c.kv_heads;
     int64_t       want  = p.row_tiles == 8 && groups >= 384 ? 1 : (512 + groups - 1) / groups;
-    want                = std::min<int64_t>(want, (tiles + 4 * kWaves - 1) / (4 * kWaves));
+    const int64_t least = p.row_tiles == 8 ? 4 : 16;
+    want                = tiles <= 32 && p.row_tiles < 8 ? 1 : std::min<int64_t>(want, (tiles + least - 1) / least);
     p.splits            = (int)std::max<int64_t>(1, std::min<int64_t>(want, 128));
     return p;
 }
