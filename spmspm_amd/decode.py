@@ -350,16 +350,30 @@ class W4Linear:
     in the activations' type (fp16 or bf16), zeros uint8 [M][K/group] (0..15), group 32, 64 or 128: see quantize_w4."""
 
     def __init__(self, codes, scales, zeros, bias=None, activation=A.ACT_NONE):
-        self.M, self.K = codes.shape
-        self.device, self.dtype = codes.device, scales.dtype
-        self.packed = w4_pack(codes, scales, zeros)
-        self.group = self.K // scales.shape[1]
-        self.activation = int(activation)
+        packed = w4_pack(codes, scales, zeros)
+        self._adopt(packed, codes.shape[0], codes.shape[1], codes.shape[1] // scales.shape[1], scales.dtype, bias, activation)
+
+    def _adopt(self, packed, M, K, group, dtype, bias, activation):
+        """Checks packed weights and takes them over."""
+        self.device, self.dtype, self.packed, self.bias = packed.device, dtype, packed, bias
+        self.M, self.K, self.group, self.activation = M, K, group, int(activation)
+        _type(dtype)
+        if packed.dtype != torch.uint8 or not packed.is_contiguous() or packed.device.type != "cuda" \
+                or packed.numel() == 0 or packed.numel() != _library().W4_PackedBytes(M, K, group):
+            raise ValueError(f"packed weights of another size than {M} x {K} in groups of {group} take")
         if self.activation not in (A.ACT_NONE, A.ACT_RELU, A.ACT_GELU):
             raise ValueError(f"unknown activation {activation}")
         if bias is not None:
-            _check("bias", bias, self.device, self.dtype, (self.M,))
-        self.bias = bias
+            _check("bias", bias, self.device, self.dtype, (M,))
+
+    def module(self):
+        """The same resident weights as a `torch.nn.Module` around the registered operator."""
+        from .torch_ops import W4LinearModule
+        return W4LinearModule(self)
+
+    def bytes_per_call(self, N):
+        """Bytes a call with N rows of x must move: codes, scales and zero points, x and y."""
+        return self.M * self.K // 2 + 5 * self.M * (self.K // self.group) // 2 + 2 * N * (self.M + self.K)
 
     def __call__(self, x, out=None, stream=None):
         if x.dim() != 2 or x.shape[1] != self.K or x.dtype != self.dtype or x.device != self.device:

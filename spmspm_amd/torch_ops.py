@@ -12,6 +12,10 @@ other kernel launch.
     layer = spmspm_amd.torch_ops.SparseLinearModule.from_compressed(comp, bias=b, activation=spmspm_amd.ACT_RELU)
     y = layer(x)                                     # x: [N][K] fp16 on the GPU  ->  [N][M] fp16
     y = torch.ops.spmspm_amd.sparse_linear(x, layer.values, layer.bitmaps, layer.offsets, None, M, 0, 0)
+
+The decode operators (include/decode_api.h; spmspm_amd/decode.py is their direct form, with less host time a call) are
+registered beside it: `w4_linear` with its `W4LinearModule`, and `kv4_append`, `kv4_gather` and `kv4_attention` over the four
+arrays of a 4-bit cache, of which kv4_append is declared to mutate them.
 """
 from typing import Optional
 
@@ -19,8 +23,9 @@ import numpy as np
 import torch
 
 from . import api as A
+from . import decode as D
 
-__all__ = ["sparse_linear", "SparseLinearModule"]
+__all__ = ["sparse_linear", "SparseLinearModule", "w4_linear", "W4LinearModule", "kv4_append", "kv4_gather", "kv4_attention"]
 
 
 @torch.library.custom_op("spmspm_amd::sparse_linear", mutates_args=(), device_types="cuda")
@@ -117,3 +122,79 @@ class SparseLinearModule(torch.nn.Module):
 
     def extra_repr(self):
         return f"M={self.M}, K={self.K}, split_k={self.split_k}, activation={self.activation}"
+
+
+@torch.library.custom_op("spmspm_amd::w4_linear", mutates_args=(), device_types="cuda")
+def w4_linear(x: torch.Tensor, packed: torch.Tensor, bias: Optional[torch.Tensor], M: int, group: int,
+              activation: int) -> torch.Tensor:
+    """y[N][M] = act(W x + bias) for 4-bit weights laid out by `spmspm_amd.w4_pack`; x [N][K], fp16 or bf16 as the scales."""
+    layer = object.__new__(D.W4Linear)
+    layer._adopt(packed, int(M), x.shape[1] if x.dim() == 2 else 0, int(group), x.dtype, bias, int(activation))
+    return layer(x)
+
+
+@w4_linear.register_fake
+def _(x, packed, bias, M, group, activation):
+    return x.new_empty((x.shape[0], M))
+
+
+class W4LinearModule(torch.nn.Module):
+    """`nn.Module` around the registered operator, over the packed weights of a `spmspm_amd.W4Linear` (shared)."""
+
+    def __init__(self, layer):
+        super().__init__()
+        self.M, self.K, self.group, self.activation = layer.M, layer.K, layer.group, layer.activation
+        self.register_buffer("packed", layer.packed)
+        self.register_buffer("bias", layer.bias)
+
+    def forward(self, x):
+        return torch.ops.spmspm_amd.w4_linear(x, self.packed, self.bias, self.M, self.group, self.activation)
+
+    def extra_repr(self):
+        return f"M={self.M}, K={self.K}, group={self.group}, activation={self.activation}"
+
+
+@torch.library.custom_op("spmspm_amd::kv4_append", mutates_args=("k_codes", "k_words", "v_codes", "v_words"),
+                         device_types="cuda")
+def kv4_append(k_codes: torch.Tensor, k_words: torch.Tensor, v_codes: torch.Tensor, v_words: torch.Tensor,
+               k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+               cu_tokens: Optional[torch.Tensor], q: Optional[torch.Tensor], rotation: Optional[torch.Tensor],
+               interleaved: bool, positions: Optional[torch.Tensor]) -> torch.Tensor:
+    """`spmspm_amd.kv4_append`; returns the rotated queries, an empty tensor without q."""
+    cache = D.KV4Cache.from_tensors(k_codes, k_words, v_codes, v_words)
+    out = D.kv4_append(cache, k, v, block_table, seq_lens, cu_tokens, q, rotation, interleaved, positions)
+    return k.new_empty(0) if out is None else out
+
+
+@kv4_append.register_fake
+def _(k_codes, k_words, v_codes, v_words, k, v, block_table, seq_lens, cu_tokens, q, rotation, interleaved, positions):
+    return k.new_empty(0) if q is None else q.new_empty(q.shape)
+
+
+@torch.library.custom_op("spmspm_amd::kv4_gather", mutates_args=(), device_types="cuda")
+def kv4_gather(k_codes: torch.Tensor, k_words: torch.Tensor, v_codes: torch.Tensor, v_words: torch.Tensor,
+               block_table: torch.Tensor, seq_lens: torch.Tensor, cu_tokens: Optional[torch.Tensor], total_tokens: int,
+               dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """`spmspm_amd.kv4_gather`."""
+    cache = D.KV4Cache.from_tensors(k_codes, k_words, v_codes, v_words)
+    return D.kv4_gather(cache, block_table, seq_lens, cu_tokens, total_tokens, dtype)
+
+
+@kv4_gather.register_fake
+def _(k_codes, k_words, v_codes, v_words, block_table, seq_lens, cu_tokens, total_tokens, dtype):
+    shape = (total_tokens, k_codes.shape[1], 2 * k_codes.shape[3])
+    return k_codes.new_empty(shape, dtype=dtype), k_codes.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("spmspm_amd::kv4_attention", mutates_args=(), device_types="cuda")
+def kv4_attention(q: torch.Tensor, k_codes: torch.Tensor, k_words: torch.Tensor, v_codes: torch.Tensor,
+                  v_words: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                  cu_tokens: Optional[torch.Tensor], scale: Optional[float], window: int, max_len: int) -> torch.Tensor:
+    """`spmspm_amd.kv4_attention`, outputs only."""
+    cache = D.KV4Cache.from_tensors(k_codes, k_words, v_codes, v_words)
+    return D.kv4_attention(q, cache, block_table, seq_lens, cu_tokens, scale, window, max_len)
+
+
+@kv4_attention.register_fake
+def _(q, k_codes, k_words, v_codes, v_words, block_table, seq_lens, cu_tokens, scale, window, max_len):
+    return q.new_empty(q.shape)
