@@ -126,12 +126,12 @@ size_t KV4_AttentionWorkspaceBytes(const KV4_Cache* cache, const KV4_Batch* batc
  * refused.
  * X: rows of K elements, x_stride elements apart (a multiple of 8, at least K), 16-byte aligned; Y contiguous [N][M].
  * `activation`: 0 none, 1 ReLU, 2 GELU (tanh form), as in spmm_api.h.  N from 0 to 16 * 65535.  `workspace` must hold
- * W4_WorkspaceBytes(M, N, K) bytes (NULL where that is 0), 16-byte aligned; contents irrelevant.
+ * W4_WorkspaceBytes(M, N, K, group) bytes (NULL where that is 0), 16-byte aligned; contents irrelevant.
  */
 size_t W4_PackedBytes(int M, int K, int group);
 int    W4_Pack(hipStream_t stream, const uint8_t* codes, const void* scales, const uint8_t* zeros, int M, int K,
                int group, int dtype, void* packed);
-size_t W4_WorkspaceBytes(int M, int N, int K);
+size_t W4_WorkspaceBytes(int M, int N, int K, int group);
 int    W4_Linear(hipStream_t stream, const void* packed, const void* X, int64_t x_stride, void* Y, int M, int N, int K,
                  int group, const void* bias, int activation, void* workspace, size_t workspace_bytes, int dtype);
 

@@ -537,11 +537,11 @@ extern "C" int W4_Pack(hipStream_t stream, const uint8_t* codes, const void* sca
                   dtype == DECODE_BF16, static_cast<uint8_t*>(packed));
 }
 
-extern "C" size_t W4_WorkspaceBytes(int M, int N, int K)
+extern "C" size_t W4_WorkspaceBytes(int M, int N, int K, int group)
 {
-    if (M < 1 || M > 16 * 65535 || N < 1 || N > kMaxColumns || K < 32)
+    if (W4_PackedBytes(M, K, group) == 0 || N < 1 || N > kMaxColumns)
         return 0;
-    return workspace_of(M, N, plan_of(M, N, K, 128)); // the split does not depend on the group
+    return workspace_of(M, N, plan_of(M, N, K, group));
 }
 
 extern "C" int W4_Linear(hipStream_t stream, const void* packed, const void* X, int64_t x_stride, void* Y, int M, int N,

@@ -69,7 +69,7 @@ def _library():
         L.W4_Linear.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p] + [C.c_int] * 4 + [
             C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_int]
         L.W4_WorkspaceBytes.restype = C.c_size_t
-        L.W4_WorkspaceBytes.argtypes = [C.c_int] * 3
+        L.W4_WorkspaceBytes.argtypes = [C.c_int] * 4
         _lib = L
     return _lib
 
@@ -389,7 +389,7 @@ class W4Linear:
             y = x.new_empty((N, self.M)) if out is None else out
             if N:
                 L = _library()
-                need = L.W4_WorkspaceBytes(self.M, N, self.K)
+                need = L.W4_WorkspaceBytes(self.M, N, self.K, self.group)
                 ws = self.packed.new_empty(need) if need else None
                 err = L.W4_Linear(handle, self.packed.data_ptr(), x.data_ptr(), stride, y.data_ptr(), self.M, N, self.K,
                                   self.group, None if self.bias is None else self.bias.data_ptr(), self.activation,

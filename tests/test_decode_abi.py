@@ -143,10 +143,52 @@ def test_linear_sizes_and_refusals(capfd):
                            a["act"], None, 0, a["dtype"]) == 1, kw
     assert L.W4_Linear(None, X, X, 128, X, 16, 0, 128, 64, None, 0, None, 0, 0) == 0
     # a split K needs its workspace
-    need = L.W4_WorkspaceBytes(9216, 64, 36864)
-    assert need > 0 and need % (4 * 9216 * 64) == 0 and L.W4_WorkspaceBytes(9216, 16, 36864) == 0
+    need = L.W4_WorkspaceBytes(9216, 64, 36864, 64)
+    assert need > 0 and need % (4 * 9216 * 64) == 0 and L.W4_WorkspaceBytes(9216, 16, 36864, 64) == 0
     for ws, size in ((None, need), (X, need - 1), (X + 8, need)):
         assert L.W4_Linear(None, X, X, 36864, X, 9216, 64, 36864, 64, None, 0, ws, size, 0) == 1
+
+
+def test_linear_workspace_is_what_the_call_asks_for(capfd):
+    """Over sizes and groups: a call with one byte less is refused, and one with the workspace is not (without a GPU it goes as
+    far as the launch, which fails in another way)."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("would launch")
+    L, rng, seen = M._library(), np.random.default_rng(0), set()
+    for _ in range(300):
+        group = int(rng.choice((32, 64, 128)))
+        m, k = int(np.exp(rng.uniform(3, 10.5))), group * max(1, int(np.exp(rng.uniform(5, 10.5))) // group)
+        n = int(np.exp(rng.uniform(2.5, 6)))
+        need = L.W4_WorkspaceBytes(m, n, k, group)
+        seen.add((group, need > 0))
+        call = lambda ws, size: L.W4_Linear(None, X, X, k, X, m, n, k, group, None, 0, ws, size, 0)
+        assert call(X, need) != 1, (m, n, k, group)
+        if need:
+            assert call(X, need - 1) == 1 and call(None, need) == 1
+    assert len(seen) == 6
+
+
+def test_attention_workspace_is_what_the_call_asks_for(capfd):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("would launch")
+    L, rng, seen = M._library(), np.random.default_rng(1), set()
+    for _ in range(300):
+        heads, share, d = int(rng.choice((1, 2, 8, 40))), int(rng.choice((1, 4, 7, 16, 64))), int(rng.choice((64, 96, 128, 256)))
+        b, width = int(np.exp(rng.uniform(0, 4))), int(np.exp(rng.uniform(0, 9)))
+        tokens = b if rng.random() < 0.5 else int(np.exp(rng.uniform(0, 8)))
+        c = cache(num_pages=9, kv_heads=heads, head_dim=d, page_size=int(rng.choice((16, 64, 256))))
+        bt = batch(batch=b, total_tokens=tokens, table_width=width, table_stride=width, cu_tokens=None if tokens == b else X)
+        window, most = int(rng.choice((0, 0, 100, 5000))), int(rng.choice((0, 300, 100000)))
+        need = L.KV4_AttentionWorkspaceBytes(c, bt, heads * share, window, most)
+        seen.add(need > 0)
+        call = lambda ws, size: attend(c=c, b=bt, heads=heads * share, q=rows(token=heads * share * d, head=d), window=window,
+                                       max_len=most, ws=ws, ws_bytes=size)
+        assert call(X, need) != 1
+        if need:
+            assert call(X, need - 1) == 1 and call(None, need) == 1
+    assert len(seen) == 2
 
 
 def test_cache_encoding_is_within_half_a_step_and_holds_zero_exactly():

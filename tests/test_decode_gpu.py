@@ -135,6 +135,24 @@ def test_append_encodes_rotates_and_reads_back(torch, d, rot, interleaved):
         assert torch.equal(got.cpu(), torch.from_numpy(want).to(ttype(torch, dtype)))
 
 
+def test_gather_rounds_the_float32_product(torch):
+    """Enough values that one lies where rounding once and rounding twice differ (one in a million does)."""
+    rng = np.random.default_rng(3)
+    for dtype in ("fp16", "bf16"):
+        pages, hkv, P, d = 64, 8, 64, 128
+        kc = rng.integers(0, 256, (pages, hkv, P, d // 2)).astype(np.uint8)
+        kw = (rng.uniform(0.01, 1, (pages, hkv, P)).astype(np.float32).view(np.uint32))
+        g = lambda a: torch.from_numpy(a).cuda()
+        cache = S.KV4Cache.from_tensors(g(kc), g(kw.view(np.int32)), g(kc), g(kw.view(np.int32)))
+        table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+        T = pages * P
+        n = torch.tensor([T], dtype=torch.int32, device="cuda")
+        k, v = S.kv4_gather(cache, table, n, cu_tokens=torch.tensor([0, T], dtype=torch.int32, device="cuda"),
+                            total_tokens=T, dtype=ttype(torch, dtype))
+        want = torch.from_numpy(D.decode32(kc, kw).transpose(0, 2, 1, 3).reshape(T, hkv, d)).to(ttype(torch, dtype))
+        assert torch.equal(k.cpu(), want) and torch.equal(v.cpu(), want)
+
+
 def test_append_special_values(torch):
     """Zeros, one sign, tiny and huge vectors, infinities and NaN: each stays within its own token and head."""
     for dtype in ("fp16", "bf16"):
@@ -477,6 +495,18 @@ def test_linear_matches_the_oracle(torch, M, K, N, G, dtype):
         big = big + np.abs(xh.astype(np.float64)) @ (256 * np.repeat(np.abs(sh.astype(np.float64)), G, 1)).T
     got = S.W4Linear(g(codes), scales, g(zeros))(x)
     assert_linear(got, y, small, big, dtype, K, G)
+
+
+@pytest.mark.parametrize("M,K,N,G", [(2213, 3744, 36, 32), (3000, 4096, 33, 64), (4100, 2048, 64, 128), (1025, 8192, 100, 32),
+                                     (5000, 1024, 20, 32), (4096, 6144, 32, 128)])
+def test_linear_with_a_split_of_k(torch, M, K, N, G):
+    """Sizes whose K the library may divide among workgroups, groups of every size."""
+    rng = np.random.default_rng(M)
+    codes, scales, sh, zeros = weights(rng, M, K, G, "fp16", torch)
+    x, xh = to16(torch, rng.standard_normal((N, K)), "fp16")
+    g = lambda a: torch.from_numpy(a).cuda()
+    y, small, big = D.linear(xh, codes, sh, zeros)
+    assert_linear(S.W4Linear(g(codes), scales, g(zeros))(x), y, small, big, "fp16", K, G)
 
 
 @pytest.mark.parametrize("K", [32, 96, 160, 224])
