@@ -221,7 +221,7 @@ __device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G
     }
 }
 
-// Few columns.  One workgroup: R row tiles of 16 rows and 16 columns, the blocks of K dealt to its waves in turn; the waves'
+// Few columns.  One workgroup: R row tiles of 16 rows and 16 columns, a share of K's blocks dealt to its waves in turn; the waves'
 // sums are joined through LDS.  G: group size.  Bound by memory where it has one workgroup for every CU: 28672x7168, N = 16,
 // groups of 128, in 26.7 us is 4.0 TB/s of weights (a large copy moves 4.9).  What it took: two sets of registers, so that no
 // wait for X includes the weights behind it; X from the cache as rarely as the registers allow (R tiles per read of it).
@@ -262,17 +262,18 @@ __global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
         multiply<1, R, G, BF16>(y, b.w, [&](int j, int) { return b.x[j]; });
         __builtin_amdgcn_sched_barrier(0);
     };
-    if (wave < l.blocks) {
-        int kb = wave;
+    const int per = (l.blocks + a.splits - 1) / a.splits, last = min((int)(blockIdx.z + 1) * per, l.blocks);
+    if ((int)blockIdx.z * per + wave < last) {
+        int kb = (int)blockIdx.z * per + wave;
         fetch(set[0], kb);
         while (true) {
-            fetch(set[1], min(kb + kWaves, l.blocks - 1)); // the last one is fetched again and not used
+            fetch(set[1], min(kb + kWaves, last - 1)); // the last one is fetched again and not used
             work(set[0]);
-            if ((kb += kWaves) >= l.blocks)
+            if ((kb += kWaves) >= last)
                 break;
-            fetch(set[0], min(kb + kWaves, l.blocks - 1));
+            fetch(set[0], min(kb + kWaves, last - 1));
             work(set[1]);
-            if ((kb += kWaves) >= l.blocks)
+            if ((kb += kWaves) >= last)
                 break;
         }
     }
@@ -289,6 +290,10 @@ __global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
 #pragma unroll
         for (int v = 0; v < kWaves; ++v)
             sum += join[v][at];
+        if (a.splits > 1) {
+            a.part[((int64_t)blockIdx.z * a.N + n) * (l.tiles * 16) + m] = sum;
+            continue;
+        }
         if (a.bias != nullptr)
             sum += from16(a.bias[m], BF16);
         a.y[(int64_t)n * a.M + m] = to16(activate(sum, a.act), BF16);
@@ -427,7 +432,7 @@ namespace {
 struct Plan {
     int row_tiles;    // of w4_linear; 0: w4_linear_wide
     int column_tiles; // of w4_linear_wide, 2 or 4
-    int splits;
+    int splits;       // shares of K
 };
 
 constexpr int kWideTiles = 2; // row tiles of a wave of the wide kernel
@@ -439,7 +444,9 @@ constexpr int most_tiles(int group) { return group == 128 ? 7 : (group == 64 ? 5
 // The cheapest by a model of a call's time in microseconds, fitted to calls of 512x1024 to 28672x7168 and 9216x36864 with 1 to
 // 64 columns.  One workgroup of w4_linear runs on a CU at a time; a step, a block of K for each of its 8 waves, takes
 // 0.4 for a row tile and 0.6 for X: 28672x7168, N = 16, fp16, groups of 128, with 7 / 4 / 2 / 1 row tiles 26.7 / 33.9 /
-// 40.7 / 59.5 us.  Columns past 16 are workgroups of their own.  The wide kernel takes a block of K in 1.13 with two column
+// 40.7 / 59.5 us.  K in shares, so that few rows fill the CUs with many row tiles each: 5120x20480, N = 16 22.6 us with five
+// row tiles in four shares, 32.5 at best in one; 7168x28672, N = 8 26.7 (seven in four) and 29.4; 4096x11008, N = 4 15.6 at
+// best in shares, 13.3 in one.  Columns past 16 are workgroups of their own.  The wide kernel takes a block of K in 1.13 with two column
 // tiles (two workgroups a CU) and 1.75 with four (one), and 8 for launch, ends and the sum of the shares: N = 32 on that
 // matrix 38.8 (w4_linear 50.7), N = 64 53.6 (103), 5120x5120 with N = 32 13.5 (13.5), 512x1024 with N = 64 8.6 (4.0).
 Plan plan_of(int M, int N, int K, int group)
@@ -448,11 +455,14 @@ Plan plan_of(int M, int N, int K, int group)
     auto          up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     Plan          p{1, 0, 1};
     double        best = 1e30;
-    for (int r = 1; r <= most_tiles(group); ++r) {
-        const double us = 3.0 + (double)(up(up(tiles, r) * up(N, 16), 256) * up(blocks, 8)) * (0.4 * r + 0.6);
-        if (us < best)
-            best = us, p.row_tiles = r;
-    }
+    for (int r = 1; r <= most_tiles(group); ++r)
+        for (int s = 1; s <= 8 && 16 * s <= std::max<int64_t>(16, blocks); ++s) {
+            double us = 3.0 + (double)(up(up(tiles, r) * up(N, 16) * s, 256) * up(up(blocks, s), 8)) * (0.4 * r + 0.6);
+            if (s > 1) // the sum of the shares: a launch, and every share written and read
+                us += 6.0 + s * (double)M * N * 8.0 / 4.9e6;
+            if (us < best)
+                best = us, p = Plan{r, 0, s};
+        }
     if (N <= 16)
         return p;
     const int     nt = N <= 32 ? 2 : 4, slots = nt == 2 ? 512 : 256;
@@ -468,6 +478,12 @@ size_t workspace_of(int M, int N, const Plan& p)
     return p.splits > 1 ? (size_t)p.splits * N * ((M + 15) / 16 * 16) * sizeof(float) : 0;
 }
 
+int run_join(hipStream_t stream, const LinearArgs& a, bool bf16)
+{
+    const int64_t quads = (int64_t)((a.M + 15) / 16) * 4 * a.N;
+    return launch(w4_join, dim3((unsigned)((quads + 255) / 256), 1, 1), dim3(256, 1, 1), stream, a, (int)bf16);
+}
+
 template <int R, int G, bool BF16>
 int run_narrow(hipStream_t stream, int row_tiles, const LinearArgs& a)
 {
@@ -475,8 +491,9 @@ int run_narrow(hipStream_t stream, int row_tiles, const LinearArgs& a)
         if (row_tiles < R)
             return run_narrow<R - 1, G, BF16>(stream, row_tiles, a);
     const unsigned tiles = (unsigned)(a.M + 15) / 16;
-    return launch(w4_linear<R, G, BF16>, dim3((tiles + R - 1) / R, (unsigned)(a.N + 15) / 16, 1), dim3(64 * kWaves, 1, 1),
-                  stream, a);
+    const int      err   = launch(w4_linear<R, G, BF16>, dim3((tiles + R - 1) / R, (unsigned)(a.N + 15) / 16, (unsigned)a.splits),
+                                  dim3(64 * kWaves, 1, 1), stream, a);
+    return err != 0 || a.splits == 1 ? err : run_join(stream, a, BF16);
 }
 
 template <int NT, int G, bool BF16>
@@ -488,10 +505,7 @@ int run_wide(hipStream_t stream, const LinearArgs& a)
     const int          err   = launch(w4_linear_wide<NT, kWideTiles, G, BF16, W>,
                                       dim3((tiles + kRows - 1) / kRows, (unsigned)(a.N + 16 * NT - 1) / (16 * NT), (unsigned)a.splits),
                                       dim3(64 * W, 1, 1), stream, a);
-    if (err != 0 || a.splits == 1)
-        return err;
-    const int64_t quads = (int64_t)tiles * 4 * a.N;
-    return launch(w4_join, dim3((unsigned)((quads + 255) / 256), 1, 1), dim3(256, 1, 1), stream, a, (int)BF16);
+    return err != 0 || a.splits == 1 ? err : run_join(stream, a, BF16);
 }
 
 template <int G, bool BF16>

@@ -144,7 +144,7 @@ def test_linear_sizes_and_refusals(capfd):
     assert L.W4_Linear(None, X, X, 128, X, 16, 0, 128, 64, None, 0, None, 0, 0) == 0
     # a split K needs its workspace
     need = L.W4_WorkspaceBytes(9216, 64, 36864, 64)
-    assert need > 0 and need % (4 * 9216 * 64) == 0 and L.W4_WorkspaceBytes(9216, 16, 36864, 64) == 0
+    assert need > 0 and need % (4 * 9216 * 64) == 0 and L.W4_WorkspaceBytes(28672, 16, 7168, 128) == 0
     for ws, size in ((None, need), (X, need - 1), (X + 8, need)):
         assert L.W4_Linear(None, X, X, 36864, X, 9216, 64, 36864, 64, None, 0, ws, size, 0) == 1
 
