@@ -223,7 +223,8 @@ __device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G
 
 // Few columns.  One workgroup: R row tiles of 16 rows and 16 columns, a share of K's blocks dealt to its waves in turn; the waves'
 // sums are joined through LDS.  G: group size.  Bound by memory where it has one workgroup for every CU: 28672x7168, N = 16,
-// groups of 128, in 26.7 us is 4.0 TB/s of weights (a large copy moves 4.9).  What it took: two sets of registers, so that no
+// groups of 128, in 24.4 us is 4.3 TB/s of weights (a large copy moves 4.9); 5120x5120, N = 1 takes 7.3, a launch, two
+// rounds of loads and the join, where its bytes are 2.8.  What it took: two sets of registers, so that no
 // wait for X includes the weights behind it; X from the cache as rarely as the registers allow (R tiles per read of it).
 template <int R, int G, bool BF16>
 __global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
@@ -302,9 +303,9 @@ __global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
 
 // Many columns.  One workgroup: WAVES waves of R row tiles each and NT column tiles, over a share of K's blocks; the X of a
 // block goes through LDS, once for all waves.  Partial sums of a split K go to `part` [split][column][row].  9216x36864, N = 64,
-// bf16, groups of 64, seven shares: 91.5 us, 2.1 TB/s of weights; bound by the SIMDs' issue of matrix products (a third of
-// them sums of X) and of the scales' multiplications, which two waves a SIMD do not overlap.  w4_linear, which reads X from
-// the cache for every wave, takes 190 to 240 there.
+// bf16, groups of 64, seven shares: 83 us with the sum of the shares (5), 2.3 TB/s of weights; bound by the SIMDs' issue of
+// vector instructions (53 % of the cycles: unpacking codes, scales into the sums) and matrix products (33 %, a third of them sums of
+// X), which two waves a SIMD do not overlap.  w4_linear, which reads X from the cache for every wave, takes 190 to 240 there.
 template <int NT, int R, int G, bool BF16, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void w4_linear_wide(LinearArgs a)
 {
@@ -407,17 +408,31 @@ __global__ __launch_bounds__(64 * WAVES, 2) void w4_linear_wide(LinearArgs a)
     }
 }
 
-// Sums the slabs of a split K: four rows of a column per thread.
-__global__ __launch_bounds__(256) void w4_join(LinearArgs a, int bf16)
+// Sums the slabs of a split K: four rows of a column per thread, and the slabs dealt to the workgroup's waves, whose sums meet
+// in LDS (66 slabs of 529x50 one after the other in every thread: 20 us more).
+constexpr int kJoinWaves = 4;
+
+__global__ __launch_bounds__(64 * kJoinWaves) void w4_join(LinearArgs a, int bf16)
 {
-    const int quads = (a.M + 15) / 16 * 4;
-    const int at    = blockIdx.x * 256 + threadIdx.x;
-    const int col = at / quads, m = at % quads * 4;
-    if (col >= a.N || m >= a.M)
+    __shared__ floatx4 sums[kJoinWaves][64];
+    const int     lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int     quads = (a.M + 15) / 16 * 4;
+    const int     at = blockIdx.x * 64 + lane, col = at / quads, m = at % quads * 4;
+    const int64_t slab = (int64_t)a.N * (quads * 4);
+    floatx4       sum{0.f, 0.f, 0.f, 0.f};
+    if (col < a.N) {
+        const float* part = a.part + (int64_t)at * 4;
+#pragma unroll 4
+        for (int s = wave; s < a.splits; s += kJoinWaves)
+            sum += *reinterpret_cast<const floatx4*>(part + s * slab);
+    }
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || col >= a.N)
         return;
-    floatx4 sum{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s)
-        sum += *reinterpret_cast<const floatx4*>(a.part + ((int64_t)s * a.N + col) * (quads * 4) + m);
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; ++w)
+        sum += sums[w][lane];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (m + i < a.M)
@@ -436,6 +451,7 @@ struct Plan {
 };
 
 constexpr int kWideTiles = 2; // row tiles of a wave of the wide kernel
+constexpr int kMostShares = 64; // of K, for the wide kernel
 constexpr int wide_waves(int column_tiles) { return column_tiles == 2 ? 4 : 8; }
 
 // The most row tiles w4_linear's registers hold (finer groups have more scales).
@@ -446,9 +462,12 @@ constexpr int most_tiles(int group) { return group == 128 ? 7 : (group == 64 ? 5
 // 0.4 for a row tile and 0.6 for X: 28672x7168, N = 16, fp16, groups of 128, with 7 / 4 / 2 / 1 row tiles 26.7 / 33.9 /
 // 40.7 / 59.5 us.  K in shares, so that few rows fill the CUs with many row tiles each: 5120x20480, N = 16 22.6 us with five
 // row tiles in four shares, 32.5 at best in one; 7168x28672, N = 8 26.7 (seven in four) and 29.4; 4096x11008, N = 4 15.6 at
-// best in shares, 13.3 in one.  Columns past 16 are workgroups of their own.  The wide kernel takes a block of K in 1.13 with two column
-// tiles (two workgroups a CU) and 1.75 with four (one), and 8 for launch, ends and the sum of the shares: N = 32 on that
-// matrix 38.8 (w4_linear 50.7), N = 64 53.6 (103), 5120x5120 with N = 32 13.5 (13.5), 512x1024 with N = 64 8.6 (4.0).
+// best in shares, 13.3 in one.  Columns past 16 are workgroups of their own.
+// The wide kernel takes a block of K in step[0] with two column tiles and one workgroup on a CU, in step[1] with two on it, and in
+// step[2] with four column tiles, 5 for launch and ends, and with shares 2 for the second launch and their bytes: 5120x5120,
+// N = 32, groups of 128 12.9 (w4_linear 12.6); 20480x5120, N = 24 22.0 (29.8) and N = 64 29.2 with four, 36.6 with two column
+// tiles (57.0); 640x8192, N = 64, groups of 64 10.2 with 16 shares, 12.7 with 8 and 14.5 with 64 (11.0); 529x25184, N = 50,
+// groups of 32 17.2 with 24 shares of two column tiles, 20.8 with 66 of four (24.0); 512x1024 with N = 64 8.6 (4.0).
 Plan plan_of(int M, int N, int K, int group)
 {
     const int64_t tiles = (M + 15) / 16, blocks = (K + kBlockK - 1) / kBlockK;
@@ -465,11 +484,25 @@ Plan plan_of(int M, int N, int K, int group)
         }
     if (N <= 16)
         return p;
-    const int     nt = N <= 32 ? 2 : 4, slots = nt == 2 ? 512 : 256;
-    const int64_t groups = up(tiles, kWideTiles * wide_waves(nt)) * up(N, 16 * nt);
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(slots / groups, blocks / 2));
-    if (8.0 + (double)(up(groups * splits, slots) * up(blocks, splits)) * (nt == 2 ? 1.13 : 1.75) < best)
-        p = Plan{0, nt, (int)splits};
+    const double step32[3] = {1.0, 1.8, 2.3}, step64[3] = {0.74, 1.25, 1.6}, step128[3] = {0.58, 1.1, 1.25};
+    const double* step = group == 32 ? step32 : (group == 64 ? step64 : step128);
+    for (int nt = 2; nt <= 4; nt += 2) {
+        const int64_t groups = up(tiles, kWideTiles * wide_waves(nt)) * up(N, 16 * nt);
+        for (int fill = 0; fill <= 512; fill += 256) { // shares for none, one or two workgroups on every CU
+            int64_t       s   = std::max<int64_t>(1, std::min<int64_t>({fill / groups, blocks, kMostShares}));
+            const int64_t per = up(blocks, s), rest = groups * up(blocks, per) % 512, full = groups * up(blocks, per) / 512;
+            s                 = up(blocks, per);
+            double us = 5.0;
+            if (nt == 4)
+                us += (double)(per * up(groups * s, 256)) * step[2];
+            else
+                us += (double)per * ((double)full * step[1] + (rest > 256 ? step[1] : (rest > 0 ? step[0] : 0.0)));
+            if (s > 1)
+                us += 2.0 + (double)s * M * N * 8.0 / 6e6;
+            if (us < best)
+                best = us, p = Plan{0, nt, (int)s};
+        }
+    }
     return p;
 }
 
@@ -481,7 +514,7 @@ size_t workspace_of(int M, int N, const Plan& p)
 int run_join(hipStream_t stream, const LinearArgs& a, bool bf16)
 {
     const int64_t quads = (int64_t)((a.M + 15) / 16) * 4 * a.N;
-    return launch(w4_join, dim3((unsigned)((quads + 255) / 256), 1, 1), dim3(256, 1, 1), stream, a, (int)bf16);
+    return launch(w4_join, dim3((unsigned)((quads + 63) / 64), 1, 1), dim3(64 * kJoinWaves, 1, 1), stream, a, (int)bf16);
 }
 
 template <int R, int G, bool BF16>

@@ -509,6 +509,21 @@ def test_linear_with_a_split_of_k(torch, M, K, N, G):
     assert_linear(S.W4Linear(g(codes), scales, g(zeros))(x), y, small, big, "fp16", K, G)
 
 
+@pytest.mark.parametrize("M,K,N,G", [(40, 8320, 50, 32), (33, 16512, 20, 128), (530, 6080, 64, 64), (700, 9024, 17, 32)])
+def test_linear_with_many_shares_of_a_long_k(torch, M, K, N, G):
+    """Few rows and a long K: dozens of shares, whose last may be shorter, and a sum of them over several waves."""
+    rng = np.random.default_rng(M)
+    codes, scales, sh, zeros = weights(rng, M, K, G, "fp16", torch)
+    x, xh = to16(torch, rng.standard_normal((N, K)), "fp16")
+    bias, bh = to16(torch, rng.standard_normal(M), "fp16")
+    g = lambda a: torch.from_numpy(a).cuda()
+    y, small, big = D.linear(xh, codes, sh, zeros, bh)
+    layer = S.W4Linear(g(codes), scales, g(zeros), bias=bias)
+    got = layer(x)
+    assert_linear(got, y, small, big + np.abs(bh), "fp16", K, G)
+    assert torch.equal(got, layer(x))
+
+
 @pytest.mark.parametrize("K", [32, 96, 160, 224])
 def test_linear_ends_inside_a_block_and_reads_nothing_past_a_row(torch, K):
     """K that is no multiple of 128: the columns behind a row's end belong to somebody else and may be NaN."""
