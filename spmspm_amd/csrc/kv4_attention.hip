@@ -18,6 +18,10 @@
 // probabilities go from one product to the next in registers, and maxima, sums and rescaling need no exchange but the
 // one between the four lanes of a row, only when the maximum rises by more than 2^8.  V^T is built from rows of V: a lane
 // loads 4 bytes of each of its 8 keys and pairs their halves (v_perm); LDS is not used until the waves' results are joined.
+//
+// Bounds.  Few rows: memory.  32 sequences of up to 16384 keys, 64 heads over 8, D = 128: 103 us, 4.6 TB/s (a large copy moves
+// 4.9); 16 of up to 2048 keys, 40 heads of their own: 36.8 us, 3.6 TB/s, the longest of one round of workgroups; 131071 keys of
+// one sequence, 32 heads over 8: 31 us and 5.5 for the join.
 #include "decode_common.hiph"
 
 #include <algorithm>
@@ -547,7 +551,9 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
 // Many rows per sequence (prompts and chunks of them): the waves of a workgroup, two row tiles each, share the keys, which go
 // unpacked through LDS, 16 for every wave at a time: half of the waves unpack the codes of 32 keys each, the others those of
 // values, as operands of the products, and the words as what a score is multiplied by (u), what is added to it (ev) and what
-// its probability counts in the sum (il).  Here z is taken off the keys' codes too, all rows of the block share the queries'
+// its probability counts in the sum (il).  Bound by the issue of vector and matrix instructions, whose times were found to add
+// up: 2 x 1024 rows over 8192 keys, 32 heads over 8 of 128 take 287 us, 715 TFLOP/s (a large product of the library reaches 1546);
+// kv4_attention, which unpacks a key for every 32 rows, took 431 before this kernel was there.  Here z is taken off the keys' codes too, all rows of the block share the queries'
 // scale, and a value's whole scale goes into the exponent, p'_t = 2^(log2 p_t + log2 s_t - m), with il = 2^-6 / s_t:
 // logarithm and reciprocal are taken once for all rows of the block, and save a product for each probability.
 template <int D>
@@ -907,7 +913,7 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
 }
 
 // Joins the splits of a row: threads of one row take 8 elements each, in `lanes` groups that deal the splits among them and
-// meet in LDS.
+// meet in LDS.  Latency decides: 32 rows of 64 splits 5.5 us, 1280 rows of a few 3.4.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_attention_join(AttentionArgs a, int lanes)
 {
