@@ -141,6 +141,7 @@ struct Source {
         }
     }
 
+    template <bool ZEROS>
     __device__ __forceinline__ void fetch(Weights<R, G>& b, int kb) const
     {
         constexpr int kGroups = kBlockK / G;
@@ -151,7 +152,8 @@ struct Source {
             for (int g = 0; g < kGroups; ++g) // a group past the end meets zeros of X
                 b.s[r][g] = *reinterpret_cast<const uintx2*>(scales[r] + min(kb * kGroups + g, groups - 1) * 16);
             const unsigned* z = reinterpret_cast<const unsigned*>(zeros[r] + (int64_t)kb * 16 * kGroups);
-            if constexpr (kGroups == 1) {
+            if constexpr (!ZEROS) {
+            } else if constexpr (kGroups == 1) {
                 b.z[r][0] = z[0];
             } else if constexpr (kGroups == 2) {
                 const uintx2 v = *reinterpret_cast<const uintx2*>(z);
@@ -166,8 +168,9 @@ struct Source {
     }
 };
 
-// y += W X of one block; x(j, n) gives the lane's operand for columns 32 j .. 32 j + 31 of column tile n.
-template <int NT, int R, int G, bool BF16, typename X>
+// y += W X of one block; x(j, n) gives the lane's operand for columns 32 j .. 32 j + 31 of column tile n.  Without ZEROS the 16 and
+// the zero points stay in the sums.
+template <int NT, int R, int G, bool BF16, bool ZEROS, typename X>
 __device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G>& b, X x)
 {
     using T   = Types<BF16>;
@@ -193,7 +196,8 @@ __device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             xv[n] = x(j, n);
-            xs[n] = T::mfma(ones, xv[n], xs[n]);
+            if constexpr (ZEROS)
+                xs[n] = T::mfma(ones, xv[n], xs[n]);
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -212,10 +216,16 @@ __device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float sc = from16((uint16_t)(b.s[r][g][i >> 1] >> (16 * (i & 1))), BF16);
-                    const float zp = (float)((b.z[r][g] >> (8 * i)) & 255u);
+                    if constexpr (ZEROS) {
+                        const float zp = (float)((b.z[r][g] >> (8 * i)) & 255u);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        y[r][n][i] = __builtin_fmaf(__builtin_fmaf(-zp, xs[n][i], acc[r][n][i]), sc, y[r][n][i]);
+                        for (int n = 0; n < NT; ++n)
+                            y[r][n][i] = __builtin_fmaf(__builtin_fmaf(-zp, xs[n][i], acc[r][n][i]), sc, y[r][n][i]);
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            y[r][n][i] = __builtin_fmaf(acc[r][n][i], sc, y[r][n][i]);
+                    }
                 }
         }
     }
@@ -247,7 +257,7 @@ __global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
         vec           x[4];
     } set[2];
     auto fetch = [&](Block& b, int kb) {
-        source.fetch(b.w, kb);
+        source.template fetch<true>(b.w, kb);
 #pragma unroll
         for (int j = 0; j < 4; ++j) { // columns past the end as zeros (K is a multiple of 32)
             const int  k      = kb * kBlockK + 32 * j;
@@ -260,7 +270,7 @@ __global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
         __builtin_amdgcn_sched_barrier(0);
     };
     auto work = [&](const Block& b) {
-        multiply<1, R, G, BF16>(y, b.w, [&](int j, int) { return b.x[j]; });
+        multiply<1, R, G, BF16, true>(y, b.w, [&](int j, int) { return b.x[j]; });
         __builtin_amdgcn_sched_barrier(0);
     };
     const int per = (l.blocks + a.splits - 1) / a.splits, last = min((int)(blockIdx.z + 1) * per, l.blocks);
@@ -303,9 +313,10 @@ __global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
 
 // Many columns.  One workgroup: WAVES waves of R row tiles each and NT column tiles, over a share of K's blocks; the X of a
 // block goes through LDS, once for all waves.  Partial sums of a split K go to `part` [split][column][row].  9216x36864, N = 64,
-// bf16, groups of 64, seven shares: 83 us with the sum of the shares (5), 2.3 TB/s of weights; bound by the SIMDs' issue of
-// vector instructions (53 % of the cycles: unpacking codes, scales into the sums) and matrix products (33 %, a third of them sums of
-// X), which two waves a SIMD do not overlap.  w4_linear, which reads X from the cache for every wave, takes 190 to 240 there.
+// bf16, groups of 64, seven shares: 76.4 us with the sum of the shares (5), 2.5 TB/s of weights.  Without its products the
+// kernel takes 57, without its loads of weights 69, and two waves a SIMD hide the one behind the other only in part; loads two and
+// three blocks ahead, operands a step ahead, vector instructions dealt between the products and XCDs with shares of their own did not help.
+// w4_linear, which reads X from the cache for every wave, takes 190 to 240 there.
 template <int NT, int R, int G, bool BF16, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void w4_linear_wide(LinearArgs a)
 {
@@ -352,37 +363,116 @@ __global__ __launch_bounds__(64 * WAVES, 2) void w4_linear_wide(LinearArgs a)
         for (int q = 0; q < kChunks; ++q)
             slab[buf][xdst[q]] = xr[q];
     };
+    // The 16 and the zero points go off a group's products with the sum of X from a product with ones, of which every wave makes its
+    // own; finer groups than 128 leave them in, and a product in float32 takes them off two blocks at once.  Measured with / without
+    // the latter: 9216x36864, N = 64, groups of 64 76.4 / 83.4 us; groups of 128, 20480x5120, N = 24 23.9 / 22.7, 4096x11008,
+    // N = 48 18.1 / 17.6.
+    constexpr bool kZeros = G == 128;
     Weights<R, G> set[2];
     auto          work = [&](const Weights<R, G>& w, int buf) {
-        multiply<NT, R, G, BF16>(y, w, [&](int j, int n) {
+        multiply<NT, R, G, BF16, kZeros>(y, w, [&](int j, int n) {
             return __builtin_bit_cast(vec, slab[buf][(j * NT + n) * 64 + h * 16 + (c ^ (4 * j + h))]);
         });
     };
+    // A span, two blocks (one with groups of 32), has four sums of X for every column, over 64 (32) columns of W each.  A wave
+    // makes two products' worth of a block's for all; `correct` takes them off, times (16 + z) scale of row c and sum h (exact in
+    // float32), a step after the span, when a barrier has made them everybody's.
+    static_assert(2 * NT == WAVES, "");
+    constexpr int kSums = G == 32 ? 4 : 2, kSpan = 4 / kSums; // sums of a block, blocks of a span
+    __shared__ float sums[2][4][16 * NT];
+    const uint16_t*  coef_s[R];
+    const uint8_t*   coef_z[R];
+    uint16_t         scale[R];
+    uint8_t          zero[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int64_t tile = min(tile0 + r, l.tiles - 1);
+        coef_s[r] = reinterpret_cast<const uint16_t*>(a.packed + l.scales) + tile * l.groups * 16 + c;
+        coef_z[r] = a.packed + l.zeros + (tile * l.blocks * 4 + (c >> 2)) * (kBlockK / G) * 4 + (c & 3);
+        scale[r] = 0, zero[r] = 0;
+    }
+    auto fetch_coef = [&](int kb) {
+        constexpr int kGroups = kBlockK / G;
+        const int     block = min(kb + h / kSums, l.blocks - 1), g = h % kGroups;
+#pragma unroll
+        for (int r = 0; r < R; ++r) { // a group past the end meets zeros of X
+            scale[r] = coef_s[r][min(block * kGroups + g, l.groups - 1) * 16];
+            zero[r]  = coef_z[r][(block * 4 * kGroups + g) * 4];
+        }
+    };
+    auto add_up = [&](int slot, int buf, int block) {
+        const vec ones = __builtin_bit_cast(vec, uintx4{Types<BF16>::kOne, Types<BF16>::kOne, Types<BF16>::kOne, Types<BF16>::kOne});
+        const int n = wave >> 1, j = 2 * (wave & 1);
+        const vec x0 = __builtin_bit_cast(vec, slab[buf][(j * NT + n) * 64 + h * 16 + (c ^ (4 * j + h))]);
+        const vec x1 = __builtin_bit_cast(vec, slab[buf][((j + 1) * NT + n) * 64 + h * 16 + (c ^ (4 * j + 4 + h))]);
+        const floatx4 none{0.f, 0.f, 0.f, 0.f};
+        floatx4       s0 = Types<BF16>::mfma(ones, x0, none);
+        if constexpr (G == 32) {
+            const floatx4 s1 = Types<BF16>::mfma(ones, x1, none);
+            if (h == 0)
+                sums[slot][j][n * 16 + c] = s0[0], sums[slot][j + 1][n * 16 + c] = s1[0];
+        } else {
+            s0 = Types<BF16>::mfma(ones, x1, s0);
+            if (h == 0)
+                sums[slot][2 * block + (wave & 1)][n * 16 + c] = s0[0];
+        }
+    };
+    auto correct = [&](const float (&coef)[R], int slot, int kb) {
+        const int  block = kb + h / kSums;
+        const bool there = block >= first && block < last;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float xs = sums[slot][h][n * 16 + c];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                y[r][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(coef[r], there ? xs : 0.f, y[r][n], 0, 0, 0);
+        }
+    };
+    auto coefs = [&](float (&coef)[R]) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            coef[r] = -(float)zero[r] * from16(scale[r], BF16);
+    };
+    int  kb   = first;
+    auto step = [&](const Weights<R, G>& now, Weights<R, G>& next, int buf) { // block kb is in slab `buf`, X of the next in registers
+        source.template fetch<kZeros>(next, min(kb + 1, last - 1));
+        store_x(buf ^ 1);
+        fetch_x(min(kb + 2, last - 1));
+        const int  at    = kb - first, slot = at / kSpan & 1;
+        const bool start = kSpan == 1 || buf == 0; // of a span
+        float      coef[R];
+        if (!kZeros && start) {
+            coefs(coef); // of the span before, zeros at first
+            fetch_coef(kb);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (!kZeros)
+            add_up(slot, buf, at % kSpan);
+        work(now, buf);
+        if (!kZeros && start)
+            correct(coef, slot ^ 1, kb - kSpan);
+        __syncthreads();
+        ++kb;
+    };
     if (first < last) {
-        int kb = first;
         fetch_x(kb);
-        source.fetch(set[0], kb);
+        source.template fetch<kZeros>(set[0], kb);
         store_x(0);
         fetch_x(min(kb + 1, last - 1));
         __syncthreads();
         while (true) {
-            // block kb is in slab 0 and set 0, X of the next in registers
-            source.fetch(set[1], min(kb + 1, last - 1));
-            store_x(1);
-            fetch_x(min(kb + 2, last - 1));
-            __builtin_amdgcn_sched_barrier(0);
-            work(set[0], 0);
-            __syncthreads();
-            if (++kb >= last)
+            step(set[0], set[1], 0);
+            if (kb >= last)
                 break;
-            source.fetch(set[0], min(kb + 1, last - 1));
-            store_x(0);
-            fetch_x(min(kb + 2, last - 1));
-            __builtin_amdgcn_sched_barrier(0);
-            work(set[1], 1);
-            __syncthreads();
-            if (++kb >= last)
+            step(set[1], set[0], 1);
+            if (kb >= last)
                 break;
+        }
+        if (!kZeros) {
+            const int span = (last - first - 1) / kSpan;
+            float     coef[R];
+            coefs(coef);
+            correct(coef, span & 1, first + span * kSpan);
         }
     }
 #pragma unroll
