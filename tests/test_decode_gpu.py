@@ -463,6 +463,58 @@ def test_cache_operators_refuse_bad_arguments(torch):
     assert S.kv4_gather(c.cache, e2, e1)[0].shape == (0, 2, 64)
 
 
+# Chunks with more than 64 rows for a key/value head in the average sequence run on blocks of 128 rows.
+
+CHUNKS = [(60, 60), (130, 230), (0, 7), (0, 0), (90, 33), (97, 128), (1, 161)]
+
+
+@pytest.mark.parametrize("window", [0, 1, 33, 100])
+@pytest.mark.parametrize("d,hq,hkv", [(64, 4, 1), (96, 6, 2), (128, 8, 2), (256, 4, 1)])
+def test_attention_of_chunks_with_windows_and_empty_rows(torch, window, d, hq, hkv):
+    """Sequences that are empty, shorter than their new tokens, or have none; tokens of no sequence at the end."""
+    c = Case(torch, CHUNKS, hq, hkv, d, 16, "fp16" if window % 2 else "bf16", seed=window + d, tail=3)
+    q, qh = c.queries(1.5)
+    want, mag, lse = c.want(qh, window)
+    got, gl = c.attend(q, window=window, return_lse=True)
+    assert_attention(got, want, mag, c.dtype)
+    assert (host(got)[-3:] == 0).all() and np.isneginf(host(gl)[-3:]).all()
+    assert np.array_equal(np.isneginf(host(gl)[:-3]), np.isneginf(lse[:-3]))
+    live = ~np.isneginf(lse[:-3])
+    assert np.allclose(host(gl)[:-3][live], lse[:-3][live], rtol=1e-5, atol=2e-4)
+    assert_attention(c.attend(q, window=window, max_len=230), want, mag, c.dtype)
+
+
+@pytest.mark.parametrize("stale", [0x7FC00000, 0xFFFFFFFF, 0x7F800000, 0xFF800000, 0x7F7FFFFF])
+def test_attention_of_chunks_does_not_see_hidden_places(torch, stale):
+    """Stale words behind the ends of sequences and in absent pages: a page number outside the cache in the middle, and one past it."""
+    c = Case(torch, [(100, 150), (80, 80), (90, 300)], 4, 2, 128, 16, "fp16", stale=stale)
+    c.table[0, 2], c.table[2, 5], c.table[2, 18] = -1, c.pages + 9, -1
+    c.gt = torch.from_numpy(c.table).cuda()
+    q, qh = c.queries()
+    want, mag, _ = c.want(qh)
+    assert np.isfinite(want).all()
+    assert_attention(c.attend(q), want, mag, "fp16")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_chunks_with_queries_of_every_size(torch, d):
+    """Rows of a block from 2^-14 to 2^6 times the usual, an infinity and a NaN among them."""
+    c = Case(torch, [(100, 300), (96, 97)], 4, 2, d, 32, "bf16", seed=d)
+    size = np.exp2(c.rng.integers(-14, 7, (c.tokens, c.hq, 1)))
+    q, qh = to16(torch, c.rng.standard_normal((c.tokens, c.hq, d)) * size, "bf16")
+    bad = np.zeros((c.tokens, c.hq), bool)
+    bad[5, 1] = bad[150, 2] = True
+    q[5, 1, 7], q[150, 2, d - 1] = float("inf"), float("nan")
+    clean = np.where(bad[..., None], 0, qh)
+    want, mag, _ = c.want(clean)
+    got = host(c.attend(q))
+    assert np.isnan(got[bad]).all()
+    # scores carry float32 errors of their own, 2^-20 of their size, as above
+    top = np.abs(clean).max(-1, keepdims=True) * d ** 0.5 * 5
+    bound = (2.0 ** -11 + 2.0 ** -13 + top * 2.0 ** -20) * mag + 2.0 ** -8 * 1.01 * np.abs(want) + 2.0 ** -25
+    assert (np.abs(got - want)[~bad] <= bound[~bad]).all()
+
+
 # ---- linears ---------------------------------------------------------------------------------------------------------------
 
 def weights(rng, M, K, G, dtype, torch):
