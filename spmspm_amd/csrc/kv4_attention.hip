@@ -714,7 +714,7 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
     float m[RT], l[RT];
     floatx4 o[RT][NV];
     uintx4  qraw[RT][kSteps];
-    float   top = 0.f;
+    float   top = 0.f, row_top[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int  row  = w0 + r * 16 + c;
@@ -728,6 +728,7 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
 #pragma unroll
         for (int d = 0; d < NV; ++d)
             o[r][d] = floatx4{0.f, 0.f, 0.f, 0.f};
+        row_top[r] = 0.f;
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
             qraw[r][j] = *reinterpret_cast<const uintx4*>(src + 8 * j);
@@ -735,12 +736,15 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
             for (int i = 0; i < 8; ++i) {
                 const float mag = fabsf(from16((uint16_t)(qraw[r][j][i >> 1] >> (16 * (i & 1))), a.bf16));
                 if (last[r] >= 0 && mag < 3.4e38f) // rows that see nothing and infinities do not count
-                    top = fmaxf(top, mag);
+                    row_top[r] = fmaxf(row_top[r], mag);
             }
         }
+        row_top[r] = fmaxf(row_top[r], __shfl_xor(row_top[r], 16));
+        row_top[r] = fmaxf(row_top[r], __shfl_xor(row_top[r], 32));
+        top        = fmaxf(top, row_top[r]);
     }
 #pragma unroll
-    for (int x = 1; x < 64; x <<= 1)
+    for (int x = 1; x < 16; x <<= 1)
         top = fmaxf(top, __shfl_xor(top, x));
     if (lane == 0)
         tops[wave] = top;
@@ -748,8 +752,23 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
 #pragma unroll
     for (int w = 0; w < W; ++w)
         top = fmaxf(top, tops[w]);
-    const int   qexp = __builtin_amdgcn_readfirstlane(top > 0.f ? min(13 - (int)__builtin_amdgcn_frexp_expf(top), 110) : 0);
+    auto exponent = [](float x) { return x > 0.f ? min(13 - (int)__builtin_amdgcn_frexp_expf(x), 110) : 0; };
+    const int   qexp = __builtin_amdgcn_readfirstlane(exponent(top));
     const float unit = ldexpf(a.scale_log2, -qexp);
+    // A wave with a row 2^16 below the block's largest (fp16 would lose its bits) scales its rows one by one and corrects the
+    // scores where it also hides keys, so that calls without such rows pay nothing for it.
+    float row_unit[RT];
+    int   row_exp[RT];
+    bool  far = false;
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+        far = far || (row_top[r] > 0.f && exponent(row_top[r]) > qexp + 16);
+    const bool apart = __ballot(far) != 0;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        row_exp[r]  = apart && row_top[r] > 0.f ? exponent(row_top[r]) : qexp;
+        row_unit[r] = ldexpf(1.f, qexp - row_exp[r]);
+    }
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -758,7 +777,7 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int x = kOrder[i];
-                q[r][j][i]  = (_Float16)ldexpf(from16((uint16_t)(qraw[r][j][x >> 1] >> (16 * (x & 1))), a.bf16), qexp);
+                q[r][j][i]  = (_Float16)ldexpf(from16((uint16_t)(qraw[r][j][x >> 1] >> (16 * (x & 1))), a.bf16), row_exp[r]);
             }
         }
 
@@ -766,7 +785,7 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
     auto work = [&](const Slab<D>& b, int tile, unsigned gone) {
         if (tile > w_hi || tile + 63 < w_lo)
             return;
-        const bool edge = (gone & 15u) != 0 || tile < all_lo || tile + 63 > all_hi;
+        const bool edge = (gone & 15u) != 0 || tile < all_lo || tile + 63 > all_hi || apart;
         floatx4    sc[4][RT];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -794,6 +813,17 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
                     sc[k][r][i] = __builtin_fmaf(sc[k][r][i], u[i], ev[i]);
         }
         if (edge) {
+            if (apart) { // (S u + ev - ev) row_unit + ev
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const floatx4 ev = *reinterpret_cast<const floatx4*>(&b.ev[32 * (k >> 1) + 8 * h + 4 * (k & 1)]);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            sc[k][r][i] = __builtin_fmaf(sc[k][r][i] - ev[i], row_unit[r], ev[i]);
+                }
+            }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int  none = -(int)((gone >> (2 * (k >> 1) + (h >> 1))) & 1u);

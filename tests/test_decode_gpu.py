@@ -515,6 +515,23 @@ def test_attention_of_chunks_with_queries_of_every_size(torch, d):
     assert (np.abs(got - want)[~bad] <= bound[~bad]).all()
 
 
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_attention_of_chunks_with_a_query_out_of_all_proportion(torch, d):
+    """Finite queries far above their neighbours in a block of rows: the neighbours' results do not change with them."""
+    c = Case(torch, [(100, 300), (96, 97)], 4, 2, d, 32, "bf16", seed=d)
+    size = np.ones((c.tokens, c.hq, 1))
+    size[3, 0], size[60, 3], size[140, 1], size[150, 0] = 2.0 ** 30, 2.0 ** 100, 2.0 ** 60, 2.0 ** -40
+    q, qh = to16(torch, c.rng.standard_normal((c.tokens, c.hq, d)) * size, "bf16")
+    want, mag, _ = c.want(np.where(size > 1, 0, qh))
+    got = host(c.attend(q))
+    keep = (size <= 1)[..., 0]
+    bound = (2.0 ** -11 + 2.0 ** -13) * mag + 1.01 * UNIT["bf16"] * np.abs(want)
+    assert (np.abs(got - want)[keep] <= bound[keep]).all()
+    # a query that large looks at one key alone
+    top = c.want(np.where(size > 1, qh / size * 2.0 ** 20, 0))[0]
+    assert np.isfinite(got[~keep]).all() and (np.abs(got - top)[~keep] <= (2.0 ** -7 * np.abs(top) + 2.0 ** -9 * np.abs(got).max())[~keep]).all()
+
+
 # ---- linears ---------------------------------------------------------------------------------------------------------------
 
 def weights(rng, M, K, G, dtype, torch):
