@@ -1,4 +1,4 @@
-"""CPU checkers of the decode operators (include/decode_api.h), numpy only, written from the formulas.
+"""CPU oracle of the decode operators (include/decode_api.h), numpy only, written from the formulas.
 
 The cache's encoding is float32 arithmetic rounded operation by operation, so codes and words are compared for equality;
 attention and linears are computed in float64."""
