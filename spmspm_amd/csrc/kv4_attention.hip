@@ -640,9 +640,9 @@ __device__ __forceinline__ void unpack(Slab<D>& slab, const Raw& t, int g, bool 
                 slab.v[g][4 * q + e][lane] = out;
             }
         }
-        if (lane < 32) { // a scale that is no positive number: NaN where it is seen, 0 where it is hidden
+        if (lane < 32) { // a scale that is no normal positive number: NaN where it is seen, 0 where it is hidden
             const float w    = __uint_as_float(t.own);
-            const bool  fine = w > 0.f && w < __builtin_inff();
+            const bool  fine = w >= 0x1p-126f && w < __builtin_inff(); // the quotient of a smaller one is infinite
             slab.ev[32 * g + lane] = fine ? __log2f(w) : __uint_as_float(0x7fc00000u);
             slab.il[32 * g + lane] = fine ? 0x1p-6f / w : 0.f;
         }

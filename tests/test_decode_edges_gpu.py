@@ -1,0 +1,51 @@
+"""Decode operators at the edges of their number ranges, on the GPU against the float64 oracle.
+
+Tolerances are those of test_decode_gpu.py; where a test adds to one, it says what for."""
+import numpy as np
+import pytest
+
+import spmspm_amd as S
+from oracle import decode_oracle as D
+from test_decode_gpu import UNIT, Case, assert_attention, host, to16, torch  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# Sequences of one row each, and of more than 64 rows, run on different kernels; both have the same formula.
+FEW, MANY = [(1, 300), (1, 77), (2, 230)], [(100, 300), (80, 80), (90, 230)]
+
+
+def put_words(c, torch):
+    """The case's words, changed by a test, onto the GPU."""
+    c.cache.k_words.copy_(torch.from_numpy(c.kw.view(np.int32)))
+    c.cache.v_words.copy_(torch.from_numpy(c.vw.view(np.int32)))
+
+
+# ---- words of the cache ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("stale", [0x00000001, 0x00007FFF, 0x007FFFFF, 0x00000000, 0x80000001])
+@pytest.mark.parametrize("seqs,d", [(FEW, 128), (MANY, 64), (MANY, 96), (MANY, 128)])
+def test_attention_does_not_see_small_words_in_hidden_places(torch, seqs, d, stale):
+    """Small integers, as reused memory holds them, are subnormal scales: behind the ends of sequences, in absent pages and
+    outside a window they change nothing."""
+    c = Case(torch, seqs, 4, 2, d, 16, "fp16", seed=d, stale=stale)
+    c.table[0, 2], c.table[2, 5] = -1, c.pages + 9
+    c.gt = torch.from_numpy(c.table).cuda()
+    q, qh = c.queries()
+    for window in (0, 40):
+        want, mag, lse = c.want(qh, window)
+        assert np.isfinite(want).all()
+        got, gl = c.attend(q, window=window, return_lse=True)
+        assert_attention(got, want, mag, "fp16")
+        assert np.allclose(host(gl), lse, rtol=1e-5, atol=2e-4)
+    # every place before a window, with the words of places that are seen kept
+    written = np.zeros((c.pages, 16), bool)
+    for b, (n, L) in enumerate(seqs):
+        for p in range(max(0, L - n - 15), L):
+            if 0 <= c.table[b, p // 16] < c.pages:
+                written[c.table[b, p // 16], p % 16] = True
+    for w in (c.kw, c.vw):
+        w[~np.broadcast_to(written[:, None, :], w.shape)] = np.uint32(stale)
+    put_words(c, torch)
+    want, mag, _ = c.want(qh, 16)
+    assert_attention(c.attend(q, window=16), want, mag, "fp16")
