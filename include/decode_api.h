@@ -20,6 +20,9 @@
  *   becomes 1), z = rint(-lo/s) in 0..15, put into the four lowest bits of s, code = clamp(rint(x/s) + z, 0, 15),
  * in float32 with quotients taken as products with the reciprocal; a vector with an infinite or NaN element is held as
  * NaN throughout, so that it shows in every row that sees it and in no other.
+ * Words that a caller writes: a scale is 0, a positive normal number below 2^127, or NaN.  0, which a cleared cache holds, is a
+ * vector of zeros; attention reads a value scale below 2^-126 as 0.  A row that sees a negative or an infinite scale has no
+ * defined result.  Words of places that no row sees may be anything.
  *
  * A batch.  Sequence b has seq_lens[b] tokens in the cache, its tokens to be processed in this step (n_b of them, the
  * last ones) included; token p of it lies in page block_table[b*table_stride + p/page_size], slot p%page_size.  The

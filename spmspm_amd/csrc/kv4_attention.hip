@@ -165,6 +165,29 @@ struct Rows {
     floatx4 o[RT][Shape<D>::kVal];
 };
 
+// Values whose scale is below the normal numbers, 0 in a cache that nothing was written to, are read as KV4_Append writes a
+// vector of zeros: a scale of 1, codes of 0.  The exponents below are then those of normal numbers.  Seldom and by whole waves.
+constexpr unsigned kLeastWord = 0x00800000u, kOneWord = 0x3f800000u;
+
+template <int D>
+__device__ __forceinline__ void zero_small(Keys<D>& t)
+{
+    unsigned least = t.vw[0][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j)
+        least = min(least, t.vw[j >> 2][j & 3]);
+    if (!__any(least < kLeastWord))
+        return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const bool small = t.vw[j >> 2][j & 3] < kLeastWord;
+        t.vw[j >> 2][j & 3] = small ? kOneWord : t.vw[j >> 2][j & 3];
+#pragma unroll
+        for (int d = 0; d < (Shape<D>::kValBytes + 3) / 4; ++d)
+            t.v[j][d] = small ? 0u : t.v[j][d];
+    }
+}
+
 // Scores, softmax and product with the values for 32 keys.  The loads of the wave's next 32 are issued where the
 // registers that they fill become free: the codes of the keys behind the scores, their words behind the exponents, the
 // values at the end.  `edge`: some key of the tile is hidden from some row; `gone`: the lane's page is not in the cache.
@@ -193,6 +216,7 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
     __builtin_amdgcn_sched_barrier(0);
     load_k();
     __builtin_amdgcn_sched_barrier(0);
+    zero_small<D>(t);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const unsigned kw = t.kw[i >> 2][i & 3], vw = t.vw[i >> 2][i & 3];
@@ -215,11 +239,13 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
     half8 pp[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        const int from = s.first[r] - tile - 8 * h, to = s.last[r] - tile - 8 * h;
+        unsigned seen = 0; // bit i: the row sees key 8 h + i
         if (edge) {
+            const int from = min(max(s.first[r] - tile - 8 * h, 0), 8), to = min(max(s.last[r] + 1 - tile - 8 * h, 0), 8);
+            seen           = gone ? 0u : ((1u << to) - 1) & ~((1u << from) - 1);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (gone || i < from || i > to)
+                if ((seen >> i & 1u) == 0)
                     sc[i >> 2][r][i & 3] = -__builtin_inff();
         }
         float mx = kNone;
@@ -243,9 +269,9 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
         if (edge) { // the words of a hidden key may be anything
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bool hidden = gone || i < from || i > to;
-                s.l[r] += hidden ? 0.f : p[i] * il[i];
-                p[i] = hidden ? 0.f : p[i] * f[i];
+                const bool shown = (seen >> i & 1u) != 0;
+                s.l[r] += shown ? p[i] * il[i] : 0.f;
+                p[i] = shown ? p[i] * f[i] : 0.f;
             }
         } else {
 #pragma unroll
@@ -609,7 +635,7 @@ __device__ __forceinline__ void load_raw(Raw& t, const AttentionArgs& a, int hea
 }
 
 template <int D>
-__device__ __forceinline__ void unpack(Slab<D>& slab, const Raw& t, int g, bool values, float unit, int lane)
+__device__ __forceinline__ void unpack(Slab<D>& slab, Raw& t, int g, bool values, float unit, int lane)
 {
     const unsigned low = in_register(0x000f000fu), up = in_register(0x00f000f0u);
     auto code = [&](unsigned w, bool high, unsigned below, unsigned above) {
@@ -618,6 +644,16 @@ __device__ __forceinline__ void unpack(Slab<D>& slab, const Raw& t, int g, bool 
         return __builtin_bit_cast(unsigned, v);
     };
     if (values) {
+        const unsigned small = (unsigned)__ballot(t.own < kLeastWord); // bit i: key i of the 32; as zero_small
+        if (__builtin_expect(small != 0, 0)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool mine = (small >> (8 * (lane >> 4) + j) & 1u) != 0;
+                t.d[j] = mine ? 0u : t.d[j];
+                t.w[j >> 2][j & 3] = mine ? kOneWord : t.w[j >> 2][j & 3];
+            }
+            t.own = t.own < kLeastWord ? kOneWord : t.own;
+        }
         unsigned below[4], above[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -640,9 +676,9 @@ __device__ __forceinline__ void unpack(Slab<D>& slab, const Raw& t, int g, bool 
                 slab.v[g][4 * q + e][lane] = out;
             }
         }
-        if (lane < 32) { // a scale that is no normal positive number: NaN where it is seen, 0 where it is hidden
+        if (lane < 32) { // a scale that is no positive number: NaN where it is seen, 0 where it is hidden
             const float w    = __uint_as_float(t.own);
-            const bool  fine = w >= 0x1p-126f && w < __builtin_inff(); // the quotient of a smaller one is infinite
+            const bool  fine = w > 0.f && w < __builtin_inff();
             slab.ev[32 * g + lane] = fine ? __log2f(w) : __uint_as_float(0x7fc00000u);
             slab.il[32 * g + lane] = fine ? 0x1p-6f / w : 0.f;
         }

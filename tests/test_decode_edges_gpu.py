@@ -6,7 +6,7 @@ import pytest
 
 import spmspm_amd as S
 from oracle import decode_oracle as D
-from test_decode_gpu import UNIT, Case, assert_attention, host, to16, torch  # noqa: F401
+from test_decode_gpu import SMALLEST, UNIT, Case, assert_attention, host, to16, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,32 @@ def test_attention_does_not_see_small_words_in_hidden_places(torch, seqs, d, sta
     put_words(c, torch)
     want, mag, _ = c.want(qh, 16)
     assert_attention(c.attend(q, window=16), want, mag, "fp16")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("seqs", [FEW, MANY])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_attention_over_scales_of_zero_and_below_the_normal_numbers(torch, d, seqs, dtype):
+    """A word of 0, which a new cache holds, is a vector of zeros for one row and for many; scales below 2^-126 count as 0 in
+    the values, at most 15 2^-126 away."""
+    c = Case(torch, seqs, 4, 2, d, 16, dtype, seed=d)
+    some = c.rng.random(c.vw.shape) < 0.3
+    c.vw[some] = c.rng.choice(np.array([0, 0, 1, 0x7FFF, 0x12345, 0x7FFFFF], np.uint32), int(some.sum()))
+    some = c.rng.random(c.kw.shape) < 0.1
+    c.kw[some] = c.rng.choice(np.array([0, 0x12345], np.uint32), int(some.sum()))
+    put_words(c, torch)
+    q, qh = c.queries()
+    want, mag, lse = c.want(qh)
+    got, gl = c.attend(q, return_lse=True)
+    bound = (2.0 ** -11 + 2.0 ** -13) * mag + 1.01 * UNIT[dtype] * np.abs(want) + max(SMALLEST[dtype], 15 * 2.0 ** -126)
+    assert (np.abs(host(got) - want) <= bound).all()
+    assert np.allclose(host(gl), lse, rtol=1e-5, atol=2e-4)
+    c.vw[:], c.kw[:] = 0, 0
+    put_words(c, torch)
+    _, _, lse = c.want(qh)
+    got, gl = c.attend(q, return_lse=True)
+    assert (host(got) == 0).all()
+    assert np.allclose(host(gl), lse, rtol=1e-5, atol=2e-4)
+    # the read-back of the same places
+    k, v = S.kv4_gather(c.cache, c.gt, c.gl, cu_tokens=c.gcu, total_tokens=c.tokens, dtype=q.dtype)
+    assert (host(k) == 0).all() and (host(v) == 0).all()
