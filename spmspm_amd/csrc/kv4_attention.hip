@@ -252,7 +252,7 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             mx = fmaxf(mx, sc[i >> 2][r][i & 3]);
-        if (__any(mx > s.m[r] + kSlack)) {
+        if (__any(mx - s.m[r] > kSlack)) { // a difference of floats is exact where their sum with 15 rounds to 16
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float m2 = fmaxf(mx - kBelow, s.m[r]), alpha = __builtin_amdgcn_exp2f(s.m[r] - m2);
@@ -881,7 +881,7 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     mx = fmaxf(mx, sc[k][r][i]);
-            if (__any(mx > m[r] + kSlack)) {
+            if (__any(mx - m[r] > kSlack)) { // exact, as in kv4_attention
                 mx = fmaxf(mx, __shfl_xor(mx, 16));
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
                 const float m2 = fmaxf(mx - kBelow, m[r]), alpha = __builtin_amdgcn_exp2f(m[r] - m2);

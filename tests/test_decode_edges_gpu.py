@@ -21,6 +21,12 @@ def put_words(c, torch):
     c.cache.v_words.copy_(torch.from_numpy(c.vw.view(np.int32)))
 
 
+def put_values(c, torch):
+    put_words(c, torch)
+    c.cache.k_codes.copy_(torch.from_numpy(c.kc))
+    c.cache.v_codes.copy_(torch.from_numpy(c.vc))
+
+
 # ---- words of the cache ----------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("stale", [0x00000001, 0x00007FFF, 0x007FFFFF, 0x00000000, 0x80000001])
@@ -78,3 +84,40 @@ def test_attention_over_scales_of_zero_and_below_the_normal_numbers(torch, d, se
     # the read-back of the same places
     k, v = S.kv4_gather(c.cache, c.gt, c.gl, cu_tokens=c.gcu, total_tokens=c.tokens, dtype=q.dtype)
     assert (host(k) == 0).all() and (host(v) == 0).all()
+
+
+# ---- scores ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("many", [False, True])
+def test_attention_of_scores_whose_float32_neighbours_are_far_apart(torch, many):
+    """Scores of 2^24 to 2^29, a few units of float32's last place apart, the larger one later: the reference of the
+    exponentials is a rounded number there, and a probability relative to it must still fit 16 bits.  Key/value heads differ in
+    the values' scale, which moves the rounding."""
+    hkv, d, page = 32, 64, 16
+    seqs, page2 = ([(70, 120)], 4) if many else ([(1, 140)], 8)  # within one split, and one wave
+    for top in (2.0 ** 14, 2.0 ** 15, 1.25 * 2.0 ** 13, 1.75 * 2.0 ** 14):
+        for word in (64.0, 128.0, 200.0, 512.0):
+            c = Case(torch, seqs, hkv, hkv, d, page, "bf16")
+            c.kc[:], c.kw[:] = 0, np.float32(1).view(np.uint32)  # a score of 0
+            first, later = (c.table[0, 0], slice(None), 0), (c.table[0, page2], slice(None), 2)  # places 0, and 66 or 130
+            c.kc[first][:, 0] = 14  # element 0
+            c.kw[first] = np.float32(word).view(np.uint32)
+            c.kc[later][:] = 0x11
+            c.kc[later][:, 0] = 0x1F  # 15 - 1, the others 1 - 1
+            c.kw[later] = np.float32(word).view(np.uint32) + np.uint32(1)
+            for h in range(hkv):  # values' scales just below powers of two
+                c.vw[:, h] = np.float32(2.0 ** (h - 16)).view(np.uint32) - np.uint32(16)
+            put_values(c, torch)
+            q = np.zeros((c.tokens, hkv, d))
+            q[..., 0] = top
+            q, qh = to16(torch, q, "bf16")
+            scale = float(np.log(2.0))
+            _, mag, _ = c.want(qh, scale=scale)
+            got = host(c.attend(q, scale=scale))
+            # between the two values, whichever way the scores were rounded
+            v = D.decode64(c.vc, c.vw)
+            a, b = v[first], v[later]
+            lo, hi = np.minimum(np.minimum(a, b), 0), np.maximum(np.maximum(a, b), 0)
+            room = 1.02 * 2.0 ** -8 * np.maximum(np.abs(lo), np.abs(hi))
+            assert np.isfinite(got).all(), (top, word)
+            assert ((got >= lo - room) & (got <= hi + room)).all(), (top, word)
