@@ -30,7 +30,7 @@ namespace decode {
 
 constexpr int   kTile   = 32;    // keys per step of a wave
 constexpr int   kWaves  = 4;     // waves of a workgroup, each with every fourth tile of the workgroup's keys
-constexpr float kNone   = -1e30f; // m before any key
+constexpr float kNone   = -3.402823466e38f; // m before any key: no score is below it
 // The reference m of the exponentials starts 7 below the first maximum and follows when a score passes it by more than 15:
 // p' stays below 2^15 and uses fp16's range down to 2^-32 of the largest.
 constexpr float kBelow = 7.f, kSlack = 15.f;

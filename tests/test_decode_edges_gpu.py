@@ -121,3 +121,21 @@ def test_attention_of_scores_whose_float32_neighbours_are_far_apart(torch, many)
             room = 1.02 * 2.0 ** -8 * np.maximum(np.abs(lo), np.abs(hi))
             assert np.isfinite(got).all(), (top, word)
             assert ((got >= lo - room) & (got <= hi + room)).all(), (top, word)
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_scores_far_below_zero(torch, d, many):
+    """The only key that a row sees has a score of -2^100: its probability is 1 all the same."""
+    c = Case(torch, [(80, 80)] if many else [(1, 1), (1, 1)], 2, 2, d, 16, "bf16", seed=d)
+    q = np.zeros((c.tokens, 2, d))
+    rows = [0] if many else [0, 1]
+    for i, t in enumerate(rows):
+        k = D.decode64(c.kc, c.kw)[c.table[i, 0], :, 0]
+        q[t] = -k * 2.0 ** 105
+    q, _ = to16(torch, q, "bf16")
+    got, lse = c.attend(q, return_lse=True)
+    for i, t in enumerate(rows):
+        v = D.decode64(c.vc, c.vw)[c.table[i, 0], :, 0]
+        assert (np.abs(host(got)[t] - v) <= (2.0 ** -8 + 2.0 ** -10) * np.abs(v) + 2.0 ** -10 * np.abs(v).max()).all()
+        assert np.isfinite(host(lse)[t]).all() and (host(lse)[t] < -2.0 ** 100).all()
