@@ -159,7 +159,8 @@ template <int D, int RT>
 struct Rows {
     half8  q[RT][Shape<D>::kSteps];
     float  qsum[RT];          // sum of the row's q, in the scores' units
-    float  unit[RT];          // what a score's unit is worth, in powers of two of a probability
+    float  unit[RT];          // what a score's unit is worth, in powers of two of a probability,
+    float  more[RT];          // times this: 1 but for rows with elements from 2^49 on, whose unit would not fit float32
     int    first[RT], last[RT]; // visible keys, last < first where there is none
     float  m[RT], l[RT];
     floatx4 o[RT][Shape<D>::kVal];
@@ -190,9 +191,10 @@ __device__ __forceinline__ void zero_small(Keys<D>& t)
 
 // Scores, softmax and product with the values for 32 keys.  The loads of the wave's next 32 are issued where the
 // registers that they fill become free: the codes of the keys behind the scores, their words behind the exponents, the
-// values at the end.  `edge`: some key of the tile is hidden from some row; `gone`: the lane's page is not in the cache.
+// values at the end.  `edge`: some key of the tile is hidden from some row, or (`large`) some row's `more` is not 1; `gone`: the
+// lane's page is not in the cache.
 template <int D, int RT, typename LoadKeys, typename LoadWords, typename LoadValues>
-__device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool edge, bool gone, int h,
+__device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool edge, bool large, bool gone, int h,
                                      LoadKeys load_k, LoadWords load_kw, LoadValues load_v)
 {
     constexpr unsigned kLow = 0x000f000fu, kHigh = 0x00f000f0u;
@@ -243,6 +245,13 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
         if (edge) {
             const int from = min(max(s.first[r] - tile - 8 * h, 0), 8), to = min(max(s.last[r] + 1 - tile - 8 * h, 0), 8);
             seen           = gone ? 0u : ((1u << to) - 1) & ~((1u << from) - 1);
+            if (large) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float ev = (float)(t.vw[i >> 2][i & 3] >> 23);
+                    sc[i >> 2][r][i & 3] = __builtin_fmaf(sc[i >> 2][r][i & 3] - ev, s.more[r], ev);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if ((seen >> i & 1u) == 0)
@@ -442,6 +451,7 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
     // the block's queries, each row scaled by a power of two that brings its largest element to 2^13: fp16 then holds them
     // exactly down to 2^-27 of that, with a factor 1/16 on those that meet the second nibble of a half
     Rows<D, RT> s;
+    bool        large = false;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int  row  = r * 16 + c;
@@ -479,7 +489,9 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         s.qsum[r] = sum * 0x1p-24f;
-        s.unit[r] = ldexpf(a.scale_log2, 24 - qexp);
+        s.unit[r] = ldexpf(a.scale_log2, min(24 - qexp, 60));
+        s.more[r] = ldexpf(1.f, max(24 - qexp, 60) - 60);
+        large     = large || s.more[r] != 1.f;
         const int place = place0 + tok;
         s.first[r] = live && a.window > 0 ? max(0, place - a.window + 1) : 0;
         s.last[r]  = live && place < cap ? place : -1;
@@ -490,6 +502,7 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
             s.o[r][e] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
 
+    large = __any(large);
     if (any) {
         for (; t < t1; t += kWaves) {
             const int  tile = t * kTile, next = tn * kTile;
@@ -498,7 +511,7 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
             tn = min(tn + kWaves, t1 - 1);
             n0 = entry_at(a, table, tn * kTile), n1 = entry_at(a, table, tn * kTile + 16);
             step<D, RT>(
-                s, keys, tile, !whole, (h < 2 ? p0 : p1) < 0, h,
+                s, keys, tile, !whole || large, large, (h < 2 ? p0 : p1) < 0, h,
                 [&] { load_keys<D>(keys, a, head, next, q0, q1, c, h); },
                 [&] { load_key_words<D>(keys, a, head, next, q0, q1, h); },
                 [&] { load_values<D>(keys, a, head, next, q0, q1, c, h); });
@@ -789,16 +802,18 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
     for (int w = 0; w < W; ++w)
         top = fmaxf(top, tops[w]);
     auto exponent = [](float x) { return x > 0.f ? min(13 - (int)__builtin_amdgcn_frexp_expf(x), 110) : 0; };
-    const int   qexp = __builtin_amdgcn_readfirstlane(exponent(top));
+    // not below -20, elements of 2^33: with the exponent of a row near the type's end the scores of its neighbours, scaled by their
+    // own, would not fit float32 before they are corrected
+    const int   qexp = max(__builtin_amdgcn_readfirstlane(exponent(top)), -20);
     const float unit = ldexpf(a.scale_log2, -qexp);
-    // A wave with a row 2^16 below the block's largest (fp16 would lose its bits) scales its rows one by one and corrects the
-    // scores where it also hides keys, so that calls without such rows pay nothing for it.
+    // A wave with a row 2^16 below the block's largest (fp16 would lose its bits) or above that exponent's range scales its rows one
+    // by one and corrects the scores where it also hides keys, so that calls without such rows pay nothing for it.
     float row_unit[RT];
     int   row_exp[RT];
     bool  far = false;
 #pragma unroll
     for (int r = 0; r < RT; ++r)
-        far = far || (row_top[r] > 0.f && exponent(row_top[r]) > qexp + 16);
+        far = far || (row_top[r] > 0.f && (exponent(row_top[r]) > qexp + 16 || exponent(row_top[r]) < qexp));
     const bool apart = __ballot(far) != 0;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {

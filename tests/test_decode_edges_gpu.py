@@ -139,3 +139,49 @@ def test_attention_of_scores_far_below_zero(torch, d, many):
         v = D.decode64(c.vc, c.vw)[c.table[i, 0], :, 0]
         assert (np.abs(host(got)[t] - v) <= (2.0 ** -8 + 2.0 ** -10) * np.abs(v) + 2.0 ** -10 * np.abs(v).max()).all()
         assert np.isfinite(host(lse)[t]).all() and (host(lse)[t] < -2.0 ** 100).all()
+
+
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("top", [2.0 ** 104, 2.0 ** 118, 3.3895e38])
+def test_attention_of_chunks_with_the_largest_queries(torch, d, top):
+    """One element of a row up to the largest finite bf16: the rows beside it are what they would be without it."""
+    c = Case(torch, [(100, 300), (96, 97)], 4, 2, d, 32, "bf16", seed=d)
+    x = c.rng.standard_normal((c.tokens, c.hq, d))
+    x[150, 0] *= 2.0 ** -40
+    x[151, 0] *= 2.0 ** -100
+    big = np.zeros((c.tokens, c.hq), bool)
+    for t, h, e in ((3, 0, 7), (60, 3, d - 1), (140, 1, 0)):
+        x[t, h, e], big[t, h] = top, True
+    q, qh = to16(torch, x, "bf16")
+    assert np.isfinite(qh).all()
+    want, mag, lse = c.want(np.where(big[..., None], 0, qh))
+    got, gl = c.attend(q, return_lse=True)
+    got, gl = host(got), host(gl)
+    bound = (2.0 ** -11 + 2.0 ** -13) * mag + 1.01 * UNIT["bf16"] * np.abs(want)
+    assert (np.abs(got - want)[~big] <= bound[~big]).all()
+    assert np.allclose(gl[~big], lse[~big], rtol=1e-5, atol=2e-4)
+    if top < 2.0 ** 120:  # the row itself looks at one key alone: its scores fit float32
+        clean = np.where(big[..., None], np.where(np.abs(qh) > 1e9, 2.0 ** 20, 0), 0)
+        one, _, _ = c.want(clean)
+        assert (np.abs(got - one)[big] <= 2.0 ** -7 * np.abs(one[big]) + 2.0 ** -9 * np.abs(one).max()).all()
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("top", [2.0 ** 90, 2.0 ** 104, 2.0 ** 118])
+def test_attention_of_single_tokens_with_the_largest_queries(torch, d, top):
+    """Rows whose scores fit float32 look at one key alone; small rows in the same block stay as they are."""
+    c = Case(torch, [(1, 300), (3, 77), (1, 1)], 4, 2, d, 16, "bf16", seed=d)
+    x = c.rng.standard_normal((c.tokens, c.hq, d))
+    size = np.ones((c.tokens, c.hq, 1))
+    size[0, 1], size[2, 0], size[3, 3], size[4] = top, top, 2.0 ** -60, top
+    q, qh = to16(torch, x * size, "bf16")
+    big = (size > 1)[..., 0]
+    want, mag, lse = c.want(np.where(big[..., None], 0, qh))
+    got, gl = c.attend(q, return_lse=True)
+    got, gl = host(got), host(gl)
+    bound = (2.0 ** -11 + 2.0 ** -13) * mag + 1.01 * UNIT["bf16"] * np.abs(want)
+    assert (np.abs(got - want)[~big] <= bound[~big]).all()
+    assert np.allclose(gl[~big], lse[~big], rtol=1e-5, atol=2e-4)
+    one = c.want(np.where(size > 1, qh / top * 2.0 ** 20, 0))[0]
+    assert (np.abs(got - one)[big] <= 2.0 ** -7 * np.abs(one[big]) + 2.0 ** -9 * np.abs(one).max()).all()
+    assert np.isfinite(gl[big]).all()
