@@ -5,7 +5,8 @@
 // the matrix cores multiply the codes themselves.  A code masked out of its dword in place is as an fp16 number the subnormal
 // k * 2^-24 (k * 2^-20 for the second nibble of a half, whose q is 1/16 of the other's), which v_mfma_f32_16x16x32_f16
 // multiplies as it is: one AND per two codes and a shift per four.  Its sums lose a few bits to that (it aligns by exponent
-// fields): scores were measured within 6e-6 of float64.
+// fields): scores of a few units were measured within 1.7e-5 of float64 (fp16; bf16 8e-6), where kv4_attention_rows, whose operands
+// are normal numbers, is within 9e-7.  The probabilities' rounding to fp16 is 2.4e-4.
 // For the values v - z goes into the product, an exact small integer in fp16: the code is put into the mantissa of 1024 (of
 // 64, where it is the second nibble) and 1024 + z (64 + z) is taken off, two codes at a time.  Their scale goes into the
 // probabilities, p'_t = p_t s_t.  p' must fit fp16 whatever the scales are, so their exponents go into the softmax: with
@@ -189,6 +190,12 @@ __device__ __forceinline__ void zero_small(Keys<D>& t)
     }
 }
 
+// e of a scale f 2^e, f in [1/2, 1).
+__device__ __forceinline__ float exponent_of(unsigned word)
+{
+    return (float)__builtin_amdgcn_frexp_expf(__uint_as_float(word));
+}
+
 // Scores, softmax and product with the values for 32 keys.  The loads of the wave's next 32 are issued where the
 // registers that they fill become free: the codes of the keys behind the scores, their words behind the exponents, the
 // values at the end.  `edge`: some key of the tile is hidden from some row, or (`large`) some row's `more` is not 1; `gone`: the
@@ -222,7 +229,7 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const unsigned kw = t.kw[i >> 2][i & 3], vw = t.vw[i >> 2][i & 3];
-        const float    zk = (float)(kw & 15u), ev = (float)(vw >> 23);
+        const float    zk = (float)(kw & 15u), ev = exponent_of(vw);
 #pragma unroll
         for (int r = 0; r < RT; ++r) // the zero point in the scale's lowest bits is part of it
             sc[i >> 2][r][i & 3] = __builtin_fmaf(__builtin_fmaf(-zk, s.qsum[r], sc[i >> 2][r][i & 3]),
@@ -236,7 +243,7 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
     for (int i = 0; i < 8; ++i) {
         const unsigned vw = t.vw[i >> 2][i & 3];
         f[i]  = __builtin_amdgcn_frexp_mantf(__uint_as_float(vw));
-        il[i] = __uint_as_float(0x7f000000u - (vw & 0x7f800000u)); // 2^(127 - e)
+        il[i] = __uint_as_float(0x7f000000u - (vw & 0x7f800000u)); // 2^(1 - e)
     }
     half8 pp[RT];
 #pragma unroll
@@ -248,7 +255,7 @@ __device__ __forceinline__ void step(Rows<D, RT>& s, Keys<D>& t, int tile, bool 
             if (large) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float ev = (float)(t.vw[i >> 2][i & 3] >> 23);
+                    const float ev = exponent_of(t.vw[i >> 2][i & 3]);
                     sc[i >> 2][r][i & 3] = __builtin_fmaf(sc[i >> 2][r][i & 3] - ev, s.more[r], ev);
                 }
             }
@@ -581,8 +588,8 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
             uintx4 v;
             __builtin_memcpy(&v, e, 16);
             *reinterpret_cast<uintx4*>(a.out + idx * D + d0) = v;
-            if (a.lse != nullptr && d0 == 0) // l is 2^127 times the sum relative to m
-                a.lse[idx] = none ? -__builtin_inff() : (__log2f(l) + (mm - 127.f)) * 0.69314718055994531f;
+            if (a.lse != nullptr && d0 == 0) // l is twice the sum relative to m
+                a.lse[idx] = none ? -__builtin_inff() : (__log2f(l) + (mm - 1.f)) * 0.69314718055994531f;
         }
     }
 }
@@ -969,7 +976,7 @@ __global__ __launch_bounds__(kWave* W, 2) void kv4_attention_rows(AttentionArgs 
                                                                            o[r][d + 2][i] * 0x1p-6f, o[r][d + 3][i] * 0x1p-6f};
             if (h == 0) {
                 float* ml = a.part_ml + ((int64_t)split * a.tokens * a.q_heads + idx) * 2;
-                ml[0] = m[r] + 133.f, ml[1] = l[r]; // as kv4_attention counts, whose sums are 2^127 times theirs
+                ml[0] = m[r] + 7.f, ml[1] = l[r]; // as kv4_attention counts, whose sums are twice theirs, these 2^-6 of them
             }
             continue;
         }
@@ -1056,7 +1063,7 @@ __global__ __launch_bounds__(256) void kv4_attention_join(AttentionArgs a, int l
     __builtin_memcpy(&v, e, 16);
     *reinterpret_cast<uintx4*>(a.out + idx * D + chunk * 8) = v;
     if (a.lse != nullptr && chunk == 0)
-        a.lse[idx] = none ? -__builtin_inff() : (__log2f(l) + (mm - 127.f)) * 0.69314718055994531f;
+        a.lse[idx] = none ? -__builtin_inff() : (__log2f(l) + (mm - 1.f)) * 0.69314718055994531f;
 }
 
 namespace {

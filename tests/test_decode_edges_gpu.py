@@ -185,3 +185,22 @@ def test_attention_of_single_tokens_with_the_largest_queries(torch, d, top):
     one = c.want(np.where(size > 1, qh / top * 2.0 ** 20, 0))[0]
     assert (np.abs(got - one)[big] <= 2.0 ** -7 * np.abs(one[big]) + 2.0 ** -9 * np.abs(one).max()).all()
     assert np.isfinite(gl[big]).all()
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_attention_scores_have_the_bits_of_float32(torch, d, many):
+    """Rows that see one key and whose queries have one element: the log of the sum is the score.  Roundings: three of the score's
+    2^-24, below 1; the score with the values' exponent, below 4; the reference 7 below it, below 8; two of the logarithm's sum."""
+    c = Case(torch, [(70, 70)] * 3 if many else [(1, 5)] * 200, 8, 4, d, 16, "bf16", seed=d)
+    c.vc, c.vw = D.encode((c.rng.uniform(0.5, 1.9, c.vw.shape + (1,)) * c.rng.choice((-7.5, 0, 7.5), c.vw.shape + (d,))).astype(np.float32))
+    c.vc = D.pack(c.vc)
+    put_values(c, torch)
+    q = np.zeros((c.tokens, 8, d))
+    at = c.rng.integers(0, d, (c.tokens, 8, 1))
+    np.put_along_axis(q, at, c.rng.uniform(-0.5, 0.5, at.shape), 2)
+    q, qh = to16(torch, q, "bf16")
+    _, lse = c.attend(q, window=1, return_lse=True)
+    _, _, want = c.want(qh, 1)
+    assert np.abs(want).max() < 0.7
+    assert np.abs(host(lse) - want).max() <= 1.5 * 2.0 ** -20
