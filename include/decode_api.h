@@ -125,7 +125,8 @@ size_t KV4_AttentionWorkspaceBytes(const KV4_Cache* cache, const KV4_Batch* batc
 
 /*
  * Linear with 4-bit weights:  Y[n][m] = act( sum_k X[n][k] * scale[m][k/group] * (code[m][k] - zero[m][k/group]) + bias[m] )
- * sums in float32, one rounding to `dtype` at the end.  W4_Pack lays the weights out for the kernels, once: from
+ * sums in float32, one rounding to `dtype` at the end; infinities and NaN in X give what the formula gives, in their own rows of Y
+ * alone.  W4_Pack lays the weights out for the kernels, once: from
  * codes uint8 [M][K] (values 0..15; higher bits are ignored), scales [M][K/group] in `dtype`, zeros uint8 [M][K/group]
  * (0..15) into `packed`, W4_PackedBytes(M, K, group) bytes, 16-byte aligned.  M is any positive number, group 32, 64 or
  * 128, K a multiple of it.  `dtype` of X, Y and bias is that of the scales.  W4_PackedBytes is 0 for sizes that are

@@ -231,6 +231,79 @@ __device__ __forceinline__ void multiply(floatx4 (&y)[R][NT], const Weights<R, G
     }
 }
 
+// Sums that came out infinite or NaN are computed once more, with w - z itself as the operand: an infinity of X, met by 16 + w, would
+// be taken off again as NaN, and bf16 values near the type's end overflow on the way (here they go in 2^16 times smaller).  Other
+// sums keep their bits.  Bit 4 (r NT + n) + i of a lane: y[r][n][i] is such a sum; a look at the sums where there are none.
+template <int NT, int R>
+__device__ __forceinline__ unsigned infinite_sums(const floatx4 (&y)[R][NT])
+{
+    static_assert(4 * R * NT <= 32, "");
+    float none = 0.f; // NaN with an infinity or a NaN
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                none = __builtin_fmaf(y[r][n][i], 0.f, none);
+    unsigned bad = 0;
+    if (__builtin_expect(__any(none != 0.f), 0)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    bad |= fabsf(y[r][n][i]) < __builtin_inff() ? 0u : 1u << (4 * (r * NT + n) + i);
+    }
+    return bad;
+}
+
+// Rows 4 h .. 4 h + 3 of a tile and column n0 + c over blocks first, first + step .. below last.  By whole waves.
+template <int G, bool BF16>
+__device__ floatx4 sum_again(const LinearArgs& a, const Layout& l, int tile, int n0, int first, int last, int step, int lane)
+{
+    using T   = Types<BF16>;
+    using vec = typename T::vec;
+    constexpr int   kGroups = kBlockK / G, kTurn = BF16 ? 3 : 6;
+    constexpr float kDown = BF16 ? 0x1p-16f : 1.f;
+    const int       c = lane & 15, h = lane >> 4;
+    const int64_t   at = min(tile, l.tiles - 1);
+    const uintx4*   codes = reinterpret_cast<const uintx4*>(a.packed) + at * l.blocks * 64 + lane;
+    const uint16_t* scales = reinterpret_cast<const uint16_t*>(a.packed + l.scales) + at * l.groups * 16 + 4 * h;
+    const uint8_t*  zeros = a.packed + l.zeros + (at * l.blocks * 4 + (c >> 2)) * kGroups * 4 + (c & 3); // of row c
+    const uint16_t* x = a.x + (int64_t)min(n0 + c, a.N - 1) * a.x_stride + 8 * h;
+    floatx4         sum{0.f, 0.f, 0.f, 0.f};
+    for (int kb = first; kb < last; kb += step) {
+        const uintx4 w = codes[(int64_t)kb * 64];
+        for (int j = 0; j < 4; ++j) {
+            const int k = kb * kBlockK + 32 * j, g = 32 * j / G;
+            if (k >= a.K)
+                break;
+            const uintx4 raw = *reinterpret_cast<const uintx4*>(x + k);
+            const float  z   = (float)zeros[(kb * 4 * kGroups + g) * 4] - 16.f;
+            vec          wv, xv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                constexpr int  kNibble[8] = {0, 4, 2, 6, 0, 4, 2, 6};
+                const unsigned dword = j < 2 ? (e < 4 ? w[0] : w[1]) : (e < 4 ? w[2] : w[3]);
+                const unsigned code  = __builtin_amdgcn_alignbit(dword, dword, (4 * (kNibble[e] + (j & 1)) + kTurn) & 31) & 15u;
+                const float    xe    = from16((uint16_t)(raw[e >> 1] >> (16 * (e & 1))), BF16) * kDown;
+                if constexpr (BF16)
+                    wv[e] = (__bf16)((float)code - z), xv[e] = (__bf16)xe;
+                else
+                    wv[e] = (_Float16)((float)code - z), xv[e] = (_Float16)xe;
+            }
+            const floatx4 acc = T::mfma(wv, xv, floatx4{0.f, 0.f, 0.f, 0.f});
+            const uintx2  s   = *reinterpret_cast<const uintx2*>(scales + (kb * kGroups + g) * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sum[i] = __builtin_fmaf(acc[i] * from16((uint16_t)(s[i >> 1] >> (16 * (i & 1))), BF16), 1.f / kDown, sum[i]);
+        }
+    }
+    return sum;
+}
+
 // Few columns.  One workgroup: R row tiles of 16 rows and 16 columns, a share of K's blocks dealt to its waves in turn; the waves'
 // sums are joined through LDS.  G: group size.  Bound by memory where it has one workgroup for every CU: 28672x7168, N = 16,
 // groups of 128, in 24.4 us is 4.3 TB/s of weights (a large copy moves 4.9); 5120x5120, N = 1 takes 7.3, a launch, two
@@ -292,6 +365,16 @@ __global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
 #pragma unroll
     for (int r = 0; r < R; ++r)
         *reinterpret_cast<floatx4*>(&join[wave][(c * R + r) * 16 + 4 * h]) = y[r][0];
+    if (const unsigned bad = infinite_sums<1, R>(y); __builtin_expect(__any(bad != 0), 0)) {
+        for (int r = 0; r < R; ++r) {
+            if (!__any((bad >> (4 * r) & 15u) != 0))
+                continue;
+            const floatx4 sum = sum_again<G, BF16>(a, l, tile0 + r, n0, (int)blockIdx.z * per + wave, last, kWaves, lane);
+            for (int i = 0; i < 4; ++i)
+                if (bad >> (4 * r + i) & 1u)
+                    join[wave][(c * R + r) * 16 + 4 * h + i] = sum[i];
+        }
+    }
     __syncthreads();
     for (int at = threadIdx.x; at < R * 256; at += 64 * kWaves) {
         const int m = tile0 * 16 + at % (R * 16), n = n0 + at / (R * 16);
@@ -475,6 +558,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void w4_linear_wide(LinearArgs a)
             correct(coef, span & 1, first + span * kSpan);
         }
     }
+    const unsigned bad = infinite_sums<NT, R>(y);
+    auto           finish = [&](int col, int m, float sum) {
+        if (a.bias != nullptr)
+            sum += from16(a.bias[m], BF16);
+        a.y[(int64_t)col * a.M + m] = to16(activate(sum, a.act), BF16);
+    };
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int col = n0 + n * 16 + c;
@@ -490,10 +579,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void w4_linear_wide(LinearArgs a)
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (m + i < a.M) {
-                    const float sum = y[r][n][i] + (a.bias != nullptr ? from16(a.bias[m + i], BF16) : 0.f);
-                    a.y[(int64_t)col * a.M + m + i] = to16(activate(sum, a.act), BF16);
-                }
+                if (m + i < a.M)
+                    finish(col, m + i, y[r][n][i]);
+        }
+    }
+    if (__builtin_expect(__any(bad != 0), 0)) {
+        for (int at = 0; at < R * NT; ++at) {
+            const int r = at / NT, n = at % NT, col = n0 + n * 16 + c;
+            if (!__any((bad >> (4 * at) & 15u) != 0))
+                continue;
+            const floatx4 sum = sum_again<G, BF16>(a, l, tile0 + r, n0 + n * 16, first, last, 1, lane);
+            for (int i = 0; i < 4; ++i) {
+                const int m = (tile0 + r) * 16 + 4 * h + i;
+                if ((bad >> (4 * at + i) & 1u) == 0 || col >= a.N || tile0 + r >= l.tiles)
+                    continue;
+                if (a.splits > 1)
+                    a.part[((int64_t)blockIdx.z * a.N + col) * (l.tiles * 16) + m] = sum[i];
+                else if (m < a.M)
+                    finish(col, m, sum[i]);
+            }
         }
     }
 }

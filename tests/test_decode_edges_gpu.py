@@ -204,3 +204,58 @@ def test_attention_scores_have_the_bits_of_float32(torch, d, many):
     _, _, want = c.want(qh, 1)
     assert np.abs(want).max() < 0.7
     assert np.abs(host(lse) - want).max() <= 1.5 * 2.0 ** -20
+
+
+# ---- linears ---------------------------------------------------------------------------------------------------------------
+
+def linear_case(torch, M, K, N, G, dtype, seed=0):
+    rng = np.random.default_rng(seed)
+    codes = rng.integers(0, 16, (M, K)).astype(np.uint8)
+    zeros = rng.integers(0, 16, (M, K // G)).astype(np.uint8)
+    scales, sh = to16(torch, rng.uniform(0.001, 0.01, (M, K // G)) * np.where(rng.random((M, K // G)) < 0.2, -1, 1), dtype)
+    g = lambda a: torch.from_numpy(a).cuda()
+    return rng, codes, sh, zeros, S.W4Linear(g(codes), scales, g(zeros))
+
+
+LINEARS = [(40, 256, 6, 32), (40, 384, 6, 64), (40, 384, 16, 128), (40, 8320, 50, 32), (640, 8192, 64, 64), (33, 16512, 20, 128)]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("M,K,N,G", LINEARS)
+def test_linear_with_infinities_in_x(torch, M, K, N, G, dtype):
+    """An infinity times a weight is one of the weight's sign, and NaN for a weight of zero; a NaN spoils its row.  The rows
+    beside them do not change by a bit."""
+    rng, codes, sh, zeros, layer = linear_case(torch, M, K, N, G, dtype, M + K)
+    x, xh = to16(torch, rng.standard_normal((N, K)), dtype)
+    ref = layer(x)
+    bad = sorted({0, N // 2, N - 1})
+    xh[bad[0], K // 3], xh[bad[1], K - 1] = np.inf, -np.inf
+    xh[bad[2], 5] = np.nan
+    x, xh = to16(torch, xh, dtype)
+    got = layer(x)
+    fine = [n for n in range(N) if n not in bad]
+    assert torch.equal(got[fine], ref[fine])
+    w = np.repeat(sh.astype(np.float64), G, 1) * (codes.astype(np.float64) - np.repeat(zeros, G, 1))
+    with np.errstate(all="ignore"):
+        want = np.stack([(w * xh[n].astype(np.float64)).sum(1) for n in bad])
+    got = host(got[bad])
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isinf(want).any()
+    inf = np.isinf(want)
+    assert np.array_equal(got[inf], want[inf])
+
+
+@pytest.mark.parametrize("M,K,N,G", LINEARS)
+def test_linear_with_the_largest_activations(torch, M, K, N, G):
+    """bf16 rows whose results are finite and whose sums with the codes as they stand are not."""
+    rng, codes, sh, zeros, layer = linear_case(torch, M, K, N, G, "bf16", M + K + 1)
+    x = rng.standard_normal((N, K))
+    x[N - 1] *= 2e37 / np.sqrt(K / 256)
+    x[0] *= 3e36
+    x, xh = to16(torch, x, "bf16")
+    y, small, _ = D.linear(xh, codes, sh, zeros)
+    assert (np.abs(y) < 3.3e38).all()
+    got = host(layer(x))
+    # rounded sums of the products themselves, and of x (16 + w) where those fit: 32 / |w - z| times as large at most
+    big = np.abs(xh.astype(np.float64)) @ (32 * np.repeat(np.abs(sh.astype(np.float64)), G, 1)).T
+    bound = (48 + K // G) * 2.0 ** -24 * big + 1.01 * UNIT["bf16"] * np.abs(y)
+    assert (np.abs(got - y) <= bound).all()
