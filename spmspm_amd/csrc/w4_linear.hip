@@ -644,6 +644,10 @@ struct Plan {
     int splits;       // shares of K
 };
 
+#ifdef SPMM_KEEP_VARIANTS
+Plan g_plan{0, 0, 0};
+#endif
+
 constexpr int kWideTiles = 2; // row tiles of a wave of the wide kernel
 constexpr int kMostShares = 64; // of K, for the wide kernel
 constexpr int wide_waves(int column_tiles) { return column_tiles == 2 ? 4 : 8; }
@@ -664,6 +668,10 @@ constexpr int most_tiles(int group) { return group == 128 ? 7 : (group == 64 ? 5
 // groups of 32 17.2 with 24 shares of two column tiles, 20.8 with 66 of four (24.0); 512x1024 with N = 64 8.6 (4.0).
 Plan plan_of(int M, int N, int K, int group)
 {
+#ifdef SPMM_KEEP_VARIANTS // the tests' build: every kernel at small sizes
+    if (g_plan.splits > 0 && g_plan.row_tiles <= most_tiles(group))
+        return g_plan;
+#endif
     const int64_t tiles = (M + 15) / 16, blocks = (K + kBlockK - 1) / kBlockK;
     auto          up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     Plan          p{1, 0, 1};
@@ -758,6 +766,17 @@ int check_weights(int M, int K, int group, int dtype)
 } // namespace decode
 
 using namespace decode;
+
+#ifdef SPMM_KEEP_VARIANTS
+// Every later call runs as the plan says (see Plan); splits 0: as the library chooses.
+extern "C" int W4_Debug_SetPlan(int row_tiles, int column_tiles, int splits)
+{
+    if (row_tiles < 0 || splits < 0 || splits > kMostShares || (splits > 0 && row_tiles == 0 && column_tiles != 2 && column_tiles != 4))
+        return 1;
+    g_plan = Plan{row_tiles, column_tiles, splits};
+    return 0;
+}
+#endif
 
 extern "C" size_t W4_PackedBytes(int M, int K, int group)
 {

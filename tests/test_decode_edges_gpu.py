@@ -1,11 +1,16 @@
 """Decode operators at the edges of their number ranges, on the GPU against the float64 oracle.
 
 Tolerances are those of test_decode_gpu.py; where a test adds to one, it says what for."""
+import ctypes as C
+import os
+
 import numpy as np
 import pytest
 
 import spmspm_amd as S
 from oracle import decode_oracle as D
+from spmspm_amd import api as A
+from spmspm_amd import decode as M
 from test_decode_gpu import SMALLEST, UNIT, Case, assert_attention, host, to16, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -259,3 +264,79 @@ def test_linear_with_the_largest_activations(torch, M, K, N, G):
     big = np.abs(xh.astype(np.float64)) @ (32 * np.repeat(np.abs(sh.astype(np.float64)), G, 1)).T
     bound = (48 + K // G) * 2.0 ** -24 * big + 1.01 * UNIT["bf16"] * np.abs(y)
     assert (np.abs(got - y) <= bound).all()
+
+
+# Every kernel of the linears at small sizes: the tests' build of the library takes a plan.
+
+@pytest.fixture
+def set_plan(monkeypatch):
+    lib = C.CDLL(os.path.join(os.path.dirname(S.library_path()), "libSpMM_API_variants.so"))
+    monkeypatch.setattr(A, "library", lambda: lib)
+    monkeypatch.setattr(M, "_lib", None)
+    yield lib.W4_Debug_SetPlan
+    lib.W4_Debug_SetPlan(0, 0, 0)
+
+
+def check_linear(torch, M_, N, K, G, dtype, act, splits):
+    """Against float64, an infinity in a row of X and the call's repetition among it."""
+    rng, codes, sh, zeros, _ = linear_case(torch, M_, K, N, G, dtype, K + splits)
+    g = lambda a: torch.from_numpy(a).cuda()
+    bias, bh = to16(torch, rng.standard_normal(M_), dtype)
+    scales, _ = to16(torch, sh, dtype)
+    layer = S.W4Linear(g(codes), scales, g(zeros), bias=bias, activation=act)
+    need = M._library().W4_WorkspaceBytes(M_, N, K, G)
+    assert need == (4 * splits * N * (-(-M_ // 16) * 16) if splits > 1 else 0)
+    x, xh = to16(torch, rng.standard_normal((N, K)), dtype)
+    y, _, big = D.linear(xh, codes, sh, zeros, bh, act)
+    got = layer(x)
+    # sums of x (16 + w) and, taken off, x (16 + z): 36 rounded additions a group at most in the matrix cores and 12 beside them,
+    # one for each group, and the shares' and waves' sums
+    s = np.repeat(np.abs(sh.astype(np.float64)), G, 1)
+    big = big + np.abs(xh.astype(np.float64)) @ (32 * s).T + np.abs(bh)
+    slope = 1.13 if act == 2 else 1.0
+    bound = slope * (48 + K // G + splits) * 2.0 ** -24 * big + (1.01 * UNIT[dtype] + (1e-5 if act == 2 else 0)) * np.abs(y) \
+        + SMALLEST[dtype] + (1e-6 if act == 2 else 0)
+    d = np.abs(host(got) - y)
+    assert (d <= bound).all(), (np.max(d / bound), np.argwhere(d > bound)[:4].tolist())
+    assert torch.equal(got, layer(x))
+    xh[N - 1, K // 2] = np.inf
+    x, xh = to16(torch, xh, dtype)
+    again = layer(x)
+    assert torch.equal(again[:N - 1], got[:N - 1])
+    with np.errstate(all="ignore"):
+        w = np.repeat(sh.astype(np.float64), G, 1) * (codes.astype(np.float64) - np.repeat(zeros, G, 1))
+        y = (w * xh[N - 1].astype(np.float64)).sum(1)
+    want = np.where(np.isnan(y), np.nan, np.where(y > 0, np.inf, 0 if act == 1 else np.nan if act == 2 else -np.inf))
+    assert np.array_equal(host(again[N - 1]), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("G,tiles", [(32, 1), (32, 2), (32, 3), (32, 4), (64, 1), (64, 2), (64, 3), (64, 4), (64, 5), (128, 1), (128, 2),
+                                     (128, 3), (128, 4), (128, 5), (128, 6), (128, 7)])
+def test_linear_of_few_columns_with_every_number_of_row_tiles(torch, set_plan, G, tiles, dtype):
+    """Rows that end inside a tile and inside a workgroup's tiles, blocks of K that end a wave's turn at either set of registers, the
+    last one not whole, and shares of which one is shorter or empty."""
+    for N, blocks, splits, act in ((3, 5, 1, 0), (18, 19, 1, 2), (16, 19, 3, 1), (1, 36, 7, 0), (20, 2, 4, 0)):
+        assert set_plan(tiles, 0, splits) == 0
+        check_linear(torch, 16 * (2 * tiles - 1) - 5, N, 128 * blocks - (G if G < 128 else 0), G, dtype, act, splits)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("tiles", [2, 4])
+def test_linear_of_many_columns_with_every_number_of_column_tiles(torch, set_plan, tiles, G, dtype):
+    """One to eight blocks of K for a workgroup, so that a span of two blocks ends at either; shares of odd numbers of blocks; columns
+    that end inside a workgroup's."""
+    rows = 300
+    for N, blocks, splits, act in ((16 * tiles, 1, 1, 0), (16 * tiles + 5, 2, 1, 1), (17, 7, 1, 2), (16 * tiles - 1, 8, 1, 0),
+                                   (16 * tiles, 9, 3, 0), (16 * tiles + 1, 10, 4, 2), (33, 5, 2, 1), (20, 3, 5, 0)):
+        assert set_plan(0, tiles, splits) == 0
+        check_linear(torch, rows, N, 128 * blocks - (G if G < 128 else 0), G, dtype, act, splits)
+
+
+@pytest.mark.parametrize("M_,N,K,G,dtype", [(512, 16, 32768, 64, "fp16"), (528, 5, 32768, 128, "bf16"), (640, 64, 8192, 64, "bf16"),
+                                            (1024, 33, 8192, 64, "fp16"), (529, 50, 25184, 32, "bf16")])
+def test_linear_with_a_k_that_the_library_splits(torch, M_, N, K, G, dtype):
+    need = M._library().W4_WorkspaceBytes(M_, N, K, G)
+    assert need > 0
+    check_linear(torch, M_, N, K, G, dtype, 1, need // (4 * N * (-(-M_ // 16) * 16)))
