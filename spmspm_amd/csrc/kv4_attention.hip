@@ -1168,6 +1168,11 @@ extern "C" int KV4_Attention(hipStream_t stream, const KV4_Cache* cache, const K
         return refuse("window %d, max_len %d, scale %f", window, max_len, (double)scale);
     if (batch->total_tokens == 0)
         return 0;
+    // one that holds the whole table hides nothing; with the others a token before its sequence's start keeps place - window + 1 within
+    // 32 bits
+    const bool whole = window >= (int64_t)batch->table_width * cache->page_size;
+    if (!whole && window > 0x7fffffff - batch->total_tokens)
+        return refuse("a window of %d with %d tokens", window, batch->total_tokens);
     if (bad_pointer(q.data, 16) || bad_pointer(out, 16) || (lse != nullptr && bad_pointer(lse, 4)) ||
         q.token_stride % 8 != 0 || q.head_stride % 8 != 0)
         return refuse("a null or misaligned q, out or lse (16 bytes, strides multiples of 8 elements)");
@@ -1189,7 +1194,7 @@ extern "C" int KV4_Attention(hipStream_t stream, const KV4_Cache* cache, const K
     a.num_pages = cache->num_pages, a.page_log2 = __builtin_ctz((unsigned)cache->page_size);
     a.kv_heads = cache->kv_heads, a.q_heads = q_heads, a.share = q_heads / cache->kv_heads;
     a.batch = batch->batch, a.width = batch->table_width, a.stride = batch->table_stride, a.tokens = batch->total_tokens;
-    a.window = window, a.splits = p.splits, a.bf16 = dtype == DECODE_BF16;
+    a.window = whole ? 0 : window, a.splits = p.splits, a.bf16 = dtype == DECODE_BF16;
     switch (cache->head_dim) {
     case 64: return run<64>(stream, p, a);
     case 96: return run<96>(stream, p, a);

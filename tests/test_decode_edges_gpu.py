@@ -340,3 +340,18 @@ def test_linear_with_a_k_that_the_library_splits(torch, M_, N, K, G, dtype):
     need = M._library().W4_WorkspaceBytes(M_, N, K, G)
     assert need > 0
     check_linear(torch, M_, N, K, G, dtype, 1, need // (4 * N * (-(-M_ // 16) * 16)))
+
+
+# ---- calls -----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("seqs", [[(5, 3), (40, 33), (1, 20)], [(120, 60), (90, 33), (97, 128)]])
+def test_attention_with_the_widest_window(torch, seqs, d):
+    """The largest int as a window, over tokens that lie before their sequence's start: it hides nothing."""
+    c = Case(torch, seqs, 4, 2, d, 16, "fp16", seed=d)
+    q, qh = c.queries()
+    want, mag, lse = c.want(qh)
+    for window in (2 ** 31 - 1, 2 ** 31 - 60, 1 << 30):
+        got, gl = c.attend(q, window=window, return_lse=True)
+        assert_attention(got, want, mag, "fp16")
+        assert np.array_equal(np.isneginf(host(gl)), np.isneginf(lse))
