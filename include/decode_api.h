@@ -114,7 +114,7 @@ int KV4_Gather(hipStream_t stream, const KV4_Cache* cache, const KV4_Batch* batc
  * natural logarithm of each row's sum of exponentials.  A row that sees no key is 0, its lse -infinity.
  * max_len: an upper bound of seq_lens where the caller knows one, 0 otherwise; it decides how the work is split and
  * nothing else.  `workspace` must hold KV4_AttentionWorkspaceBytes of the same arguments (may be NULL when that is 0),
- * 16-byte aligned; contents irrelevant.  q: rows aligned to 16 bytes (strides multiples of 8 elements).
+ * 16-byte aligned; contents irrelevant.  q: rows aligned to 16 bytes (strides multiples of 8 elements, where they are used).
  * Roundings.  Scores, their maxima and the sums are float32; a score is within 2^-21 of sum_d |q_d| w (code + z) (as measured,
  * with few rows to a sequence; 2^-24 with many).  A probability is rounded to fp16 (11 bits, of either sign) before it is
  * multiplied by the values; the sum of probabilities is not.  out is rounded once. */

@@ -1174,7 +1174,7 @@ extern "C" int KV4_Attention(hipStream_t stream, const KV4_Cache* cache, const K
     if (!whole && window > 0x7fffffff - batch->total_tokens)
         return refuse("a window of %d with %d tokens", window, batch->total_tokens);
     if (bad_pointer(q.data, 16) || bad_pointer(out, 16) || (lse != nullptr && bad_pointer(lse, 4)) ||
-        q.token_stride % 8 != 0 || q.head_stride % 8 != 0)
+        (batch->total_tokens > 1 && q.token_stride % 8 != 0) || (q_heads > 1 && q.head_stride % 8 != 0))
         return refuse("a null or misaligned q, out or lse (16 bytes, strides multiples of 8 elements)");
     const Plan p = plan_of(*cache, *batch, q_heads, window, max_len);
     if (p.blocks * cache->kv_heads > 0x7fffffff || (int64_t)batch->total_tokens * q_heads > 0x7fffffff)

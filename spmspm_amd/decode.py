@@ -157,7 +157,7 @@ class KV4Cache:
 
 def _batch(cache, block_table, seq_lens, cu_tokens, tokens):
     shape, strides = block_table.shape, block_table.stride()
-    if len(shape) != 2 or block_table.dtype != torch.int32 or strides[1] != 1 or seq_lens.dtype != torch.int32 \
+    if len(shape) != 2 or block_table.dtype != torch.int32 or (shape[1] > 1 and strides[1] != 1) or seq_lens.dtype != torch.int32 \
             or not seq_lens.is_contiguous() or seq_lens.shape != shape[:1]:
         raise ValueError("block_table must be int32 [batch][pages], seq_lens int32 [batch]")
     n, device = seq_lens.shape[0], cache.device
@@ -279,7 +279,7 @@ def kv4_attention(q, cache, block_table, seq_lens, cu_tokens=None, scale=None, w
         raise ValueError(f"{heads} query heads over {cache.kv_heads} key/value heads")
     if window < 0 or max_len < 0:
         raise ValueError("window and max_len must not be negative")
-    if tokens and (rows.data % 16 or rows.token_stride % 8 or rows.head_stride % 8):
+    if tokens and (rows.data % 16 or (tokens > 1 and rows.token_stride % 8) or (heads > 1 and rows.head_stride % 8)):
         raise ValueError("q's rows must be aligned to 16 bytes")
     if out is not None:
         _check("out", out, cache.device, q.dtype, (tokens, heads, cache.head_dim))

@@ -355,3 +355,27 @@ def test_attention_with_the_widest_window(torch, seqs, d):
         got, gl = c.attend(q, window=window, return_lse=True)
         assert_attention(got, want, mag, "fp16")
         assert np.array_equal(np.isneginf(host(gl)), np.isneginf(lse))
+
+
+def test_strides_of_dimensions_of_one_do_not_matter(torch):
+    """One token, one head, one page: views whose stride there is any number."""
+    c = Case(torch, [(1, 20)], 4, 2, 64, 32, "fp16")
+    q, _ = c.queries()
+    ref = c.attend(q)
+    buf = torch.zeros(600, dtype=torch.float16, device="cuda")
+    odd = buf.as_strided((1, 4, 64), (333, 64, 1))
+    odd.copy_(q)
+    assert torch.equal(c.attend(odd), ref)
+    table = torch.as_strided(c.gt, (1, 1), (1, 7))
+    assert torch.equal(S.kv4_attention(odd, c.cache, table, c.gl), ref)
+    k, v = S.kv4_gather(c.cache, table, c.gl)
+    c1 = Case(torch, [(1, 20), (1, 9), (1, 32)], 1, 1, 64, 32, "fp16")
+    q, _ = c1.queries()
+    ref = c1.attend(q)
+    one = torch.empty(3 * 64, dtype=torch.float16, device="cuda").as_strided((3, 1, 64), (64, 13, 1))
+    one.copy_(q)
+    assert torch.equal(S.kv4_attention(one, c1.cache, c1.gt.t().contiguous().t(), c1.gl), ref)
+    S.kv4_append(c.cache, odd[:, :2], odd[:, 2:], table, c.gl)
+    back = S.kv4_gather(c.cache, table, c.gl)
+    want = S.kv4_gather(c.cache, c.gt, c.gl)
+    assert torch.equal(back[0], want[0]) and torch.equal(back[1], want[1]) and not torch.equal(back[0], k)
