@@ -67,7 +67,8 @@ struct Keys {
 };
 
 // Codes that one workgroup reads once go past the caches (measured: 3 to 6 % less time, 24 to 96 sequences of 4k to 16k keys);
-// ONCE is false where other blocks of rows read them again.
+// ONCE is false where other blocks of rows read them again, as the average sequence has more than one: 4 x 128 tokens over 16384
+// keys, 32 heads of 256 over 4, 504 us past the caches and 468 through them; 32 x 12 tokens over 8192, 32 heads of 128 over 8, 133 and 128.
 template <bool ONCE, typename T>
 __device__ __forceinline__ T load_as(const uint8_t* p)
 {
@@ -102,7 +103,7 @@ __device__ __forceinline__ int page_of(const AttentionArgs& a, int entry, int po
 }
 
 // Loads of the 32 keys from `tile` on (a multiple of 32); p0 and p1 are the pages of its two halves of 16.
-template <int D>
+template <int D, bool ONCE>
 __device__ __forceinline__ void load_keys(Keys<D>& t, const AttentionArgs& a, int head, int tile, int p0, int p1, int c, int h)
 {
     const int P = 1 << a.page_log2;
@@ -111,8 +112,8 @@ __device__ __forceinline__ void load_keys(Keys<D>& t, const AttentionArgs& a, in
     const int      kp  = max(c < 8 ? p0 : p1, 0);
     const int64_t  kat = (((int64_t)kp * a.kv_heads + head) << a.page_log2) + ((tile + kr) & (P - 1));
     const uint8_t* kc  = a.k_codes + kat * (D / 2) + h * (D / 8);
-    load_dwords<true>(t.k[0], kc);
-    load_dwords<true>(t.k[1], kc + 4 * (D / 2));
+    load_dwords<ONCE>(t.k[0], kc);
+    load_dwords<ONCE>(t.k[1], kc + 4 * (D / 2));
 }
 
 __device__ __forceinline__ int64_t word_index(const AttentionArgs& a, int head, int tile, int p0, int p1, int h)
@@ -128,7 +129,7 @@ __device__ __forceinline__ void load_key_words(Keys<D>& t, const AttentionArgs& 
     t.kw[0] = kw[0], t.kw[1] = kw[1];
 }
 
-template <int D>
+template <int D, bool ONCE>
 __device__ __forceinline__ void load_values(Keys<D>& t, const AttentionArgs& a, int head, int tile, int p0, int p1, int c, int h)
 {
     const int64_t  vat = word_index(a, head, tile, p0, p1, h);
@@ -141,9 +142,9 @@ __device__ __forceinline__ void load_values(Keys<D>& t, const AttentionArgs& a, 
         if constexpr (Shape<D>::kValBytes == 2)
             t.v[j][0] = *reinterpret_cast<const uint16_t*>(vb + j * (D / 2));
         else if constexpr (Shape<D>::kValBytes == 4)
-            t.v[j][0] = load_as<true, unsigned>(vb + j * (D / 2));
+            t.v[j][0] = load_as<ONCE, unsigned>(vb + j * (D / 2));
         else {
-            const uintx2 w = load_as<true, uintx2>(vb + j * (D / 2));
+            const uintx2 w = load_as<ONCE, uintx2>(vb + j * (D / 2));
             t.v[j][0] = w[0], t.v[j][1] = w[1];
         }
     }
@@ -413,7 +414,7 @@ __device__ __forceinline__ void zero_idle(const AttentionArgs& a, int head, int 
     }
 }
 
-template <int D, int RT>
+template <int D, int RT, bool ONCE>
 __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attention(AttentionArgs a)
 {
     constexpr int NV = Shape<D>::kVal, kRows = 16 * RT;
@@ -449,9 +450,9 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
         p1 = page_of(a, entry_at(a, table, t * kTile + 16), t * kTile + 16);
         tn = min(t + kWaves, t1 - 1); // the wave's last tile is loaded once more and not used
         n0 = entry_at(a, table, tn * kTile), n1 = entry_at(a, table, tn * kTile + 16);
-        load_keys<D>(keys, a, head, t * kTile, p0, p1, c, h);
+        load_keys<D, ONCE>(keys, a, head, t * kTile, p0, p1, c, h);
         load_key_words<D>(keys, a, head, t * kTile, p0, p1, h);
-        load_values<D>(keys, a, head, t * kTile, p0, p1, c, h);
+        load_values<D, ONCE>(keys, a, head, t * kTile, p0, p1, c, h);
     }
     __builtin_amdgcn_sched_barrier(0);
 
@@ -519,9 +520,9 @@ __global__ __launch_bounds__(kWave* kWaves, Shape<D>::waves(RT)) void kv4_attent
             n0 = entry_at(a, table, tn * kTile), n1 = entry_at(a, table, tn * kTile + 16);
             step<D, RT>(
                 s, keys, tile, !whole || large, large, (h < 2 ? p0 : p1) < 0, h,
-                [&] { load_keys<D>(keys, a, head, next, q0, q1, c, h); },
+                [&] { load_keys<D, ONCE>(keys, a, head, next, q0, q1, c, h); },
                 [&] { load_key_words<D>(keys, a, head, next, q0, q1, h); },
-                [&] { load_values<D>(keys, a, head, next, q0, q1, c, h); });
+                [&] { load_values<D, ONCE>(keys, a, head, next, q0, q1, c, h); });
             p0 = q0, p1 = q1;
         }
     }
@@ -1070,6 +1071,7 @@ namespace {
 
 struct Plan {
     int     row_tiles, splits; // row tiles of a block; 8: kv4_attention_rows
+    bool    once; // the average sequence has one block of rows
     int64_t blocks;
 };
 
@@ -1090,6 +1092,7 @@ Plan plan_of(const KV4_Cache& c, const KV4_Batch& b, int q_heads, int window, in
     const int64_t rows  = (int64_t)b.total_tokens * share, each = (rows + b.batch - 1) / b.batch;
     p.row_tiles = each <= 16 || c.head_dim == 256 ? 1 : (each <= kManyRows ? 2 : 8);
     const int64_t per = 16 * p.row_tiles;
+    p.once            = each <= per;
     p.blocks          = (b.cu_tokens == nullptr ? b.batch * ((share + per - 1) / per) : rows / per + b.batch);
     const int64_t capacity = (int64_t)b.table_width * c.page_size;
     int64_t       len      = max_len > 0 ? std::min<int64_t>(max_len, capacity) : capacity;
@@ -1124,9 +1127,10 @@ int run(hipStream_t stream, const Plan& p, const AttentionArgs& a)
     const dim3 grid((unsigned)p.blocks * a.kv_heads, (unsigned)p.splits, 1), block(kWave * kWaves, 1, 1);
     int        err;
     if (p.row_tiles == 1)
-        err = launch(kv4_attention<D, 1>, grid, block, stream, a);
+        err = launch(p.once ? kv4_attention<D, 1, true> : kv4_attention<D, 1, false>, grid, block, stream, a);
     else if constexpr (D < 256)
-        err = launch(p.row_tiles == 2 ? kv4_attention<D, 2> : kv4_attention_rows<D, 4>, grid, block, stream, a);
+        err = launch(p.row_tiles == 8 ? kv4_attention_rows<D, 4> : (p.once ? kv4_attention<D, 2, true> : kv4_attention<D, 2, false>),
+                     grid, block, stream, a);
     else
         return (int)hipErrorInvalidValue; // plan_of gives heads of 256 one row tile: two would not fit the registers
     if (err != 0 || p.splits == 1)
