@@ -109,12 +109,22 @@ def _check(name, t, device, dtype, shape):
         raise ValueError(f"{name} is on {t.device}, the cache or weight on {device}")
 
 
+def _check_sizes(pages, size, heads, head_dim):
+    if head_dim not in (64, 96, 128, 256):
+        raise ValueError(f"head_dim {head_dim} is not 64, 96, 128 or 256")
+    if size < 16 or size > 1024 or size & (size - 1):
+        raise ValueError(f"page_size {size} is not a power of two from 16 to 1024")
+    if pages < 1 or pages >= 1 << 31 or heads < 1 or heads > 4096:
+        raise ValueError(f"a cache of {pages} pages and {heads} heads (1 to 2^31 - 1, 1 to 4096)")
+
+
 class KV4Cache:
     """A paged key/value cache of one layer in 4 bits (format: include/decode_api.h): `k_codes`, `v_codes` uint8
     [num_pages][kv_heads][page_size][head_dim/2] and `k_words`, `v_words` int32 [num_pages][kv_heads][page_size], which may
     be copied, saved and moved page by page like any tensors."""
 
     def __init__(self, num_pages, page_size, kv_heads, head_dim, device="cuda:0"):
+        _check_sizes(num_pages, page_size, kv_heads, head_dim)  # before anything is allocated
         device = torch.device(device)
         codes = (num_pages, kv_heads, page_size, head_dim // 2)
         self._adopt(torch.zeros(codes, dtype=torch.uint8, device=device),
@@ -133,12 +143,7 @@ class KV4Cache:
         if k_codes.dim() != 4 or k_codes.device.type != "cuda":
             raise ValueError("k_codes must be [num_pages][kv_heads][page_size][head_dim/2] on the GPU")
         pages, heads, size, half = k_codes.shape
-        if 2 * half not in (64, 96, 128, 256):
-            raise ValueError(f"head_dim {2 * half} is not 64, 96, 128 or 256")
-        if size < 16 or size > 1024 or size & (size - 1):
-            raise ValueError(f"page_size {size} is not a power of two from 16 to 1024")
-        if pages < 1 or heads < 1:
-            raise ValueError("a cache needs a page and a head")
+        _check_sizes(pages, size, heads, 2 * half)
         device = k_codes.device
         for name, t, dtype, shape in (("k_codes", k_codes, torch.uint8, k_codes.shape),
                                       ("v_codes", v_codes, torch.uint8, k_codes.shape),

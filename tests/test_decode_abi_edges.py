@@ -1,4 +1,7 @@
 """More refusals of the decode operators' C ABI, on a machine without a GPU."""
+import pytest
+
+import spmspm_amd as S
 from spmspm_amd import decode as M
 from test_decode_abi import X, attend, batch, cache
 
@@ -10,3 +13,11 @@ def test_a_window_whose_arithmetic_would_leave_32_bits_is_refused(capfd):
     need = M._library().KV4_AttentionWorkspaceBytes(c, b, 4, 0x7ffffb00, 0)
     assert attend(c=c, b=b, window=0x7ffffb00, ws=X, ws_bytes=need) == 1
     assert "a window of" in capfd.readouterr().out
+
+
+def test_a_cache_of_sizes_that_are_not_supported_is_refused_before_it_is_allocated():
+    """An odd head dimension is not the even one below it."""
+    for args in ((4, 16, 2, 65), (4, 16, 2, 97), (4, 16, 2, 129), (4, 16, 2, 257), (4, 16, 2, 80), (4, 24, 2, 64), (4, 8, 2, 64),
+                 (4, 2048, 2, 64), (0, 16, 2, 64), (1 << 31, 16, 2, 64), (4, 16, 0, 64), (4, 16, 4097, 64)):
+        with pytest.raises(ValueError):
+            S.KV4Cache(*args)
