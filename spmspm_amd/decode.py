@@ -178,6 +178,8 @@ def _batch(cache, block_table, seq_lens, cu_tokens, tokens):
             raise ValueError("cu_tokens must be int32 [batch + 1] on the cache's device")
         cu = cu_tokens.data_ptr()
     width = shape[1]
+    if tokens >= 1 << 31 or (n > 1 and strides[0] >= 1 << 31):
+        raise ValueError(f"{tokens} tokens, a block table of stride {strides[0]}: more than 32 bits hold")
     return _Batch(block_table.data_ptr(), seq_lens.data_ptr(), cu, n, width, strides[0] if n > 1 else max(width, 1), tokens)
 
 
@@ -284,6 +286,7 @@ def kv4_attention(q, cache, block_table, seq_lens, cu_tokens=None, scale=None, w
         raise ValueError(f"{heads} query heads over {cache.kv_heads} key/value heads")
     if window < 0 or max_len < 0:
         raise ValueError("window and max_len must not be negative")
+    window, max_len = min(window, 0x7fffffff), min(max_len, 0x7fffffff)  # what a sequence can hold; ctypes would cut the bits off
     if tokens and (rows.data % 16 or (tokens > 1 and rows.token_stride % 8) or (heads > 1 and rows.head_stride % 8)):
         raise ValueError("q's rows must be aligned to 16 bytes")
     if out is not None:

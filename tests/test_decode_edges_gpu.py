@@ -379,3 +379,15 @@ def test_strides_of_dimensions_of_one_do_not_matter(torch):
     back = S.kv4_gather(c.cache, table, c.gl)
     want = S.kv4_gather(c.cache, c.gt, c.gl)
     assert torch.equal(back[0], want[0]) and torch.equal(back[1], want[1]) and not torch.equal(back[0], k)
+
+
+def test_attention_takes_any_int_as_a_window_and_a_bound(torch):
+    """Numbers past 32 bits hide nothing and bound nothing; they are not cut off to their lowest bits."""
+    c = Case(torch, [(1, 77), (2, 30)], 4, 2, 64, 16, "fp16")
+    q, _ = c.queries()
+    ref = c.attend(q)
+    for many in (2 ** 31, 2 ** 32 + 5, 2 ** 40 + 1, 2 ** 63 - 1):
+        assert torch.equal(c.attend(q, window=many), ref)
+        assert torch.equal(c.attend(q, max_len=many), ref)
+    with pytest.raises(ValueError):
+        S.kv4_gather(c.cache, c.gt, c.gl, cu_tokens=c.gcu, total_tokens=2 ** 32 + 3)
