@@ -129,7 +129,7 @@ size_t KV4_AttentionWorkspaceBytes(const KV4_Cache* cache, const KV4_Batch* batc
  * alone.  W4_Pack lays the weights out for the kernels, once: from
  * codes uint8 [M][K] (values 0..15; higher bits are ignored), scales [M][K/group] in `dtype`, zeros uint8 [M][K/group]
  * (0..15) into `packed`, W4_PackedBytes(M, K, group) bytes, 16-byte aligned.  M is any positive number, group 32, 64 or
- * 128, K a multiple of it.  `dtype` of X, Y and bias is that of the scales.  W4_PackedBytes is 0 for sizes that are
+ * 128, K a multiple of it, at most 2^30.  `dtype` of X, Y and bias is that of the scales.  W4_PackedBytes is 0 for sizes that are
  * refused.
  * X: rows of K elements, x_stride elements apart (a multiple of 8, at least K), 16-byte aligned; Y contiguous [N][M].
  * `activation`: 0 none, 1 ReLU, 2 GELU (tanh form), as in spmm_api.h.  N from 0 to 16 * 65535.  `workspace` must hold

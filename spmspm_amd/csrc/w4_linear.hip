@@ -14,6 +14,7 @@ namespace decode {
 constexpr int kBlockK     = 128;        // columns of W in a block: 16 rows x 128 columns, 16 bytes a lane
 constexpr int kWaves      = 8;          // waves of a workgroup of w4_linear
 constexpr int kMaxColumns = 16 * 65535; // column tiles are the y dimension of the grid
+constexpr int kMaxK       = 1 << 30;    // column numbers of the last block, and of those fetched behind it, are ints
 
 // Packed weights: codes [row tile of 16][block of 128 columns][lane][4 dwords], scales [row tile][group][16 rows] in 16
 // bits, zero points plus 16 [row tile][block][h][group of the block][rows 4 h .. 4 h + 3] in 8.  Lane r + 16 h of a block holds, of row r, for each half p of 64 columns
@@ -755,8 +756,8 @@ int check_weights(int M, int K, int group, int dtype)
 {
     if (group != 32 && group != 64 && group != 128)
         return refuse("a group of %d columns: 32, 64 or 128", group);
-    if (M < 1 || M > 16 * 65535 || K < group || K % group != 0)
-        return refuse("weights of %d rows (at most 16 * 65535) and %d columns (a multiple of %d)", M, K, group);
+    if (M < 1 || M > 16 * 65535 || K < group || K > kMaxK || K % group != 0)
+        return refuse("weights of %d rows (at most 16 * 65535) and %d columns (a multiple of %d, at most 2^30)", M, K, group);
     if (dtype != DECODE_FP16 && dtype != DECODE_BF16)
         return refuse("unknown element type %d", dtype);
     return 0;
@@ -780,7 +781,7 @@ extern "C" int W4_Debug_SetPlan(int row_tiles, int column_tiles, int splits)
 
 extern "C" size_t W4_PackedBytes(int M, int K, int group)
 {
-    if ((group != 32 && group != 64 && group != 128) || M < 1 || M > 16 * 65535 || K < group || K % group != 0)
+    if ((group != 32 && group != 64 && group != 128) || M < 1 || M > 16 * 65535 || K < group || K > kMaxK || K % group != 0)
         return 0;
     return (size_t)layout_of(M, K, group).bytes;
 }

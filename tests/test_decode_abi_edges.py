@@ -21,3 +21,13 @@ def test_a_cache_of_sizes_that_are_not_supported_is_refused_before_it_is_allocat
                  (4, 2048, 2, 64), (0, 16, 2, 64), (1 << 31, 16, 2, 64), (4, 16, 0, 64), (4, 16, 4097, 64)):
         with pytest.raises(ValueError):
             S.KV4Cache(*args)
+
+
+def test_a_k_whose_last_block_would_end_past_32_bits_is_refused(capfd):
+    L = M._library()
+    for K, group in ((2 ** 31 - 32, 32), (2 ** 31 - 64, 64), (2 ** 31 - 128, 128), (2 ** 30 + 128, 128)):
+        assert L.W4_PackedBytes(16, K, group) == 0 and L.W4_WorkspaceBytes(16, 1, K, group) == 0
+        assert L.W4_Pack(None, X, X, X, 16, K, group, 0, X) == 1
+        assert L.W4_Linear(None, X, X, K, X, 16, 1, K, group, None, 0, None, 0, 0) == 1
+    assert L.W4_PackedBytes(16, 2 ** 30, 32) == 2 ** 30 * 8 + 2 ** 25 * 32 + 2 ** 23 * 64
+    # codes 8 bytes a column, scales 32 and zero points 16 a group
