@@ -319,8 +319,10 @@ def quantize_w4(weight, group=128, dtype=None):
         raise ValueError(f"K = {K} is not a multiple of the group {group}")
     w = weight.float().view(M, K // group, group)
     hi, lo = w.amax(-1).clamp_min(0), w.amin(-1).clamp_max(0)
-    scales = ((hi - lo) / 15).to(dtype)
-    scales = torch.where(scales > 0, scales, torch.ones_like(scales))  # a group of zeros, or one too small for the type
+    scales, info = (hi - lo) / 15, torch.finfo(dtype)
+    last = info.smallest_normal * info.eps  # subnormal scales have few bits: rounded up, or codes would not reach the group's ends
+    scales = torch.where(scales < info.smallest_normal, torch.ceil(scales / last) * last, scales).clamp(max=info.max).to(dtype)
+    scales = torch.where(scales > 0, scales, torch.ones_like(scales))  # a group of zeros
     zeros = torch.round(-lo / scales.float()).clamp(0, 15)
     codes = (torch.round(w / scales.float()[..., None]) + zeros[..., None]).clamp(0, 15)
     return codes.to(torch.uint8).view(M, K), scales, zeros.to(torch.uint8)

@@ -31,3 +31,20 @@ def test_a_k_whose_last_block_would_end_past_32_bits_is_refused(capfd):
         assert L.W4_Linear(None, X, X, K, X, 16, 1, K, group, None, 0, None, 0, 0) == 1
     assert L.W4_PackedBytes(16, 2 ** 30, 32) == 2 ** 30 * 8 + 2 ** 25 * 32 + 2 ** 23 * 64
     # codes 8 bytes a column, scales 32 and zero points 16 a group
+
+
+def test_quantize_w4_of_ranges_at_the_ends_of_the_scale_s_type():
+    """Scales among fp16's subnormal numbers are rounded up, so that codes reach the group's ends; those past its largest one are it."""
+    import torch
+    torch.manual_seed(0)
+    w = torch.randn(64, 128) * torch.logspace(-9, -3, 64)[:, None]
+    codes, scales, zeros = S.quantize_w4(w, 128, torch.float16)
+    back = (codes.double() - zeros.double()) * scales.double()
+    step = scales.double()
+    # half a step, half of one where the zero point's rounding cuts an end off, and the scale's own rounding
+    assert ((back - w.double()).abs() <= 1.01 * step).all()
+    w = torch.randn(8, 128) * 2e6
+    codes, scales, zeros = S.quantize_w4(w, 128, torch.float16)
+    assert torch.isfinite(scales).all()
+    back = (codes.double() - zeros.double()) * scales.double()
+    assert (back.sign() * w.double().sign() >= 0).all() and (back.abs().amax(1) >= 65504).all()
