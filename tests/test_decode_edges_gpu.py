@@ -391,3 +391,65 @@ def test_attention_takes_any_int_as_a_window_and_a_bound(torch):
         assert torch.equal(c.attend(q, max_len=many), ref)
     with pytest.raises(ValueError):
         S.kv4_gather(c.cache, c.gt, c.gl, cu_tokens=c.gcu, total_tokens=2 ** 32 + 3)
+
+
+# ---- work that is dealt in other ways at larger sizes ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("hq,hkv,seqs,window", [(8, 2, [(1, 2100), (1, 700), (1, 1)], 0), (8, 1, [(3, 1500), (1, 40)], 0),
+                                                (6, 2, [(9, 1300), (6, 33), (3, 2)], 1100), (8, 2, [(11, 1800), (13, 64)], 0),
+                                                (4, 2, [(60, 1500), (20, 20)], 0), (4, 1, [(30, 1200), (5, 9)], 1100)])
+def test_attention_with_keys_split_among_workgroups(torch, hq, hkv, seqs, window, d, dtype):
+    """Every kernel with more than one share of the keys, some of them empty; rows of no sequence at the end."""
+    tail = 2 if sum(n for n, _ in seqs) > len(seqs) else 0
+    c = Case(torch, seqs, hq, hkv, d, 16, dtype, seed=d + hq, tail=tail, width=1300)
+    need = M._library().KV4_AttentionWorkspaceBytes(c.cache._desc, M._batch(c.cache, c.gt, c.gl, c.gcu, c.tokens), hq, window, 0)
+    splits = need // (4 * c.tokens * hq * (d + 2))
+    assert splits > 1 and need == 4 * c.tokens * hq * (d + 2) * splits
+    q, qh = c.queries(1.5)
+    want, mag, lse = c.want(qh, window)
+    got, gl = c.attend(q, window=window, return_lse=True)
+    assert_attention(got, want, mag, dtype)
+    live = np.isfinite(lse)
+    assert np.array_equal(np.isneginf(host(gl)), ~live) and np.allclose(host(gl)[live], lse[live], rtol=1e-5, atol=2e-4)
+    assert torch.equal(got, c.attend(q, window=window))
+
+
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("d,rot,interleaved", [(64, 64, False), (64, 20, False), (96, 96, True), (128, 64, False), (128, 10, True),
+                                               (256, 256, False), (128, 0, False)])
+def test_append_and_gather_of_long_prompts(torch, d, rot, interleaved, odd):
+    """So many tokens that a group of lanes takes several of a token's vectors, the next one's loads ahead of the present one's work;
+    rows at odd addresses are read element by element."""
+    hq, hkv, page, dtype = (24 if rot else 0), 8, 32, "bf16" if odd else "fp16"
+    lens, rng = [5003, 2999], np.random.default_rng(d + rot)
+    T, heads = sum(lens), hq + 2 * hkv
+    groups = {64: 32, 96: 16, 128: 16, 256: 8}[d]
+    assert heads * -(-T // groups) // 2048 >= 2 and 2 * hkv * -(-T // groups) // 2048 >= 1
+    flat, fh = to16(torch, rng.standard_normal(T * heads * d + 1), dtype)
+    rows, h = flat[odd:T * heads * d + odd].view(T, heads, d), fh[odd:T * heads * d + odd].reshape(T, heads, d)
+    counts = [-(-n // page) for n in lens]
+    order = rng.permutation(sum(counts) + 2).astype(np.int32)
+    table = np.full((2, max(counts)), -1, np.int32)
+    table[0, :counts[0]], table[1, :counts[1]] = order[:counts[0]], order[counts[0]:sum(counts)]
+    g = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    cache = S.KV4Cache(len(order), page, hkv, d)
+    batch = (g(table), g(np.array(lens, np.int32)), g(np.array([0, lens[0], T], np.int32)))
+    turn = rng.uniform(-1, 1, (max(lens), rot)).astype(np.float32)
+    q = S.kv4_append(cache, rows[:, hq:hq + hkv], rows[:, hq + hkv:], *batch, q=rows[:, :hq] if rot else None,
+                     rotation=g(turn) if rot else None, interleaved=interleaved)
+    place = np.concatenate([np.arange(n) for n in lens])
+    pages, slot = table[np.repeat([0, 1], lens), place // page], place % page
+    k = h[:, hq:hq + hkv]
+    if rot:
+        k = D.rotate(k, turn, place, interleaved)
+        want = D.rotate(h[:, :hq], turn, place, interleaved)
+        assert torch.equal(q.cpu(), torch.from_numpy(want).to(q.dtype))
+    back = S.kv4_gather(cache, *batch, total_tokens=T, dtype=rows.dtype)
+    for x, codes, words, read in ((k, cache.k_codes, cache.k_words, back[0]), (h[:, hq + hkv:], cache.v_codes, cache.v_words, back[1])):
+        wc, ww = D.encode(x)
+        wc = D.pack(wc)
+        assert np.array_equal(codes.cpu().numpy()[pages, :, slot], wc)
+        assert np.array_equal(words.cpu().numpy().view(np.uint32)[pages, :, slot], ww)
+        assert torch.equal(read.cpu(), torch.from_numpy(D.decode32(wc, ww)).to(read.dtype))
