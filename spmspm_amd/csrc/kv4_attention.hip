@@ -21,8 +21,8 @@
 // loads 4 bytes of each of its 8 keys and pairs their halves (v_perm); LDS is not used until the waves' results are joined.
 //
 // Bounds.  Few rows: memory.  32 sequences of up to 16384 keys, 64 heads over 8, D = 128: 103 us, 4.6 TB/s (a large copy moves
-// 4.9); 16 of up to 2048 keys, 40 heads of their own: 36.8 us, 3.6 TB/s, the longest of one round of workgroups; 131071 keys of
-// one sequence, 32 heads over 8: 31 us and 5.5 for the join.
+// 4.9); 16 of up to 2048 keys, 40 heads of their own: 36.3 us, 3.6 TB/s, the longest of one round of workgroups; 131071 keys of
+// one sequence, 32 heads over 8: 32 us and 5.5 for the join.
 #include "decode_common.hiph"
 
 #include <algorithm>

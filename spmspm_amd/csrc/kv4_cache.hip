@@ -96,8 +96,8 @@ __device__ __forceinline__ float element(const uintx4& v, int i, bool bf16)
 // and takes `per` of its vectors one after the other: keys, values, then queries.  A vector is read once, rotated and encoded
 // in registers (its extremes pass between the group's lanes) and written as one dword of codes per lane.  Tokens in a row lie
 // side by side in a page, so that a workgroup writes whole lines of codes and words; with a workgroup for each token, codes
-// and above all single words went to memory as parts of lines (12k tokens, 8 key/value and 32 query heads of 128: 105 us;
-// 80 now, 3.4 TB/s of reads and writes mixed).  The lane's part of the rotation's row is read once for all of the token's vectors.
+// and above all single words went to memory as parts of lines (14247 tokens, 8 key/value and 32 query heads of 128, 307 MB:
+// 105 us; 80 now, 3.8 TB/s of reads and writes mixed).  The lane's part of the rotation's row is read once for all of the token's vectors.
 template <int L>
 __global__ __launch_bounds__(256) void kv4_append(AppendArgs a, int heads, int per)
 {
@@ -259,7 +259,7 @@ struct GatherArgs {
 };
 
 // As kv4_append deals tokens: a lane reads one dword of codes and writes the 8 elements that it holds.  Bound by its writes:
-// 12k tokens, 8 key/value heads of 128, 61 MB in 20 us; a few tokens take 2.4 us, a launch.
+// 14247 tokens, 8 key/value heads of 128, 74 MB in 20 us, 3.7 TB/s; a few tokens take 2.7 us, a launch.
 template <int L>
 __global__ __launch_bounds__(256) void kv4_gather(GatherArgs a, int per)
 {

@@ -307,7 +307,7 @@ __device__ floatx4 sum_again(const LinearArgs& a, const Layout& l, int tile, int
 
 // Few columns.  One workgroup: R row tiles of 16 rows and 16 columns, a share of K's blocks dealt to its waves in turn; the waves'
 // sums are joined through LDS.  G: group size.  Bound by memory where it has one workgroup for every CU: 28672x7168, N = 16,
-// groups of 128, in 24.4 us is 4.3 TB/s of weights (a large copy moves 4.9); 5120x5120, N = 1 takes 7.3, a launch, two
+// groups of 128, in 24.6 us is 4.3 TB/s of weights (a large copy moves 4.9); 5120x5120, N = 1 takes 7.4, a launch, two
 // rounds of loads and the join, where its bytes are 2.8.  What it took: two sets of registers, so that no
 // wait for X includes the weights behind it; X from the cache as rarely as the registers allow (R tiles per read of it).
 template <int R, int G, bool BF16>
@@ -397,8 +397,8 @@ __global__ __launch_bounds__(64 * kWaves) void w4_linear(LinearArgs a)
 
 // Many columns.  One workgroup: WAVES waves of R row tiles each and NT column tiles, over a share of K's blocks; the X of a
 // block goes through LDS, once for all waves.  Partial sums of a split K go to `part` [split][column][row].  9216x36864, N = 64,
-// bf16, groups of 64, seven shares: 76.4 us with the sum of the shares (5), 2.5 TB/s of weights.  Without its products the
-// kernel takes 57, without its loads of weights 69, and two waves a SIMD hide the one behind the other only in part; loads two and
+// bf16, groups of 64, seven shares: 76.9 us with the sum of the shares (5), 2.4 TB/s of weights.  Without its products the
+// kernel takes 57, without its loads of weights 69 (of 76.4), and two waves a SIMD hide the one behind the other only in part; loads two and
 // three blocks ahead, operands a step ahead, vector instructions dealt between the products and XCDs with shares of their own did not help.
 // w4_linear, which reads X from the cache for every wave, takes 190 to 240 there.
 template <int NT, int R, int G, bool BF16, int WAVES>
@@ -657,8 +657,9 @@ constexpr int wide_waves(int column_tiles) { return column_tiles == 2 ? 4 : 8; }
 constexpr int most_tiles(int group) { return group == 128 ? 7 : (group == 64 ? 5 : 4); }
 
 // The cheapest by a model of a call's time in microseconds, fitted to calls of 512x1024 to 28672x7168 and 9216x36864 with 1 to
-// 64 columns.  One workgroup of w4_linear runs on a CU at a time; a step, a block of K for each of its 8 waves, takes
-// 0.4 for a row tile and 0.6 for X: 28672x7168, N = 16, fp16, groups of 128, with 7 / 4 / 2 / 1 row tiles 26.7 / 33.9 /
+// 64 columns.  w4_linear's workgroups are counted in rounds of 256, one for every CU.  That is what the registers leave from three row
+// tiles on (two in groups of 32); of fewer a CU holds two or three, which the model does not count.  A step, a block of K for each
+// of a workgroup's 8 waves, takes 0.4 for a row tile and 0.6 for X: 28672x7168, N = 16, fp16, groups of 128, with 7 / 4 / 2 / 1 row tiles 26.7 / 33.9 /
 // 40.7 / 59.5 us.  K in shares, so that few rows fill the CUs with many row tiles each: 5120x20480, N = 16 22.6 us with five
 // row tiles in four shares, 32.5 at best in one; 7168x28672, N = 8 26.7 (seven in four) and 29.4; 4096x11008, N = 4 15.6 at
 // best in shares, 13.3 in one.  Columns past 16 are workgroups of their own.
