@@ -117,7 +117,8 @@ int KV4_Gather(hipStream_t stream, const KV4_Cache* cache, const KV4_Batch* batc
  * 16-byte aligned; contents irrelevant.  q: rows aligned to 16 bytes (strides multiples of 8 elements, where they are used).
  * Roundings.  Scores, their maxima and the sums are float32; a score is within 2^-21 of sum_d |q_d| w (code + z) (as measured,
  * with few rows to a sequence; 2^-24 with many).  A probability is rounded to fp16 (11 bits, of either sign) before it is
- * multiplied by the values; the sum of probabilities is not.  out is rounded once. */
+ * multiplied by the values; the sum of probabilities is not.  With its value's scale (1 for a vector of zeros) it keeps those bits
+ * down to 2^-21 of the row's largest such product, and counts as 0 below 2^-31 of it.  out is rounded once. */
 int    KV4_Attention(hipStream_t stream, const KV4_Cache* cache, const KV4_Batch* batch, KV4_Rows q, int q_heads,
                      void* out, float* lse, float scale, int window, int max_len, void* workspace,
                      size_t workspace_bytes, int dtype);

@@ -134,7 +134,8 @@ class KV4Cache:
 
     @classmethod
     def from_tensors(cls, k_codes, k_words, v_codes, v_words):
-        """A cache over existing arrays, which it shares."""
+        """A cache over existing arrays, which it shares.  Words of places that some row sees must be those of kv4_append, or have a
+        scale of 0 (a vector of zeros) or a positive normal one; the others may be anything."""
         self = object.__new__(cls)
         self._adopt(k_codes, k_words, v_codes, v_words)
         return self
