@@ -14,6 +14,7 @@ from .api import (  # noqa: F401
     ACT_GELU,
     ACT_NONE,
     ACT_RELU,
+    ACT_SILU,
     NOALLOC_SCRATCH_BYTES,
     SpMM_SplitK_API,
     SpMM_SplitK_API_NoAlloc,
@@ -38,9 +39,13 @@ from .api import (  # noqa: F401
 
 
 def __getattr__(name):
-    # the decode operators need torch, which the host encoder and the C ABI do without: imported when first asked for
+    # the decode operators and the 8-bit linears need torch, which the host encoder and the C ABI do without: imported when first asked for
     if name in ("KV4Cache", "kv4_append", "kv4_gather", "kv4_attention", "W4Linear", "quantize_w4", "w4_pack"):
         from . import decode
         value = globals()[name] = getattr(decode, name)
+        return value
+    if name in ("rms_norm", "rms_norm_x8", "quantize_x8", "quantize_w8", "w8_pack", "W8Linear", "W8GatedLinear"):
+        from . import w8
+        value = globals()[name] = getattr(w8, name)
         return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -331,6 +331,7 @@ def SpMM_SplitK_API_NoAlloc(stream, values, bitmaps, offsets, X, C_out, M, N, K,
 
 
 ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
+ACT_SILU = 3  # of the 8-bit linears alone (include/w8_api.h)
 
 
 def InitSparseMatrixA_bitmap_device(W, stream=None):

@@ -10,7 +10,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 LIBPATH = os.path.join(LIBDIR, "libSpMM_API.so")
 
-SOURCES = ["spmm_api.hip", "encoder_device.hip", "encoder.cpp", "kv4_cache.hip", "kv4_attention.hip", "w4_linear.hip"]
+SOURCES = ["spmm_api.hip", "encoder_device.hip", "encoder.cpp", "kv4_cache.hip", "kv4_attention.hip", "w4_linear.hip",
+           "rms_norm.hip", "w8_linear.hip"]
 # Packed-fp32 VALU forms are switched off for every device compile.  Kernel arguments are preloaded into scalar
 # registers when a wave starts (gfx950 supports it; a kernel then begins without the round trip for its argument
 # block): 0.25-0.4 us per call on every shape measured, 3 % of a 5120x5120 call.

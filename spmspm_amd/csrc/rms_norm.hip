@@ -1,0 +1,284 @@
+// RMS_Norm, W8_Quantize (w8_api.h): a row of 16-bit numbers is read once, held in registers, reduced and written.
+//
+// Mathematics.  With t = h w the codes of a normed row are those of t itself, since the division by the rms scales all of a row
+// alike: rint(127 t / max|t|).  So they do not depend on the sum of squares, whose rounding varies with its order, and one pass
+// takes the sum of h^2 and the maximum of |t| together.
+//
+// Bound by memory: 2 bytes for x, 2 for the residual and 2 for h, 2 or 1 for the result of every element.
+#include "w8_common.hiph"
+
+namespace decode {
+namespace {
+
+struct NormArgs {
+    const uint16_t *x, *residual, *weight;
+    uint16_t *      h, *y;
+    int8_t*         codes;
+    float*          scales;
+    int64_t         x_stride, r_stride, h_stride, y_stride, c_stride;
+    int             N, K;
+    float           eps;
+    int             norm; // 0: the row is only rounded to 8 bits
+};
+
+__device__ __forceinline__ shortx8 load8(const uint16_t* p, int left)
+{
+    if (left >= 8)
+        return *reinterpret_cast<const loose8*>(p);
+    shortx8 v = 0;
+    for (int i = 0; i < 7; ++i)
+        if (i < left)
+            v[i] = p[i];
+    return v;
+}
+
+__device__ __forceinline__ void store8(uint16_t* p, shortx8 v, int left)
+{
+    if (left >= 8) {
+        *reinterpret_cast<loose8*>(p) = v;
+        return;
+    }
+    for (int i = 0; i < 7; ++i)
+        if (i < left)
+            p[i] = v[i];
+}
+
+template <bool BF16>
+__device__ __forceinline__ float up(uint16_t v)
+{
+    return from16(v, BF16);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint16_t down(float x)
+{
+    return BF16 ? __builtin_bit_cast(uint16_t, (__bf16)x) : __builtin_bit_cast(uint16_t, (_Float16)x);
+}
+
+// Sum of `a` and maximum of `b` over the WAVES waves of a row, in every lane.
+template <int WAVES>
+__device__ __forceinline__ void reduce(float& a, unsigned& b, float (*sum)[16], unsigned (*top)[16], int turn)
+{
+    for (int d = 32; d > 0; d >>= 1) {
+        a += __shfl_xor(a, d);
+        b = max(b, (unsigned)__shfl_xor((int)b, d));
+    }
+    if constexpr (WAVES > 1) {
+        const int wave = threadIdx.x / kWave;
+        if (threadIdx.x % kWave == 0)
+            sum[turn][wave] = a, top[turn][wave] = b;
+        __syncthreads();
+        a = 0.f, b = 0;
+        for (int w = 0; w < WAVES; ++w)
+            a += sum[turn][w], b = max(b, top[turn][w]);
+    }
+}
+
+// One row by WAVES waves, V vectors of eight elements a lane in registers; V = 0: a row of any length, read twice.
+template <bool BF16, bool QUANT, int WAVES, int V>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(NormArgs a)
+{
+    constexpr int      kThreads = WAVES * kWave, kHeld = V > 0 ? V : 1;
+    __shared__ float    sum[2][16];
+    __shared__ unsigned top[2][16];
+    const int           lane = WAVES == 1 ? threadIdx.x % kWave : threadIdx.x;
+    const int64_t       row  = WAVES == 1 ? (int64_t)blockIdx.x * 4 + threadIdx.x / kWave : (int64_t)blockIdx.x;
+    if (WAVES == 1 && row >= a.N)
+        return;
+    const uint16_t* x = a.x + row * a.x_stride;
+    const uint16_t* r = a.residual + row * a.r_stride;
+    uint16_t*       h = a.h + row * a.h_stride;
+    const int       n = V > 0 ? V : (a.K + kThreads * 8 - 1) / (kThreads * 8);
+
+    shortx8 held[kHeld], gain[kHeld];
+    // The vector at element e as the norm sees it; what lies behind the row is 0.
+    auto fetch = [&](int e) {
+        shortx8 v = load8(x + e, a.K - e);
+        if (a.residual != nullptr) {
+            const shortx8 d = load8(r + e, a.K - e);
+            for (int i = 0; i < 8; ++i)
+                v[i] = down<BF16>(up<BF16>(v[i]) + up<BF16>(d[i]));
+        }
+        return v;
+    };
+    float    squares = 0.f;
+    unsigned most    = 0; // bits of max |t|: an infinity or a NaN is larger than every number
+    auto     take    = [&](shortx8 v, shortx8 w) {
+        for (int i = 0; i < 8; ++i) {
+            const float f = up<BF16>(v[i]), t = a.weight != nullptr ? f * up<BF16>(w[i]) : f;
+            squares       = __builtin_fmaf(f, f, squares);
+            if (QUANT)
+                most = max(most, __float_as_uint(t) & 0x7fffffffu);
+        }
+    };
+    for (int j = 0; j < n; ++j) {
+        const int e = (j * kThreads + lane) * 8, k = V > 0 ? j : 0;
+        held[k] = 0, gain[k] = 0;
+        if (e < a.K) {
+            held[k] = fetch(e);
+            if (a.weight != nullptr)
+                gain[k] = load8(a.weight + e, a.K - e);
+            if (a.h != nullptr)
+                store8(h + e, held[k], a.K - e);
+            if (V == 0)
+                take(held[0], gain[0]);
+        }
+    }
+    if (V > 0)
+        for (int j = 0; j < V; ++j)
+            take(held[j], gain[j]);
+    // The row once more, for rows that are not held: h where it was written (it may have taken x's place), x and the residual otherwise.
+    auto again = [&](int j, int e) {
+        if (V > 0)
+            return held[V > 0 ? j : 0];
+        return a.h != nullptr ? load8(h + e, a.K - e) : fetch(e);
+    };
+    reduce<WAVES>(squares, most, sum, top, 0);
+
+    float inverse_rms = 1.f;
+    if (a.norm) {
+        float mean = squares / (float)a.K, unit = 1.f;
+        if (BF16 && !(squares < INFINITY)) { // squares of bf16 numbers from 2^64 on: once more with h / 2^96
+            float    small = 0.f;
+            unsigned none  = 0;
+            for (int j = 0; j < n; ++j) {
+                const int e = (j * kThreads + lane) * 8;
+                if (e < a.K) {
+                    const shortx8 v = again(j, e);
+                    for (int i = 0; i < 8; ++i) {
+                        const float f = up<BF16>(v[i]) * 0x1p-96f;
+                        small         = __builtin_fmaf(f, f, small);
+                    }
+                }
+            }
+            reduce<WAVES>(small, none, sum, top, 1);
+            mean = small / (float)a.K, unit = 0x1p-96f;
+        }
+        inverse_rms = 1.f / sqrtf(mean + (unit == 1.f ? a.eps : 0.f)) * unit;
+    }
+    const float m       = __uint_as_float(most);
+    const bool  bad     = QUANT && most >= 0x7f800000u, none = QUANT && (bad || m < kNoRow8);
+    const float inverse = none ? 0.f : 127.f / m;
+    if (QUANT && lane == 0)
+        a.scales[row] = bad ? NAN : (none ? 0.f : m / 127.f * inverse_rms);
+    for (int j = 0; j < n; ++j) {
+        const int e = (j * kThreads + lane) * 8;
+        if (e >= a.K)
+            continue;
+        const shortx8 v = again(j, e);
+        shortx8       w = gain[V > 0 ? j : 0];
+        if (V == 0 && a.weight != nullptr)
+            w = load8(a.weight + e, a.K - e);
+        if constexpr (QUANT) {
+            float t[8];
+            for (int i = 0; i < 8; ++i)
+                t[i] = none ? 0.f : (a.weight != nullptr ? up<BF16>(v[i]) * up<BF16>(w[i]) : up<BF16>(v[i]));
+            // rows are readable, and here written, up to 16 bytes: the codes of the zeros behind the row are 0
+            *reinterpret_cast<uintx2*>(a.codes + row * a.c_stride + e) = codes8(t, m, inverse);
+        } else {
+            shortx8 y;
+            for (int i = 0; i < 8; ++i)
+                y[i] = down<BF16>(up<BF16>(v[i]) * inverse_rms * up<BF16>(w[i]));
+            store8(a.y + row * a.y_stride + e, y, a.K - e);
+        }
+    }
+}
+
+template <bool BF16, bool QUANT, int WAVES, int V>
+int start(hipStream_t stream, const NormArgs& a)
+{
+    const unsigned rows = WAVES == 1 ? (unsigned)(((int64_t)a.N + 3) / 4) : (unsigned)a.N;
+    return launch(rms_norm<BF16, QUANT, WAVES, V>, dim3(rows, 1, 1), dim3(WAVES == 1 ? 256 : WAVES * kWave, 1, 1), stream, a);
+}
+
+template <bool BF16, bool QUANT>
+int start(hipStream_t stream, const NormArgs& a)
+{
+    const int vectors = (a.K + 7) / 8;
+    if (vectors <= 64)
+        return start<BF16, QUANT, 1, 1>(stream, a);
+    if (vectors <= 256)
+        return start<BF16, QUANT, 4, 1>(stream, a);
+    if (vectors <= 512)
+        return start<BF16, QUANT, 4, 2>(stream, a);
+    if (vectors <= 1024)
+        return start<BF16, QUANT, 4, 4>(stream, a);
+    if (vectors <= 4096)
+        return start<BF16, QUANT, 16, 4>(stream, a);
+    return start<BF16, QUANT, 16, 0>(stream, a);
+}
+
+int start(hipStream_t stream, const NormArgs& a, int dtype)
+{
+    if (a.codes != nullptr)
+        return dtype == DECODE_BF16 ? start<true, true>(stream, a) : start<false, true>(stream, a);
+    return dtype == DECODE_BF16 ? start<true, false>(stream, a) : start<false, false>(stream, a);
+}
+
+int check_sizes(int N, int K, int most, int dtype)
+{
+    if (N < 0 || K < 1 || K > most)
+        return refuse("%d rows of %d numbers (1 to %d)", N, K, most);
+    if (dtype != DECODE_FP16 && dtype != DECODE_BF16)
+        return refuse("unknown element type %d", dtype);
+    return 0;
+}
+
+} // namespace
+
+int run_quantize(hipStream_t stream, const void* x, int64_t x_stride, int N, int K, int8_t* codes, int64_t codes_stride,
+                 float* scales, int dtype)
+{
+    NormArgs a{};
+    a.x = static_cast<const uint16_t*>(x), a.x_stride = x_stride;
+    a.codes = codes, a.c_stride = codes_stride, a.scales = scales;
+    a.N = N, a.K = K;
+    return start(stream, a, dtype);
+}
+
+} // namespace decode
+
+using namespace decode;
+
+extern "C" int RMS_Norm(hipStream_t stream, W8_Rows x, W8_Rows residual, const void* weight, float eps, int N, int K,
+                        W8_Rows h_out, W8_Rows y, const W8_Codes* codes, int dtype)
+{
+    if (int e = check_sizes(N, K, codes != nullptr ? kMaxK8 : 1 << 24, dtype))
+        return e;
+    if (!(eps >= 1e-20f) || !(eps < INFINITY))
+        return refuse("eps %g: 1e-20 or more", (double)eps);
+    if ((codes != nullptr) == (y.data != nullptr))
+        return refuse("a norm writes either 16-bit rows or codes");
+    if (N == 0)
+        return 0;
+    if (bad_rows16(x) || bad_pointer(weight, 2) || (residual.data != nullptr && bad_rows16(residual)) ||
+        (h_out.data != nullptr && bad_rows16(h_out)) || (y.data != nullptr && bad_rows16(y)))
+        return refuse("a null or misaligned x, residual, weight, h or y (2 bytes)");
+    if (codes != nullptr && (bad_codes(*codes, N, K) || bad_pointer(codes->scales, 4)))
+        return refuse("codes null or misaligned (16 bytes, rows too), or scales (4)");
+    if (N > 1 && ((h_out.data != nullptr && h_out.stride < K) || (y.data != nullptr && y.stride < K)))
+        return refuse("rows of an output less than %d numbers apart", K);
+    NormArgs a{};
+    a.x = static_cast<const uint16_t*>(x.data), a.x_stride = x.stride;
+    a.residual = static_cast<const uint16_t*>(residual.data), a.r_stride = residual.stride;
+    a.weight = static_cast<const uint16_t*>(weight);
+    a.h = static_cast<uint16_t*>(const_cast<void*>(h_out.data)), a.h_stride = h_out.stride;
+    a.y = static_cast<uint16_t*>(const_cast<void*>(y.data)), a.y_stride = y.stride;
+    if (codes != nullptr)
+        a.codes = codes->codes, a.c_stride = codes->stride, a.scales = codes->scales;
+    a.N = N, a.K = K, a.eps = eps, a.norm = 1;
+    return start(stream, a, dtype);
+}
+
+extern "C" int W8_Quantize(hipStream_t stream, W8_Rows x, int N, int K, const W8_Codes* codes, int dtype)
+{
+    if (int e = check_sizes(N, K, kMaxK8, dtype))
+        return e;
+    if (codes == nullptr)
+        return refuse("no codes given");
+    if (N == 0)
+        return 0;
+    if (bad_rows16(x) || bad_codes(*codes, N, K) || bad_pointer(codes->scales, 4))
+        return refuse("x null or misaligned (2 bytes), codes (16, rows too) or scales (4)");
+    return run_quantize(stream, x.data, x.stride, N, K, codes->codes, codes->stride, codes->scales, dtype);
+}

@@ -1,0 +1,296 @@
+// Linears of 8-bit integers: W8_Pack, W8_Linear, W8_Gated (w8_api.h).
+//
+// Mathematics.  Y[n][m] = act(sx[n] sw[m] sum_k cx[n][k] cw[m][k] + b[m]): the matrix cores take the sums in whole numbers, exactly and
+// in any order, so that K may be split among waves and workgroups at will without a result changing; scales, bias and
+// activation are applied to a sum in float32.
+//
+// Packed weights.  Blocks of 16 rows x 64 columns, 1 KB, in the order in which v_mfma_i32_16x16x64_i8 takes its first operand: 16 bytes a
+// lane, lane r + 16 q has columns 16 q .. 16 q + 15 of row r.  Four row tiles make a group of 64 rows, whose order is chosen for the
+// results: after the product a lane r + 16 q holds, of column r of X, rows 4 q .. 4 q + 3 of every tile.  Row 16 q + 4 t + i of the group
+// is put at row 4 q + i of tile t, so that these are 16 consecutive outputs, 32 bytes of Y.  In gated weights tiles 0 and 1 hold 32
+// rows of the gate (row 8 q + 4 t + i), tiles 2 and 3 the same rows of up: both sums of an output meet in one lane.
+// K is filled up with zeros to a multiple of 128: what X has there does not matter.
+#include "w8_common.hiph"
+
+#include <algorithm>
+
+namespace decode {
+namespace {
+
+constexpr int kMaxRows8 = 1 << 24;
+
+struct Layout8 {
+    int     groups, steps; // groups of 64 packed rows, steps of 64 columns (an even number)
+    int64_t scales, bytes; // offset of the scales (float32; of the gate, then of up), size
+};
+
+__host__ __device__ inline Layout8 layout8(int M, int K, bool gated)
+{
+    Layout8 l;
+    l.groups = gated ? (M + 31) / 32 : (M + 63) / 64;
+    l.steps  = (K + 127) / 128 * 2;
+    l.scales = (int64_t)l.groups * l.steps * 4096;
+    l.bytes  = l.scales + (int64_t)l.groups * 64 * 4;
+    return l;
+}
+
+struct PackArgs {
+    const int8_t *w, *up;
+    const float * scales, *up_scales;
+    int64_t       w_stride, up_stride;
+    int           M, K;
+    uint8_t*      packed;
+};
+
+// One wave lays out one block of 16 rows x 64 columns.
+__global__ __launch_bounds__(64) void w8_pack(PackArgs a)
+{
+    const bool    gated = a.up != nullptr;
+    const Layout8 l     = layout8(a.M, a.K, gated);
+    const int     lane = threadIdx.x, r = lane & 15, q = lane >> 4, tile = blockIdx.x & 3;
+    const int64_t block = blockIdx.x;
+    const int     group = (int)(block / 4 % l.groups), step = (int)(block / 4 / l.groups);
+    const bool    second = gated && tile >= 2;
+    const int     row = gated ? group * 32 + (r >> 2) * 8 + (tile & 1) * 4 + (r & 3) : group * 64 + (r >> 2) * 16 + tile * 4 + (r & 3);
+    const int8_t* src = second ? a.up + row * a.up_stride : a.w + row * a.w_stride;
+    uintx4        out = 0;
+    for (int b = 0; b < 16; ++b) {
+        const int k = step * 64 + q * 16 + b;
+        if (row < a.M && k < a.K)
+            out[b / 4] |= (unsigned)(uint8_t)src[k] << (8 * (b % 4));
+    }
+    reinterpret_cast<uintx4*>(a.packed)[(((int64_t)group * 4 + tile) * l.steps + step) * 64 + lane] = out;
+    if (step == 0 && tile == 0) { // 64 scales: of the group's rows, or of 32 rows of the gate and of up
+        const int  per = gated ? 32 : 64, m = group * per + lane % per;
+        const bool u = gated && lane >= 32;
+        reinterpret_cast<float*>(a.packed + l.scales)[(u ? (int64_t)l.groups * 32 : 0) + m] =
+            m < a.M ? (u ? a.up_scales[m] : a.scales[m]) : 0.f;
+    }
+}
+
+struct ProductArgs {
+    const uint8_t* packed;
+    const int8_t*  x;
+    const float*   x_scales;
+    int64_t        x_stride;
+    uint16_t*      y;
+    const uint16_t *bias, *up_bias;
+    int            M, N, K, act;
+};
+
+__device__ __forceinline__ float activate8(float y, int act)
+{
+    if (act == 1)
+        return y < 0.f ? 0.f : y; // a NaN stays one
+    if (act == 2) { // y * sigmoid(2u) = y/2 (1 + tanh u); large |u| ends at 0 and y
+        const float u = 0.7978845608028654f * (y + 0.044715f * y * y * y);
+        return y / (1.f + __expf(-2.f * u));
+    }
+    if (act == W8_ACT_SILU)
+        return y / (1.f + __expf(-y));
+    return y;
+}
+
+// Eight 16-bit numbers from p on, of which `left` are there.
+__device__ __forceinline__ shortx8 bias8(const uint16_t* p, int left)
+{
+    if (left >= 8)
+        return *reinterpret_cast<const loose8*>(p);
+    shortx8 v = 0;
+    for (int i = 0; i < 7; ++i)
+        if (i < left)
+            v[i] = p[i];
+    return v;
+}
+
+// The end of a sum: eight consecutive outputs from row m on, of column n.  `up` is read by gated products only.
+template <bool BF16, bool GATED>
+__device__ __forceinline__ void finish8(const ProductArgs& a, const Layout8& l, int m, int n, const int* sum, const int* up)
+{
+    const int left = a.M - m;
+    if (left <= 0)
+        return;
+    const float   sx = a.x_scales[n];
+    const float*  sw = reinterpret_cast<const float*>(a.packed + l.scales) + m;
+    const float*  su = sw + (int64_t)l.groups * 32;
+    const shortx8 b  = a.bias != nullptr ? bias8(a.bias + m, left) : (shortx8)0;
+    const shortx8 bu = GATED && a.up_bias != nullptr ? bias8(a.up_bias + m, left) : (shortx8)0;
+    shortx8       out;
+    for (int i = 0; i < 8; ++i) {
+        float y = (float)sum[i] * sw[i] * sx;
+        if (a.bias != nullptr)
+            y += from16(b[i], BF16);
+        y = activate8(y, a.act);
+        if constexpr (GATED) {
+            float u = (float)up[i] * su[i] * sx;
+            if (a.up_bias != nullptr)
+                u += from16(bu[i], BF16);
+            y *= u;
+        }
+        out[i] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y) : __builtin_bit_cast(uint16_t, (_Float16)y);
+    }
+    uint16_t* y = a.y + (int64_t)n * a.M + m;
+    if (left >= 8) {
+        *reinterpret_cast<loose8*>(y) = out;
+        return;
+    }
+    for (int i = 0; i < 7; ++i)
+        if (i < left)
+            y[i] = out[i];
+}
+
+// A workgroup takes one group of 64 packed rows and 16 columns of X; its four waves take every fourth step of K and meet in LDS.
+template <bool BF16, bool GATED>
+__global__ __launch_bounds__(256) void w8_product(ProductArgs a)
+{
+    __shared__ intx4 part[4][4][64];
+    const Layout8    l    = layout8(a.M, a.K, GATED);
+    const int        lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int        group = blockIdx.x, n = blockIdx.y * 16 + (lane & 15), q = lane >> 4;
+    const int8_t*    x     = a.x + (int64_t)min(n, a.N - 1) * a.x_stride;
+    const int        last  = (a.K - 1) / 16; // the last 16 columns that X has; behind them the weights are 0
+    const intx4*     w     = reinterpret_cast<const intx4*>(a.packed) + (int64_t)group * 4 * l.steps * 64 + lane;
+    intx4            sum[4] = {0, 0, 0, 0};
+    for (int s = wave; s < l.steps; s += 4) {
+        const intx4 b = *reinterpret_cast<const intx4*>(x + 16 * min(4 * s + q, last));
+        for (int t = 0; t < 4; ++t)
+            sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[((int64_t)t * l.steps + s) * 64], b, sum[t], 0, 0, 0);
+    }
+    for (int t = 0; t < 4; ++t)
+        part[wave][t][lane] = sum[t];
+    __syncthreads();
+    if (wave > 0 || n >= a.N)
+        return;
+    for (int t = 0; t < 4; ++t)
+        for (int w = 1; w < 4; ++w)
+            sum[t] += part[w][t][lane];
+    int v[16];
+    for (int i = 0; i < 16; ++i)
+        v[i] = sum[i / 4][i % 4];
+    if constexpr (GATED) {
+        finish8<BF16, true>(a, l, group * 32 + 8 * q, n, v, v + 8);
+    } else {
+        finish8<BF16, false>(a, l, group * 64 + 16 * q, n, v, nullptr);
+        finish8<BF16, false>(a, l, group * 64 + 16 * q + 8, n, v + 8, nullptr);
+    }
+}
+
+template <bool BF16, bool GATED>
+int run_product(hipStream_t stream, const ProductArgs& a)
+{
+    const Layout8 l = layout8(a.M, a.K, GATED);
+    return launch(w8_product<BF16, GATED>, dim3((unsigned)l.groups, (unsigned)(a.N + 15) / 16, 1), dim3(256, 1, 1), stream, a);
+}
+
+int check_sizes8(int M, int K)
+{
+    if (M < 1 || M > kMaxRows8 || K < 1 || K > kMaxK8)
+        return refuse("weights of %d rows (1 to 2^24) and %d columns (1 to %d)", M, K, kMaxK8);
+    return 0;
+}
+
+// Workspace of a call on 16-bit rows: codes, then scales.
+struct Space8 {
+    int64_t stride, scales, bytes;
+};
+
+Space8 space8(int N, int K, bool x16)
+{
+    Space8 s{};
+    if (x16) {
+        s.stride = (K + 15) / 16 * 16;
+        s.scales = s.stride * N;
+        s.bytes  = s.scales + ((int64_t)N * 4 + 15) / 16 * 16;
+    }
+    return s;
+}
+
+int run_product(hipStream_t stream, const void* packed, const W8_Codes& x, void* Y, int M, int N, int K, const void* bias,
+                const void* up_bias, int activation, void* workspace, size_t workspace_bytes, int dtype, bool gated)
+{
+    if (int e = check_sizes8(M, K))
+        return e;
+    if (N < 0 || N > 16 * 65535)
+        return refuse("%d rows of X (0 to %d)", N, 16 * 65535);
+    if (dtype != DECODE_FP16 && dtype != DECODE_BF16)
+        return refuse("unknown element type %d", dtype);
+    if (activation < 0 || activation > W8_ACT_SILU)
+        return refuse("unknown activation %d (0 none, 1 ReLU, 2 GELU, 3 SiLU)", activation);
+    if (N == 0)
+        return 0;
+    if (bad_pointer(packed, 16) || bad_pointer(Y, 2) || (bias != nullptr && bad_pointer(bias, 2)) ||
+        (up_bias != nullptr && bad_pointer(up_bias, 2)))
+        return refuse("a null or misaligned weight (16 bytes), Y or bias (2)");
+    const bool   x16 = x.scales == nullptr;
+    const Space8 s   = space8(N, K, x16);
+    if (x16 ? bad_pointer(x.codes, 2) : bad_codes(x, N, K) || bad_pointer(x.scales, 4))
+        return refuse("X null or misaligned (16-bit rows: 2 bytes; codes: 16, rows too, scales 4)");
+    const size_t need = (size_t)s.bytes;
+    if (need > 0 && (bad_pointer(workspace, 16) || workspace_bytes < need))
+        return refuse("workspace of %zu bytes (16-byte aligned), %zu needed", workspace == nullptr ? (size_t)0 : workspace_bytes, need);
+    ProductArgs a{};
+    a.packed = static_cast<const uint8_t*>(packed);
+    a.x = x.codes, a.x_scales = x.scales, a.x_stride = x.stride;
+    if (x16) {
+        int8_t* codes  = static_cast<int8_t*>(workspace);
+        float*  scales = reinterpret_cast<float*>(codes + s.scales);
+        if (int e = run_quantize(stream, x.codes, x.stride, N, K, codes, s.stride, scales, dtype))
+            return e;
+        a.x = codes, a.x_scales = scales, a.x_stride = s.stride;
+    }
+    a.y = static_cast<uint16_t*>(Y), a.bias = static_cast<const uint16_t*>(bias), a.up_bias = static_cast<const uint16_t*>(up_bias);
+    a.M = M, a.N = N, a.K = K, a.act = activation;
+    if (gated)
+        return dtype == DECODE_BF16 ? run_product<true, true>(stream, a) : run_product<false, true>(stream, a);
+    return dtype == DECODE_BF16 ? run_product<true, false>(stream, a) : run_product<false, false>(stream, a);
+}
+
+} // namespace
+} // namespace decode
+
+using namespace decode;
+
+extern "C" size_t W8_PackedBytes(int M, int K, int gated)
+{
+    if (M < 1 || M > kMaxRows8 || K < 1 || K > kMaxK8)
+        return 0;
+    return (size_t)layout8(M, K, gated != 0).bytes;
+}
+
+extern "C" int W8_Pack(hipStream_t stream, W8_Weights w, const W8_Weights* up, int M, int K, void* packed)
+{
+    if (int e = check_sizes8(M, K))
+        return e;
+    if (w.codes == nullptr || bad_pointer(w.scales, 4) || (up != nullptr && (up->codes == nullptr || bad_pointer(up->scales, 4))) ||
+        bad_pointer(packed, 16) || (M > 1 && (w.w_stride < K || (up != nullptr && up->w_stride < K))))
+        return refuse("null or misaligned codes, scales (4 bytes) or packed weights (16), or rows less than %d codes apart", K);
+    PackArgs a{};
+    a.w = w.codes, a.scales = w.scales, a.w_stride = w.w_stride;
+    if (up != nullptr)
+        a.up = up->codes, a.up_scales = up->scales, a.up_stride = up->w_stride;
+    a.M = M, a.K = K, a.packed = static_cast<uint8_t*>(packed);
+    const Layout8 l      = layout8(M, K, up != nullptr);
+    const int64_t blocks = (int64_t)l.groups * l.steps * 4;
+    if (blocks > 0x7fffffff)
+        return refuse("weights of %d rows and %d columns: more than 2^31 blocks", M, K);
+    return launch(w8_pack, dim3((unsigned)blocks, 1, 1), dim3(64, 1, 1), stream, a);
+}
+
+extern "C" size_t W8_WorkspaceBytes(int M, int N, int K, int gated, int x16)
+{
+    if (W8_PackedBytes(M, K, gated) == 0 || N < 1)
+        return 0;
+    return (size_t)space8(N, K, x16 != 0).bytes;
+}
+
+extern "C" int W8_Linear(hipStream_t stream, const void* packed, W8_Codes x, void* Y, int M, int N, int K, const void* bias,
+                         int activation, void* workspace, size_t workspace_bytes, int dtype)
+{
+    return run_product(stream, packed, x, Y, M, N, K, bias, nullptr, activation, workspace, workspace_bytes, dtype, false);
+}
+
+extern "C" int W8_Gated(hipStream_t stream, const void* packed, W8_Codes x, void* Y, int M, int N, int K, const void* gate_bias,
+                        const void* up_bias, int activation, void* workspace, size_t workspace_bytes, int dtype)
+{
+    return run_product(stream, packed, x, Y, M, N, K, gate_bias, up_bias, activation, workspace, workspace_bytes, dtype, true);
+}

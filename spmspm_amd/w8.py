@@ -1,0 +1,329 @@
+"""8-bit linears and the norm before them: for layers that are neither pruned nor held in 4 bits, above all over prompts.
+
+Thin host layer over include/w8_api.h, in the manner of spmspm_amd/decode.py: every size, type and stride is checked here before a
+kernel sees a pointer (ValueError), an error of the library raises RuntimeError, calls run on torch's current stream unless
+`stream` names another.  There is no CPU fallback.
+
+    codes, scales, h = rms_norm_x8(x, norm_weight, residual=h)      # h + x, normed, in 8 bits with a scale per token
+    gates = W8GatedLinear(*quantize_w8(w_gate), *quantize_w8(w_up))  # silu(gate) * up in one kernel
+    down = W8Linear(*quantize_w8(w_down))
+    y = down(gates(codes, scales))                                   # 16-bit rows are rounded to 8 bits within the call
+
+No counterpart in the reference, whose dense linears and norms are those of its FasterTransformer host
+(third_party/ft_spinfer.patch:3722-3753 is the one call that its library takes over there).
+"""
+import ctypes as C
+
+import torch
+
+from . import api as A
+from .decode import _TYPES, _check, _raise, _run, _type
+
+__all__ = ["rms_norm", "rms_norm_x8", "quantize_x8", "quantize_w8", "w8_pack", "W8Linear", "W8GatedLinear"]
+
+MAX_K = 131071  # sums of products of codes stay in 32 bits
+
+
+class _Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_int64)]
+
+
+class _Codes(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("stride", C.c_int64), ("scales", C.c_void_p)]
+
+
+class _Weights(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("w_stride", C.c_int64), ("scales", C.c_void_p)]
+
+
+_lib = None
+
+
+def _library():
+    global _lib
+    if _lib is None:
+        L = A.library()
+        codes, weights = C.POINTER(_Codes), C.POINTER(_Weights)
+        L.RMS_Norm.restype = C.c_int
+        L.RMS_Norm.argtypes = [C.c_void_p, _Rows, _Rows, C.c_void_p, C.c_float, C.c_int, C.c_int, _Rows, _Rows, codes, C.c_int]
+        L.W8_Quantize.restype = C.c_int
+        L.W8_Quantize.argtypes = [C.c_void_p, _Rows, C.c_int, C.c_int, codes, C.c_int]
+        L.W8_PackedBytes.restype = C.c_size_t
+        L.W8_PackedBytes.argtypes = [C.c_int] * 3
+        L.W8_Pack.restype = C.c_int
+        L.W8_Pack.argtypes = [C.c_void_p, _Weights, weights, C.c_int, C.c_int, C.c_void_p]
+        L.W8_WorkspaceBytes.restype = C.c_size_t
+        L.W8_WorkspaceBytes.argtypes = [C.c_int] * 5
+        L.W8_Linear.restype = C.c_int
+        L.W8_Linear.argtypes = [C.c_void_p, C.c_void_p, _Codes, C.c_void_p] + [C.c_int] * 3 + [
+            C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_int]
+        L.W8_Gated.restype = C.c_int
+        L.W8_Gated.argtypes = [C.c_void_p, C.c_void_p, _Codes, C.c_void_p] + [C.c_int] * 3 + [
+            C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_int]
+        _lib = L
+    return _lib
+
+
+_NONE = _Rows(None, 0)
+
+
+def _rows(name, t, dtype, shape, device):
+    """16-bit rows of any stride."""
+    if t.dtype != dtype or t.shape != shape or t.device != device or (shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on {device} with contiguous rows")
+    return _Rows(t.data_ptr(), t.stride(0))
+
+
+def _out_rows(name, t, like, inputs, outputs=()):
+    """Rows of an output, which may be an input itself but not a part of one, nor lap over another output."""
+    rows = _rows(name, t, like.dtype, like.shape, like.device)
+    if like.shape[0] > 1 and t.stride(0) < like.shape[1]:
+        raise ValueError(f"{name}: rows of an output must not overlap")
+    for other in inputs:
+        if other is not None and _overlap(t, other) and not (
+                t.data_ptr() == other.data_ptr() and (like.shape[0] < 2 or t.stride(0) == other.stride(0)) and t.shape == other.shape):
+            raise ValueError(f"{name} overlaps an input without being it")
+    for other in outputs:
+        if other is not None and _overlap(t, other):
+            raise ValueError(f"{name} overlaps another output")
+    return rows
+
+
+def _overlap(a, b):
+    """Whether the address ranges of two tensors meet (ranges that interlace without sharing an element count too)."""
+    span = lambda t: (t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size())
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _new_codes(x, N, K):
+    """Room for N rows of K codes, 16-byte aligned, and their scales."""
+    width = (K + 15) // 16 * 16
+    codes = torch.empty((N, width), dtype=torch.int8, device=x.device)
+    return codes if width == K else codes[:, :K], torch.empty(N, dtype=torch.float32, device=x.device)
+
+
+def _norm_args(x, weight, eps, residual):
+    _type(x.dtype)
+    if x.dim() != 2 or x.shape[1] == 0 or x.device.type != "cuda":
+        raise ValueError("x must be [tokens][K] on the GPU")
+    if x.shape[0] >= 1 << 31:
+        raise ValueError(f"{x.shape[0]} tokens: 2^31 - 1 at most")
+    if x.shape[1] > 1 << 24:
+        raise ValueError(f"rows of {x.shape[1]} numbers: 2^24 at most")
+    _check("weight", weight, x.device, x.dtype, (x.shape[1],))
+    if not 1e-20 <= eps < 3e38:
+        raise ValueError(f"eps {eps}: from 1e-20 up")
+    xr = _rows("x", x, x.dtype, x.shape, x.device)
+    return xr, _NONE if residual is None else _rows("residual", residual, x.dtype, x.shape, x.device)
+
+
+def rms_norm(x, weight, eps=1e-5, residual=None, out=None, residual_out=None, stream=None):
+    """y = h / sqrt(mean(h^2) + eps) * weight of rows h = x + residual (rounded to their type), or h = x.
+
+    x, residual [tokens][K], fp16 or bf16, contiguous rows of any stride; weight [K] of that type.  Returns y, with a residual
+    (y, h).  `out` and `residual_out` take y and h: new tensors by default; either may be x or the residual itself."""
+    xr, rr = _norm_args(x, weight, eps, residual)
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out without a residual: h is x itself")
+    given = (x, residual, weight)
+    hr = None if residual_out is None else _out_rows("residual_out", residual_out, x, given[:2])
+    yr = None if out is None else _out_rows("out", out, x, given[:2], (residual_out,))
+    for name, t in (("out", out), ("residual_out", residual_out)):
+        if t is not None and _overlap(t, weight):
+            raise ValueError(f"{name} overlaps the weight")
+
+    def call(handle):
+        y = x.new_empty(x.shape) if out is None else out
+        h = residual_out
+        if residual is not None and h is None:
+            h = x.new_empty(x.shape)
+        if x.shape[0]:
+            err = _library().RMS_Norm(handle, xr, rr, weight.data_ptr(), eps, x.shape[0], x.shape[1],
+                                      hr or (_NONE if h is None else _Rows(h.data_ptr(), x.shape[1])),
+                                      yr or _Rows(y.data_ptr(), x.shape[1]), None, _TYPES[x.dtype])
+            _raise(err, "rms_norm")
+        return y if residual is None else (y, h)
+
+    return _run(x.device, stream, call)
+
+
+def rms_norm_x8(x, weight, eps=1e-5, residual=None, residual_out=None, stream=None):
+    """rms_norm with its result in 8 bits: (codes, scales), with a residual (codes, scales, h).
+
+    codes int8 [tokens][K] (rows 16-byte aligned: a slice of wider ones where K is not a multiple of 16), scales float32 [tokens];
+    y ~ codes * scales.  What a W8Linear and a W8GatedLinear take."""
+    xr, rr = _norm_args(x, weight, eps, residual)
+    N, K = x.shape
+    if K > MAX_K:
+        raise ValueError(f"rows of {K} codes: {MAX_K} at most")
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out without a residual: h is x itself")
+    hr = None
+    if residual_out is not None:
+        hr = _out_rows("residual_out", residual_out, x, (x, residual))
+        if _overlap(residual_out, weight):
+            raise ValueError("residual_out overlaps the weight")
+
+    def call(handle):
+        codes, scales = _new_codes(x, N, K)
+        h = residual_out
+        if residual is not None and h is None:
+            h = x.new_empty(x.shape)
+        if N:
+            err = _library().RMS_Norm(handle, xr, rr, weight.data_ptr(), eps, N, K,
+                                      hr or (_NONE if h is None else _Rows(h.data_ptr(), K)), _NONE,
+                                      _Codes(codes.data_ptr(), (K + 15) // 16 * 16, scales.data_ptr()), _TYPES[x.dtype])
+            _raise(err, "rms_norm_x8")
+        return (codes, scales) if residual is None else (codes, scales, h)
+
+    return _run(x.device, stream, call)
+
+
+def quantize_x8(x, stream=None):
+    """Rows in 8 bits: (codes, scales) with x ~ codes * scales, as rms_norm_x8 returns them.  x [tokens][K], fp16 or bf16, of any stride."""
+    kind = _type(x.dtype)
+    if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] > MAX_K or x.shape[0] >= 1 << 31 or x.device.type != "cuda":
+        raise ValueError(f"x must be [tokens][K] on the GPU, K at most {MAX_K}")
+    xr = _rows("x", x, x.dtype, x.shape, x.device)
+    N, K = x.shape
+
+    def call(handle):
+        codes, scales = _new_codes(x, N, K)
+        if N:
+            err = _library().W8_Quantize(handle, xr, N, K, _Codes(codes.data_ptr(), (K + 15) // 16 * 16, scales.data_ptr()), kind)
+            _raise(err, "quantize_x8")
+        return codes, scales
+
+    return _run(x.device, stream, call)
+
+
+def quantize_w8(weight):
+    """Round a [M][K] weight to 8 bits: codes int8 [M][K] (-127..127), scales float32 [M], weight ~ scale * code.  Plain torch
+    operations, on any device."""
+    w = weight.float()
+    scales = w.abs().amax(-1) / 127
+    scales = torch.where(scales > 2.0 ** -100, scales, torch.ones_like(scales))  # a row of zeros
+    return torch.round(w / scales[:, None]).clamp(-127, 127).to(torch.int8), scales
+
+
+def w8_pack(codes, scales, up_codes=None, up_scales=None, stream=None):
+    """The layout that the kernels read, laid out once: an uint8 tensor.  codes int8 [M][K] and scales float32 [M] on the GPU; with a
+    second pair, of the same sizes, the weights of a gated product."""
+    if codes.dim() != 2 or codes.device.type != "cuda" or codes.numel() == 0:
+        raise ValueError("codes must be [M][K] on the GPU")
+    (M, K), device = codes.shape, codes.device
+    pairs = [(codes, scales)] + ([] if up_codes is None else [(up_codes, up_scales)])
+    for c, s in pairs:
+        _check("codes", c, device, torch.int8, (M, K))
+        _check("scales", s, device, torch.float32, (M,))
+    need = _library().W8_PackedBytes(M, K, len(pairs) == 2) if M < 1 << 31 and K < 1 << 31 else 0
+    if need == 0:
+        raise ValueError(f"weights of {M} x {K} are not supported")
+
+    def call(handle):
+        packed = torch.empty(need, dtype=torch.uint8, device=device)
+        w = [_Weights(c.data_ptr(), K, s.data_ptr()) for c, s in pairs]
+        _raise(_library().W8_Pack(handle, w[0], w[1] if len(w) == 2 else None, M, K, packed.data_ptr()), "w8_pack")
+        return packed
+
+    return _run(device, stream, call)
+
+
+class _Product:
+    """What the two linears share: packed weights and the call."""
+
+    def _adopt(self, packed, M, K, dtype, biases, activation, gated):
+        """Checks packed weights and takes them over."""
+        _type(dtype)
+        self.M, self.K, self.gated, self.dtype, self.activation = M, K, gated, dtype, int(activation)
+        self.packed, self.device, self.biases = packed, packed.device, biases
+        if packed.dtype != torch.uint8 or not packed.is_contiguous() or packed.device.type != "cuda" or packed.numel() == 0 \
+                or packed.numel() != _library().W8_PackedBytes(M, K, gated):
+            raise ValueError(f"packed weights of another size than {'two of ' if gated else ''}{M} x {K} take")
+        if self.activation not in (A.ACT_NONE, A.ACT_RELU, A.ACT_GELU, A.ACT_SILU):
+            raise ValueError(f"unknown activation {activation}")
+        for b in biases:
+            if b is not None:
+                _check("bias", b, self.device, dtype, (M,))
+
+    def bytes_per_call(self, N):
+        """Bytes a call with N rows of 8-bit x must move: weights and scales, x and y."""
+        return (2 if self.gated else 1) * self.M * (self.K + 4) + N * (self.K + 4 + 2 * self.M)
+
+    def __call__(self, x, scales=None, out=None, stream=None):
+        """x int8 [N][K] with float32 scales [N] (of rms_norm_x8 or quantize_x8), or 16-bit [N][K] in the layer's type, which is rounded
+        to 8 bits first.  Returns [N][M] in the layer's type."""
+        if x.dim() != 2 or x.shape[1] != self.K or x.device != self.device:
+            raise ValueError(f"x must be [N][{self.K}] on {self.device}")
+        N, stride = x.shape[0], x.stride(0)
+        if N > 16 * 65535:
+            raise ValueError(f"{N} rows of x: {16 * 65535} at most")
+        if N and self.K > 1 and x.stride(1) != 1:
+            raise ValueError("x must have contiguous rows")
+        if scales is None:
+            if x.dtype != self.dtype:
+                raise ValueError(f"x must be {self.dtype}, or int8 with its scales")
+        else:
+            if x.dtype != torch.int8:
+                raise ValueError("scales belong to int8 codes")
+            _check("scales", scales, self.device, torch.float32, (N,))
+            wide = (self.K + 15) // 16 * 16
+            if N and (x.data_ptr() % 16 or (N > 1 and (stride % 16 or stride < wide))
+                      or x.storage_offset() + (N - 1) * stride + wide > x.untyped_storage().nbytes()):
+                raise ValueError("rows of codes must be aligned to 16 bytes and readable up to a multiple of 16")
+            if N == 1:
+                stride = wide
+        if out is not None:
+            _check("out", out, self.device, self.dtype, (N, self.M))
+            if any(_overlap(out, t) for t in (x, scales, self.packed, *self.biases) if t is not None):
+                raise ValueError("out overlaps an input")
+
+        def call(handle):
+            y = torch.empty((N, self.M), dtype=self.dtype, device=self.device) if out is None else out
+            if N:
+                L, kind = _library(), _TYPES[self.dtype]
+                need = L.W8_WorkspaceBytes(self.M, N, self.K, self.gated, scales is None)
+                ws = self.packed.new_empty(need) if need else None
+                source = _Codes(x.data_ptr(), stride, None if scales is None else scales.data_ptr())
+                biases = [None if b is None else b.data_ptr() for b in self.biases]
+                err = (L.W8_Gated if self.gated else L.W8_Linear)(
+                    handle, self.packed.data_ptr(), source, y.data_ptr(), self.M, N, self.K, *biases, self.activation,
+                    None if ws is None else ws.data_ptr(), need, kind)
+                _raise(err, type(self).__name__)
+            return y
+
+        return _run(self.device, stream, call)
+
+
+class W8Linear(_Product):
+    """One 8-bit weight matrix resident in HBM: y = act(x W^T + bias), W[m][k] = scale[m] * code[m][k], x in 8 bits with a scale per row.
+
+    codes int8 [M][K], scales float32 [M] (see quantize_w8); bias [M] and y in `dtype`, fp16 or bf16."""
+
+    def __init__(self, codes, scales, bias=None, activation=A.ACT_NONE, dtype=torch.float16):
+        _type(dtype)
+        self._adopt(w8_pack(codes, scales), codes.shape[0], codes.shape[1], dtype, (bias,), activation, False)
+
+    def module(self):
+        """The same resident weights as a `torch.nn.Module` around the registered operator."""
+        from .torch_ops import W8LinearModule
+        return W8LinearModule(self)
+
+
+class W8GatedLinear(_Product):
+    """Gate and up of a feed-forward block in one kernel: y = act(x G^T + gate_bias) * (x U^T + up_bias), weights and x in 8 bits as
+    W8Linear's, `activation` of the gate (SiLU by default)."""
+
+    def __init__(self, gate_codes, gate_scales, up_codes, up_scales, gate_bias=None, up_bias=None, activation=A.ACT_SILU,
+                 dtype=torch.float16):
+        _type(dtype)
+        self._adopt(w8_pack(gate_codes, gate_scales, up_codes, up_scales), gate_codes.shape[0], gate_codes.shape[1], dtype,
+                    (gate_bias, up_bias), activation, True)
+
+    def module(self):
+        """The same resident weights as a `torch.nn.Module` around the registered operator."""
+        from .torch_ops import W8LinearModule
+        return W8LinearModule(self)
