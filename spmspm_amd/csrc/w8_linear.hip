@@ -103,40 +103,62 @@ __device__ __forceinline__ shortx8 bias8(const uint16_t* p, int left)
     return v;
 }
 
-// The end of a sum: eight consecutive outputs from row m on, of column n.  `up` is read by gated products only.
+// What the outputs of eight consecutive rows from `m` on have in common over the columns.
 template <bool BF16, bool GATED>
-__device__ __forceinline__ void finish8(const ProductArgs& a, const Layout8& l, int m, int n, const int* sum, const int* up)
-{
-    const int left = a.M - m;
-    if (left <= 0)
-        return;
-    const float   sx = a.x_scales[n];
-    const float*  sw = reinterpret_cast<const float*>(a.packed + l.scales) + m;
-    const float*  su = sw + (int64_t)l.groups * 32;
-    const shortx8 b  = a.bias != nullptr ? bias8(a.bias + m, left) : (shortx8)0;
-    const shortx8 bu = GATED && a.up_bias != nullptr ? bias8(a.up_bias + m, left) : (shortx8)0;
-    shortx8       out;
-    for (int i = 0; i < 8; ++i) {
-        float y = (float)sum[i] * sw[i] * sx;
-        if (a.bias != nullptr)
-            y += from16(b[i], BF16);
-        y = activate8(y, a.act);
-        if constexpr (GATED) {
-            float u = (float)up[i] * su[i] * sx;
-            if (a.up_bias != nullptr)
-                u += from16(bu[i], BF16);
-            y *= u;
+struct Tail8 {
+    float   sw[8], su[8];
+    shortx8 b, bu;
+    int     m, left;
+
+    __device__ __forceinline__ Tail8(const ProductArgs& a, const Layout8& l, int row) : m(row), left(a.M - row)
+    {
+        if (left <= 0)
+            return;
+        const float* s = reinterpret_cast<const float*>(a.packed + l.scales) + m; // the layout's rows go past M
+        for (int i = 0; i < 8; ++i) {
+            sw[i] = s[i];
+            if (GATED)
+                su[i] = s[i + (int64_t)l.groups * 32];
         }
-        out[i] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y) : __builtin_bit_cast(uint16_t, (_Float16)y);
+        b  = a.bias != nullptr ? bias8(a.bias + m, left) : (shortx8)0;
+        bu = GATED && a.up_bias != nullptr ? bias8(a.up_bias + m, left) : (shortx8)0;
     }
-    uint16_t* y = a.y + (int64_t)n * a.M + m;
-    if (left >= 8) {
-        *reinterpret_cast<loose8*>(y) = out;
-        return;
+
+    // The end of the sums of column n, of its row of X the scale sx; `up` is read by gated products only.
+    __device__ __forceinline__ void store(const ProductArgs& a, int n, float sx, const int* sum, const int* up) const
+    {
+        if (left <= 0)
+            return;
+        shortx8 out;
+        for (int i = 0; i < 8; ++i) {
+            float y = (float)sum[i] * sw[i] * sx;
+            if (a.bias != nullptr)
+                y += from16(b[i], BF16);
+            y = activate8(y, a.act);
+            if constexpr (GATED) {
+                float u = (float)up[i] * su[i] * sx;
+                if (a.up_bias != nullptr)
+                    u += from16(bu[i], BF16);
+                y *= u;
+            }
+            out[i] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y) : __builtin_bit_cast(uint16_t, (_Float16)y);
+        }
+        uint16_t* y = a.y + (int64_t)n * a.M + m;
+        if (left >= 8) {
+            *reinterpret_cast<loose8*>(y) = out;
+            return;
+        }
+        for (int i = 0; i < 7; ++i)
+            if (i < left)
+                y[i] = out[i];
     }
-    for (int i = 0; i < 7; ++i)
-        if (i < left)
-            y[i] = out[i];
+};
+
+// Row of its group that a lane's outputs begin at: 16 of them, or 8 of a gated product.
+template <bool GATED>
+__device__ __forceinline__ int first_row8(int group, int q)
+{
+    return GATED ? group * 32 + 8 * q : group * 64 + 16 * q;
 }
 
 // A workgroup takes one group of 64 packed rows and 16 columns of X; its four waves take every fourth step of K and meet in LDS.
@@ -167,11 +189,134 @@ __global__ __launch_bounds__(256) void w8_product(ProductArgs a)
     int v[16];
     for (int i = 0; i < 16; ++i)
         v[i] = sum[i / 4][i % 4];
-    if constexpr (GATED) {
-        finish8<BF16, true>(a, l, group * 32 + 8 * q, n, v, v + 8);
-    } else {
-        finish8<BF16, false>(a, l, group * 64 + 16 * q, n, v, nullptr);
-        finish8<BF16, false>(a, l, group * 64 + 16 * q + 8, n, v + 8, nullptr);
+    const float sx = a.x_scales[n];
+    const int   m  = first_row8<GATED>(group, q);
+    Tail8<BF16, GATED>(a, l, m).store(a, n, sx, v, v + 8);
+    if constexpr (!GATED)
+        Tail8<BF16, false>(a, l, m + 8).store(a, n, sx, v + 8, nullptr);
+}
+
+// A wave's 1 KB of 16 bytes a lane goes from global memory straight into LDS.  In assembly, since the compiler would wait for it
+// ahead of the next read of LDS; the kernel waits for it itself, before the barrier that hands the tile over.
+__device__ __forceinline__ void to_lds(unsigned lds, const void* base, unsigned offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+
+__device__ __forceinline__ void to_lds(unsigned lds, const void* address)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(address) : "memory");
+}
+
+// Workgroups are dealt to the eight dies in turn, each with an L2 of its own: consecutive numbers on one die, and there a band of
+// kBand row tiles by as many column tiles as run at once.
+__device__ __forceinline__ void place8(int id, int row_tiles, int column_tiles, int& row, int& column)
+{
+    constexpr int kBand = 8;
+    const int     total = row_tiles * column_tiles, xcd = id % 8, rest = total % 8;
+    const int     at   = xcd * (total / 8) + min(xcd, rest) + id / 8;
+    const int     band = at / (kBand * column_tiles), first = band * kBand, height = min(kBand, row_tiles - first);
+    const int     in   = at - first * column_tiles;
+    row = first + in % height, column = in / height;
+}
+
+// A workgroup of WM x WN waves takes WM MT x WN NT tiles of 16 x 16 outputs (packed rows x rows of X), a wave MT x NT of them.  K goes by in
+// blocks of 128 through two buffers in LDS: W's blocks lie there as they are packed, one operand a KB; of X 8 rows lie in a KB,
+// row r's chunk c of 16 bytes at place 8 r + (c ^ r), which the matrix operands' reads find without bank conflicts.
+// While the products of a block's first half run, the second half's operands are read; then the waves meet, the buffer that
+// all have read takes the block after next, and the next block's first operands are read under the second half's products.
+template <bool BF16, bool GATED, int MT, int NT, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_tiles, int column_tiles)
+{
+    constexpr int kWaves = WM * WN, kRows = WM * MT, kCols = WN * NT * 2, kStage = (2 * kRows + kCols) * 1024; // tiles of W, KBs of X
+    constexpr int kLoads = (2 * kRows + kCols) / kWaves, kWLoads = 2 * kRows / kWaves;
+    static_assert(2 * kRows % kWaves == 0 && kCols % kWaves == 0 && MT % 4 == 0);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][kStage];
+    const Layout8 l    = layout8(a.M, a.K, GATED);
+    const int     lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int     q = lane >> 4, c = lane & 15, wm = wave / WN, wn = wave % WN, blocks = l.steps / 2;
+    int           row, column;
+    place8(blockIdx.x, row_tiles, column_tiles, row, column);
+    const int tile0 = row * kRows, n0 = column * WN * NT * 16;
+
+    // What a wave brings of every block: KBs of W first, then of X.
+    const uint8_t* w_at[kWLoads];
+    const int8_t*  x_at[kLoads - kWLoads];
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0][0];
+    for (int i = 0; i < kWLoads; ++i) { // tiles behind the last are the last again: computed, not stored
+        const int j = wave * kWLoads + i;
+        w_at[i]     = a.packed + ((int64_t)min(tile0 + j / 2, l.groups * 4 - 1) * l.steps + j % 2) * 1024;
+    }
+    const int chunk = 16 * ((lane & 7) ^ (lane >> 3)), last = (a.K - 1) / 16 * 16;
+    for (int i = 0; i < kLoads - kWLoads; ++i) {
+        const int j = wave * (kLoads - kWLoads) + i;
+        x_at[i]     = a.x + (int64_t)min(n0 + 8 * j + (lane >> 3), a.N - 1) * a.x_stride;
+    }
+    auto stage = [&](int block, int buffer) {
+        const unsigned to = lds0 + buffer * kStage;
+        for (int i = 0; i < kWLoads; ++i)
+            to_lds(to + (wave * kWLoads + i) * 1024, w_at[i] + (int64_t)block * 2048, lane * 16);
+        const int at = min(block * 128 + chunk, last); // behind the last 16 columns of X the weights are 0
+        for (int i = 0; i < kLoads - kWLoads; ++i)
+            to_lds(to + (2 * kRows + wave * (kLoads - kWLoads) + i) * 1024, x_at[i] + at);
+    };
+    struct Operands {
+        intx4 w[MT], x[NT];
+    };
+    auto fetch = [&](Operands& o, int buffer, int half) {
+        const uint8_t* from = lds[buffer];
+        for (int t = 0; t < MT; ++t)
+            o.w[t] = *reinterpret_cast<const intx4*>(from + ((wm * MT + t) * 2 + half) * 1024 + lane * 16);
+        for (int t = 0; t < NT; ++t)
+            o.x[t] = *reinterpret_cast<const intx4*>(from + (2 * kRows + (wn * NT + t) * 2 + (c >> 3)) * 1024 + (c & 7) * 128 +
+                                                     (((4 * half + q) ^ (c & 7)) * 16));
+    };
+    intx4 sum[MT][NT];
+    for (int t = 0; t < MT; ++t)
+        for (int u = 0; u < NT; ++u)
+            sum[t][u] = 0;
+    auto multiply = [&](const Operands& o) {
+        for (int u = 0; u < NT; ++u)
+            for (int t = 0; t < MT; ++t)
+                sum[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[t], o.x[u], sum[t][u], 0, 0, 0);
+    };
+    Operands first, second;
+    stage(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (blocks > 1)
+        stage(1, 1);
+    fetch(first, 0, 0);
+    for (int i = 0; i < blocks; ++i) {
+        const int buffer = i & 1;
+        fetch(second, buffer, 1);
+        multiply(first);
+        __builtin_amdgcn_sched_barrier(0); // products stay ahead of the barrier: they run while the waves meet
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (i + 2 < blocks)
+            stage(i + 2, buffer);
+        if (i + 1 < blocks)
+            fetch(first, buffer ^ 1, 0);
+        multiply(second);
+    }
+
+#pragma unroll
+    for (int g = 0; g < MT / 4; ++g) {
+        const int                group = (tile0 + wm * MT) / 4 + g, m = first_row8<GATED>(group, q);
+        const Tail8<BF16, GATED> one(a, l, m);
+        const Tail8<BF16, GATED> two(a, l, GATED ? a.M : m + 8);
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            const int n = n0 + (wn * NT + u) * 16 + c;
+            if (n >= a.N)
+                continue;
+            int v[16];
+            for (int i = 0; i < 16; ++i)
+                v[i] = sum[g * 4 + i / 4][u][i % 4];
+            const float sx = a.x_scales[n];
+            one.store(a, n, sx, v, v + 8);
+            if (!GATED)
+                two.store(a, n, sx, v + 8, nullptr);
+        }
     }
 }
 
@@ -179,6 +324,10 @@ template <bool BF16, bool GATED>
 int run_product(hipStream_t stream, const ProductArgs& a)
 {
     const Layout8 l = layout8(a.M, a.K, GATED);
+    if (a.N > 64) {
+        const int rows = (l.groups * 4 + 15) / 16, cols = (a.N + 255) / 256;
+        return launch(w8_tiles<BF16, GATED, 8, 4, 2, 4>, dim3((unsigned)rows * cols, 1, 1), dim3(512, 1, 1), stream, a, rows, cols);
+    }
     return launch(w8_product<BF16, GATED>, dim3((unsigned)l.groups, (unsigned)(a.N + 15) / 16, 1), dim3(256, 1, 1), stream, a);
 }
 
