@@ -13,6 +13,7 @@
 #include "w8_common.hiph"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace decode {
 namespace {
@@ -78,17 +79,20 @@ struct ProductArgs {
     int            M, N, K, act;
 };
 
-__device__ __forceinline__ float activate8(float y, int act)
+// ReLU, GELU (tanh form) or SiLU of eight sums.  The last two are y / (1 + exp(-z)), with z = 2 sqrt(2/pi) (y + 0.044715 y^3), since
+// (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), or z = y; far from 0 they end at 0 and y.  The reciprocal's last bit is far below 16 bits.
+__device__ __forceinline__ void activate8(float* y, int act)
 {
-    if (act == 1)
-        return y < 0.f ? 0.f : y; // a NaN stays one
-    if (act == 2) { // y * sigmoid(2u) = y/2 (1 + tanh u); large |u| ends at 0 and y
-        const float u = 0.7978845608028654f * (y + 0.044715f * y * y * y);
-        return y / (1.f + __expf(-2.f * u));
+    if (act == 1) {
+        for (int i = 0; i < 8; ++i)
+            y[i] = y[i] < 0.f ? 0.f : y[i]; // a NaN stays one
+    } else if (act > 1) {
+        const float cube = act == 2 ? 1.5957691216057308f * 0.044715f : 0.f, one = act == 2 ? 1.5957691216057308f : 1.f;
+        for (int i = 0; i < 8; ++i) {
+            const float z = y[i] * (one + cube * y[i] * y[i]);
+            y[i]          = y[i] * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+        }
     }
-    if (act == W8_ACT_SILU)
-        return y / (1.f + __expf(-y));
-    return y;
 }
 
 // Eight 16-bit numbers from p on, of which `left` are there.
@@ -129,28 +133,24 @@ struct Tail8 {
     {
         if (left <= 0)
             return;
+        float y[8];
+        for (int i = 0; i < 8; ++i)
+            y[i] = (float)sum[i] * sw[i] * sx + from16(b[i], BF16);
+        activate8(y, a.act);
+        if constexpr (GATED)
+            for (int i = 0; i < 8; ++i)
+                y[i] *= (float)up[i] * su[i] * sx + from16(bu[i], BF16);
         shortx8 out;
-        for (int i = 0; i < 8; ++i) {
-            float y = (float)sum[i] * sw[i] * sx;
-            if (a.bias != nullptr)
-                y += from16(b[i], BF16);
-            y = activate8(y, a.act);
-            if constexpr (GATED) {
-                float u = (float)up[i] * su[i] * sx;
-                if (a.up_bias != nullptr)
-                    u += from16(bu[i], BF16);
-                y *= u;
-            }
-            out[i] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y) : __builtin_bit_cast(uint16_t, (_Float16)y);
-        }
-        uint16_t* y = a.y + (int64_t)n * a.M + m;
+        for (int i = 0; i < 8; ++i)
+            out[i] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y[i]) : __builtin_bit_cast(uint16_t, (_Float16)y[i]);
+        uint16_t* to = a.y + (int64_t)n * a.M + m;
         if (left >= 8) {
-            *reinterpret_cast<loose8*>(y) = out;
+            *reinterpret_cast<loose8*>(to) = out;
             return;
         }
         for (int i = 0; i < 7; ++i)
             if (i < left)
-                y[i] = out[i];
+                to[i] = out[i];
     }
 };
 
@@ -194,6 +194,16 @@ __global__ __launch_bounds__(256) void w8_product(ProductArgs a)
     Tail8<BF16, GATED>(a, l, m).store(a, n, sx, v, v + 8);
     if constexpr (!GATED)
         Tail8<BF16, false>(a, l, m + 8).store(a, n, sx, v + 8, nullptr);
+}
+
+// f(0) .. f(N - 1) with constants: arrays of registers have no others for an index.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F f)
+{
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>());
+        each<N, I + 1>(f);
+    }
 }
 
 // A wave's 1 KB of 16 bytes a lane goes from global memory straight into LDS.  In assembly, since the compiler would wait for it
@@ -252,63 +262,84 @@ __global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_
         const int j = wave * (kLoads - kWLoads) + i;
         x_at[i]     = a.x + (int64_t)min(n0 + 8 * j + (lane >> 3), a.N - 1) * a.x_stride;
     }
-    auto stage = [&](int block, int buffer) {
+    // The i-th of a wave's loads of a block.  Behind the last 16 columns of X the weights are 0: what is there does not matter.
+    auto stage = [&](int i, int block, int buffer) {
         const unsigned to = lds0 + buffer * kStage;
-        for (int i = 0; i < kWLoads; ++i)
+        if (i < kWLoads)
             to_lds(to + (wave * kWLoads + i) * 1024, w_at[i] + (int64_t)block * 2048, lane * 16);
-        const int at = min(block * 128 + chunk, last); // behind the last 16 columns of X the weights are 0
-        for (int i = 0; i < kLoads - kWLoads; ++i)
-            to_lds(to + (2 * kRows + wave * (kLoads - kWLoads) + i) * 1024, x_at[i] + at);
+        else
+            to_lds(to + (2 * kRows + wave * (kLoads - kWLoads) + i - kWLoads) * 1024,
+                   x_at[i - kWLoads] + min(block * 128 + chunk, last));
     };
     struct Operands {
         intx4 w[MT], x[NT];
     };
-    auto fetch = [&](Operands& o, int buffer, int half) {
+    constexpr int kReads = MT + NT, kProducts = MT * NT;
+    auto fetch = [&](Operands& o, int i, int buffer, int half) {
         const uint8_t* from = lds[buffer];
-        for (int t = 0; t < MT; ++t)
-            o.w[t] = *reinterpret_cast<const intx4*>(from + ((wm * MT + t) * 2 + half) * 1024 + lane * 16);
-        for (int t = 0; t < NT; ++t)
-            o.x[t] = *reinterpret_cast<const intx4*>(from + (2 * kRows + (wn * NT + t) * 2 + (c >> 3)) * 1024 + (c & 7) * 128 +
-                                                     (((4 * half + q) ^ (c & 7)) * 16));
+        if (i < MT)
+            o.w[i] = *reinterpret_cast<const intx4*>(from + ((wm * MT + i) * 2 + half) * 1024 + lane * 16);
+        else
+            o.x[i - MT] = *reinterpret_cast<const intx4*>(from + (2 * kRows + (wn * NT + i - MT) * 2 + (c >> 3)) * 1024 +
+                                                          (c & 7) * 128 + (((4 * half + q) ^ (c & 7)) * 16));
     };
     intx4 sum[MT][NT];
     for (int t = 0; t < MT; ++t)
         for (int u = 0; u < NT; ++u)
             sum[t][u] = 0;
-    auto multiply = [&](const Operands& o) {
-        for (int u = 0; u < NT; ++u)
-            for (int t = 0; t < MT; ++t)
-                sum[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[t], o.x[u], sum[t][u], 0, 0, 0);
+    // The products of one half in kParts parts, with `between(part)` behind each: loads issued all at once would hold the wave up
+    // ahead of its products until the memory pipe has taken them.
+    constexpr int kParts = kProducts / 4;
+    auto multiply = [&](const Operands& o, auto between) {
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+            for (int f = 4 * part; f < 4 * part + 4; ++f)
+                sum[f % MT][f / MT] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[f % MT], o.x[f / MT], sum[f % MT][f / MT], 0, 0, 0);
+            between(part);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
+    // Items `part` of `parts` of n, as a range.
+#define W8_SHARE(i, n, part, parts) for (int i = (n) * (part) / (parts); i < (n) * ((part) + 1) / (parts); ++i)
     Operands first, second;
-    stage(0, 0);
+    for (int i = 0; i < kLoads; ++i)
+        stage(i, 0, 0);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     if (blocks > 1)
-        stage(1, 1);
-    fetch(first, 0, 0);
+        for (int i = 0; i < kLoads; ++i)
+            stage(i, 1, 1);
+    for (int i = 0; i < kReads; ++i)
+        fetch(first, i, 0, 0);
+    constexpr int kEarly = kParts * 3 / 4; // parts under which operands are read: the rest covers their latency
     for (int i = 0; i < blocks; ++i) {
-        const int buffer = i & 1;
-        fetch(second, buffer, 1);
-        multiply(first);
-        __builtin_amdgcn_sched_barrier(0); // products stay ahead of the barrier: they run while the waves meet
+        const int  buffer = i & 1;
+        const bool more = i + 2 < blocks;
+        multiply(first, [&](int part) {
+            if (part < kEarly)
+                W8_SHARE(j, kReads, part, kEarly)
+                    fetch(second, j, buffer, 1);
+        });
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (i + 2 < blocks)
-            stage(i + 2, buffer);
-        if (i + 1 < blocks)
-            fetch(first, buffer ^ 1, 0);
-        multiply(second);
+        multiply(second, [&](int part) {
+            if (part < kEarly)
+                W8_SHARE(j, kReads, part, kEarly) // behind the last block stale bytes, which nothing takes
+                    fetch(first, j, buffer ^ 1, 0);
+            if (more)
+                W8_SHARE(j, kLoads, part, kParts)
+                    stage(j, i + 2, buffer);
+        });
     }
+#undef W8_SHARE
 
-#pragma unroll
-    for (int g = 0; g < MT / 4; ++g) {
+    each<MT / 4>([&](auto g) {
         const int                group = (tile0 + wm * MT) / 4 + g, m = first_row8<GATED>(group, q);
         const Tail8<BF16, GATED> one(a, l, m);
         const Tail8<BF16, GATED> two(a, l, GATED ? a.M : m + 8);
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
+        each<NT>([&](auto u) {
             const int n = n0 + (wn * NT + u) * 16 + c;
             if (n >= a.N)
-                continue;
+                return;
             int v[16];
             for (int i = 0; i < 16; ++i)
                 v[i] = sum[g * 4 + i / 4][u][i % 4];
@@ -316,8 +347,8 @@ __global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_
             one.store(a, n, sx, v, v + 8);
             if (!GATED)
                 two.store(a, n, sx, v + 8, nullptr);
-        }
-    }
+        });
+    });
 }
 
 template <bool BF16, bool GATED>
