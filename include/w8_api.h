@@ -12,7 +12,7 @@
  *   m = max |t_k|, code_k = the whole number nearest to 127 t_k / m (the even one of two), exactly; value_k = code_k * scale
  *   scale = m / 127, or m / 127 / rms where the norm below writes it
  * m below 2^-100: a row of zeros, codes and scale 0.  A row with an infinity or a NaN has codes 0 and scale NaN, and so NaN in
- * all that is computed from it.  Rows lie `stride` bytes apart, a multiple of 16, 16-byte aligned, each readable up to K rounded
+ * all that is computed from it.  Rows lie `stride` bytes apart, a multiple of 16, at most 2^28, 16-byte aligned, each readable up to K rounded
  * up to 16 bytes; what the bytes behind K hold does not matter.
  */
 #ifndef W8_API_H

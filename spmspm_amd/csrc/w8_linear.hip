@@ -110,22 +110,31 @@ __device__ __forceinline__ shortx8 bias8(const uint16_t* p, int left)
 // What the outputs of eight consecutive rows from `m` on have in common over the columns.
 template <bool BF16, bool GATED>
 struct Tail8 {
-    float   sw[8], su[8];
-    shortx8 b, bu;
-    int     m, left;
+    float sw[8], su[8], b[8], bu[8];
+    int   m, left;
 
     __device__ __forceinline__ Tail8(const ProductArgs& a, const Layout8& l, int row) : m(row), left(a.M - row)
     {
         if (left <= 0)
             return;
-        const float* s = reinterpret_cast<const float*>(a.packed + l.scales) + m; // the layout's rows go past M
+        const float*  s  = reinterpret_cast<const float*>(a.packed + l.scales) + m; // the layout's rows go past M
+        const shortx8 v  = a.bias != nullptr ? bias8(a.bias + m, left) : (shortx8)0;
+        const shortx8 vu = GATED && a.up_bias != nullptr ? bias8(a.up_bias + m, left) : (shortx8)0;
         for (int i = 0; i < 8; ++i) {
-            sw[i] = s[i];
+            sw[i] = s[i], b[i] = from16(v[i], BF16);
             if (GATED)
-                su[i] = s[i + (int64_t)l.groups * 32];
+                su[i] = s[i + (int64_t)l.groups * 32], bu[i] = from16(vu[i], BF16);
         }
-        b  = a.bias != nullptr ? bias8(a.bias + m, left) : (shortx8)0;
-        bu = GATED && a.up_bias != nullptr ? bias8(a.up_bias + m, left) : (shortx8)0;
+    }
+
+    // From LDS: scales, and biases as 32-bit words of 16 bits; those of up `up` words behind the gate's.
+    __device__ __forceinline__ Tail8(const ProductArgs& a, int row, const float* s, const unsigned* bias, int up) : m(row), left(a.M - row)
+    {
+        for (int i = 0; i < 8; ++i) {
+            sw[i] = s[i], b[i] = a.bias != nullptr ? from16((uint16_t)bias[i], BF16) : 0.f;
+            if (GATED)
+                su[i] = s[up + i], bu[i] = a.up_bias != nullptr ? from16((uint16_t)bias[up + i], BF16) : 0.f;
+        }
     }
 
     // The end of the sums of column n, of its row of X the scale sx; `up` is read by gated products only.
@@ -135,11 +144,11 @@ struct Tail8 {
             return;
         float y[8];
         for (int i = 0; i < 8; ++i)
-            y[i] = (float)sum[i] * sw[i] * sx + from16(b[i], BF16);
+            y[i] = (float)sum[i] * sw[i] * sx + b[i];
         activate8(y, a.act);
         if constexpr (GATED)
             for (int i = 0; i < 8; ++i)
-                y[i] *= (float)up[i] * su[i] * sx + from16(bu[i], BF16);
+                y[i] *= (float)up[i] * su[i] * sx + bu[i];
         shortx8 out;
         for (int i = 0; i < 8; ++i)
             out[i] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y[i]) : __builtin_bit_cast(uint16_t, (_Float16)y[i]);
@@ -213,9 +222,15 @@ __device__ __forceinline__ void to_lds(unsigned lds, const void* base, unsigned 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
-__device__ __forceinline__ void to_lds(unsigned lds, const void* address)
+// The same of one word, or of 16 bits in a word, a lane.
+__device__ __forceinline__ void word_to_lds(unsigned lds, const void* address)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(address) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(address) : "memory");
+}
+
+__device__ __forceinline__ void short_to_lds(unsigned lds, const void* address)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, off" ::"s"(lds), "v"(address) : "memory");
 }
 
 // Workgroups are dealt to the eight dies in turn, each with an L2 of its own: consecutive numbers on one die, and there a band of
@@ -227,7 +242,8 @@ __device__ __forceinline__ void place8(int id, int row_tiles, int column_tiles, 
     const int     at   = xcd * (total / 8) + min(xcd, rest) + id / 8;
     const int     band = at / (kBand * column_tiles), first = band * kBand, height = min(kBand, row_tiles - first);
     const int     in   = at - first * column_tiles;
-    row = first + in % height, column = in / height;
+    // divisions are done by vector instructions: back to scalars, which the addresses are made of
+    row = __builtin_amdgcn_readfirstlane(first + in % height), column = __builtin_amdgcn_readfirstlane(in / height);
 }
 
 // A workgroup of WM x WN waves takes WM MT x WN NT tiles of 16 x 16 outputs (packed rows x rows of X), a wave MT x NT of them.  K goes by in
@@ -235,33 +251,63 @@ __device__ __forceinline__ void place8(int id, int row_tiles, int column_tiles, 
 // row r's chunk c of 16 bytes at place 8 r + (c ^ r), which the matrix operands' reads find without bank conflicts.
 // While the products of a block's first half run, the second half's operands are read; then the waves meet, the buffer that
 // all have read takes the block after next, and the next block's first operands are read under the second half's products.
+// A workgroup stays on its CU and takes every gridDim-th tile: the blocks of all its tiles are one stream, so that the next tile is
+// loaded while the results of the last are written, and a tile costs its products alone.
 template <bool BF16, bool GATED, int MT, int NT, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_tiles, int column_tiles)
 {
     constexpr int kWaves = WM * WN, kRows = WM * MT, kCols = WN * NT * 2, kStage = (2 * kRows + kCols) * 1024; // tiles of W, KBs of X
     constexpr int kLoads = (2 * kRows + kCols) / kWaves, kWLoads = 2 * kRows / kWaves;
-    static_assert(2 * kRows % kWaves == 0 && kCols % kWaves == 0 && MT % 4 == 0);
+    constexpr int kM = kRows * 16, kN = WN * NT * 16; // packed rows, rows of X
+    static_assert(2 * kRows % kWaves == 0 && kCols % kWaves == 0 && MT % 4 == 0 && kM % 64 == 0 && kN % 64 == 0);
+    struct Ends { // of a tile: scales and biases of its rows (of the gate, then of up), scales of its rows of X
+        float    sw[kM];
+        unsigned b[kM];
+        float    sx[kN];
+    };
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2][kStage];
+    __shared__ __attribute__((aligned(16))) Ends      ends[4]; // loads are at most two tiles ahead of the products
     const Layout8 l    = layout8(a.M, a.K, GATED);
     const int     lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int     q = lane >> 4, c = lane & 15, wm = wave / WN, wn = wave % WN, blocks = l.steps / 2;
-    int           row, column;
-    place8(blockIdx.x, row_tiles, column_tiles, row, column);
-    const int tile0 = row * kRows, n0 = column * WN * NT * 16;
+    const int     tiles = row_tiles * column_tiles;
 
     // What a wave brings of every block: KBs of W first, then of X.
     const uint8_t* w_at[kWLoads];
     const int8_t*  x_at[kLoads - kWLoads];
-    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&lds[0][0];
-    for (int i = 0; i < kWLoads; ++i) { // tiles behind the last are the last again: computed, not stored
-        const int j = wave * kWLoads + i;
-        w_at[i]     = a.packed + ((int64_t)min(tile0 + j / 2, l.groups * 4 - 1) * l.steps + j % 2) * 1024;
-    }
-    const int chunk = 16 * ((lane & 7) ^ (lane >> 3)), last = (a.K - 1) / 16 * 16;
-    for (int i = 0; i < kLoads - kWLoads; ++i) {
-        const int j = wave * (kLoads - kWLoads) + i;
-        x_at[i]     = a.x + (int64_t)min(n0 + 8 * j + (lane >> 3), a.N - 1) * a.x_stride;
-    }
+    unsigned       x_row[kLoads - kWLoads];
+    auto address = [](const void* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p; };
+    const unsigned lds0 = address(lds), ends0 = address(ends);
+    const int      chunk = 16 * ((lane & 7) ^ (lane >> 3)), last = (a.K - 1) / 16 * 16;
+    // Turns the loads to a tile, the `turn`-th, and brings its ends.
+    auto enter = [&](int tile, int turn) {
+        int row, column;
+        place8(tile, row_tiles, column_tiles, row, column);
+        const int tile0 = row * kRows, n0 = column * kN;
+        for (int i = 0; i < kWLoads; ++i) { // tiles behind the last are the last again: computed, not stored
+            const int j = wave * kWLoads + i;
+            w_at[i]     = a.packed + ((int64_t)min(tile0 + j / 2, l.groups * 4 - 1) * l.steps + j % 2) * 1024;
+        }
+        for (int i = 0; i < kLoads - kWLoads; ++i) {
+            const int j = wave * (kLoads - kWLoads) + i;
+            const int n = min(n0 + 8 * j, a.N - 1); // rows behind the last are the last again
+            x_at[i]     = a.x + (int64_t)n * a.x_stride;
+            x_row[i]    = min(lane >> 3, a.N - 1 - n) * (unsigned)a.x_stride;
+        }
+        const unsigned to = ends0 + (turn & 3) * sizeof(Ends);
+        const float*   sw = reinterpret_cast<const float*>(a.packed + l.scales);
+        for (int i = wave; i < kM / 64; i += kWaves) { // 64 rows, all of the gate or all of up
+            const bool up = GATED && i >= kM / 128;
+            const int  at = (GATED ? tile0 * 8 + (up ? i - kM / 128 : i) * 64 : tile0 * 16 + i * 64) + lane;
+            const int  most = l.groups * (GATED ? 32 : 64) - 1;
+            word_to_lds(to + i * 256, sw + (up ? (int64_t)l.groups * 32 : 0) + min(at, most));
+            const uint16_t* bias = up ? a.up_bias : a.bias;
+            if (bias != nullptr)
+                short_to_lds(to + kM * 4 + i * 256, bias + min(at, a.M - 1));
+        }
+        for (int i = kWaves - 1 - wave; i < kN / 64; i += kWaves)
+            word_to_lds(to + kM * 8 + i * 256, a.x_scales + min(n0 + i * 64 + lane, a.N - 1));
+    };
     // The i-th of a wave's loads of a block.  Behind the last 16 columns of X the weights are 0: what is there does not matter.
     auto stage = [&](int i, int block, int buffer) {
         const unsigned to = lds0 + buffer * kStage;
@@ -269,7 +315,7 @@ __global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_
             to_lds(to + (wave * kWLoads + i) * 1024, w_at[i] + (int64_t)block * 2048, lane * 16);
         else
             to_lds(to + (2 * kRows + wave * (kLoads - kWLoads) + i - kWLoads) * 1024,
-                   x_at[i - kWLoads] + min(block * 128 + chunk, last));
+                   x_at[i - kWLoads], x_row[i - kWLoads] + min(block * 128 + chunk, last));
     };
     struct Operands {
         intx4 w[MT], x[NT];
@@ -284,9 +330,11 @@ __global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_
                                                           (c & 7) * 128 + (((4 * half + q) ^ (c & 7)) * 16));
     };
     intx4 sum[MT][NT];
-    for (int t = 0; t < MT; ++t)
-        for (int u = 0; u < NT; ++u)
-            sum[t][u] = 0;
+    auto clear = [&] {
+        for (int t = 0; t < MT; ++t)
+            for (int u = 0; u < NT; ++u)
+                sum[t][u] = 0;
+    };
     // The products of one half in kParts parts, with `between(part)` behind each: loads issued all at once would hold the wave up
     // ahead of its products until the memory pipe has taken them.
     constexpr int kParts = kProducts / 4;
@@ -303,52 +351,80 @@ __global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_
     // Items `part` of `parts` of n, as a range.
 #define W8_SHARE(i, n, part, parts) for (int i = (n) * (part) / (parts); i < (n) * ((part) + 1) / (parts); ++i)
     Operands first, second;
-    for (int i = 0; i < kLoads; ++i)
-        stage(i, 0, 0);
+    // Tile and block of the next load, and how many tiles it has seen; tile, block and number of the next products.
+    int ahead_tile = blockIdx.x, ahead_block = 0, ahead_turn = 0, tile = blockIdx.x, block = 0, turn = 0;
+    auto advance = [&] {
+        if (++ahead_block == blocks) {
+            ahead_block = 0, ahead_tile += gridDim.x, ++ahead_turn;
+            if (ahead_tile < tiles)
+                enter(ahead_tile, ahead_turn);
+        }
+    };
+    enter(tile, 0);
+    for (int s = 0; s < 2; ++s) {
+        if (ahead_tile < tiles)
+            for (int i = 0; i < kLoads; ++i)
+                stage(i, ahead_block, s);
+        advance();
+    }
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    if (blocks > 1)
-        for (int i = 0; i < kLoads; ++i)
-            stage(i, 1, 1);
     for (int i = 0; i < kReads; ++i)
         fetch(first, i, 0, 0);
-    constexpr int kEarly = kParts * 3 / 4; // parts under which operands are read: the rest covers their latency
-    for (int i = 0; i < blocks; ++i) {
-        const int  buffer = i & 1;
-        const bool more = i + 2 < blocks;
+    clear();
+    constexpr int kEarly  = kParts * 3 / 4;                      // parts under which operands are read: the rest covers their latency
+    constexpr int kStores = MT / 4 * NT * (GATED ? 1 : 2);       // of a wave for a tile that is full
+    bool          relaxed = false;                               // the last results' stores may still be under way
+    for (int buffer = 0;; buffer ^= 1) {
+        const bool more = ahead_tile < tiles;
         multiply(first, [&](int part) {
             if (part < kEarly)
                 W8_SHARE(j, kReads, part, kEarly)
                     fetch(second, j, buffer, 1);
         });
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        // The next block has come: its loads are older than the stores, which are counted with them.
+        if (relaxed)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kStores) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        relaxed = false;
         multiply(second, [&](int part) {
             if (part < kEarly)
                 W8_SHARE(j, kReads, part, kEarly) // behind the last block stale bytes, which nothing takes
                     fetch(first, j, buffer ^ 1, 0);
             if (more)
                 W8_SHARE(j, kLoads, part, kParts)
-                    stage(j, i + 2, buffer);
+                    stage(j, ahead_block, buffer);
         });
+        if (++block == blocks) {
+            int row, column;
+            place8(tile, row_tiles, column_tiles, row, column);
+            const Ends& e = ends[turn & 3];
+            each<MT / 4>([&](auto g) {
+                const int group = wm * (MT / 4) + g;
+                each<GATED ? 1 : 2>([&](auto h) {
+                    const int                j = GATED ? group * 32 + 8 * q : group * 64 + 16 * q + 8 * h;
+                    const Tail8<BF16, GATED> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
+                    each<NT>([&](auto u) {
+                        const int n = column * kN + (wn * NT + u) * 16 + c;
+                        if (n >= a.N)
+                            return;
+                        int v[16];
+                        for (int i = 0; i < 16; ++i)
+                            v[i] = sum[g * 4 + i / 4][u][i % 4];
+                        tail.store(a, n, e.sx[(wn * NT + u) * 16 + c], v + 8 * h, v + 8);
+                    });
+                });
+            });
+            // With all its stores made, and blocks enough that the loads of a tile's ends are waited for by another barrier.
+            relaxed = (row + 1) * (GATED ? kM / 2 : kM) <= a.M && (column + 1) * kN <= a.N && blocks > 2;
+            block = 0, tile += gridDim.x, ++turn;
+            if (tile >= tiles)
+                return;
+            clear();
+        }
+        advance();
     }
 #undef W8_SHARE
-
-    each<MT / 4>([&](auto g) {
-        const int                group = (tile0 + wm * MT) / 4 + g, m = first_row8<GATED>(group, q);
-        const Tail8<BF16, GATED> one(a, l, m);
-        const Tail8<BF16, GATED> two(a, l, GATED ? a.M : m + 8);
-        each<NT>([&](auto u) {
-            const int n = n0 + (wn * NT + u) * 16 + c;
-            if (n >= a.N)
-                return;
-            int v[16];
-            for (int i = 0; i < 16; ++i)
-                v[i] = sum[g * 4 + i / 4][u][i % 4];
-            const float sx = a.x_scales[n];
-            one.store(a, n, sx, v, v + 8);
-            if (!GATED)
-                two.store(a, n, sx, v + 8, nullptr);
-        });
-    });
 }
 
 template <bool BF16, bool GATED>
@@ -357,7 +433,8 @@ int run_product(hipStream_t stream, const ProductArgs& a)
     const Layout8 l = layout8(a.M, a.K, GATED);
     if (a.N > 64) {
         const int rows = (l.groups * 4 + 15) / 16, cols = (a.N + 255) / 256;
-        return launch(w8_tiles<BF16, GATED, 8, 4, 2, 4>, dim3((unsigned)rows * cols, 1, 1), dim3(512, 1, 1), stream, a, rows, cols);
+        return launch(w8_tiles<BF16, GATED, 8, 4, 2, 4>, dim3((unsigned)std::min(rows * cols, 256), 1, 1), dim3(512, 1, 1),
+                      stream, a, rows, cols);
     }
     return launch(w8_product<BF16, GATED>, dim3((unsigned)l.groups, (unsigned)(a.N + 15) / 16, 1), dim3(256, 1, 1), stream, a);
 }
