@@ -9,7 +9,9 @@
 // results: after the product a lane r + 16 q holds, of column r of X, rows 4 q .. 4 q + 3 of every tile.  Row 16 q + 4 t + i of the group
 // is put at row 4 q + i of tile t, so that these are 16 consecutive outputs, 32 bytes of Y.  In gated weights tiles 0 and 1 hold 32
 // rows of the gate (row 8 q + 4 t + i), tiles 2 and 3 the same rows of up: both sums of an output meet in one lane.
-// K is filled up with zeros to a multiple of 128: what X has there does not matter.
+// K is filled up with zeros to a multiple of 128: what X has there does not matter.  Of every 128 columns the groups lie one behind the
+// other, 8 KB each, two steps of four tiles: workgroups that are equally far along K read one stretch of memory, where rows that
+// lay whole would be a power of two apart and meet on the same channels.
 #include "w8_common.hiph"
 
 #include <algorithm>
@@ -19,6 +21,8 @@ namespace decode {
 namespace {
 
 constexpr int kMaxRows8 = 1 << 24;
+constexpr int kGroup8   = 8192; // bytes of a group's 128 columns
+constexpr int kMaxN8    = 16 * 65535;
 
 struct Layout8 {
     int     groups, steps; // groups of 64 packed rows, steps of 64 columns (an even number)
@@ -60,7 +64,7 @@ __global__ __launch_bounds__(64) void w8_pack(PackArgs a)
         if (row < a.M && k < a.K)
             out[b / 4] |= (unsigned)(uint8_t)src[k] << (8 * (b % 4));
     }
-    reinterpret_cast<uintx4*>(a.packed)[(((int64_t)group * 4 + tile) * l.steps + step) * 64 + lane] = out;
+    reinterpret_cast<uintx4*>(a.packed + ((int64_t)(step / 2) * l.groups + group) * kGroup8)[(step % 2 * 4 + tile) * 64 + lane] = out;
     if (step == 0 && tile == 0) { // 64 scales: of the group's rows, or of 32 rows of the gate and of up
         const int  per = gated ? 32 : 64, m = group * per + lane % per;
         const bool u = gated && lane >= 32;
@@ -76,64 +80,75 @@ struct ProductArgs {
     int64_t        x_stride;
     uint16_t*      y;
     const uint16_t *bias, *up_bias;
-    int            M, N, K, act;
+    int*           part; // sums of the shares of K, [share][N][packed row]; null where K is not split
+    int            M, N, K, act, bf16;
+    int            shares, per; // shares of K, blocks of 128 columns in each but the last
 };
 
-// ReLU, GELU (tanh form) or SiLU of eight sums.  The last two are y / (1 + exp(-z)), with z = 2 sqrt(2/pi) (y + 0.044715 y^3), since
+// ReLU, GELU (tanh form) or SiLU of W sums.  The last two are y / (1 + exp(-z)), with z = 2 sqrt(2/pi) (y + 0.044715 y^3), since
 // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), or z = y; far from 0 they end at 0 and y.  The reciprocal's last bit is far below 16 bits.
+template <int W>
 __device__ __forceinline__ void activate8(float* y, int act)
 {
     if (act == 1) {
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < W; ++i)
             y[i] = y[i] < 0.f ? 0.f : y[i]; // a NaN stays one
     } else if (act > 1) {
         const float cube = act == 2 ? 1.5957691216057308f * 0.044715f : 0.f, one = act == 2 ? 1.5957691216057308f : 1.f;
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < W; ++i) {
             const float z = y[i] * (one + cube * y[i] * y[i]);
             y[i]          = y[i] * __builtin_amdgcn_rcpf(1.f + __expf(-z));
         }
     }
 }
 
-// Eight 16-bit numbers from p on, of which `left` are there.
-__device__ __forceinline__ shortx8 bias8(const uint16_t* p, int left)
-{
-    if (left >= 8)
-        return *reinterpret_cast<const loose8*>(p);
-    shortx8 v = 0;
-    for (int i = 0; i < 7; ++i)
-        if (i < left)
-            v[i] = p[i];
-    return v;
-}
+template <int W>
+struct Loose { // W 16-bit numbers at any alignment of theirs
+    typedef uint16_t type __attribute__((ext_vector_type(W)));
+    typedef type __attribute__((aligned(2))) loose;
+};
 
-// What the outputs of eight consecutive rows from `m` on have in common over the columns.
-template <bool BF16, bool GATED>
+// What W consecutive outputs from row `m` on have in common over the columns.
+template <bool GATED, int W>
 struct Tail8 {
-    float sw[8], su[8], b[8], bu[8];
+    float sw[W], su[W], b[W], bu[W];
     int   m, left;
+
+    static __device__ __forceinline__ void biases(float* to, const uint16_t* p, int left, bool bf16)
+    {
+        typename Loose<W>::type v = 0;
+        if (p != nullptr && left >= W)
+            v = *reinterpret_cast<const typename Loose<W>::loose*>(p);
+        else if (p != nullptr)
+            for (int i = 0; i < W - 1; ++i)
+                if (i < left)
+                    v[i] = p[i];
+        for (int i = 0; i < W; ++i)
+            to[i] = from16(v[i], bf16);
+    }
 
     __device__ __forceinline__ Tail8(const ProductArgs& a, const Layout8& l, int row) : m(row), left(a.M - row)
     {
         if (left <= 0)
             return;
-        const float*  s  = reinterpret_cast<const float*>(a.packed + l.scales) + m; // the layout's rows go past M
-        const shortx8 v  = a.bias != nullptr ? bias8(a.bias + m, left) : (shortx8)0;
-        const shortx8 vu = GATED && a.up_bias != nullptr ? bias8(a.up_bias + m, left) : (shortx8)0;
-        for (int i = 0; i < 8; ++i) {
-            sw[i] = s[i], b[i] = from16(v[i], BF16);
+        const float* s = reinterpret_cast<const float*>(a.packed + l.scales) + m; // the layout's rows go past M
+        biases(b, a.bias == nullptr ? nullptr : a.bias + m, left, a.bf16);
+        if (GATED)
+            biases(bu, a.up_bias == nullptr ? nullptr : a.up_bias + m, left, a.bf16);
+        for (int i = 0; i < W; ++i) {
+            sw[i] = s[i];
             if (GATED)
-                su[i] = s[i + (int64_t)l.groups * 32], bu[i] = from16(vu[i], BF16);
+                su[i] = s[i + (int64_t)l.groups * 32];
         }
     }
 
     // From LDS: scales, and biases as 32-bit words of 16 bits; those of up `up` words behind the gate's.
     __device__ __forceinline__ Tail8(const ProductArgs& a, int row, const float* s, const unsigned* bias, int up) : m(row), left(a.M - row)
     {
-        for (int i = 0; i < 8; ++i) {
-            sw[i] = s[i], b[i] = a.bias != nullptr ? from16((uint16_t)bias[i], BF16) : 0.f;
+        for (int i = 0; i < W; ++i) {
+            sw[i] = s[i], b[i] = a.bias != nullptr ? from16((uint16_t)bias[i], a.bf16) : 0.f;
             if (GATED)
-                su[i] = s[up + i], bu[i] = a.up_bias != nullptr ? from16((uint16_t)bias[up + i], BF16) : 0.f;
+                su[i] = s[up + i], bu[i] = a.up_bias != nullptr ? from16((uint16_t)bias[up + i], a.bf16) : 0.f;
         }
     }
 
@@ -142,67 +157,147 @@ struct Tail8 {
     {
         if (left <= 0)
             return;
-        float y[8];
-        for (int i = 0; i < 8; ++i)
+        float y[W];
+        for (int i = 0; i < W; ++i)
             y[i] = (float)sum[i] * sw[i] * sx + b[i];
-        activate8(y, a.act);
+        activate8<W>(y, a.act);
         if constexpr (GATED)
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < W; ++i)
                 y[i] *= (float)up[i] * su[i] * sx + bu[i];
-        shortx8 out;
-        for (int i = 0; i < 8; ++i)
-            out[i] = BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y[i]) : __builtin_bit_cast(uint16_t, (_Float16)y[i]);
+        typename Loose<W>::type out;
+        if (a.bf16)
+            for (int i = 0; i < W; ++i)
+                out[i] = __builtin_bit_cast(uint16_t, (__bf16)y[i]);
+        else
+            for (int i = 0; i < W; ++i)
+                out[i] = __builtin_bit_cast(uint16_t, (_Float16)y[i]);
         uint16_t* to = a.y + (int64_t)n * a.M + m;
-        if (left >= 8) {
-            *reinterpret_cast<loose8*>(to) = out;
+        if (left >= W) {
+            *reinterpret_cast<typename Loose<W>::loose*>(to) = out;
             return;
         }
-        for (int i = 0; i < 7; ++i)
+        for (int i = 0; i < W - 1; ++i)
             if (i < left)
                 to[i] = out[i];
     }
 };
 
-// Row of its group that a lane's outputs begin at: 16 of them, or 8 of a gated product.
+// The sums of a share of K: of column n, tile t of a group, rows 4 q .. 4 q + 3.  The order within a group is that of the outputs, of
+// a gated product 32 of the gate and 32 of up.
 template <bool GATED>
-__device__ __forceinline__ int first_row8(int group, int q)
+__device__ __forceinline__ void store_part(const ProductArgs& a, int groups, int share, int n, int group, int t, int q, intx4 sum)
 {
-    return GATED ? group * 32 + 8 * q : group * 64 + 16 * q;
+    const int at = GATED ? t / 2 * 32 + 8 * q + t % 2 * 4 : 16 * q + 4 * t;
+    *reinterpret_cast<intx4*>(a.part + (((int64_t)share * a.N + n) * groups + group) * 64 + at) = sum;
 }
 
-// A workgroup takes one group of 64 packed rows and 16 columns of X; its four waves take every fourth step of K and meet in LDS.
-template <bool BF16, bool GATED>
-__global__ __launch_bounds__(256) void w8_product(ProductArgs a)
+// Eight outputs a thread from the sums of all shares.
+template <bool GATED>
+__global__ __launch_bounds__(256) void w8_join(ProductArgs a)
 {
-    __shared__ intx4 part[4][4][64];
-    const Layout8    l    = layout8(a.M, a.K, GATED);
-    const int        lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int        group = blockIdx.x, n = blockIdx.y * 16 + (lane & 15), q = lane >> 4;
-    const int8_t*    x     = a.x + (int64_t)min(n, a.N - 1) * a.x_stride;
-    const int        last  = (a.K - 1) / 16; // the last 16 columns that X has; behind them the weights are 0
-    const intx4*     w     = reinterpret_cast<const intx4*>(a.packed) + (int64_t)group * 4 * l.steps * 64 + lane;
-    intx4            sum[4] = {0, 0, 0, 0};
-    for (int s = wave; s < l.steps; s += 4) {
-        const intx4 b = *reinterpret_cast<const intx4*>(x + 16 * min(4 * s + q, last));
-        for (int t = 0; t < 4; ++t)
-            sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[((int64_t)t * l.steps + s) * 64], b, sum[t], 0, 0, 0);
-    }
-    for (int t = 0; t < 4; ++t)
-        part[wave][t][lane] = sum[t];
-    __syncthreads();
-    if (wave > 0 || n >= a.N)
+    constexpr int kPer  = GATED ? 4 : 8; // threads for a group's outputs
+    const Layout8 l     = layout8(a.M, a.K, GATED);
+    const int64_t id    = (int64_t)blockIdx.x * 256 + threadIdx.x, unit = id / kPer;
+    const int     n     = (int)(unit / l.groups), group = (int)(unit % l.groups), j = (int)(id % kPer) * 8;
+    if (n >= a.N)
         return;
-    for (int t = 0; t < 4; ++t)
-        for (int w = 1; w < 4; ++w)
-            sum[t] += part[w][t][lane];
+    const intx4*  p    = reinterpret_cast<const intx4*>(a.part + ((int64_t)n * l.groups + group) * 64 + j);
+    const int64_t next = (int64_t)a.N * l.groups * 16;
+    intx4         sum[4] = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < a.shares; ++s) {
+        sum[0] += p[s * next], sum[1] += p[s * next + 1];
+        if (GATED)
+            sum[2] += p[s * next + 8], sum[3] += p[s * next + 9];
+    }
     int v[16];
     for (int i = 0; i < 16; ++i)
         v[i] = sum[i / 4][i % 4];
-    const float sx = a.x_scales[n];
-    const int   m  = first_row8<GATED>(group, q);
-    Tail8<BF16, GATED>(a, l, m).store(a, n, sx, v, v + 8);
-    if constexpr (!GATED)
-        Tail8<BF16, false>(a, l, m + 8).store(a, n, sx, v + 8, nullptr);
+    Tail8<GATED, 8>(a, l, group * (GATED ? 32 : 64) + j).store(a, n, a.x_scales[n], v, v + 8);
+}
+
+// Few columns: a workgroup of kNarrowWaves waves takes R row tiles and NT column tiles, its waves every kNarrowWaves-th block of 128 columns of
+// its share of K.  W is read once and goes from memory into the matrix operands as it is packed, X by way of the caches; a wave
+// has D blocks of both in flight.  The waves' sums meet in LDS.  A gated product has rows of the gate and of up in every
+// workgroup: tiles t and t + 2 with R = 2.
+constexpr int kNarrowWaves = 8;
+
+template <bool GATED, int R, int NT, int D>
+__global__ __launch_bounds__(64 * kNarrowWaves) void w8_narrow(ProductArgs a, int column_tiles)
+{
+    static_assert(!GATED || R >= 2);
+    __shared__ int total[R * NT][kWave][4];
+    const Layout8  l    = layout8(a.M, a.K, GATED);
+    const int      lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), c = lane & 15, q = lane >> 4;
+    const int      unit = blockIdx.x / column_tiles, n0 = blockIdx.x % column_tiles * (NT * 16), share = blockIdx.y;
+    const int      group = unit * R / 4, first = unit % (4 / R) * (GATED ? 1 : R), apart = GATED && R == 2 ? 2 : 1; // of its row tiles
+    const int      from = share * a.per, to = min(from + a.per, l.steps / 2);
+    const int      last = (a.K - 1) / 16 * 16;
+    for (int i = threadIdx.x; i < R * NT * kWave; i += 64 * kNarrowWaves)
+        reinterpret_cast<intx4*>(total)[i] = 0;
+    __syncthreads();
+
+    const intx4*  w = reinterpret_cast<const intx4*>(a.packed + (int64_t)group * kGroup8) + first * 64 + lane;
+    const int8_t* x[NT];
+    for (int u = 0; u < NT; ++u) // rows behind the last are the last again
+        x[u] = a.x + (int64_t)min(n0 + u * 16 + c, a.N - 1) * a.x_stride;
+    struct Block {
+        intx4 w[2][R], x[2][NT];
+    };
+    Block held[D];
+    auto  fetch = [&](Block& h, int block) {
+        for (int s = 0; s < 2; ++s) {
+            for (int t = 0; t < R; ++t)
+                h.w[s][t] = __builtin_nontemporal_load(w + (int64_t)block * l.groups * (kGroup8 / 16) + (s * 4 + t * apart) * 64);
+            for (int u = 0; u < NT; ++u) // behind the last 16 columns of X the weights are 0
+                h.x[s][u] = *reinterpret_cast<const intx4*>(x[u] + min(block * 128 + s * 64 + 16 * q, last));
+        }
+    };
+    intx4 sum[R][NT];
+    for (int t = 0; t < R; ++t)
+        for (int u = 0; u < NT; ++u)
+            sum[t][u] = 0;
+    for (int d = 0; d < D; ++d)
+        if (from + wave + d * kNarrowWaves < to)
+            fetch(held[d], from + wave + d * kNarrowWaves);
+    for (int block = from + wave; block < to;) {
+#pragma unroll
+        for (int d = 0; d < D; ++d, block += kNarrowWaves) {
+            if (block >= to)
+                break;
+            for (int s = 0; s < 2; ++s)
+                for (int u = 0; u < NT; ++u)
+                    for (int t = 0; t < R; ++t)
+                        sum[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(held[d].w[s][t], held[d].x[s][u], sum[t][u], 0, 0, 0);
+            if (block + D * kNarrowWaves < to)
+                fetch(held[d], block + D * kNarrowWaves);
+        }
+    }
+    for (int t = 0; t < R; ++t)
+        for (int u = 0; u < NT; ++u)
+            for (int i = 0; i < 4; ++i)
+                __hip_atomic_fetch_add(&total[t * NT + u][lane][i], sum[t][u][i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    __syncthreads();
+    if (wave >= NT) // wave u ends column tile u
+        return;
+    const int n = n0 + wave * 16 + c;
+    if (n >= a.N)
+        return;
+    int v[4 * R];
+    for (int t = 0; t < R; ++t) {
+        const intx4 s = *reinterpret_cast<const intx4*>(total[t * NT + wave][lane]);
+        if (a.part != nullptr)
+            store_part<GATED>(a, l.groups, share, n, group, first + t * apart, q, s);
+        for (int i = 0; i < 4; ++i)
+            v[4 * t + i] = s[i];
+    }
+    if (a.part != nullptr)
+        return;
+    constexpr int W  = GATED ? 2 * R : (R == 1 ? 4 : 8); // consecutive outputs of a lane
+    const float   sx = a.x_scales[n];
+    const int     m  = GATED ? group * 32 + 8 * q + 4 * first : group * 64 + 16 * q + 4 * first;
+    for (int i = 0; i < (GATED ? 1 : R * 4 / W); ++i)
+        Tail8<GATED, W>(a, l, m + i * W).store(a, n, sx, v + i * W, v + 2 * R);
 }
 
 // f(0) .. f(N - 1) with constants: arrays of registers have no others for an index.
@@ -234,12 +329,14 @@ __device__ __forceinline__ void short_to_lds(unsigned lds, const void* address)
 }
 
 // Workgroups are dealt to the eight dies in turn, each with an L2 of its own: consecutive numbers on one die, and there a band of
-// kBand row tiles by as many column tiles as run at once.
-__device__ __forceinline__ void place8(int id, int row_tiles, int column_tiles, int& row, int& column)
+// kBand row tiles by as many column tiles as run at once; shares of K one after another.
+__device__ __forceinline__ void place8(int id, int row_tiles, int column_tiles, int shares, int& row, int& column, int& share)
 {
     constexpr int kBand = 8;
-    const int     total = row_tiles * column_tiles, xcd = id % 8, rest = total % 8;
-    const int     at   = xcd * (total / 8) + min(xcd, rest) + id / 8;
+    const int     one = row_tiles * column_tiles, total = one * shares, xcd = id % 8, rest = total % 8;
+    int           at = xcd * (total / 8) + min(xcd, rest) + id / 8;
+    share            = __builtin_amdgcn_readfirstlane(at / one);
+    at -= share * one;
     const int     band = at / (kBand * column_tiles), first = band * kBand, height = min(kBand, row_tiles - first);
     const int     in   = at - first * column_tiles;
     // divisions are done by vector instructions: back to scalars, which the addresses are made of
@@ -247,54 +344,59 @@ __device__ __forceinline__ void place8(int id, int row_tiles, int column_tiles, 
 }
 
 // A workgroup of WM x WN waves takes WM MT x WN NT tiles of 16 x 16 outputs (packed rows x rows of X), a wave MT x NT of them.  K goes by in
-// blocks of 128 through two buffers in LDS: W's blocks lie there as they are packed, one operand a KB; of X 8 rows lie in a KB,
+// blocks of 128 through a ring of S places in LDS: W's blocks lie there as they are packed, one operand a KB; of X 8 rows lie in a KB,
 // row r's chunk c of 16 bytes at place 8 r + (c ^ r), which the matrix operands' reads find without bank conflicts.
-// While the products of a block's first half run, the second half's operands are read; then the waves meet, the buffer that
-// all have read takes the block after next, and the next block's first operands are read under the second half's products.
+// While the products of a block's first half run, the second half's operands are read; then the waves meet, the place that
+// all have read takes the block S further on, and the next block's first operands are read under the second half's products.
 // A workgroup stays on its CU and takes every gridDim-th tile: the blocks of all its tiles are one stream, so that the next tile is
 // loaded while the results of the last are written, and a tile costs its products alone.
-template <bool BF16, bool GATED, int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_tiles, int column_tiles)
+template <bool GATED, int MT, int NT, int WM, int WN, int S>
+__global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs a, int row_tiles, int column_tiles)
 {
-    constexpr int kWaves = WM * WN, kRows = WM * MT, kCols = WN * NT * 2, kStage = (2 * kRows + kCols) * 1024; // tiles of W, KBs of X
-    constexpr int kLoads = (2 * kRows + kCols) / kWaves, kWLoads = 2 * kRows / kWaves;
-    constexpr int kM = kRows * 16, kN = WN * NT * 16; // packed rows, rows of X
-    static_assert(2 * kRows % kWaves == 0 && kCols % kWaves == 0 && MT % 4 == 0 && kM % 64 == 0 && kN % 64 == 0);
+    constexpr int kWaves = WM * WN, kRows = WM * MT, kCols = WN * NT, kStage = (kRows + kCols) * 2048; // tiles of W, of X
+    constexpr int kLoads = 2 * (kRows + kCols) / kWaves;
+    constexpr int kM = kRows * 16, kN = kCols * 16; // packed rows, rows of X
+    constexpr int kEnds = S + 2; // loads are at most S + 1 tiles ahead of the products
+    static_assert(2 * (kRows + kCols) % kWaves == 0 && MT % 4 == 0 && kM % 128 == 0 && kN % 64 == 0 && S >= 2);
     struct Ends { // of a tile: scales and biases of its rows (of the gate, then of up), scales of its rows of X
         float    sw[kM];
         unsigned b[kM];
         float    sx[kN];
     };
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][kStage];
-    __shared__ __attribute__((aligned(16))) Ends      ends[4]; // loads are at most two tiles ahead of the products
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S][kStage];
+    __shared__ __attribute__((aligned(16))) Ends      ends[kEnds];
     const Layout8 l    = layout8(a.M, a.K, GATED);
     const int     lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int     q = lane >> 4, c = lane & 15, wm = wave / WN, wn = wave % WN, blocks = l.steps / 2;
-    const int     tiles = row_tiles * column_tiles;
+    const int     q = lane >> 4, c = lane & 15, wm = wave / WN, wn = wave % WN;
+    const int     tiles = row_tiles * column_tiles * a.shares;
 
-    // What a wave brings of every block: KBs of W first, then of X.
-    const uint8_t* w_at[kWLoads];
-    const int8_t*  x_at[kLoads - kWLoads];
-    unsigned       x_row[kLoads - kWLoads];
+    // What a wave brings of every block: KBs wave, wave + kWaves, ... of W's, as they are packed, then of X's.
+    const uint8_t* from[kLoads];
+    unsigned       off[kLoads];
     auto address = [](const void* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p; };
     const unsigned lds0 = address(lds), ends0 = address(ends);
     const int      chunk = 16 * ((lane & 7) ^ (lane >> 3)), last = (a.K - 1) / 16 * 16;
+    // Tile and block of the next load, the end of its blocks, and how many tiles it has seen; tile and number of the next products, and
+    // how many blocks of it are left.
+    int ahead_tile = blockIdx.x, ahead_block, ahead_end, ahead_turn = 0, tile = blockIdx.x, left, turn = 0;
     // Turns the loads to a tile, the `turn`-th, and brings its ends.
     auto enter = [&](int tile, int turn) {
-        int row, column;
-        place8(tile, row_tiles, column_tiles, row, column);
+        int row, column, share;
+        place8(tile, row_tiles, column_tiles, a.shares, row, column, share);
         const int tile0 = row * kRows, n0 = column * kN;
-        for (int i = 0; i < kWLoads; ++i) { // tiles behind the last are the last again: computed, not stored
-            const int j = wave * kWLoads + i;
-            w_at[i]     = a.packed + ((int64_t)min(tile0 + j / 2, l.groups * 4 - 1) * l.steps + j % 2) * 1024;
+        ahead_block = share * a.per, ahead_end = min(ahead_block + a.per, l.steps / 2);
+        for (int i = 0; i < kLoads; ++i) { // groups and rows behind the last are the last again: computed, not stored
+            const int j = wave + i * kWaves;
+            if (j < 2 * kRows) {
+                from[i] = a.packed + (int64_t)min(tile0 / 4 + j / 8, l.groups - 1) * kGroup8 + j % 8 * 1024;
+                off[i]  = lane * 16;
+            } else {
+                const int n = min(n0 + 8 * (j - 2 * kRows), a.N - 1);
+                from[i]     = reinterpret_cast<const uint8_t*>(a.x) + (int64_t)n * a.x_stride;
+                off[i]      = min(lane >> 3, a.N - 1 - n) * (unsigned)a.x_stride;
+            }
         }
-        for (int i = 0; i < kLoads - kWLoads; ++i) {
-            const int j = wave * (kLoads - kWLoads) + i;
-            const int n = min(n0 + 8 * j, a.N - 1); // rows behind the last are the last again
-            x_at[i]     = a.x + (int64_t)n * a.x_stride;
-            x_row[i]    = min(lane >> 3, a.N - 1 - n) * (unsigned)a.x_stride;
-        }
-        const unsigned to = ends0 + (turn & 3) * sizeof(Ends);
+        const unsigned to = ends0 + turn % kEnds * (unsigned)sizeof(Ends);
         const float*   sw = reinterpret_cast<const float*>(a.packed + l.scales);
         for (int i = wave; i < kM / 64; i += kWaves) { // 64 rows, all of the gate or all of up
             const bool up = GATED && i >= kM / 128;
@@ -308,25 +410,26 @@ __global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_
         for (int i = kWaves - 1 - wave; i < kN / 64; i += kWaves)
             word_to_lds(to + kM * 8 + i * 256, a.x_scales + min(n0 + i * 64 + lane, a.N - 1));
     };
+    const int64_t block_bytes = (int64_t)l.groups * kGroup8;
     // The i-th of a wave's loads of a block.  Behind the last 16 columns of X the weights are 0: what is there does not matter.
-    auto stage = [&](int i, int block, int buffer) {
-        const unsigned to = lds0 + buffer * kStage;
-        if (i < kWLoads)
-            to_lds(to + (wave * kWLoads + i) * 1024, w_at[i] + (int64_t)block * 2048, lane * 16);
+    auto stage = [&](int i, int block, int place) {
+        const int      j  = wave + i * kWaves;
+        const unsigned to = lds0 + place * kStage + j * 1024;
+        if ((i + 1) * kWaves <= 2 * kRows || j < 2 * kRows)
+            to_lds(to, from[i] + block * block_bytes, off[i]);
         else
-            to_lds(to + (2 * kRows + wave * (kLoads - kWLoads) + i - kWLoads) * 1024,
-                   x_at[i - kWLoads], x_row[i - kWLoads] + min(block * 128 + chunk, last));
+            to_lds(to, from[i], off[i] + min(block * 128 + chunk, last));
     };
     struct Operands {
         intx4 w[MT], x[NT];
     };
     constexpr int kReads = MT + NT, kProducts = MT * NT;
-    auto fetch = [&](Operands& o, int i, int buffer, int half) {
-        const uint8_t* from = lds[buffer];
+    auto fetch = [&](Operands& o, int i, int place, int half) {
+        const uint8_t* p = lds[place];
         if (i < MT)
-            o.w[i] = *reinterpret_cast<const intx4*>(from + ((wm * MT + i) * 2 + half) * 1024 + lane * 16);
+            o.w[i] = *reinterpret_cast<const intx4*>(p + ((wm * MT + i) / 4 * 8 + half * 4 + i % 4) * 1024 + lane * 16);
         else
-            o.x[i - MT] = *reinterpret_cast<const intx4*>(from + (2 * kRows + (wn * NT + i - MT) * 2 + (c >> 3)) * 1024 +
+            o.x[i - MT] = *reinterpret_cast<const intx4*>(p + (2 * kRows + (wn * NT + i - MT) * 2 + (c >> 3)) * 1024 +
                                                           (c & 7) * 128 + (((4 * half + q) ^ (c & 7)) * 16));
     };
     intx4 sum[MT][NT];
@@ -350,93 +453,219 @@ __global__ __launch_bounds__(64 * WM * WN) void w8_tiles(ProductArgs a, int row_
     };
     // Items `part` of `parts` of n, as a range.
 #define W8_SHARE(i, n, part, parts) for (int i = (n) * (part) / (parts); i < (n) * ((part) + 1) / (parts); ++i)
-    Operands first, second;
-    // Tile and block of the next load, and how many tiles it has seen; tile, block and number of the next products.
-    int ahead_tile = blockIdx.x, ahead_block = 0, ahead_turn = 0, tile = blockIdx.x, block = 0, turn = 0;
     auto advance = [&] {
-        if (++ahead_block == blocks) {
-            ahead_block = 0, ahead_tile += gridDim.x, ++ahead_turn;
+        if (++ahead_block >= ahead_end) {
+            ahead_tile += gridDim.x, ++ahead_turn;
             if (ahead_tile < tiles)
                 enter(ahead_tile, ahead_turn);
         }
     };
+    auto begin = [&] { // blocks of the tile that the products come to
+        int row, column, share;
+        place8(tile, row_tiles, column_tiles, a.shares, row, column, share);
+        left = min(a.per, l.steps / 2 - share * a.per);
+    };
     enter(tile, 0);
-    for (int s = 0; s < 2; ++s) {
-        if (ahead_tile < tiles)
+    begin();
+    for (int s = 0; s < S; ++s) {
+        if (ahead_tile < tiles) {
             for (int i = 0; i < kLoads; ++i)
                 stage(i, ahead_block, s);
-        advance();
+            advance();
+        }
     }
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (ahead_tile < tiles)
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * kLoads) : "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    Operands first, second;
     for (int i = 0; i < kReads; ++i)
         fetch(first, i, 0, 0);
     clear();
-    constexpr int kEarly  = kParts * 3 / 4;                      // parts under which operands are read: the rest covers their latency
-    constexpr int kStores = MT / 4 * NT * (GATED ? 1 : 2);       // of a wave for a tile that is full
-    bool          relaxed = false;                               // the last results' stores may still be under way
-    for (int buffer = 0;; buffer ^= 1) {
-        const bool more = ahead_tile < tiles;
+    constexpr int kEarly  = kParts > 2 ? kParts * 3 / 4 : kParts; // parts under which operands are read: the rest covers their latency
+    constexpr int kStores = MT / 4 * NT * (GATED ? 1 : 2);  // of a wave for a tile that is full
+    constexpr int kAway   = (S - 2) * kLoads;               // a wave's loads of the blocks behind the next
+    static_assert(kAway + kStores < 64);
+    int place = 0, relaxed = 0; // relaxed: barriers ahead of which the last results' stores may still be under way
+    for (;;) {
+const bool more = ahead_tile < tiles;
         multiply(first, [&](int part) {
             if (part < kEarly)
                 W8_SHARE(j, kReads, part, kEarly)
-                    fetch(second, j, buffer, 1);
+                    fetch(second, j, place, 1);
         });
-        // The next block has come: its loads are older than the stores, which are counted with them.
-        if (relaxed)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kStores) : "memory");
-        else
+        // The next block has come.  Loads and stores are counted in their order: behind it are kAway loads, and stores.
+        if (!more)
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        relaxed = false;
+        else if (relaxed > 0)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kAway + kStores) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kAway) : "memory");
+        --relaxed;
+        const int next = place + 1 == S ? 0 : place + 1;
         multiply(second, [&](int part) {
             if (part < kEarly)
                 W8_SHARE(j, kReads, part, kEarly) // behind the last block stale bytes, which nothing takes
-                    fetch(first, j, buffer ^ 1, 0);
+                    fetch(first, j, next, 0);
             if (more)
                 W8_SHARE(j, kLoads, part, kParts)
-                    stage(j, ahead_block, buffer);
+                    stage(j, ahead_block, place);
         });
-        if (++block == blocks) {
-            int row, column;
-            place8(tile, row_tiles, column_tiles, row, column);
-            const Ends& e = ends[turn & 3];
-            each<MT / 4>([&](auto g) {
-                const int group = wm * (MT / 4) + g;
-                each<GATED ? 1 : 2>([&](auto h) {
-                    const int                j = GATED ? group * 32 + 8 * q : group * 64 + 16 * q + 8 * h;
-                    const Tail8<BF16, GATED> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
-                    each<NT>([&](auto u) {
-                        const int n = column * kN + (wn * NT + u) * 16 + c;
-                        if (n >= a.N)
-                            return;
-                        int v[16];
-                        for (int i = 0; i < 16; ++i)
-                            v[i] = sum[g * 4 + i / 4][u][i % 4];
-                        tail.store(a, n, e.sx[(wn * NT + u) * 16 + c], v + 8 * h, v + 8);
+        if (more)
+            advance();
+        place = next;
+        --left;
+        if (left == 0) {
+            int row, column, share;
+            place8(tile, row_tiles, column_tiles, a.shares, row, column, share);
+            const Ends& e = ends[turn % kEnds];
+            if (a.part == nullptr) {
+                each<MT / 4>([&](auto g) {
+                    const int group = wm * (MT / 4) + g;
+                    each<GATED ? 1 : 2>([&](auto h) {
+                        const int             j = GATED ? group * 32 + 8 * q : group * 64 + 16 * q + 8 * h;
+                        const Tail8<GATED, 8> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
+                        each<NT>([&](auto u) {
+                            const int n = column * kN + (wn * NT + u) * 16 + c;
+                            if (n >= a.N)
+                                return;
+                            int v[16];
+                            for (int i = 0; i < 16; ++i)
+                                v[i] = sum[g * 4 + i / 4][u][i % 4];
+                            tail.store(a, n, e.sx[(wn * NT + u) * 16 + c], v + 8 * h, v + 8);
+                        });
                     });
                 });
-            });
-            // With all its stores made, and blocks enough that the loads of a tile's ends are waited for by another barrier.
-            relaxed = (row + 1) * (GATED ? kM / 2 : kM) <= a.M && (column + 1) * kN <= a.N && blocks > 2;
-            block = 0, tile += gridDim.x, ++turn;
+                // With all its stores made: of the barriers that wait for loads older than they are.
+                relaxed = (row + 1) * (GATED ? kM / 2 : kM) <= a.M && (column + 1) * kN <= a.N ? S - 1 : 0;
+            } else {
+                each<NT>([&](auto u) {
+                    const int n = column * kN + (wn * NT + u) * 16 + c;
+                    each<MT>([&](auto t) {
+                        const int group = row * (kM / 64) + wm * (MT / 4) + t / 4;
+                        if (n < a.N && group < l.groups)
+                            store_part<GATED>(a, l.groups, share, n, group, t % 4, q, sum[t][u]);
+                    });
+                });
+            }
+            tile += gridDim.x, ++turn;
             if (tile >= tiles)
                 return;
+            begin();
             clear();
         }
-        advance();
     }
 #undef W8_SHARE
 }
 
-template <bool BF16, bool GATED>
-int run_product(hipStream_t stream, const ProductArgs& a)
+// How a call runs.
+struct Plan8 {
+    int kind;        // 0: w8_narrow, otherwise a w8_tiles of kTiles[kind - 1]
+    int rows, cols;  // row and column tiles of 16 that a workgroup takes
+    int shares, per; // shares of K, blocks of 128 columns in each
+};
+
+struct Tiles8 {
+    int rows, cols, resident; // workgroups that fit a CU
+};
+constexpr Tiles8 kTiles[] = {{16, 16, 1}, {8, 16, 1}, {16, 8, 1}, {8, 8, 1}, {8, 8, 2}, {8, 4, 2}, {16, 4, 1}};
+
+#ifdef SPMM_KEEP_VARIANTS
+Plan8 g_plan8{0, 0, 0, 0, 0};
+#endif
+
+int64_t up8(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+void share8(Plan8& p, int blocks, int shares)
 {
-    const Layout8 l = layout8(a.M, a.K, GATED);
-    if (a.N > 64) {
-        const int rows = (l.groups * 4 + 15) / 16, cols = (a.N + 255) / 256;
-        return launch(w8_tiles<BF16, GATED, 8, 4, 2, 4>, dim3((unsigned)std::min(rows * cols, 256), 1, 1), dim3(512, 1, 1),
-                      stream, a, rows, cols);
+    p.per    = (int)up8(blocks, std::max(1, std::min(shares, blocks)));
+    p.shares = (int)up8(blocks, p.per);
+}
+
+Plan8 plan8(int M, int N, int K, bool gated)
+{
+    const Layout8 l      = layout8(M, K, gated);
+    const int     blocks = l.steps / 2;
+    Plan8         p{};
+#ifdef SPMM_KEEP_VARIANTS // the tests' build: every kernel at small sizes
+    if (g_plan8.shares > 0) {
+        p = g_plan8;
+        share8(p, blocks, g_plan8.shares);
+        return p;
     }
-    return launch(w8_product<BF16, GATED>, dim3((unsigned)l.groups, (unsigned)(a.N + 15) / 16, 1), dim3(256, 1, 1), stream, a);
+#endif
+    if (N > 64) {
+        p.kind = 1;
+        share8(p, blocks, 1);
+    } else {
+        p.rows = 4, p.cols = N > 32 ? 4 : (N > 16 ? 2 : 1);
+        share8(p, blocks, 1);
+    }
+    return p;
+}
+
+size_t part_bytes8(int M, int N, int K, bool gated, const Plan8& p)
+{
+    return p.shares > 1 ? (size_t)p.shares * N * layout8(M, K, gated).groups * 64 * sizeof(int) : 0;
+}
+
+template <bool GATED, int MT, int NT, int WM, int WN, int S>
+int run_tiles8(hipStream_t stream, const ProductArgs& a, int resident)
+{
+    const Layout8 l    = layout8(a.M, a.K, GATED);
+    const int     rows = (int)up8(l.groups * 4, MT * WM), cols = (int)up8(a.N, NT * WN * 16);
+    const int64_t tiles = (int64_t)rows * cols * a.shares;
+    if (tiles > 0x7fffffff)
+        return refuse("%lld tiles of outputs", (long long)tiles);
+    return launch(w8_tiles<GATED, MT, NT, WM, WN, S>, dim3((unsigned)std::min<int64_t>(tiles, 256 * resident), 1, 1),
+                  dim3(64 * WM * WN, 1, 1), stream, a, rows, cols);
+}
+
+template <bool GATED, int R, int NT, int D>
+int run_narrow8(hipStream_t stream, const ProductArgs& a)
+{
+    const int     cols  = (int)up8(a.N, NT * 16);
+    const int64_t units = (int64_t)layout8(a.M, a.K, GATED).groups * (4 / R) * cols;
+    if (units > 0x7fffffff)
+        return refuse("%lld tiles of outputs", (long long)units);
+    return launch(w8_narrow<GATED, R, NT, D>, dim3((unsigned)units, (unsigned)a.shares, 1), dim3(64 * kNarrowWaves, 1, 1), stream, a, cols);
+}
+
+template <bool GATED, int R>
+int run_narrow8(hipStream_t stream, const Plan8& p, const ProductArgs& a)
+{
+    if (p.cols == 1)
+        return run_narrow8<GATED, R, 1, R == 4 ? 3 : 4>(stream, a);
+    if (p.cols == 2)
+        return run_narrow8<GATED, R, 2, R == 4 ? 3 : 4>(stream, a);
+    return run_narrow8<GATED, R, 4, 2>(stream, a);
+}
+
+template <bool GATED>
+int run_plan8(hipStream_t stream, const Plan8& p, const ProductArgs& a)
+{
+    int e;
+    switch (p.kind) {
+    case 0:
+        if constexpr (!GATED)
+            if (p.rows == 1) {
+                e = run_narrow8<false, 1>(stream, p, a);
+                break;
+            }
+        e = p.rows == 2 ? run_narrow8<GATED, 2>(stream, p, a) : run_narrow8<GATED, 4>(stream, p, a);
+        break;
+    case 1: e = run_tiles8<GATED, 8, 4, 2, 4, 2>(stream, a, 1); break;
+    case 2: e = run_tiles8<GATED, 4, 4, 2, 4, 3>(stream, a, 1); break;
+    case 3: e = run_tiles8<GATED, 4, 4, 4, 2, 3>(stream, a, 1); break;
+    case 4: e = run_tiles8<GATED, 4, 2, 2, 4, 4>(stream, a, 1); break;
+    case 5: e = run_tiles8<GATED, 4, 4, 2, 2, 2>(stream, a, 2); break;
+    case 6: e = run_tiles8<GATED, 4, 2, 2, 2, 3>(stream, a, 2); break;
+    default: e = run_tiles8<GATED, 4, 2, 4, 2, 3>(stream, a, 1); break;
+    }
+    if (e != 0 || a.shares == 1)
+        return e;
+    const int64_t threads = (int64_t)a.N * layout8(a.M, a.K, GATED).groups * (GATED ? 4 : 8);
+    return launch(w8_join<GATED>, dim3((unsigned)up8(threads, 256), 1, 1), dim3(256, 1, 1), stream, a);
 }
 
 int check_sizes8(int M, int K)
@@ -446,17 +675,18 @@ int check_sizes8(int M, int K)
     return 0;
 }
 
-// Workspace of a call on 16-bit rows: codes, then scales.
+// Workspace of a call: sums of the shares of K; of 16-bit rows codes, then scales.
 struct Space8 {
-    int64_t stride, scales, bytes;
+    int64_t part, codes, stride, scales, bytes; // bytes of the sums, offsets
 };
 
-Space8 space8(int N, int K, bool x16)
+Space8 space8(int M, int N, int K, bool gated, bool x16, const Plan8& p)
 {
     Space8 s{};
+    s.part = s.codes = s.bytes = (int64_t)part_bytes8(M, N, K, gated, p);
     if (x16) {
         s.stride = (K + 15) / 16 * 16;
-        s.scales = s.stride * N;
+        s.scales = s.codes + s.stride * N;
         s.bytes  = s.scales + ((int64_t)N * 4 + 15) / 16 * 16;
     }
     return s;
@@ -467,8 +697,8 @@ int run_product(hipStream_t stream, const void* packed, const W8_Codes& x, void*
 {
     if (int e = check_sizes8(M, K))
         return e;
-    if (N < 0 || N > 16 * 65535)
-        return refuse("%d rows of X (0 to %d)", N, 16 * 65535);
+    if (N < 0 || N > kMaxN8)
+        return refuse("%d rows of X (0 to %d)", N, kMaxN8);
     if (dtype != DECODE_FP16 && dtype != DECODE_BF16)
         return refuse("unknown element type %d", dtype);
     if (activation < 0 || activation > W8_ACT_SILU)
@@ -479,7 +709,8 @@ int run_product(hipStream_t stream, const void* packed, const W8_Codes& x, void*
         (up_bias != nullptr && bad_pointer(up_bias, 2)))
         return refuse("a null or misaligned weight (16 bytes), Y or bias (2)");
     const bool   x16 = x.scales == nullptr;
-    const Space8 s   = space8(N, K, x16);
+    const Plan8  p   = plan8(M, N, K, gated);
+    const Space8 s   = space8(M, N, K, gated, x16, p);
     if (x16 ? bad_pointer(x.codes, 2) : bad_codes(x, N, K) || bad_pointer(x.scales, 4))
         return refuse("X null or misaligned (16-bit rows: 2 bytes; codes: 16, rows too, scales 4)");
     const size_t need = (size_t)s.bytes;
@@ -489,23 +720,34 @@ int run_product(hipStream_t stream, const void* packed, const W8_Codes& x, void*
     a.packed = static_cast<const uint8_t*>(packed);
     a.x = x.codes, a.x_scales = x.scales, a.x_stride = x.stride;
     if (x16) {
-        int8_t* codes  = static_cast<int8_t*>(workspace);
-        float*  scales = reinterpret_cast<float*>(codes + s.scales);
+        int8_t* codes  = static_cast<int8_t*>(workspace) + s.codes;
+        float*  scales = reinterpret_cast<float*>(static_cast<int8_t*>(workspace) + s.scales);
         if (int e = run_quantize(stream, x.codes, x.stride, N, K, codes, s.stride, scales, dtype))
             return e;
         a.x = codes, a.x_scales = scales, a.x_stride = s.stride;
     }
     a.y = static_cast<uint16_t*>(Y), a.bias = static_cast<const uint16_t*>(bias), a.up_bias = static_cast<const uint16_t*>(up_bias);
-    a.M = M, a.N = N, a.K = K, a.act = activation;
-    if (gated)
-        return dtype == DECODE_BF16 ? run_product<true, true>(stream, a) : run_product<false, true>(stream, a);
-    return dtype == DECODE_BF16 ? run_product<true, false>(stream, a) : run_product<false, false>(stream, a);
+    a.M = M, a.N = N, a.K = K, a.act = activation, a.bf16 = dtype == DECODE_BF16;
+    a.shares = p.shares, a.per = p.per, a.part = p.shares > 1 ? static_cast<int*>(workspace) : nullptr;
+    return gated ? run_plan8<true>(stream, p, a) : run_plan8<false>(stream, p, a);
 }
 
 } // namespace
 } // namespace decode
 
 using namespace decode;
+
+#ifdef SPMM_KEEP_VARIANTS
+// Every later call runs as the plan says (see Plan8); shares 0: as the library chooses.
+extern "C" int W8_Debug_SetPlan(int kind, int rows, int cols, int shares)
+{
+    if (kind < 0 || kind > (int)(sizeof kTiles / sizeof *kTiles) || shares < 0 ||
+        (kind == 0 && shares > 0 && ((rows != 1 && rows != 2 && rows != 4) || (cols != 1 && cols != 2 && cols != 4))))
+        return 1;
+    g_plan8 = Plan8{kind, rows, cols, shares, 0};
+    return 0;
+}
+#endif
 
 extern "C" size_t W8_PackedBytes(int M, int K, int gated)
 {
@@ -535,9 +777,9 @@ extern "C" int W8_Pack(hipStream_t stream, W8_Weights w, const W8_Weights* up, i
 
 extern "C" size_t W8_WorkspaceBytes(int M, int N, int K, int gated, int x16)
 {
-    if (W8_PackedBytes(M, K, gated) == 0 || N < 1)
+    if (W8_PackedBytes(M, K, gated) == 0 || N < 1 || N > kMaxN8)
         return 0;
-    return (size_t)space8(N, K, x16 != 0).bytes;
+    return (size_t)space8(M, N, K, gated != 0, x16 != 0, plan8(M, N, K, gated != 0)).bytes;
 }
 
 extern "C" int W8_Linear(hipStream_t stream, const void* packed, W8_Codes x, void* Y, int M, int N, int K, const void* bias,
