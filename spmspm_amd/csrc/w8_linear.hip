@@ -80,7 +80,7 @@ struct ProductArgs {
     int64_t        x_stride;
     uint16_t*      y;
     const uint16_t *bias, *up_bias;
-    int*           part; // sums of the shares of K, [share][N][packed row]; null where K is not split
+    int*           part; // sums of the shares of K (part_of); null where K is not split
     int            M, N, K, act, bf16;
     int            shares, per; // shares of K, blocks of 128 columns in each but the last
 };
@@ -182,51 +182,61 @@ struct Tail8 {
     }
 };
 
-// The sums of a share of K: of column n, tile t of a group, rows 4 q .. 4 q + 3.  The order within a group is that of the outputs, of
-// a gated product 32 of the gate and 32 of up.
-template <bool GATED>
-__device__ __forceinline__ void store_part(const ProductArgs& a, int groups, int share, int n, int group, int t, int q, intx4 sum)
+// The sums of a share of K go to memory as the matrix cores leave them: of a group and a tile of 16 columns, four tiles of 1 KB.
+__device__ __forceinline__ intx4* part_of(const ProductArgs& a, int groups, int share, int columns, int group, int column)
 {
-    const int at = GATED ? t / 2 * 32 + 8 * q + t % 2 * 4 : 16 * q + 4 * t;
-    *reinterpret_cast<intx4*>(a.part + (((int64_t)share * a.N + n) * groups + group) * 64 + at) = sum;
+    return reinterpret_cast<intx4*>(a.part) + (((int64_t)share * columns + column) * groups + group) * 256;
 }
 
-// Eight outputs a thread from the sums of all shares.
+// A wave ends half a group, tiles h and h + 2 of a gated product, 2 h and 2 h + 1 otherwise, of 16 columns from the sums of all shares.
 template <bool GATED>
 __global__ __launch_bounds__(256) void w8_join(ProductArgs a)
 {
-    constexpr int kPer  = GATED ? 4 : 8; // threads for a group's outputs
-    const Layout8 l     = layout8(a.M, a.K, GATED);
-    const int64_t id    = (int64_t)blockIdx.x * 256 + threadIdx.x, unit = id / kPer;
-    const int     n     = (int)(unit / l.groups), group = (int)(unit % l.groups), j = (int)(id % kPer) * 8;
+    const Layout8 l = layout8(a.M, a.K, GATED);
+    const int     lane = threadIdx.x % kWave, columns = (a.N + 15) / 16;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int     h = (int)(unit & 1), group = (int)(unit / 2 % l.groups), column = (int)(unit / 2 / l.groups);
+    const int     n = column * 16 + (lane & 15), q = lane >> 4;
     if (n >= a.N)
         return;
-    const intx4*  p    = reinterpret_cast<const intx4*>(a.part + ((int64_t)n * l.groups + group) * 64 + j);
-    const int64_t next = (int64_t)a.N * l.groups * 16;
-    intx4         sum[4] = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int s = 0; s < a.shares; ++s) {
-        sum[0] += p[s * next], sum[1] += p[s * next + 1];
-        if (GATED)
-            sum[2] += p[s * next + 8], sum[3] += p[s * next + 9];
-    }
-    int v[16];
-    for (int i = 0; i < 16; ++i)
+    const intx4*  p    = part_of(a, l.groups, 0, columns, group, column) + (GATED ? h : 2 * h) * 64 + lane;
+    const int64_t next = (int64_t)columns * l.groups * 256;
+    intx4         sum[2] = {0, 0};
+#pragma unroll 8
+    for (int s = 0; s < a.shares; ++s)
+        for (int t = 0; t < 2; ++t)
+            sum[t] += p[s * next + t * (GATED ? 128 : 64)];
+    int v[8];
+    for (int i = 0; i < 8; ++i)
         v[i] = sum[i / 4][i % 4];
-    Tail8<GATED, 8>(a, l, group * (GATED ? 32 : 64) + j).store(a, n, a.x_scales[n], v, v + 8);
+    if constexpr (GATED)
+        Tail8<true, 4>(a, l, group * 32 + 8 * q + 4 * h).store(a, n, a.x_scales[n], v, v + 4);
+    else
+        Tail8<false, 8>(a, l, group * 64 + 16 * q + 8 * h).store(a, n, a.x_scales[n], v, nullptr);
 }
 
 // Few columns: a workgroup of kNarrowWaves waves takes R row tiles and NT column tiles, its waves every kNarrowWaves-th block of 128 columns of
-// its share of K.  W is read once and goes from memory into the matrix operands as it is packed, X by way of the caches; a wave
-// has D blocks of both in flight.  The waves' sums meet in LDS.  A gated product has rows of the gate and of up in every
-// workgroup: tiles t and t + 2 with R = 2.
+// its share of K.  W is read once and goes from memory into the matrix operands as it is packed.  X comes eight rows of 128 bytes to a
+// load and takes the operands' order in a corner of LDS that the wave has for itself (read in that order, 16 rows at once, a load
+// keeps the address unit four times as long: 2.3 us for every 16 columns of 5120).  A wave has D blocks of both in flight.  The
+// waves' sums meet in LDS.  A gated product has rows of the gate and of up in every workgroup: tiles t and t + 2 with R = 2.
 constexpr int kNarrowWaves = 8;
+
+// What a wave wrote to LDS is there for its other lanes, and what they read may be written over: no instruction, the wave's
+// accesses keep their order.
+__device__ __forceinline__ void wave_handoff8()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 template <bool GATED, int R, int NT, int D>
 __global__ __launch_bounds__(64 * kNarrowWaves) void w8_narrow(ProductArgs a, int column_tiles)
 {
     static_assert(!GATED || R >= 2);
-    __shared__ int total[R * NT][kWave][4];
+    __shared__ int   total[R * NT][kWave][4];
+    __shared__ intx4 turned[kNarrowWaves][NT][2][kWave]; // X: 8 rows a KB, row r's chunk c at place 8 r + (c ^ r)
     const Layout8  l    = layout8(a.M, a.K, GATED);
     const int      lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), c = lane & 15, q = lane >> 4;
     const int      unit = blockIdx.x / column_tiles, n0 = blockIdx.x % column_tiles * (NT * 16), share = blockIdx.y;
@@ -238,20 +248,21 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void w8_narrow(ProductArgs a, in
     __syncthreads();
 
     const intx4*  w = reinterpret_cast<const intx4*>(a.packed + (int64_t)group * kGroup8) + first * 64 + lane;
-    const int8_t* x[NT];
+    const int8_t* x[NT][2];
     for (int u = 0; u < NT; ++u) // rows behind the last are the last again
-        x[u] = a.x + (int64_t)min(n0 + u * 16 + c, a.N - 1) * a.x_stride;
+        for (int s = 0; s < 2; ++s)
+            x[u][s] = a.x + (int64_t)min(n0 + u * 16 + s * 8 + (lane >> 3), a.N - 1) * a.x_stride;
     struct Block {
-        intx4 w[2][R], x[2][NT];
+        intx4 w[2][R], x[NT][2];
     };
     Block held[D];
     auto  fetch = [&](Block& h, int block) {
-        for (int s = 0; s < 2; ++s) {
+        for (int u = 0; u < NT; ++u) // behind the last 16 columns of X the weights are 0
+            for (int s = 0; s < 2; ++s)
+                h.x[u][s] = *reinterpret_cast<const intx4*>(x[u][s] + min(block * 128 + 16 * (lane & 7), last));
+        for (int s = 0; s < 2; ++s)
             for (int t = 0; t < R; ++t)
                 h.w[s][t] = __builtin_nontemporal_load(w + (int64_t)block * l.groups * (kGroup8 / 16) + (s * 4 + t * apart) * 64);
-            for (int u = 0; u < NT; ++u) // behind the last 16 columns of X the weights are 0
-                h.x[s][u] = *reinterpret_cast<const intx4*>(x[u] + min(block * 128 + s * 64 + 16 * q, last));
-        }
     };
     intx4 sum[R][NT];
     for (int t = 0; t < R; ++t)
@@ -265,10 +276,17 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void w8_narrow(ProductArgs a, in
         for (int d = 0; d < D; ++d, block += kNarrowWaves) {
             if (block >= to)
                 break;
+            for (int u = 0; u < NT; ++u)
+                for (int s = 0; s < 2; ++s)
+                    turned[wave][u][s][(lane & 56) | ((lane & 7) ^ (lane >> 3))] = held[d].x[u][s];
+            wave_handoff8();
             for (int s = 0; s < 2; ++s)
-                for (int u = 0; u < NT; ++u)
+                for (int u = 0; u < NT; ++u) {
+                    const intx4 b = turned[wave][u][c >> 3][(c & 7) * 8 + ((4 * s + q) ^ (c & 7))];
                     for (int t = 0; t < R; ++t)
-                        sum[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(held[d].w[s][t], held[d].x[s][u], sum[t][u], 0, 0, 0);
+                        sum[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(held[d].w[s][t], b, sum[t][u], 0, 0, 0);
+                }
+            wave_handoff8();
             if (block + D * kNarrowWaves < to)
                 fetch(held[d], block + D * kNarrowWaves);
         }
@@ -281,17 +299,15 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void w8_narrow(ProductArgs a, in
     if (wave >= NT) // wave u ends column tile u
         return;
     const int n = n0 + wave * 16 + c;
-    if (n >= a.N)
-        return;
-    int v[4 * R];
+    int       v[4 * R];
     for (int t = 0; t < R; ++t) {
         const intx4 s = *reinterpret_cast<const intx4*>(total[t * NT + wave][lane]);
-        if (a.part != nullptr)
-            store_part<GATED>(a, l.groups, share, n, group, first + t * apart, q, s);
+        if (a.part != nullptr && n0 + wave * 16 < a.N)
+            part_of(a, l.groups, share, (a.N + 15) / 16, group, n0 / 16 + wave)[(first + t * apart) * 64 + lane] = s;
         for (int i = 0; i < 4; ++i)
             v[4 * t + i] = s[i];
     }
-    if (a.part != nullptr)
+    if (a.part != nullptr || n >= a.N)
         return;
     constexpr int W  = GATED ? 2 * R : (R == 1 ? 4 : 8); // consecutive outputs of a lane
     const float   sx = a.x_scales[n];
@@ -315,6 +331,12 @@ __device__ __forceinline__ void each(F f)
 __device__ __forceinline__ void to_lds(unsigned lds, const void* base, unsigned offset)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+
+// The same of memory that is read once: the caches are kept for what is read again (36864x9216 with 64 columns 92 -> 87 us).
+__device__ __forceinline__ void to_lds_once(unsigned lds, const void* base, unsigned offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
 // The same of one word, or of 16 bits in a word, a lane.
@@ -415,9 +437,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs a, int r
     auto stage = [&](int i, int block, int place) {
         const int      j  = wave + i * kWaves;
         const unsigned to = lds0 + place * kStage + j * 1024;
-        if ((i + 1) * kWaves <= 2 * kRows || j < 2 * kRows)
-            to_lds(to, from[i] + block * block_bytes, off[i]);
-        else
+        if ((i + 1) * kWaves <= 2 * kRows || j < 2 * kRows) {
+            if (column_tiles == 1)
+                to_lds_once(to, from[i] + block * block_bytes, off[i]);
+            else
+                to_lds(to, from[i] + block * block_bytes, off[i]);
+        } else
             to_lds(to, from[i], off[i] + min(block * 128 + chunk, last));
     };
     struct Operands {
@@ -539,12 +564,13 @@ const bool more = ahead_tile < tiles;
                 // With all its stores made: of the barriers that wait for loads older than they are.
                 relaxed = (row + 1) * (GATED ? kM / 2 : kM) <= a.M && (column + 1) * kN <= a.N ? S - 1 : 0;
             } else {
+                const int columns = (a.N + 15) / 16;
                 each<NT>([&](auto u) {
-                    const int n = column * kN + (wn * NT + u) * 16 + c;
+                    const int at = column * kCols + wn * NT + u;
                     each<MT>([&](auto t) {
                         const int group = row * (kM / 64) + wm * (MT / 4) + t / 4;
-                        if (n < a.N && group < l.groups)
-                            store_part<GATED>(a, l.groups, share, n, group, t % 4, q, sum[t][u]);
+                        if (at < columns && group < l.groups)
+                            part_of(a, l.groups, share, columns, group, at)[t % 4 * 64 + lane] = sum[t][u];
                     });
                 });
             }
@@ -561,14 +587,19 @@ const bool more = ahead_tile < tiles;
 // How a call runs.
 struct Plan8 {
     int kind;        // 0: w8_narrow, otherwise a w8_tiles of kTiles[kind - 1]
-    int rows, cols;  // row and column tiles of 16 that a workgroup takes
+    int rows, cols;  // row and column tiles of 16 that a workgroup of w8_narrow takes
     int shares, per; // shares of K, blocks of 128 columns in each
 };
 
+// What plan8 knows of the shapes of w8_tiles: a workgroup's row and column tiles, how many fit a CU, and in microseconds what a tile costs
+// beside its blocks, a block with one workgroup on the CU and with two.
 struct Tiles8 {
-    int rows, cols, resident; // workgroups that fit a CU
+    int    rows, cols, resident;
+    double tile, block, both;
 };
-constexpr Tiles8 kTiles[] = {{16, 16, 1}, {8, 16, 1}, {16, 8, 1}, {8, 8, 1}, {8, 8, 2}, {8, 4, 2}, {16, 4, 1}};
+constexpr Tiles8 kTiles[] = {{16, 16, 1, 5.3, 1.41, 0},    {8, 16, 1, 4.3, 0.85, 0},     {16, 8, 1, 4.2, 0.86, 0},
+                             {8, 8, 1, 3.2, 0.50, 0},      {8, 8, 2, 3.2, 0.70, 0.99},   {8, 4, 2, 2.6, 0.41, 0.68}};
+constexpr int kShapes = sizeof kTiles / sizeof *kTiles;
 
 #ifdef SPMM_KEEP_VARIANTS
 Plan8 g_plan8{0, 0, 0, 0, 0};
@@ -576,17 +607,24 @@ Plan8 g_plan8{0, 0, 0, 0, 0};
 
 int64_t up8(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-void share8(Plan8& p, int blocks, int shares)
+void share8(Plan8& p, int64_t blocks, int64_t shares)
 {
-    p.per    = (int)up8(blocks, std::max(1, std::min(shares, blocks)));
+    p.per    = (int)up8(blocks, std::max<int64_t>(1, std::min(shares, blocks)));
     p.shares = (int)up8(blocks, p.per);
 }
 
+// The cheapest by a model of a call's time in microseconds, fitted to 1328 calls of 51 shapes, from 256x256 to 36864x9216 and from 1 to 6000
+// columns, on which it is 1.5 % off the best on average and 17 % at worst.  Workgroups are counted in rounds, one (or two) for every CU;
+// W's bytes are added to them; K in shares costs a launch and the shares' bytes.  Examples, us: 5120x5120, N = 37 10.3 narrow
+// with two row and three column tiles, 12.7 in tiles of 128 x 64; 20480x5120, N = 64 25.7 in tiles of 128 x 64, 30.4
+// narrow; 9216x36864, N = 193 97 in tiles of 256 x 256 and seven shares of K, 113 in tiles of 128 x 256 and three, 410 in one.
 Plan8 plan8(int M, int N, int K, bool gated)
 {
     const Layout8 l      = layout8(M, K, gated);
-    const int     blocks = l.steps / 2;
-    Plan8         p{};
+    const int64_t blocks = l.steps / 2, tiles = (int64_t)l.groups * 4;
+    const double  w_mb = (double)tiles * (double)blocks * 2048e-6, part_mb = (double)tiles * (double)up8(N, 16) * 2048e-6;
+    Plan8         p{}, best{};
+    double        least = 1e300;
 #ifdef SPMM_KEEP_VARIANTS // the tests' build: every kernel at small sizes
     if (g_plan8.shares > 0) {
         p = g_plan8;
@@ -594,19 +632,46 @@ Plan8 plan8(int M, int N, int K, bool gated)
         return p;
     }
 #endif
-    if (N > 64) {
-        p.kind = 1;
-        share8(p, blocks, 1);
-    } else {
-        p.rows = 4, p.cols = N > 32 ? 4 : (N > 16 ? 2 : 1);
-        share8(p, blocks, 1);
+    auto consider = [&](double us) {
+        if (p.shares > 1)
+            us += 3.0 + p.shares * part_mb / 8.4;
+        if (us < least)
+            least = us, best = p;
+    };
+    if (N <= 128)
+        for (p.rows = gated ? 2 : 1; p.rows <= 4; p.rows *= 2)
+            for (p.cols = 1; p.cols <= std::min<int64_t>(4, up8(N, 16)); ++p.cols) {
+                const int64_t columns = up8(N, 16 * p.cols), groups = tiles / p.rows * columns;
+                for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+                    if (s > 1 && (s > blocks || groups * s > 2048))
+                        break;
+                    share8(p, blocks, s);
+                    consider(2.8 + w_mb * (double)columns / 12.7 +
+                             (double)(up8(groups * p.shares, 256) * up8(p.per, 8)) * (0.20 * p.rows + 0.25 * p.cols));
+                }
+            }
+    for (p.kind = 1; p.kind <= kShapes; ++p.kind) {
+        const Tiles8& k      = kTiles[p.kind - 1];
+        const int64_t groups = up8(tiles, k.rows) * up8(N, 16 * k.cols);
+        p.rows = p.cols = 0;
+        for (int fill = 0; fill <= k.resident; ++fill) { // shares for none, one or two workgroups on every CU
+            if (fill > 0 && 256 * fill / groups < 2)
+                continue;
+            share8(p, blocks, fill > 0 ? std::min<int64_t>(64, 256 * fill / groups) : 1);
+            const int64_t slots = 256 * k.resident, full = groups * p.shares / slots, rest = groups * p.shares % slots;
+            double        us = 2.4 + w_mb / 25;
+            us += (double)full * (k.tile + p.per * (k.resident > 1 ? k.both : k.block));
+            if (rest > 0)
+                us += k.tile + p.per * (rest > 256 ? k.both : k.block);
+            consider(us);
+        }
     }
-    return p;
+    return best;
 }
 
 size_t part_bytes8(int M, int N, int K, bool gated, const Plan8& p)
 {
-    return p.shares > 1 ? (size_t)p.shares * N * layout8(M, K, gated).groups * 64 * sizeof(int) : 0;
+    return p.shares > 1 ? (size_t)p.shares * up8(N, 16) * layout8(M, K, gated).groups * 4096 : 0;
 }
 
 template <bool GATED, int MT, int NT, int WM, int WN, int S>
@@ -638,6 +703,8 @@ int run_narrow8(hipStream_t stream, const Plan8& p, const ProductArgs& a)
         return run_narrow8<GATED, R, 1, R == 4 ? 3 : 4>(stream, a);
     if (p.cols == 2)
         return run_narrow8<GATED, R, 2, R == 4 ? 3 : 4>(stream, a);
+    if (p.cols == 3)
+        return run_narrow8<GATED, R, 3, 2>(stream, a);
     return run_narrow8<GATED, R, 4, 2>(stream, a);
 }
 
@@ -659,13 +726,12 @@ int run_plan8(hipStream_t stream, const Plan8& p, const ProductArgs& a)
     case 3: e = run_tiles8<GATED, 4, 4, 4, 2, 3>(stream, a, 1); break;
     case 4: e = run_tiles8<GATED, 4, 2, 2, 4, 4>(stream, a, 1); break;
     case 5: e = run_tiles8<GATED, 4, 4, 2, 2, 2>(stream, a, 2); break;
-    case 6: e = run_tiles8<GATED, 4, 2, 2, 2, 3>(stream, a, 2); break;
-    default: e = run_tiles8<GATED, 4, 2, 4, 2, 3>(stream, a, 1); break;
+    default: e = run_tiles8<GATED, 4, 2, 2, 2, 3>(stream, a, 2); break;
     }
     if (e != 0 || a.shares == 1)
         return e;
-    const int64_t threads = (int64_t)a.N * layout8(a.M, a.K, GATED).groups * (GATED ? 4 : 8);
-    return launch(w8_join<GATED>, dim3((unsigned)up8(threads, 256), 1, 1), dim3(256, 1, 1), stream, a);
+    const int64_t waves = up8(a.N, 16) * layout8(a.M, a.K, GATED).groups * 2;
+    return launch(w8_join<GATED>, dim3((unsigned)up8(waves, 4), 1, 1), dim3(256, 1, 1), stream, a);
 }
 
 int check_sizes8(int M, int K)
@@ -673,6 +739,13 @@ int check_sizes8(int M, int K)
     if (M < 1 || M > kMaxRows8 || K < 1 || K > kMaxK8)
         return refuse("weights of %d rows (1 to 2^24) and %d columns (1 to %d)", M, K, kMaxK8);
     return 0;
+}
+
+// Bytes from row to row of codes that the library makes room for.  From 1 KB on an odd multiple of 128: the rows of a tile then lie on
+// different channels (8192 columns in rows of 8192 bytes 220 us, of 8320 209; 20480x5120, N = 4096 345 and 336).
+int64_t stride8(int K)
+{
+    return K < 1024 ? (K + 15) / 16 * 16 : ((K + 127) / 128 | 1) * 128;
 }
 
 // Workspace of a call: sums of the shares of K; of 16-bit rows codes, then scales.
@@ -685,7 +758,7 @@ Space8 space8(int M, int N, int K, bool gated, bool x16, const Plan8& p)
     Space8 s{};
     s.part = s.codes = s.bytes = (int64_t)part_bytes8(M, N, K, gated, p);
     if (x16) {
-        s.stride = (K + 15) / 16 * 16;
+        s.stride = stride8(K);
         s.scales = s.codes + s.stride * N;
         s.bytes  = s.scales + ((int64_t)N * 4 + 15) / 16 * 16;
     }
@@ -741,8 +814,8 @@ using namespace decode;
 // Every later call runs as the plan says (see Plan8); shares 0: as the library chooses.
 extern "C" int W8_Debug_SetPlan(int kind, int rows, int cols, int shares)
 {
-    if (kind < 0 || kind > (int)(sizeof kTiles / sizeof *kTiles) || shares < 0 ||
-        (kind == 0 && shares > 0 && ((rows != 1 && rows != 2 && rows != 4) || (cols != 1 && cols != 2 && cols != 4))))
+    if (kind < 0 || kind > kShapes || shares < 0 ||
+        (kind == 0 && shares > 0 && ((rows != 1 && rows != 2 && rows != 4) || cols < 1 || cols > 4)))
         return 1;
     g_plan8 = Plan8{kind, rows, cols, shares, 0};
     return 0;

@@ -99,8 +99,9 @@ def _overlap(a, b):
 
 
 def _new_codes(x, N, K):
-    """Room for N rows of K codes, 16-byte aligned, and their scales."""
-    width = (K + 15) // 16 * 16
+    """Room for N rows of K codes, 16-byte aligned, and their scales.  Long rows lie an odd multiple of 128 bytes apart: rows a power of
+    two apart would meet on the same memory channels."""
+    width = (K + 15) // 16 * 16 if K < 1024 else ((K + 127) // 128 | 1) * 128
     codes = torch.empty((N, width), dtype=torch.int8, device=x.device)
     return codes if width == K else codes[:, :K], torch.empty(N, dtype=torch.float32, device=x.device)
 
@@ -153,7 +154,7 @@ def rms_norm(x, weight, eps=1e-5, residual=None, out=None, residual_out=None, st
 def rms_norm_x8(x, weight, eps=1e-5, residual=None, residual_out=None, stream=None):
     """rms_norm with its result in 8 bits: (codes, scales), with a residual (codes, scales, h).
 
-    codes int8 [tokens][K] (rows 16-byte aligned: a slice of wider ones where K is not a multiple of 16), scales float32 [tokens];
+    codes int8 [tokens][K] (rows 16-byte aligned, in general a slice of wider ones), scales float32 [tokens];
     y ~ codes * scales.  What a W8Linear and a W8GatedLinear take."""
     xr, rr = _norm_args(x, weight, eps, residual)
     N, K = x.shape
@@ -175,7 +176,7 @@ def rms_norm_x8(x, weight, eps=1e-5, residual=None, residual_out=None, stream=No
         if N:
             err = _library().RMS_Norm(handle, xr, rr, weight.data_ptr(), eps, N, K,
                                       hr or (_NONE if h is None else _Rows(h.data_ptr(), K)), _NONE,
-                                      _Codes(codes.data_ptr(), (K + 15) // 16 * 16, scales.data_ptr()), _TYPES[x.dtype])
+                                      _Codes(codes.data_ptr(), codes.stride(0), scales.data_ptr()), _TYPES[x.dtype])
             _raise(err, "rms_norm_x8")
         return (codes, scales) if residual is None else (codes, scales, h)
 
@@ -193,7 +194,7 @@ def quantize_x8(x, stream=None):
     def call(handle):
         codes, scales = _new_codes(x, N, K)
         if N:
-            err = _library().W8_Quantize(handle, xr, N, K, _Codes(codes.data_ptr(), (K + 15) // 16 * 16, scales.data_ptr()), kind)
+            err = _library().W8_Quantize(handle, xr, N, K, _Codes(codes.data_ptr(), codes.stride(0), scales.data_ptr()), kind)
             _raise(err, "quantize_x8")
         return codes, scales
 
