@@ -18,7 +18,6 @@ struct NormArgs {
     int64_t         x_stride, r_stride, h_stride, y_stride, c_stride;
     int             N, K;
     float           eps;
-    int             norm; // 0: the row is only rounded to 8 bits
 };
 
 __device__ __forceinline__ shortx8 load8(const uint16_t* p, int left)
@@ -74,8 +73,9 @@ __device__ __forceinline__ void reduce(float& a, unsigned& b, float (*sum)[16], 
     }
 }
 
-// One row by WAVES waves, V vectors of eight elements a lane in registers; V = 0: a row of any length, read twice.
-template <bool BF16, bool QUANT, int WAVES, int V>
+// One row by WAVES waves, V vectors of eight elements a lane in registers; V = 0: a row of any length, read twice.  Without NORM the row
+// is only rounded to 8 bits.
+template <bool BF16, bool NORM, bool QUANT, int WAVES, int V>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(NormArgs a)
 {
     constexpr int      kThreads = WAVES * kWave, kHeld = V > 0 ? V : 1;
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
     // The vector at element e as the norm sees it; what lies behind the row is 0.
     auto fetch = [&](int e) {
         shortx8 v = load8(x + e, a.K - e);
-        if (a.residual != nullptr) {
+        if (NORM && a.residual != nullptr) {
             const shortx8 d = load8(r + e, a.K - e);
             for (int i = 0; i < 8; ++i)
                 v[i] = down<BF16>(up<BF16>(v[i]) + up<BF16>(d[i]));
@@ -105,20 +105,22 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
     unsigned most    = 0; // bits of max |t|: an infinity or a NaN is larger than every number
     auto     take    = [&](shortx8 v, shortx8 w) {
         for (int i = 0; i < 8; ++i) {
-            const float f = up<BF16>(v[i]), t = a.weight != nullptr ? f * up<BF16>(w[i]) : f;
-            squares       = __builtin_fmaf(f, f, squares);
+            const float f = up<BF16>(v[i]), t = NORM ? f * up<BF16>(w[i]) : f;
+            if (NORM)
+                squares = __builtin_fmaf(f, f, squares);
             if (QUANT)
                 most = max(most, __float_as_uint(t) & 0x7fffffffu);
         }
     };
+#pragma unroll kHeld
     for (int j = 0; j < n; ++j) {
         const int e = (j * kThreads + lane) * 8, k = V > 0 ? j : 0;
         held[k] = 0, gain[k] = 0;
         if (e < a.K) {
             held[k] = fetch(e);
-            if (a.weight != nullptr)
+            if (NORM)
                 gain[k] = load8(a.weight + e, a.K - e);
-            if (a.h != nullptr)
+            if (NORM && a.h != nullptr)
                 store8(h + e, held[k], a.K - e);
             if (V == 0)
                 take(held[0], gain[0]);
@@ -131,12 +133,12 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
     auto again = [&](int j, int e) {
         if (V > 0)
             return held[V > 0 ? j : 0];
-        return a.h != nullptr ? load8(h + e, a.K - e) : fetch(e);
+        return NORM && a.h != nullptr ? load8(h + e, a.K - e) : fetch(e);
     };
     reduce<WAVES>(squares, most, sum, top, 0);
 
     float inverse_rms = 1.f;
-    if (a.norm) {
+    if constexpr (NORM) {
         float mean = squares / (float)a.K, unit = 1.f;
         if (BF16 && !(squares < INFINITY)) { // squares of bf16 numbers from 2^64 on: once more with h / 2^96
             float    small = 0.f;
@@ -161,18 +163,19 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
     const float inverse = none ? 0.f : 127.f / m;
     if (QUANT && lane == 0)
         a.scales[row] = bad ? NAN : (none ? 0.f : m / 127.f * inverse_rms);
+#pragma unroll kHeld
     for (int j = 0; j < n; ++j) {
         const int e = (j * kThreads + lane) * 8;
         if (e >= a.K)
             continue;
         const shortx8 v = again(j, e);
         shortx8       w = gain[V > 0 ? j : 0];
-        if (V == 0 && a.weight != nullptr)
+        if (V == 0 && NORM)
             w = load8(a.weight + e, a.K - e);
         if constexpr (QUANT) {
             float t[8];
             for (int i = 0; i < 8; ++i)
-                t[i] = none ? 0.f : (a.weight != nullptr ? up<BF16>(v[i]) * up<BF16>(w[i]) : up<BF16>(v[i]));
+                t[i] = none ? 0.f : (NORM ? up<BF16>(v[i]) * up<BF16>(w[i]) : up<BF16>(v[i]));
             // rows are readable, and here written, up to 16 bytes: the codes of the zeros behind the row are 0
             *reinterpret_cast<uintx2*>(a.codes + row * a.c_stride + e) = codes8(t, m, inverse);
         } else {
@@ -184,35 +187,65 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
     }
 }
 
-template <bool BF16, bool QUANT, int WAVES, int V>
+template <bool BF16, bool NORM, bool QUANT, int WAVES, int V>
 int start(hipStream_t stream, const NormArgs& a)
 {
     const unsigned rows = WAVES == 1 ? (unsigned)(((int64_t)a.N + 3) / 4) : (unsigned)a.N;
-    return launch(rms_norm<BF16, QUANT, WAVES, V>, dim3(rows, 1, 1), dim3(WAVES == 1 ? 256 : WAVES * kWave, 1, 1), stream, a);
+    return launch(rms_norm<BF16, NORM, QUANT, WAVES, V>, dim3(rows, 1, 1), dim3(WAVES == 1 ? 256 : WAVES * kWave, 1, 1), stream, a);
 }
 
-template <bool BF16, bool QUANT>
+// Waves to a row and vectors to a lane.  Many rows: few waves, as many vectors as leave few lanes without one, since rows in flight
+// hide each other's latency (4099 rows of 9216 to 8 bits: four waves with five vectors 57 us, sixteen with four 87).  Few rows: all the
+// waves there are (64 rows of 7168 4.6 us, four waves with four vectors 6.3).  Longer rows than registers hold are read twice.
+template <bool BF16, bool NORM, bool QUANT>
 int start(hipStream_t stream, const NormArgs& a)
 {
     const int vectors = (a.K + 7) / 8;
+    if (vectors > 4096) {
+        if constexpr (!NORM) // no weights to hold
+            if (vectors <= 8192)
+                return start<BF16, NORM, QUANT, 16, 8>(stream, a);
+        return start<BF16, NORM, QUANT, 16, 0>(stream, a);
+    }
+    if (a.N < 256 && vectors > 256) {
+        if (vectors <= 1024)
+            return start<BF16, NORM, QUANT, 16, 1>(stream, a);
+        if (vectors <= 2048)
+            return start<BF16, NORM, QUANT, 16, 2>(stream, a);
+        return start<BF16, NORM, QUANT, 16, 4>(stream, a);
+    }
     if (vectors <= 64)
-        return start<BF16, QUANT, 1, 1>(stream, a);
+        return start<BF16, NORM, QUANT, 1, 1>(stream, a);
+    if (vectors <= 128)
+        return start<BF16, NORM, QUANT, 1, 2>(stream, a);
     if (vectors <= 256)
-        return start<BF16, QUANT, 4, 1>(stream, a);
+        return start<BF16, NORM, QUANT, 4, 1>(stream, a);
     if (vectors <= 512)
-        return start<BF16, QUANT, 4, 2>(stream, a);
+        return start<BF16, NORM, QUANT, 4, 2>(stream, a);
+    if (vectors <= 768)
+        return start<BF16, NORM, QUANT, 4, 3>(stream, a);
     if (vectors <= 1024)
-        return start<BF16, QUANT, 4, 4>(stream, a);
-    if (vectors <= 4096)
-        return start<BF16, QUANT, 16, 4>(stream, a);
-    return start<BF16, QUANT, 16, 0>(stream, a);
+        return start<BF16, NORM, QUANT, 4, 4>(stream, a);
+    if (vectors <= 1280)
+        return start<BF16, NORM, QUANT, 4, 5>(stream, a);
+    if (vectors <= 1536)
+        return start<BF16, NORM, QUANT, 4, 6>(stream, a);
+    if (vectors <= 2048)
+        return start<BF16, NORM, QUANT, 8, 4>(stream, a);
+    if (vectors <= 2560)
+        return start<BF16, NORM, QUANT, 8, 5>(stream, a);
+    if (vectors <= 3072)
+        return start<BF16, NORM, QUANT, 8, 6>(stream, a);
+    return start<BF16, NORM, QUANT, 8, 8>(stream, a);
 }
 
 int start(hipStream_t stream, const NormArgs& a, int dtype)
 {
+    if (a.weight == nullptr)
+        return dtype == DECODE_BF16 ? start<true, false, true>(stream, a) : start<false, false, true>(stream, a);
     if (a.codes != nullptr)
-        return dtype == DECODE_BF16 ? start<true, true>(stream, a) : start<false, true>(stream, a);
-    return dtype == DECODE_BF16 ? start<true, false>(stream, a) : start<false, false>(stream, a);
+        return dtype == DECODE_BF16 ? start<true, true, true>(stream, a) : start<false, true, true>(stream, a);
+    return dtype == DECODE_BF16 ? start<true, true, false>(stream, a) : start<false, true, false>(stream, a);
 }
 
 int check_sizes(int N, int K, int most, int dtype)
@@ -266,7 +299,7 @@ extern "C" int RMS_Norm(hipStream_t stream, W8_Rows x, W8_Rows residual, const v
     a.y = static_cast<uint16_t*>(const_cast<void*>(y.data)), a.y_stride = y.stride;
     if (codes != nullptr)
         a.codes = codes->codes, a.c_stride = codes->stride, a.scales = codes->scales;
-    a.N = N, a.K = K, a.eps = eps, a.norm = 1;
+    a.N = N, a.K = K, a.eps = eps;
     return start(stream, a, dtype);
 }
 
