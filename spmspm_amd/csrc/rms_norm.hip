@@ -20,14 +20,33 @@ struct NormArgs {
     float           eps;
 };
 
-__device__ __forceinline__ shortx8 load8(const uint16_t* p, int left)
+// Eight elements of a row from e on; what lies behind its K is 0.  The row's end is taken by a whole vector too, the last one there
+// is, and moved down: no lane's loads wait for another's branch.
+__device__ __forceinline__ shortx8 load8(const uint16_t* row, int e, int K)
 {
-    if (left >= 8)
-        return *reinterpret_cast<const loose8*>(p);
-    shortx8 v = 0;
-    for (int i = 0; i < 7; ++i)
-        if (i < left)
-            v[i] = p[i];
+    if (K < 8) {
+        shortx8 v = 0;
+        for (int i = 0; i < 7; ++i)
+            if (e + i < K)
+                v[i] = row[e + i];
+        return v;
+    }
+    const int at = min(e, K - 8);
+    shortx8   v  = *reinterpret_cast<const loose8*>(row + at);
+    if (e > at) {
+        const int by = e - at;
+        uintx4    u  = __builtin_bit_cast(uintx4, v);
+        if (by & 2)
+            u = uintx4{u[1], u[2], u[3], 0};
+        if (by & 4)
+            u = uintx4{u[2], u[3], 0, 0};
+        if (by & 1)
+            for (int i = 0; i < 4; ++i)
+                u[i] = u[i] >> 16 | (i < 3 ? u[i + 1] << 16 : 0);
+        if (by >= 8)
+            u = 0;
+        v = __builtin_bit_cast(shortx8, u);
+    }
     return v;
 }
 
@@ -93,9 +112,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
     shortx8 held[kHeld], gain[kHeld];
     // The vector at element e as the norm sees it; what lies behind the row is 0.
     auto fetch = [&](int e) {
-        shortx8 v = load8(x + e, a.K - e);
+        shortx8 v = load8(x, e, a.K);
         if (NORM && a.residual != nullptr) {
-            const shortx8 d = load8(r + e, a.K - e);
+            const shortx8 d = load8(r, e, a.K);
             for (int i = 0; i < 8; ++i)
                 v[i] = down<BF16>(up<BF16>(v[i]) + up<BF16>(d[i]));
         }
@@ -119,21 +138,24 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
         if (e < a.K) {
             held[k] = fetch(e);
             if (NORM)
-                gain[k] = load8(a.weight + e, a.K - e);
-            if (NORM && a.h != nullptr)
-                store8(h + e, held[k], a.K - e);
-            if (V == 0)
-                take(held[0], gain[0]);
+                gain[k] = load8(a.weight, e, a.K);
+        }
+        if (NORM && a.h != nullptr && e < a.K)
+            store8(h + e, held[k], a.K - e);
+        if (V == 0)
+            take(held[0], gain[0]);
+    }
+    if (V > 0) { // behind all loads: h may take x's place
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            take(held[j], gain[j]);
         }
     }
-    if (V > 0)
-        for (int j = 0; j < V; ++j)
-            take(held[j], gain[j]);
     // The row once more, for rows that are not held: h where it was written (it may have taken x's place), x and the residual otherwise.
     auto again = [&](int j, int e) {
         if (V > 0)
             return held[V > 0 ? j : 0];
-        return NORM && a.h != nullptr ? load8(h + e, a.K - e) : fetch(e);
+        return NORM && a.h != nullptr ? load8(h, e, a.K) : fetch(e);
     };
     reduce<WAVES>(squares, most, sum, top, 0);
 
@@ -171,7 +193,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
         const shortx8 v = again(j, e);
         shortx8       w = gain[V > 0 ? j : 0];
         if (V == 0 && NORM)
-            w = load8(a.weight + e, a.K - e);
+            w = load8(a.weight, e, a.K);
         if constexpr (QUANT) {
             float t[8];
             for (int i = 0; i < 8; ++i)

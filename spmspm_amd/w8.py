@@ -69,9 +69,10 @@ _NONE = _Rows(None, 0)
 
 def _rows(name, t, dtype, shape, device):
     """16-bit rows of any stride."""
-    if t.dtype != dtype or t.shape != shape or t.device != device or (shape[1] > 1 and t.stride(1) != 1):
+    strides = t.stride()
+    if t.dtype != dtype or t.shape != shape or t.device != device or (strides[1] != 1 and shape[1] > 1):
         raise ValueError(f"{name} must be {dtype} {list(shape)} on {device} with contiguous rows")
-    return _Rows(t.data_ptr(), t.stride(0))
+    return _Rows(t.data_ptr(), strides[0])
 
 
 def _out_rows(name, t, like, inputs, outputs=()):
@@ -102,23 +103,40 @@ def _new_codes(x, N, K):
     """Room for N rows of K codes, 16-byte aligned, and their scales.  Long rows lie an odd multiple of 128 bytes apart: rows a power of
     two apart would meet on the same memory channels."""
     width = (K + 15) // 16 * 16 if K < 1024 else ((K + 127) // 128 | 1) * 128
-    codes = torch.empty((N, width), dtype=torch.int8, device=x.device)
-    return codes if width == K else codes[:, :K], torch.empty(N, dtype=torch.float32, device=x.device)
+    if K % 16:  # the last row too is readable up to a multiple of 16
+        codes = x.new_empty((N, width), dtype=torch.int8)[:, :K]
+    else:
+        codes = x.new_empty_strided((N, K), (width, 1), dtype=torch.int8)
+    return codes, width, x.new_empty(N, dtype=torch.float32)
 
 
-def _norm_args(x, weight, eps, residual):
-    _type(x.dtype)
-    if x.dim() != 2 or x.shape[1] == 0 or x.device.type != "cuda":
+def _norm_args(x, weight, eps, residual, most):
+    """Checked rows of x and of the residual, the kind of their type, N and K."""
+    shape, dtype, device = x.shape, x.dtype, x.device
+    kind = _type(dtype)
+    if len(shape) != 2 or shape[1] == 0 or not x.is_cuda:
         raise ValueError("x must be [tokens][K] on the GPU")
-    if x.shape[0] >= 1 << 31:
-        raise ValueError(f"{x.shape[0]} tokens: 2^31 - 1 at most")
-    if x.shape[1] > 1 << 24:
-        raise ValueError(f"rows of {x.shape[1]} numbers: 2^24 at most")
-    _check("weight", weight, x.device, x.dtype, (x.shape[1],))
+    N, K = shape
+    if N >= 1 << 31 or K > most:
+        raise ValueError(f"{N} tokens of {K} numbers: 2^31 - 1 tokens and {most} numbers at most")
+    if weight.shape != (K,) or weight.dtype != dtype or weight.device != device or not weight.is_contiguous():
+        raise ValueError(f"weight must be {dtype} [{K}], contiguous, on {device}")
     if not 1e-20 <= eps < 3e38:
         raise ValueError(f"eps {eps}: from 1e-20 up")
-    xr = _rows("x", x, x.dtype, x.shape, x.device)
-    return xr, _NONE if residual is None else _rows("residual", residual, x.dtype, x.shape, x.device)
+    xr = _rows("x", x, dtype, shape, device)
+    return xr, _NONE if residual is None else _rows("residual", residual, dtype, shape, device), kind, N, K
+
+
+def _given(x, residual, weight, residual_out, out):
+    """Checked rows of outputs that a caller gives, None for those that are to be made."""
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out without a residual: h is x itself")
+    hr = None if residual_out is None else _out_rows("residual_out", residual_out, x, (x, residual))
+    yr = None if out is None else _out_rows("out", out, x, (x, residual), (residual_out,))
+    for name, t in (("out", out), ("residual_out", residual_out)):
+        if t is not None and _overlap(t, weight):
+            raise ValueError(f"{name} overlaps the weight")
+    return hr, yr
 
 
 def rms_norm(x, weight, eps=1e-5, residual=None, out=None, residual_out=None, stream=None):
@@ -126,26 +144,21 @@ def rms_norm(x, weight, eps=1e-5, residual=None, out=None, residual_out=None, st
 
     x, residual [tokens][K], fp16 or bf16, contiguous rows of any stride; weight [K] of that type.  Returns y, with a residual
     (y, h).  `out` and `residual_out` take y and h: new tensors by default; either may be x or the residual itself."""
-    xr, rr = _norm_args(x, weight, eps, residual)
-    if residual is None and residual_out is not None:
-        raise ValueError("residual_out without a residual: h is x itself")
-    given = (x, residual, weight)
-    hr = None if residual_out is None else _out_rows("residual_out", residual_out, x, given[:2])
-    yr = None if out is None else _out_rows("out", out, x, given[:2], (residual_out,))
-    for name, t in (("out", out), ("residual_out", residual_out)):
-        if t is not None and _overlap(t, weight):
-            raise ValueError(f"{name} overlaps the weight")
+    xr, rr, kind, N, K = _norm_args(x, weight, eps, residual, 1 << 24)
+    hr, yr = (None, None) if residual_out is None and out is None else _given(x, residual, weight, residual_out, out)
 
     def call(handle):
-        y = x.new_empty(x.shape) if out is None else out
-        h = residual_out
-        if residual is not None and h is None:
-            h = x.new_empty(x.shape)
-        if x.shape[0]:
-            err = _library().RMS_Norm(handle, xr, rr, weight.data_ptr(), eps, x.shape[0], x.shape[1],
-                                      hr or (_NONE if h is None else _Rows(h.data_ptr(), x.shape[1])),
-                                      yr or _Rows(y.data_ptr(), x.shape[1]), None, _TYPES[x.dtype])
-            _raise(err, "rms_norm")
+        y, h, hrows, yrows = out, residual_out, hr or _NONE, yr
+        if y is None:
+            y = x.new_empty((N, K))
+            yrows = _Rows(y.data_ptr(), K)
+        if h is None and residual is not None:
+            h = x.new_empty((N, K))
+            hrows = _Rows(h.data_ptr(), K)
+        if N:
+            err = _library().RMS_Norm(handle, xr, rr, weight.data_ptr(), eps, N, K, hrows, yrows, None, kind)
+            if err:
+                _raise(err, "rms_norm")
         return y if residual is None else (y, h)
 
     return _run(x.device, stream, call)
@@ -156,28 +169,20 @@ def rms_norm_x8(x, weight, eps=1e-5, residual=None, residual_out=None, stream=No
 
     codes int8 [tokens][K] (rows 16-byte aligned, in general a slice of wider ones), scales float32 [tokens];
     y ~ codes * scales.  What a W8Linear and a W8GatedLinear take."""
-    xr, rr = _norm_args(x, weight, eps, residual)
-    N, K = x.shape
-    if K > MAX_K:
-        raise ValueError(f"rows of {K} codes: {MAX_K} at most")
-    if residual is None and residual_out is not None:
-        raise ValueError("residual_out without a residual: h is x itself")
-    hr = None
-    if residual_out is not None:
-        hr = _out_rows("residual_out", residual_out, x, (x, residual))
-        if _overlap(residual_out, weight):
-            raise ValueError("residual_out overlaps the weight")
+    xr, rr, kind, N, K = _norm_args(x, weight, eps, residual, MAX_K)
+    hr = None if residual_out is None else _given(x, residual, weight, residual_out, None)[0]
 
     def call(handle):
-        codes, scales = _new_codes(x, N, K)
-        h = residual_out
-        if residual is not None and h is None:
-            h = x.new_empty(x.shape)
+        codes, width, scales = _new_codes(x, N, K)
+        h, hrows = residual_out, hr or _NONE
+        if h is None and residual is not None:
+            h = x.new_empty((N, K))
+            hrows = _Rows(h.data_ptr(), K)
         if N:
-            err = _library().RMS_Norm(handle, xr, rr, weight.data_ptr(), eps, N, K,
-                                      hr or (_NONE if h is None else _Rows(h.data_ptr(), K)), _NONE,
-                                      _Codes(codes.data_ptr(), codes.stride(0), scales.data_ptr()), _TYPES[x.dtype])
-            _raise(err, "rms_norm_x8")
+            err = _library().RMS_Norm(handle, xr, rr, weight.data_ptr(), eps, N, K, hrows, _NONE,
+                                      _Codes(codes.data_ptr(), width, scales.data_ptr()), kind)
+            if err:
+                _raise(err, "rms_norm_x8")
         return (codes, scales) if residual is None else (codes, scales, h)
 
     return _run(x.device, stream, call)
@@ -192,10 +197,11 @@ def quantize_x8(x, stream=None):
     N, K = x.shape
 
     def call(handle):
-        codes, scales = _new_codes(x, N, K)
+        codes, width, scales = _new_codes(x, N, K)
         if N:
-            err = _library().W8_Quantize(handle, xr, N, K, _Codes(codes.data_ptr(), codes.stride(0), scales.data_ptr()), kind)
-            _raise(err, "quantize_x8")
+            err = _library().W8_Quantize(handle, xr, N, K, _Codes(codes.data_ptr(), width, scales.data_ptr()), kind)
+            if err:
+                _raise(err, "quantize_x8")
         return codes, scales
 
     return _run(x.device, stream, call)
@@ -249,6 +255,7 @@ class _Product:
         for b in biases:
             if b is not None:
                 _check("bias", b, self.device, dtype, (M,))
+        self._kind = _TYPES[dtype]
 
     def bytes_per_call(self, N):
         """Bytes a call with N rows of 8-bit x must move: weights and scales, x and y."""
@@ -257,12 +264,13 @@ class _Product:
     def __call__(self, x, scales=None, out=None, stream=None):
         """x int8 [N][K] with float32 scales [N] (of rms_norm_x8 or quantize_x8), or 16-bit [N][K] in the layer's type, which is rounded
         to 8 bits first.  Returns [N][M] in the layer's type."""
-        if x.dim() != 2 or x.shape[1] != self.K or x.device != self.device:
-            raise ValueError(f"x must be [N][{self.K}] on {self.device}")
-        N, stride = x.shape[0], x.stride(0)
+        shape, K = x.shape, self.K
+        if len(shape) != 2 or shape[1] != K or x.device != self.device:
+            raise ValueError(f"x must be [N][{K}] on {self.device}")
+        N, (stride, inner) = shape[0], x.stride()
         if N > 16 * 65535:
             raise ValueError(f"{N} rows of x: {16 * 65535} at most")
-        if N and self.K > 1 and x.stride(1) != 1:
+        if inner != 1 and N and K > 1:
             raise ValueError("x must have contiguous rows")
         if scales is None:
             if x.dtype != self.dtype:
@@ -270,11 +278,12 @@ class _Product:
         else:
             if x.dtype != torch.int8:
                 raise ValueError("scales belong to int8 codes")
-            _check("scales", scales, self.device, torch.float32, (N,))
-            wide = (self.K + 15) // 16 * 16
-            if N and (x.data_ptr() % 16 or (N > 1 and (stride % 16 or stride < wide))
-                      or x.storage_offset() + (N - 1) * stride + wide > x.untyped_storage().nbytes()):
-                raise ValueError("rows of codes must be aligned to 16 bytes and readable up to a multiple of 16")
+            if scales.shape != (N,) or scales.dtype != torch.float32 or scales.device != self.device or not scales.is_contiguous():
+                raise ValueError(f"scales must be float32 [{N}], contiguous, on {self.device}")
+            wide = (K + 15) // 16 * 16
+            if N and (x.data_ptr() % 16 or (N > 1 and (stride % 16 or stride < wide or stride > 1 << 28))
+                      or (wide != K and x.storage_offset() + (N - 1) * stride + wide > x.untyped_storage().nbytes())):
+                raise ValueError("rows of codes must be aligned to 16 bytes, at most 2^28 apart and readable up to a multiple of 16")
             if N == 1:
                 stride = wide
         if out is not None:
@@ -283,17 +292,17 @@ class _Product:
                 raise ValueError("out overlaps an input")
 
         def call(handle):
-            y = torch.empty((N, self.M), dtype=self.dtype, device=self.device) if out is None else out
+            y = self.packed.new_empty((N, self.M), dtype=self.dtype) if out is None else out
             if N:
-                L, kind = _library(), _TYPES[self.dtype]
-                need = L.W8_WorkspaceBytes(self.M, N, self.K, self.gated, scales is None)
+                L, M, gated = _library(), self.M, self.gated
+                need = L.W8_WorkspaceBytes(M, N, K, gated, scales is None)
                 ws = self.packed.new_empty(need) if need else None
-                source = _Codes(x.data_ptr(), stride, None if scales is None else scales.data_ptr())
-                biases = [None if b is None else b.data_ptr() for b in self.biases]
-                err = (L.W8_Gated if self.gated else L.W8_Linear)(
-                    handle, self.packed.data_ptr(), source, y.data_ptr(), self.M, N, self.K, *biases, self.activation,
-                    None if ws is None else ws.data_ptr(), need, kind)
-                _raise(err, type(self).__name__)
+                err = (L.W8_Gated if gated else L.W8_Linear)(
+                    handle, self.packed.data_ptr(), _Codes(x.data_ptr(), stride, None if scales is None else scales.data_ptr()),
+                    y.data_ptr(), M, N, K, *[None if b is None else b.data_ptr() for b in self.biases], self.activation, None if ws is None else ws.data_ptr(), need,
+                    self._kind)
+                if err:
+                    _raise(err, type(self).__name__)
             return y
 
         return _run(self.device, stream, call)
