@@ -82,24 +82,8 @@ struct ProductArgs {
     const uint16_t *bias, *up_bias;
     int*           part; // sums of the shares of K (part_of); null where K is not split
     int            M, N, K, act, bf16;
-    int            shares, per; // of w8_narrow: shares of K, blocks of 128 columns in each but the last
-    int            full;        // of w8_tiles: tiles that one workgroup takes whole; the others are cut up among all
-    int            row_tiles, column_tiles, grid; // of w8_tiles: its tiles and workgroups
+    int            shares, per; // shares of K, blocks of 128 columns in each but the last
 };
-
-// The kernel's arguments, read from memory once more where a tile begins and ends: kept in registers from the kernel's start they would
-// leave too few scalars for its loop.
-__device__ __forceinline__ ProductArgs late_args8()
-{
-    typedef const __attribute__((address_space(4))) ProductArgs* Pointer;
-    Pointer p = (Pointer)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(p));
-    ProductArgs a{};
-    a.packed = p->packed, a.x = p->x, a.x_scales = p->x_scales, a.x_stride = p->x_stride, a.y = p->y, a.bias = p->bias;
-    a.up_bias = p->up_bias, a.part = p->part, a.M = p->M, a.N = p->N, a.K = p->K, a.act = p->act, a.bf16 = p->bf16, a.full = p->full;
-    a.row_tiles = p->row_tiles, a.column_tiles = p->column_tiles, a.grid = p->grid;
-    return a;
-}
 
 // ReLU, GELU (tanh form) or SiLU of W sums.  The last two are y / (1 + exp(-z)), with z = 2 sqrt(2/pi) (y + 0.044715 y^3), since
 // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), or z = y; far from 0 they end at 0 and y.  The reciprocal's last bit is far below 16 bits.
@@ -343,21 +327,16 @@ __device__ __forceinline__ void each(F f)
 }
 
 // A wave's 1 KB of 16 bytes a lane goes from global memory straight into LDS.  In assembly, since the compiler would wait for it
-// ahead of the next read of LDS; the kernel waits for it itself, before the barrier that hands the tile over.  OFFSET counts for both
-// addresses.
-template <int OFFSET>
+// ahead of the next read of LDS; the kernel waits for it itself, before the barrier that hands the tile over.
 __device__ __forceinline__ void to_lds(unsigned lds, const void* base, unsigned offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds), "v"(offset), "s"(base), "n"(OFFSET)
-                 : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
 // The same of memory that is read once: the caches are kept for what is read again (36864x9216 with 64 columns 92 -> 87 us).
-template <int OFFSET>
 __device__ __forceinline__ void to_lds_once(unsigned lds, const void* base, unsigned offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3 nt" ::"s"(lds), "v"(offset), "s"(base), "n"(OFFSET)
-                 : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
 // The same of one word, or of 16 bits in a word, a lane.
@@ -371,98 +350,19 @@ __device__ __forceinline__ void short_to_lds(unsigned lds, const void* address)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, off" ::"s"(lds), "v"(address) : "memory");
 }
 
-// Workgroups are dealt to the eight dies in turn, each with an L2 of its own: place of the id-th of `total` things in an order that has
-// those of a die one behind the other.
-__device__ __forceinline__ int dealt8(int id, int total)
-{
-    const int die = id % 8;
-    return die * (total / 8) + min(die, total % 8) + id / 8;
-}
-
-// The order of tiles: bands of kBand row tiles, in a band column by column, so that what a die works on at once shares W and X.
-__device__ __forceinline__ void tile8(const ProductArgs& a, int at, int& row, int& column)
+// Workgroups are dealt to the eight dies in turn, each with an L2 of its own: consecutive numbers on one die, and there a band of
+// kBand row tiles by as many column tiles as run at once; shares of K one after another.
+__device__ __forceinline__ void place8(int id, int row_tiles, int column_tiles, int shares, int& row, int& column, int& share)
 {
     constexpr int kBand = 8;
-    const int     band = at / (kBand * a.column_tiles), first = band * kBand, height = min(kBand, a.row_tiles - first);
-    const int     in   = at - first * a.column_tiles;
+    const int     one = row_tiles * column_tiles, total = one * shares, xcd = id % 8, rest = total % 8;
+    int           at = xcd * (total / 8) + min(xcd, rest) + id / 8;
+    share            = __builtin_amdgcn_readfirstlane(at / one);
+    at -= share * one;
+    const int     band = at / (kBand * column_tiles), first = band * kBand, height = min(kBand, row_tiles - first);
+    const int     in   = at - first * column_tiles;
     // divisions are done by vector instructions: back to scalars, which the addresses are made of
     row = __builtin_amdgcn_readfirstlane(first + in % height), column = __builtin_amdgcn_readfirstlane(in / height);
-}
-
-// What a workgroup of w8_tiles works on: every grid-th of the first `full` tiles, then its part of the others, whose blocks of K are one
-// row that is cut into `grid` parts of a length.  A part crosses from tile to tile; what is not a whole tile goes to memory as sums.
-struct Work8 {
-    int next, at, end; // next tile; next block of its part of the others, and end
-
-    __device__ __forceinline__ explicit Work8(const ProductArgs& a) : next(blockIdx.x)
-    {
-        const int64_t rest = (int64_t)(a.row_tiles * a.column_tiles - a.full) * ((a.K + 127) / 128);
-        const int     part = dealt8(blockIdx.x, a.grid);
-        at  = __builtin_amdgcn_readfirstlane((int)(part * rest / a.grid));
-        end = __builtin_amdgcn_readfirstlane((int)((part + 1) * rest / a.grid));
-    }
-
-    // Place of the next tile, its first block and how many; false: there is none.
-    __device__ __forceinline__ bool take(const ProductArgs& a, int& place, int& first, int& count)
-    {
-        const int blocks = (a.K + 127) / 128;
-        if (next < a.full) {
-            place = dealt8(next, a.full), first = 0, count = blocks;
-            next += a.grid;
-            return true;
-        }
-        if (at >= end)
-            return false;
-        const int other = __builtin_amdgcn_readfirstlane(at / blocks);
-        place = a.full + other, first = at - other * blocks, count = min(blocks - first, end - at);
-        at += count;
-        return true;
-    }
-};
-
-// The part that block `at` of the others lies in, of `parts` over `rest` blocks: the inverse of Work8's bounds.
-__device__ __forceinline__ int part8(int at, int rest, int parts)
-{
-    return (int)((((int64_t)at + 1) * parts - 1) / rest);
-}
-
-// Sums of a part of a tile: parts and tiles are crossed one at a time, so that the sum of their numbers names a place of its own.
-// In it, of 16 columns after the other, the row groups, four tiles of 1 KB.
-__device__ __forceinline__ intx4* cut_of(int* part, int place, int cols, int groups, int column, int group)
-{
-    return reinterpret_cast<intx4*>(part) + (((int64_t)place * cols + column) * groups + group) * 256;
-}
-
-// A wave ends half a group (as in w8_join) of 16 columns of a tile of w8_tiles that was cut up.
-template <bool GATED>
-__global__ __launch_bounds__(256) void w8_join_cut(ProductArgs a, int rows, int cols)
-{
-    const Layout8 l = layout8(a.M, a.K, GATED);
-    const int     lane = threadIdx.x % kWave, groups = rows / 4, blocks = l.steps / 2, rest = a.row_tiles * a.column_tiles - a.full;
-    int           unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
-    const int     h = unit & 1, g = (unit >>= 1) % groups, u = (unit /= groups) % cols, tile = unit / cols;
-    if (tile >= rest)
-        return;
-    int row, column;
-    tile8(a, a.full + tile, row, column);
-    const int group = row * groups + g, n = (column * cols + u) * 16 + (lane & 15), q = lane >> 4;
-    const int lowest = part8(tile * blocks, rest * blocks, a.grid), highest = part8((tile + 1) * blocks - 1, rest * blocks, a.grid);
-    if (lowest == highest || group >= l.groups || n >= a.N)
-        return; // one workgroup had all of it
-    const intx4*  p    = cut_of(a.part, lowest + tile, cols, groups, u, g) + (GATED ? h : 2 * h) * 64 + lane;
-    const int64_t next = (int64_t)cols * groups * 256;
-    intx4         sum[2] = {0, 0};
-#pragma unroll 8
-    for (int s = 0; s <= highest - lowest; ++s)
-        for (int t = 0; t < 2; ++t)
-            sum[t] += p[s * next + t * (GATED ? 128 : 64)];
-    int v[8];
-    for (int i = 0; i < 8; ++i)
-        v[i] = sum[i / 4][i % 4];
-    if constexpr (GATED)
-        Tail8<true, 4>(a, l, group * 32 + 8 * q + 4 * h).store(a, n, a.x_scales[n], v, v + 4);
-    else
-        Tail8<false, 8>(a, l, group * 64 + 16 * q + 8 * h).store(a, n, a.x_scales[n], v, nullptr);
 }
 
 // A workgroup of WM x WN waves takes WM MT x WN NT tiles of 16 x 16 outputs (packed rows x rows of X), a wave MT x NT of them.  K goes by in
@@ -470,18 +370,16 @@ __global__ __launch_bounds__(256) void w8_join_cut(ProductArgs a, int rows, int 
 // row r's chunk c of 16 bytes at place 8 r + (c ^ r), which the matrix operands' reads find without bank conflicts.
 // While the products of a block's first half run, the second half's operands are read; then the waves meet, the place that
 // all have read takes the block S further on, and the next block's first operands are read under the second half's products.
-// A workgroup stays on its CU for many tiles (Work8), whose blocks are one stream: the next tile is loaded while the results of the last
-// are written, and a tile costs its products alone.
+// A workgroup stays on its CU and takes every gridDim-th tile: the blocks of all its tiles are one stream, so that the next tile is
+// loaded while the results of the last are written, and a tile costs its products alone.
 template <bool GATED, int MT, int NT, int WM, int WN, int S>
-__global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs args)
+__global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs a, int row_tiles, int column_tiles)
 {
     constexpr int kWaves = WM * WN, kRows = WM * MT, kCols = WN * NT, kStage = (kRows + kCols) * 2048; // tiles of W, of X
     constexpr int kLoads = 2 * (kRows + kCols) / kWaves;
     constexpr int kM = kRows * 16, kN = kCols * 16; // packed rows, rows of X
     constexpr int kEnds = S + 2; // loads are at most S + 1 tiles ahead of the products
-    constexpr int kWLoads = 2 * kRows / kWaves, kXLoads = 2 * kCols / kWaves; // of a wave, of W and of X
-    static_assert(2 * kRows % kWaves == 0 && 2 * kCols % kWaves == 0 && (kWLoads == 2 || kWLoads == 4));
-    static_assert(MT % 4 == 0 && kM % 128 == 0 && kN % 64 == 0 && S >= 2);
+    static_assert(2 * (kRows + kCols) % kWaves == 0 && MT % 4 == 0 && kM % 128 == 0 && kN % 64 == 0 && S >= 2);
     struct Ends { // of a tile: scales and biases of its rows (of the gate, then of up), scales of its rows of X
         float    sw[kM];
         unsigned b[kM];
@@ -489,41 +387,38 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs args)
     };
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S][kStage];
     __shared__ __attribute__((aligned(16))) Ends      ends[kEnds];
+    const Layout8 l    = layout8(a.M, a.K, GATED);
     const int     lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int     q = lane >> 4, c = lane & 15, wm = wave / WN, wn = wave % WN;
+    const int     tiles = row_tiles * column_tiles * a.shares;
 
-    // What a wave brings of every block: kWLoads KBs of W, as they are packed, half a group's or a quarter's, then kXLoads of X.
-    const uint8_t* w_now; // W's block of the next load, from the tile's first group on
-    const int8_t*  x_at[kXLoads];
-    unsigned       w_off, x_off[kXLoads];
+    // What a wave brings of every block: KBs wave, wave + kWaves, ... of W's, as they are packed, then of X's.
+    const uint8_t* from[kLoads];
+    unsigned       off[kLoads];
     auto address = [](const void* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p; };
     const unsigned lds0 = address(lds), ends0 = address(ends);
-    const int      chunk = 16 * ((lane & 7) ^ (lane >> 3)), last = (args.K - 1) / 16 * 16;
-    const int64_t block_bytes = (int64_t)layout8(args.M, args.K, GATED).groups * kGroup8;
-    const bool    once        = args.column_tiles == 1;
-    Work8 ahead(args), now = ahead; // of the loads, of the products
-    int   ahead_block, ahead_end, ahead_turn = 0, turn = 0;                  // block of the next load and end of its tile's; tiles seen
-    int   place_now, left;                                                   // of the products' tile: place, blocks left
-    // Turns the loads to the next tile, the ahead_turn-th, and brings its ends.
-    auto enter = [&] {
-        int at, row, column;
-        const ProductArgs a = late_args8();
-        int               from, many;
-        if (!ahead.take(a, at, from, many))
-            return;
-        ahead_block = from, ahead_end = from + many;
-        const Layout8     l = layout8(a.M, a.K, GATED);
-        tile8(a, at, row, column);
+    const int      chunk = 16 * ((lane & 7) ^ (lane >> 3)), last = (a.K - 1) / 16 * 16;
+    // Tile and block of the next load, the end of its blocks, and how many tiles it has seen; tile and number of the next products, and
+    // how many blocks of it are left.
+    int ahead_tile = blockIdx.x, ahead_block, ahead_end, ahead_turn = 0, tile = blockIdx.x, left, turn = 0;
+    // Turns the loads to a tile, the `turn`-th, and brings its ends.
+    auto enter = [&](int tile, int turn) {
+        int row, column, share;
+        place8(tile, row_tiles, column_tiles, a.shares, row, column, share);
         const int tile0 = row * kRows, n0 = column * kN;
-        w_now = a.packed + (int64_t)ahead_block * block_bytes + (int64_t)(tile0 / 4) * kGroup8;
-        // groups and rows behind the last are the last again: computed, not stored
-        w_off = min(wave * kWLoads / 8, l.groups - 1 - tile0 / 4) * kGroup8 + wave * kWLoads % 8 * 1024 + lane * 16;
-        for (int i = 0; i < kXLoads; ++i) {
-            const int n = min(n0 + 8 * (wave * kXLoads + i), a.N - 1);
-            x_at[i]     = a.x + (int64_t)n * a.x_stride;
-            x_off[i]    = min(lane >> 3, a.N - 1 - n) * (unsigned)a.x_stride;
+        ahead_block = share * a.per, ahead_end = min(ahead_block + a.per, l.steps / 2);
+        for (int i = 0; i < kLoads; ++i) { // groups and rows behind the last are the last again: computed, not stored
+            const int j = wave + i * kWaves;
+            if (j < 2 * kRows) {
+                from[i] = a.packed + (int64_t)min(tile0 / 4 + j / 8, l.groups - 1) * kGroup8 + j % 8 * 1024;
+                off[i]  = lane * 16;
+            } else {
+                const int n = min(n0 + 8 * (j - 2 * kRows), a.N - 1);
+                from[i]     = reinterpret_cast<const uint8_t*>(a.x) + (int64_t)n * a.x_stride;
+                off[i]      = min(lane >> 3, a.N - 1 - n) * (unsigned)a.x_stride;
+            }
         }
-        const unsigned to = ends0 + ahead_turn++ % kEnds * (unsigned)sizeof(Ends);
+        const unsigned to = ends0 + turn % kEnds * (unsigned)sizeof(Ends);
         const float*   sw = reinterpret_cast<const float*>(a.packed + l.scales);
         for (int i = wave; i < kM / 64; i += kWaves) { // 64 rows, all of the gate or all of up
             const bool up = GATED && i >= kM / 128;
@@ -537,18 +432,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs args)
         for (int i = kWaves - 1 - wave; i < kN / 64; i += kWaves)
             word_to_lds(to + kM * 8 + i * 256, a.x_scales + min(n0 + i * 64 + lane, a.N - 1));
     };
+    const int64_t block_bytes = (int64_t)l.groups * kGroup8;
     // The i-th of a wave's loads of a block.  Behind the last 16 columns of X the weights are 0: what is there does not matter.
-    auto stage = [&](auto i, int place) {
-        const unsigned to = lds0 + place * kStage;
-        if constexpr (i < kWLoads) {
-            if (kCols <= 4 && once)
-                to_lds_once<i * 1024>(to + wave * kWLoads * 1024, w_now, w_off);
+    auto stage = [&](int i, int block, int place) {
+        const int      j  = wave + i * kWaves;
+        const unsigned to = lds0 + place * kStage + j * 1024;
+        if ((i + 1) * kWaves <= 2 * kRows || j < 2 * kRows) {
+            if (column_tiles == 1)
+                to_lds_once(to, from[i] + block * block_bytes, off[i]);
             else
-                to_lds<i * 1024>(to + wave * kWLoads * 1024, w_now, w_off);
-        } else {
-            constexpr int x = i - kWLoads;
-            to_lds<0>(to + (2 * kRows + wave * kXLoads + x) * 1024, x_at[x], x_off[x] + min(ahead_block * 128 + chunk, last));
-        }
+                to_lds(to, from[i] + block * block_bytes, off[i]);
+        } else
+            to_lds(to, from[i], off[i] + min(block * 128 + chunk, last));
     };
     struct Operands {
         intx4 w[MT], x[NT];
@@ -572,84 +467,93 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs args)
     // ahead of its products until the memory pipe has taken them.
     constexpr int kParts = kProducts / 4;
     auto multiply = [&](const Operands& o, auto between) {
-        each<kParts>([&](auto part) {
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
 #pragma unroll
             for (int f = 4 * part; f < 4 * part + 4; ++f)
                 sum[f % MT][f / MT] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[f % MT], o.x[f / MT], sum[f % MT][f / MT], 0, 0, 0);
             between(part);
             __builtin_amdgcn_sched_barrier(0);
-        });
+        }
     };
-    // f(i) for items `part` of `parts` of N.
-    auto share = [](auto n, auto part, auto parts, auto f) {
-        each<n * (part + 1) / parts - n * part / parts>([&](auto i) { f(std::integral_constant<int, n * part / parts + i>()); });
+    // Items `part` of `parts` of n, as a range.
+#define W8_SHARE(i, n, part, parts) for (int i = (n) * (part) / (parts); i < (n) * ((part) + 1) / (parts); ++i)
+    auto advance = [&] {
+        if (++ahead_block >= ahead_end) {
+            ahead_tile += gridDim.x, ++ahead_turn;
+            if (ahead_tile < tiles)
+                enter(ahead_tile, ahead_turn);
+        }
     };
-    constexpr std::integral_constant<int, kReads> reads;
-    constexpr std::integral_constant<int, kLoads> loads;
-    constexpr std::integral_constant<int, kParts> parts;
-    auto advance = [&] { // behind the last block there is that block again, which nobody reads: loads are made, and counted, all the same
-        if (ahead_block + 1 < ahead_end)
-            ++ahead_block, w_now += block_bytes;
-        else
-            enter();
+    auto begin = [&] { // blocks of the tile that the products come to
+        int row, column, share;
+        place8(tile, row_tiles, column_tiles, a.shares, row, column, share);
+        left = min(a.per, l.steps / 2 - share * a.per);
     };
-    int first_now;
-    if (!now.take(args, place_now, first_now, left)) // no block: there are fewer than workgroups
-        return;
-    enter();
-    int count = left;
+    enter(tile, 0);
+    begin();
     for (int s = 0; s < S; ++s) {
-        each<kLoads>([&](auto i) { stage(i, s); });
-        advance();
+        if (ahead_tile < tiles) {
+            for (int i = 0; i < kLoads; ++i)
+                stage(i, ahead_block, s);
+            advance();
+        }
     }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * kLoads) : "memory");
+    if (ahead_tile < tiles)
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * kLoads) : "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     Operands first, second;
     for (int i = 0; i < kReads; ++i)
         fetch(first, i, 0, 0);
     clear();
-    constexpr int kEarly = kParts > 2 ? kParts * 3 / 4 : kParts; // parts under which operands are read: the rest covers their latency
-    constexpr std::integral_constant<int, kEarly> early;
+    constexpr int kEarly  = kParts > 2 ? kParts * 3 / 4 : kParts; // parts under which operands are read: the rest covers their latency
     constexpr int kStores = MT / 4 * NT * (GATED ? 1 : 2);  // of a wave for a tile that is full
     constexpr int kAway   = (S - 2) * kLoads;               // a wave's loads of the blocks behind the next
     static_assert(kAway + kStores < 64);
     int place = 0, relaxed = 0; // relaxed: barriers ahead of which the last results' stores may still be under way
     for (;;) {
-        multiply(first, [&](auto part) {
-            if constexpr (part < kEarly)
-                share(reads, part, early, [&](auto i) { fetch(second, i, place, 1); });
+const bool more = ahead_tile < tiles;
+        multiply(first, [&](int part) {
+            if (part < kEarly)
+                W8_SHARE(j, kReads, part, kEarly)
+                    fetch(second, j, place, 1);
         });
         // The next block has come.  Loads and stores are counted in their order: behind it are kAway loads, and stores.
-        if (relaxed > 0)
+        if (!more)
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else if (relaxed > 0)
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kAway + kStores) : "memory");
         else
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kAway) : "memory");
         --relaxed;
         const int next = place + 1 == S ? 0 : place + 1;
-        multiply(second, [&](auto part) {
-            if constexpr (part < kEarly) // behind the last block bytes that nothing takes
-                share(reads, part, early, [&](auto i) { fetch(first, i, next, 0); });
-            share(loads, part, parts, [&](auto i) { stage(i, place); });
+        multiply(second, [&](int part) {
+            if (part < kEarly)
+                W8_SHARE(j, kReads, part, kEarly) // behind the last block stale bytes, which nothing takes
+                    fetch(first, j, next, 0);
+            if (more)
+                W8_SHARE(j, kLoads, part, kParts)
+                    stage(j, ahead_block, place);
         });
-        advance();
+        if (more)
+            advance();
         place = next;
         --left;
         if (left == 0) {
-            const ProductArgs a = late_args8();
-            const Layout8     l = layout8(a.M, a.K, GATED);
-            int               row, column;
-            tile8(a, place_now, row, column);
+            int row, column, share;
+            place8(tile, row_tiles, column_tiles, a.shares, row, column, share);
             const Ends& e = ends[turn % kEnds];
-            if (count == l.steps / 2) {
+            if (a.part == nullptr) {
                 each<MT / 4>([&](auto g) {
                     const int group = wm * (MT / 4) + g;
                     each<GATED ? 1 : 2>([&](auto h) {
-                        const int j = GATED ? group * 32 + 8 * q : group * 64 + 16 * q + 8 * h;
+                        const int             j = GATED ? group * 32 + 8 * q : group * 64 + 16 * q + 8 * h;
+                        const Tail8<GATED, 8> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
                         each<NT>([&](auto u) {
                             const int n = column * kN + (wn * NT + u) * 16 + c;
                             if (n >= a.N)
                                 return;
-                            asm volatile("" ::: "memory"); // scales and biases once more, rather than in registers there are not enough of
-                            const Tail8<GATED, 8> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
                             int v[16];
                             for (int i = 0; i < 16; ++i)
                                 v[i] = sum[g * 4 + i / 4][u][i % 4];
@@ -660,33 +564,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs args)
                 // With all its stores made: of the barriers that wait for loads older than they are.
                 relaxed = (row + 1) * (GATED ? kM / 2 : kM) <= a.M && (column + 1) * kN <= a.N ? S - 1 : 0;
             } else {
+                const int columns = (a.N + 15) / 16;
                 each<NT>([&](auto u) {
-                    each<MT / 4>([&](auto g) {
-                        const int group = wm * (MT / 4) + g;
-                        if (column * kN + (wn * NT + u) * 16 < a.N && row * (kM / 64) + group < l.groups)
-                            each<4>([&](auto t) {
-                                cut_of(a.part, dealt8(blockIdx.x, a.grid) + place_now - a.full, kCols, kM / 64, wn * NT + u, group)[t * 64 + lane] =
-                                    sum[g * 4 + t][u];
-                            });
+                    const int at = column * kCols + wn * NT + u;
+                    each<MT>([&](auto t) {
+                        const int group = row * (kM / 64) + wm * (MT / 4) + t / 4;
+                        if (at < columns && group < l.groups)
+                            part_of(a, l.groups, share, columns, group, at)[t % 4 * 64 + lane] = sum[t][u];
                     });
                 });
             }
-            ++turn;
-            if (!now.take(a, place_now, first_now, left))
-                break;
-            count = left;
+            tile += gridDim.x, ++turn;
+            if (tile >= tiles)
+                return;
+            begin();
             clear();
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the LDS that loads are on their way to is the workgroup's until they are there
+#undef W8_SHARE
 }
 
 // How a call runs.
 struct Plan8 {
     int kind;        // 0: w8_narrow, otherwise a w8_tiles of kTiles[kind - 1]
     int rows, cols;  // row and column tiles of 16 that a workgroup of w8_narrow takes
-    int shares, per; // of w8_narrow: shares of K, blocks of 128 columns in each
-    int grid, full;  // of w8_tiles: workgroups, and tiles that they take whole (Work8)
+    int shares, per; // shares of K, blocks of 128 columns in each
 };
 
 // What plan8 knows of the shapes of w8_tiles: a workgroup's row and column tiles, how many fit a CU, and in microseconds what a tile costs
@@ -700,7 +602,7 @@ constexpr Tiles8 kTiles[] = {{16, 16, 1, 5.3, 1.41, 0},    {8, 16, 1, 4.3, 0.85,
 constexpr int kShapes = sizeof kTiles / sizeof *kTiles;
 
 #ifdef SPMM_KEEP_VARIANTS
-Plan8 g_plan8{};
+Plan8 g_plan8{0, 0, 0, 0, 0};
 #endif
 
 int64_t up8(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -724,19 +626,6 @@ Plan8 plan8(int M, int N, int K, bool gated)
     Plan8         p{}, best{};
     double        least = 1e300;
 #ifdef SPMM_KEEP_VARIANTS // the tests' build: every kernel at small sizes
-    if (g_plan8.kind > 0) {
-        p               = g_plan8;
-        const int64_t n = up8(tiles, kTiles[p.kind - 1].rows) * up8(N, 16 * kTiles[p.kind - 1].cols);
-        if (p.grid == 0)
-            p.grid = 256 * kTiles[p.kind - 1].resident, p.full = (int)n;
-        else
-            p.full = (int)(n / p.grid * p.grid);
-        if ((n - p.full) * blocks < p.grid)
-            p.full = (int)n;
-        if (p.full == n)
-            p.grid = (int)std::min<int64_t>(p.grid, n);
-        return p;
-    }
     if (g_plan8.shares > 0) {
         p = g_plan8;
         share8(p, blocks, g_plan8.shares);
@@ -744,6 +633,8 @@ Plan8 plan8(int M, int N, int K, bool gated)
     }
 #endif
     auto consider = [&](double us) {
+        if (p.shares > 1)
+            us += 3.0 + p.shares * part_mb / 8.4;
         if (us < least)
             least = us, best = p;
     };
@@ -756,31 +647,23 @@ Plan8 plan8(int M, int N, int K, bool gated)
                         break;
                     share8(p, blocks, s);
                     consider(2.8 + w_mb * (double)columns / 12.7 +
-                             (double)(up8(groups * p.shares, 256) * up8(p.per, 8)) * (0.20 * p.rows + 0.25 * p.cols) +
-                             (p.shares > 1 ? 3.0 + p.shares * part_mb / 8.4 : 0));
+                             (double)(up8(groups * p.shares, 256) * up8(p.per, 8)) * (0.20 * p.rows + 0.25 * p.cols));
                 }
             }
     for (p.kind = 1; p.kind <= kShapes; ++p.kind) {
-        const Tiles8& k = kTiles[p.kind - 1];
-        const int64_t n = up8(tiles, k.rows) * up8(N, 16 * k.cols), slots = 256 * k.resident;
-        if (n > 0x3fffffff)
-            continue;
-        p.rows = p.cols = p.shares = p.per = 0;
-        auto block = [&](int64_t workgroups) { return workgroups > 256 ? k.both : k.block; };
-        // every tile whole
-        p.grid = (int)std::min(n, slots), p.full = (int)n;
-        const int64_t full = n / slots, rest = n % slots;
-        consider(2.4 + w_mb / 25 + (double)full * (k.tile + (double)blocks * block(slots)) +
-                 (rest > 0 ? k.tile + (double)blocks * block(rest) : 0));
-        // the last round's tiles cut up among all workgroups, or among so many that every tile has the same number of them
-        for (int64_t grid : {slots, (int64_t)256, rest > 0 ? 256 / rest * rest : 0, rest > 0 ? slots / rest * rest : 0}) {
-            grid = std::min(grid, rest * blocks);
-            if (rest == 0 || grid <= rest || (full > 0 && grid != slots))
+        const Tiles8& k      = kTiles[p.kind - 1];
+        const int64_t groups = up8(tiles, k.rows) * up8(N, 16 * k.cols);
+        p.rows = p.cols = 0;
+        for (int fill = 0; fill <= k.resident; ++fill) { // shares for none, one or two workgroups on every CU
+            if (fill > 0 && 256 * fill / groups < 2)
                 continue;
-            p.grid = (int)grid, p.full = (int)(full * slots);
-            const double cuts = (double)(grid % rest == 0 ? grid : grid + rest), mb = (double)(k.rows * k.cols) * 2048e-6;
-            consider(2.4 + w_mb / 25 + (double)full * (k.tile + (double)blocks * block(slots)) + k.tile +
-                     (double)up8(rest * blocks, grid) * block(grid) + 3.0 + cuts * mb / 8.4);
+            share8(p, blocks, fill > 0 ? std::min<int64_t>(64, 256 * fill / groups) : 1);
+            const int64_t slots = 256 * k.resident, full = groups * p.shares / slots, rest = groups * p.shares % slots;
+            double        us = 2.4 + w_mb / 25;
+            us += (double)full * (k.tile + p.per * (k.resident > 1 ? k.both : k.block));
+            if (rest > 0)
+                us += k.tile + p.per * (rest > 256 ? k.both : k.block);
+            consider(us);
         }
     }
     return best;
@@ -788,24 +671,19 @@ Plan8 plan8(int M, int N, int K, bool gated)
 
 size_t part_bytes8(int M, int N, int K, bool gated, const Plan8& p)
 {
-    if (p.kind > 0) {
-        const Tiles8& k = kTiles[p.kind - 1];
-        const int64_t n = up8((int64_t)layout8(M, K, gated).groups * 4, k.rows) * up8(N, 16 * k.cols);
-        return n > p.full ? (size_t)(p.grid + n - p.full) * k.rows * k.cols * 1024 : 0;
-    }
     return p.shares > 1 ? (size_t)p.shares * up8(N, 16) * layout8(M, K, gated).groups * 4096 : 0;
 }
 
 template <bool GATED, int MT, int NT, int WM, int WN, int S>
-int run_tiles8(hipStream_t stream, const Plan8& p, ProductArgs a)
+int run_tiles8(hipStream_t stream, const ProductArgs& a, int resident)
 {
-    constexpr int kRows = MT * WM, kCols = NT * WN;
-    const int     rows = (int)up8(layout8(a.M, a.K, GATED).groups * 4, kRows), cols = (int)up8(a.N, kCols * 16), rest = rows * cols - a.full;
-    a.row_tiles = rows, a.column_tiles = cols, a.grid = p.grid;
-    const int e = launch(w8_tiles<GATED, MT, NT, WM, WN, S>, dim3((unsigned)p.grid, 1, 1), dim3(64 * WM * WN, 1, 1), stream, a);
-    if (e != 0 || rest == 0)
-        return e;
-    return launch(w8_join_cut<GATED>, dim3((unsigned)up8(rest * (kRows / 4) * kCols * 2, 4), 1, 1), dim3(256, 1, 1), stream, a, kRows, kCols);
+    const Layout8 l    = layout8(a.M, a.K, GATED);
+    const int     rows = (int)up8(l.groups * 4, MT * WM), cols = (int)up8(a.N, NT * WN * 16);
+    const int64_t tiles = (int64_t)rows * cols * a.shares;
+    if (tiles > 0x7fffffff)
+        return refuse("%lld tiles of outputs", (long long)tiles);
+    return launch(w8_tiles<GATED, MT, NT, WM, WN, S>, dim3((unsigned)std::min<int64_t>(tiles, 256 * resident), 1, 1),
+                  dim3(64 * WM * WN, 1, 1), stream, a, rows, cols);
 }
 
 template <bool GATED, int R, int NT, int D>
@@ -843,14 +721,14 @@ int run_plan8(hipStream_t stream, const Plan8& p, const ProductArgs& a)
             }
         e = p.rows == 2 ? run_narrow8<GATED, 2>(stream, p, a) : run_narrow8<GATED, 4>(stream, p, a);
         break;
-    case 1: e = run_tiles8<GATED, 8, 4, 2, 4, 2>(stream, p, a); break;
-    case 2: e = run_tiles8<GATED, 4, 4, 2, 4, 3>(stream, p, a); break;
-    case 3: e = run_tiles8<GATED, 4, 4, 4, 2, 3>(stream, p, a); break;
-    case 4: e = run_tiles8<GATED, 4, 2, 2, 4, 4>(stream, p, a); break;
-    case 5: e = run_tiles8<GATED, 4, 4, 2, 2, 2>(stream, p, a); break;
-    default: e = run_tiles8<GATED, 4, 2, 2, 2, 3>(stream, p, a); break;
+    case 1: e = run_tiles8<GATED, 8, 4, 2, 4, 2>(stream, a, 1); break;
+    case 2: e = run_tiles8<GATED, 4, 4, 2, 4, 3>(stream, a, 1); break;
+    case 3: e = run_tiles8<GATED, 4, 4, 4, 2, 3>(stream, a, 1); break;
+    case 4: e = run_tiles8<GATED, 4, 2, 2, 4, 4>(stream, a, 1); break;
+    case 5: e = run_tiles8<GATED, 4, 4, 2, 2, 2>(stream, a, 2); break;
+    default: e = run_tiles8<GATED, 4, 2, 2, 2, 3>(stream, a, 2); break;
     }
-    if (e != 0 || p.kind > 0 || a.shares == 1)
+    if (e != 0 || a.shares == 1)
         return e;
     const int64_t waves = up8(a.N, 16) * layout8(a.M, a.K, GATED).groups * 2;
     return launch(w8_join<GATED>, dim3((unsigned)up8(waves, 4), 1, 1), dim3(256, 1, 1), stream, a);
@@ -923,7 +801,7 @@ int run_product(hipStream_t stream, const void* packed, const W8_Codes& x, void*
     }
     a.y = static_cast<uint16_t*>(Y), a.bias = static_cast<const uint16_t*>(bias), a.up_bias = static_cast<const uint16_t*>(up_bias);
     a.M = M, a.N = N, a.K = K, a.act = activation, a.bf16 = dtype == DECODE_BF16;
-    a.shares = p.shares, a.per = p.per, a.full = p.full, a.part = s.part > 0 ? static_cast<int*>(workspace) : nullptr;
+    a.shares = p.shares, a.per = p.per, a.part = p.shares > 1 ? static_cast<int*>(workspace) : nullptr;
     return gated ? run_plan8<true>(stream, p, a) : run_plan8<false>(stream, p, a);
 }
 
@@ -933,14 +811,13 @@ int run_product(hipStream_t stream, const void* packed, const W8_Codes& x, void*
 using namespace decode;
 
 #ifdef SPMM_KEEP_VARIANTS
-// Every later call runs as the plan says (see Plan8): kind 0 with row and column tiles and shares of K (0: as the library chooses), or tiles
-// of a kind, with `shares` workgroups (0: tiles whole).
+// Every later call runs as the plan says (see Plan8); shares 0: as the library chooses.
 extern "C" int W8_Debug_SetPlan(int kind, int rows, int cols, int shares)
 {
     if (kind < 0 || kind > kShapes || shares < 0 ||
         (kind == 0 && shares > 0 && ((rows != 1 && rows != 2 && rows != 4) || cols < 1 || cols > 4)))
         return 1;
-    g_plan8 = kind > 0 ? Plan8{kind, 0, 0, 0, 0, shares, 0} : Plan8{0, rows, cols, shares, 0, 0, 0};
+    g_plan8 = Plan8{kind, rows, cols, shares, 0};
     return 0;
 }
 #endif
