@@ -83,7 +83,22 @@ struct ProductArgs {
     int*           part; // sums of the shares of K (part_of); null where K is not split
     int            M, N, K, act, bf16;
     int            shares, per; // shares of K, blocks of 128 columns in each but the last
+    int            row_tiles, column_tiles; // of w8_tiles
 };
+
+// The kernel's arguments, read from memory once more where a tile begins and ends: kept in registers from the kernel's start they would
+// leave too few scalars for its loop.
+__device__ __forceinline__ ProductArgs late_args8()
+{
+    typedef const __attribute__((address_space(4))) ProductArgs* Pointer;
+    Pointer p = (Pointer)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    ProductArgs a{};
+    a.packed = p->packed, a.x = p->x, a.x_scales = p->x_scales, a.x_stride = p->x_stride, a.y = p->y, a.bias = p->bias;
+    a.up_bias = p->up_bias, a.part = p->part, a.M = p->M, a.N = p->N, a.K = p->K, a.act = p->act, a.bf16 = p->bf16, a.shares = p->shares;
+    a.per = p->per, a.row_tiles = p->row_tiles, a.column_tiles = p->column_tiles;
+    return a;
+}
 
 // ReLU, GELU (tanh form) or SiLU of W sums.  The last two are y / (1 + exp(-z)), with z = 2 sqrt(2/pi) (y + 0.044715 y^3), since
 // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), or z = y; far from 0 they end at 0 and y.  The reciprocal's last bit is far below 16 bits.
@@ -327,16 +342,21 @@ __device__ __forceinline__ void each(F f)
 }
 
 // A wave's 1 KB of 16 bytes a lane goes from global memory straight into LDS.  In assembly, since the compiler would wait for it
-// ahead of the next read of LDS; the kernel waits for it itself, before the barrier that hands the tile over.
+// ahead of the next read of LDS; the kernel waits for it itself, before the barrier that hands the tile over.  OFFSET counts for both
+// addresses.
+template <int OFFSET>
 __device__ __forceinline__ void to_lds(unsigned lds, const void* base, unsigned offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds), "v"(offset), "s"(base), "n"(OFFSET)
+                 : "memory");
 }
 
 // The same of memory that is read once: the caches are kept for what is read again (36864x9216 with 64 columns 92 -> 87 us).
+template <int OFFSET>
 __device__ __forceinline__ void to_lds_once(unsigned lds, const void* base, unsigned offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3 nt" ::"s"(lds), "v"(offset), "s"(base), "n"(OFFSET)
+                 : "memory");
 }
 
 // The same of one word, or of 16 bits in a word, a lane.
@@ -352,15 +372,15 @@ __device__ __forceinline__ void short_to_lds(unsigned lds, const void* address)
 
 // Workgroups are dealt to the eight dies in turn, each with an L2 of its own: consecutive numbers on one die, and there a band of
 // kBand row tiles by as many column tiles as run at once; shares of K one after another.
-__device__ __forceinline__ void place8(int id, int row_tiles, int column_tiles, int shares, int& row, int& column, int& share)
+__device__ __forceinline__ void place8(const ProductArgs& a, int id, int& row, int& column, int& share)
 {
     constexpr int kBand = 8;
-    const int     one = row_tiles * column_tiles, total = one * shares, xcd = id % 8, rest = total % 8;
-    int           at = xcd * (total / 8) + min(xcd, rest) + id / 8;
+    const int     one = a.row_tiles * a.column_tiles, total = one * a.shares, die = id % 8;
+    int           at = die * (total / 8) + min(die, total % 8) + id / 8;
     share            = __builtin_amdgcn_readfirstlane(at / one);
     at -= share * one;
-    const int     band = at / (kBand * column_tiles), first = band * kBand, height = min(kBand, row_tiles - first);
-    const int     in   = at - first * column_tiles;
+    const int band = at / (kBand * a.column_tiles), first = band * kBand, height = min(kBand, a.row_tiles - first);
+    const int in   = at - first * a.column_tiles;
     // divisions are done by vector instructions: back to scalars, which the addresses are made of
     row = __builtin_amdgcn_readfirstlane(first + in % height), column = __builtin_amdgcn_readfirstlane(in / height);
 }
@@ -373,13 +393,15 @@ __device__ __forceinline__ void place8(int id, int row_tiles, int column_tiles, 
 // A workgroup stays on its CU and takes every gridDim-th tile: the blocks of all its tiles are one stream, so that the next tile is
 // loaded while the results of the last are written, and a tile costs its products alone.
 template <bool GATED, int MT, int NT, int WM, int WN, int S>
-__global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs a, int row_tiles, int column_tiles)
+__global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs args)
 {
     constexpr int kWaves = WM * WN, kRows = WM * MT, kCols = WN * NT, kStage = (kRows + kCols) * 2048; // tiles of W, of X
     constexpr int kLoads = 2 * (kRows + kCols) / kWaves;
     constexpr int kM = kRows * 16, kN = kCols * 16; // packed rows, rows of X
     constexpr int kEnds = S + 2; // loads are at most S + 1 tiles ahead of the products
-    static_assert(2 * (kRows + kCols) % kWaves == 0 && MT % 4 == 0 && kM % 128 == 0 && kN % 64 == 0 && S >= 2);
+    constexpr int kWLoads = 2 * kRows / kWaves, kXLoads = 2 * kCols / kWaves; // of a wave, of W and of X
+    static_assert(2 * kRows % kWaves == 0 && 2 * kCols % kWaves == 0 && (kWLoads == 2 || kWLoads == 4));
+    static_assert(MT % 4 == 0 && kM % 128 == 0 && kN % 64 == 0 && S >= 2);
     struct Ends { // of a tile: scales and biases of its rows (of the gate, then of up), scales of its rows of X
         float    sw[kM];
         unsigned b[kM];
@@ -387,38 +409,41 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs a, int r
     };
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S][kStage];
     __shared__ __attribute__((aligned(16))) Ends      ends[kEnds];
-    const Layout8 l    = layout8(a.M, a.K, GATED);
     const int     lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int     q = lane >> 4, c = lane & 15, wm = wave / WN, wn = wave % WN;
-    const int     tiles = row_tiles * column_tiles * a.shares;
 
-    // What a wave brings of every block: KBs wave, wave + kWaves, ... of W's, as they are packed, then of X's.
-    const uint8_t* from[kLoads];
-    unsigned       off[kLoads];
+    // What a wave brings of every block: kWLoads KBs of W, as they are packed, half a group's or a quarter's, then kXLoads of X.
+    const uint8_t* w_now; // W's block of the next load, from the tile's first group on
+    const int8_t*  x_at[kXLoads];
+    unsigned       w_off, x_off[kXLoads];
     auto address = [](const void* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p; };
     const unsigned lds0 = address(lds), ends0 = address(ends);
-    const int      chunk = 16 * ((lane & 7) ^ (lane >> 3)), last = (a.K - 1) / 16 * 16;
-    // Tile and block of the next load, the end of its blocks, and how many tiles it has seen; tile and number of the next products, and
-    // how many blocks of it are left.
-    int ahead_tile = blockIdx.x, ahead_block, ahead_end, ahead_turn = 0, tile = blockIdx.x, left, turn = 0;
-    // Turns the loads to a tile, the `turn`-th, and brings its ends.
-    auto enter = [&](int tile, int turn) {
-        int row, column, share;
-        place8(tile, row_tiles, column_tiles, a.shares, row, column, share);
-        const int tile0 = row * kRows, n0 = column * kN;
+    const int      chunk = 16 * ((lane & 7) ^ (lane >> 3)), last = (args.K - 1) / 16 * 16;
+    const int64_t block_bytes = (int64_t)layout8(args.M, args.K, GATED).groups * kGroup8;
+    const bool    once        = args.column_tiles == 1;
+    const int tiles = args.row_tiles * args.column_tiles * args.shares, apart = gridDim.x;
+    // Tile of the loads, their next block and the end of the tile's, tiles seen; tile of the products, blocks of it left, tiles seen.
+    int ahead = blockIdx.x - apart, ahead_block, ahead_end, ahead_turn = 0, now = blockIdx.x, left, turn = 0;
+    // Turns the loads to the next tile, if there is one, and brings its ends.
+    auto enter = [&] {
+        if (ahead + apart >= tiles)
+            return;
+        ahead += apart;
+        const ProductArgs a = late_args8();
+        const Layout8     l = layout8(a.M, a.K, GATED);
+        int               row, column, share;
+        place8(a, ahead, row, column, share);
         ahead_block = share * a.per, ahead_end = min(ahead_block + a.per, l.steps / 2);
-        for (int i = 0; i < kLoads; ++i) { // groups and rows behind the last are the last again: computed, not stored
-            const int j = wave + i * kWaves;
-            if (j < 2 * kRows) {
-                from[i] = a.packed + (int64_t)min(tile0 / 4 + j / 8, l.groups - 1) * kGroup8 + j % 8 * 1024;
-                off[i]  = lane * 16;
-            } else {
-                const int n = min(n0 + 8 * (j - 2 * kRows), a.N - 1);
-                from[i]     = reinterpret_cast<const uint8_t*>(a.x) + (int64_t)n * a.x_stride;
-                off[i]      = min(lane >> 3, a.N - 1 - n) * (unsigned)a.x_stride;
-            }
+        const int tile0 = row * kRows, n0 = column * kN;
+        w_now = a.packed + (int64_t)ahead_block * block_bytes + (int64_t)(tile0 / 4) * kGroup8;
+        // groups and rows behind the last are the last again: computed, not stored
+        w_off = min(wave * kWLoads / 8, l.groups - 1 - tile0 / 4) * kGroup8 + wave * kWLoads % 8 * 1024 + lane * 16;
+        for (int i = 0; i < kXLoads; ++i) {
+            const int n = min(n0 + 8 * (wave * kXLoads + i), a.N - 1);
+            x_at[i]     = a.x + (int64_t)n * a.x_stride;
+            x_off[i]    = min(lane >> 3, a.N - 1 - n) * (unsigned)a.x_stride;
         }
-        const unsigned to = ends0 + turn % kEnds * (unsigned)sizeof(Ends);
+        const unsigned to = ends0 + ahead_turn++ % kEnds * (unsigned)sizeof(Ends);
         const float*   sw = reinterpret_cast<const float*>(a.packed + l.scales);
         for (int i = wave; i < kM / 64; i += kWaves) { // 64 rows, all of the gate or all of up
             const bool up = GATED && i >= kM / 128;
@@ -432,18 +457,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs a, int r
         for (int i = kWaves - 1 - wave; i < kN / 64; i += kWaves)
             word_to_lds(to + kM * 8 + i * 256, a.x_scales + min(n0 + i * 64 + lane, a.N - 1));
     };
-    const int64_t block_bytes = (int64_t)l.groups * kGroup8;
     // The i-th of a wave's loads of a block.  Behind the last 16 columns of X the weights are 0: what is there does not matter.
-    auto stage = [&](int i, int block, int place) {
-        const int      j  = wave + i * kWaves;
-        const unsigned to = lds0 + place * kStage + j * 1024;
-        if ((i + 1) * kWaves <= 2 * kRows || j < 2 * kRows) {
-            if (column_tiles == 1)
-                to_lds_once(to, from[i] + block * block_bytes, off[i]);
+    auto stage = [&](auto i, int place) {
+        const unsigned to = lds0 + place * kStage;
+        if constexpr (i < kWLoads) {
+            if (kCols <= 4 && once)
+                to_lds_once<i * 1024>(to + wave * kWLoads * 1024, w_now, w_off);
             else
-                to_lds(to, from[i] + block * block_bytes, off[i]);
-        } else
-            to_lds(to, from[i], off[i] + min(block * 128 + chunk, last));
+                to_lds<i * 1024>(to + wave * kWLoads * 1024, w_now, w_off);
+        } else {
+            constexpr int x = i - kWLoads;
+            to_lds<0>(to + (2 * kRows + wave * kXLoads + x) * 1024, x_at[x], x_off[x] + min(ahead_block * 128 + chunk, last));
+        }
     };
     struct Operands {
         intx4 w[MT], x[NT];
@@ -467,93 +492,86 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs a, int r
     // ahead of its products until the memory pipe has taken them.
     constexpr int kParts = kProducts / 4;
     auto multiply = [&](const Operands& o, auto between) {
-#pragma unroll
-        for (int part = 0; part < kParts; ++part) {
+        each<kParts>([&](auto part) {
 #pragma unroll
             for (int f = 4 * part; f < 4 * part + 4; ++f)
                 sum[f % MT][f / MT] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[f % MT], o.x[f / MT], sum[f % MT][f / MT], 0, 0, 0);
             between(part);
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
     };
-    // Items `part` of `parts` of n, as a range.
-#define W8_SHARE(i, n, part, parts) for (int i = (n) * (part) / (parts); i < (n) * ((part) + 1) / (parts); ++i)
-    auto advance = [&] {
-        if (++ahead_block >= ahead_end) {
-            ahead_tile += gridDim.x, ++ahead_turn;
-            if (ahead_tile < tiles)
-                enter(ahead_tile, ahead_turn);
-        }
+    // f(i) for items `part` of `parts` of N.
+    auto share = [](auto n, auto part, auto parts, auto f) {
+        each<n * (part + 1) / parts - n * part / parts>([&](auto i) { f(std::integral_constant<int, n * part / parts + i>()); });
     };
-    auto begin = [&] { // blocks of the tile that the products come to
+    constexpr std::integral_constant<int, kReads> reads;
+    constexpr std::integral_constant<int, kLoads> loads;
+    constexpr std::integral_constant<int, kParts> parts;
+    auto advance = [&] { // behind the last block there is that block again, which nobody reads: loads are made, and counted, all the same
+        if (ahead_block + 1 < ahead_end)
+            ++ahead_block, w_now += block_bytes;
+        else
+            enter();
+    };
+    auto begin = [&](const ProductArgs& a) { // blocks of the products' tile
         int row, column, share;
-        place8(tile, row_tiles, column_tiles, a.shares, row, column, share);
-        left = min(a.per, l.steps / 2 - share * a.per);
+        place8(a, now, row, column, share);
+        left = min(a.per, (a.K + 127) / 128 - share * a.per);
     };
-    enter(tile, 0);
-    begin();
+    enter();
+    begin(args);
     for (int s = 0; s < S; ++s) {
-        if (ahead_tile < tiles) {
-            for (int i = 0; i < kLoads; ++i)
-                stage(i, ahead_block, s);
-            advance();
-        }
+        each<kLoads>([&](auto i) { stage(i, s); });
+        advance();
     }
-    if (ahead_tile < tiles)
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * kLoads) : "memory");
-    else
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * kLoads) : "memory");
     Operands first, second;
     for (int i = 0; i < kReads; ++i)
         fetch(first, i, 0, 0);
     clear();
-    constexpr int kEarly  = kParts > 2 ? kParts * 3 / 4 : kParts; // parts under which operands are read: the rest covers their latency
+    constexpr int kEarly = kParts > 2 ? kParts * 3 / 4 : kParts; // parts under which operands are read: the rest covers their latency
+    constexpr std::integral_constant<int, kEarly> early;
     constexpr int kStores = MT / 4 * NT * (GATED ? 1 : 2);  // of a wave for a tile that is full
     constexpr int kAway   = (S - 2) * kLoads;               // a wave's loads of the blocks behind the next
     static_assert(kAway + kStores < 64);
     int place = 0, relaxed = 0; // relaxed: barriers ahead of which the last results' stores may still be under way
     for (;;) {
-const bool more = ahead_tile < tiles;
-        multiply(first, [&](int part) {
-            if (part < kEarly)
-                W8_SHARE(j, kReads, part, kEarly)
-                    fetch(second, j, place, 1);
+        multiply(first, [&](auto part) {
+            if constexpr (part < kEarly)
+                share(reads, part, early, [&](auto i) { fetch(second, i, place, 1); });
         });
         // The next block has come.  Loads and stores are counted in their order: behind it are kAway loads, and stores.
-        if (!more)
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        else if (relaxed > 0)
+        if (relaxed > 0)
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kAway + kStores) : "memory");
         else
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kAway) : "memory");
         --relaxed;
         const int next = place + 1 == S ? 0 : place + 1;
-        multiply(second, [&](int part) {
-            if (part < kEarly)
-                W8_SHARE(j, kReads, part, kEarly) // behind the last block stale bytes, which nothing takes
-                    fetch(first, j, next, 0);
-            if (more)
-                W8_SHARE(j, kLoads, part, kParts)
-                    stage(j, ahead_block, place);
+        multiply(second, [&](auto part) {
+            if constexpr (part < kEarly) // behind the last block bytes that nothing takes
+                share(reads, part, early, [&](auto i) { fetch(first, i, next, 0); });
+            share(loads, part, parts, [&](auto i) { stage(i, place); });
         });
-        if (more)
-            advance();
+        advance();
         place = next;
         --left;
         if (left == 0) {
-            int row, column, share;
-            place8(tile, row_tiles, column_tiles, a.shares, row, column, share);
+            const ProductArgs a = late_args8();
+            const Layout8     l = layout8(a.M, a.K, GATED);
+            int               row, column, share;
+            place8(a, now, row, column, share);
             const Ends& e = ends[turn % kEnds];
             if (a.part == nullptr) {
                 each<MT / 4>([&](auto g) {
                     const int group = wm * (MT / 4) + g;
                     each<GATED ? 1 : 2>([&](auto h) {
-                        const int             j = GATED ? group * 32 + 8 * q : group * 64 + 16 * q + 8 * h;
-                        const Tail8<GATED, 8> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
+                        const int j = GATED ? group * 32 + 8 * q : group * 64 + 16 * q + 8 * h;
                         each<NT>([&](auto u) {
                             const int n = column * kN + (wn * NT + u) * 16 + c;
                             if (n >= a.N)
                                 return;
+                            asm volatile("" ::: "memory"); // scales and biases once more, rather than in registers there are not enough of
+                            const Tail8<GATED, 8> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
                             int v[16];
                             for (int i = 0; i < 16; ++i)
                                 v[i] = sum[g * 4 + i / 4][u][i % 4];
@@ -567,21 +585,21 @@ const bool more = ahead_tile < tiles;
                 const int columns = (a.N + 15) / 16;
                 each<NT>([&](auto u) {
                     const int at = column * kCols + wn * NT + u;
-                    each<MT>([&](auto t) {
-                        const int group = row * (kM / 64) + wm * (MT / 4) + t / 4;
+                    each<MT / 4>([&](auto g) {
+                        const int group = row * (kM / 64) + wm * (MT / 4) + g;
                         if (at < columns && group < l.groups)
-                            part_of(a, l.groups, share, columns, group, at)[t % 4 * 64 + lane] = sum[t][u];
+                            each<4>([&](auto t) { part_of(a, l.groups, share, columns, group, at)[t * 64 + lane] = sum[g * 4 + t][u]; });
                     });
                 });
             }
-            tile += gridDim.x, ++turn;
-            if (tile >= tiles)
-                return;
-            begin();
+            now += apart, ++turn;
+            if (now >= tiles)
+                break;
+            begin(a);
             clear();
         }
     }
-#undef W8_SHARE
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the LDS that loads are on their way to is the workgroup's until they are there
 }
 
 // How a call runs.
@@ -597,8 +615,8 @@ struct Tiles8 {
     int    rows, cols, resident;
     double tile, block, both;
 };
-constexpr Tiles8 kTiles[] = {{16, 16, 1, 5.3, 1.41, 0},    {8, 16, 1, 4.3, 0.85, 0},     {16, 8, 1, 4.2, 0.86, 0},
-                             {8, 8, 1, 3.2, 0.50, 0},      {8, 8, 2, 3.2, 0.70, 0.99},   {8, 4, 2, 2.6, 0.41, 0.68}};
+constexpr Tiles8 kTiles[] = {{16, 16, 1, 2.6, 1.27, 0},    {8, 16, 1, 2.3, 0.73, 0},     {16, 8, 1, 2.2, 0.69, 0},
+                             {8, 8, 1, 1.6, 0.43, 0},      {8, 8, 2, 1.3, 0.57, 0.81},   {8, 4, 2, 1.2, 0.36, 0.58}};
 constexpr int kShapes = sizeof kTiles / sizeof *kTiles;
 
 #ifdef SPMM_KEEP_VARIANTS
@@ -613,16 +631,18 @@ void share8(Plan8& p, int64_t blocks, int64_t shares)
     p.shares = (int)up8(blocks, p.per);
 }
 
-// The cheapest by a model of a call's time in microseconds, fitted to 1328 calls of 51 shapes, from 256x256 to 36864x9216 and from 1 to 6000
-// columns, on which it is 1.5 % off the best on average and 17 % at worst.  Workgroups are counted in rounds, one (or two) for every CU;
-// W's bytes are added to them; K in shares costs a launch and the shares' bytes.  Examples, us: 5120x5120, N = 37 10.3 narrow
-// with two row and three column tiles, 12.7 in tiles of 128 x 64; 20480x5120, N = 64 25.7 in tiles of 128 x 64, 30.4
-// narrow; 9216x36864, N = 193 97 in tiles of 256 x 256 and seven shares of K, 113 in tiles of 128 x 256 and three, 410 in one.
+// The cheapest by a model of a call's time in microseconds, fitted to 2815 calls of 97 shapes, from 256x256 to 36864x9216 and from 1 to 6000
+// columns, on which it is 2 % off the best on average and 32 % at worst (rows of an odd length with few columns of K).  Workgroups are
+// counted in rounds, one (or two) for every CU; W's and Y's bytes are added to them; K in shares costs a launch and the shares'
+// bytes.  Examples, us: 5120x5120, N = 37 10.2 narrow with two row and three column tiles, 12.9 in tiles of 128 x 64;
+// 20480x5120, N = 64 25.6 in tiles of 128 x 64, 30.3 narrow; 9216x36864, N = 193 97 in tiles of 256 x 256 and seven shares of K,
+// 113 in tiles of 128 x 256 and three, 410 in one.
 Plan8 plan8(int M, int N, int K, bool gated)
 {
     const Layout8 l      = layout8(M, K, gated);
     const int64_t blocks = l.steps / 2, tiles = (int64_t)l.groups * 4;
-    const double  w_mb = (double)tiles * (double)blocks * 2048e-6, part_mb = (double)tiles * (double)up8(N, 16) * 2048e-6;
+    const double  w_mb = (double)tiles * (double)blocks * 2048e-6, part_mb = (double)tiles * (double)up8(N, 16) * 2048e-6,
+                  y_mb = (double)M * N * 2e-6;
     Plan8         p{}, best{};
     double        least = 1e300;
 #ifdef SPMM_KEEP_VARIANTS // the tests' build: every kernel at small sizes
@@ -634,7 +654,7 @@ Plan8 plan8(int M, int N, int K, bool gated)
 #endif
     auto consider = [&](double us) {
         if (p.shares > 1)
-            us += 3.0 + p.shares * part_mb / 8.4;
+            us += 3.2 + p.shares * part_mb / 7.6;
         if (us < least)
             least = us, best = p;
     };
@@ -646,8 +666,8 @@ Plan8 plan8(int M, int N, int K, bool gated)
                     if (s > 1 && (s > blocks || groups * s > 2048))
                         break;
                     share8(p, blocks, s);
-                    consider(2.8 + w_mb * (double)columns / 12.7 +
-                             (double)(up8(groups * p.shares, 256) * up8(p.per, 8)) * (0.20 * p.rows + 0.25 * p.cols));
+                    consider(2.8 + w_mb * (double)columns / 12.6 +
+                             (double)(up8(groups * p.shares, 256) * up8(p.per, 8)) * (0.19 * p.rows + 0.24 * p.cols));
                 }
             }
     for (p.kind = 1; p.kind <= kShapes; ++p.kind) {
@@ -659,7 +679,7 @@ Plan8 plan8(int M, int N, int K, bool gated)
                 continue;
             share8(p, blocks, fill > 0 ? std::min<int64_t>(64, 256 * fill / groups) : 1);
             const int64_t slots = 256 * k.resident, full = groups * p.shares / slots, rest = groups * p.shares % slots;
-            double        us = 2.4 + w_mb / 25;
+            double        us = 4.7 + w_mb / 16 + y_mb / 3.3;
             us += (double)full * (k.tile + p.per * (k.resident > 1 ? k.both : k.block));
             if (rest > 0)
                 us += k.tile + p.per * (rest > 256 ? k.both : k.block);
@@ -675,15 +695,14 @@ size_t part_bytes8(int M, int N, int K, bool gated, const Plan8& p)
 }
 
 template <bool GATED, int MT, int NT, int WM, int WN, int S>
-int run_tiles8(hipStream_t stream, const ProductArgs& a, int resident)
+int run_tiles8(hipStream_t stream, ProductArgs a, int resident)
 {
-    const Layout8 l    = layout8(a.M, a.K, GATED);
-    const int     rows = (int)up8(l.groups * 4, MT * WM), cols = (int)up8(a.N, NT * WN * 16);
-    const int64_t tiles = (int64_t)rows * cols * a.shares;
-    if (tiles > 0x7fffffff)
+    a.row_tiles         = (int)up8(layout8(a.M, a.K, GATED).groups * 4, MT * WM), a.column_tiles = (int)up8(a.N, NT * WN * 16);
+    const int64_t tiles = (int64_t)a.row_tiles * a.column_tiles * a.shares;
+    if (tiles > 0x3fffffff)
         return refuse("%lld tiles of outputs", (long long)tiles);
     return launch(w8_tiles<GATED, MT, NT, WM, WN, S>, dim3((unsigned)std::min<int64_t>(tiles, 256 * resident), 1, 1),
-                  dim3(64 * WM * WN, 1, 1), stream, a, rows, cols);
+                  dim3(64 * WM * WN, 1, 1), stream, a);
 }
 
 template <bool GATED, int R, int NT, int D>
