@@ -47,25 +47,29 @@ struct PackArgs {
     uint8_t*      packed;
 };
 
-// One wave lays out one block of 16 rows x 64 columns.
-__global__ __launch_bounds__(64) void w8_pack(PackArgs a)
+// A workgroup lays out the 128 columns of a group, a wave a row tile's.
+__global__ __launch_bounds__(256) void w8_pack(PackArgs a)
 {
     const bool    gated = a.up != nullptr;
     const Layout8 l     = layout8(a.M, a.K, gated);
-    const int     lane = threadIdx.x, r = lane & 15, q = lane >> 4, tile = blockIdx.x & 3;
-    const int64_t block = blockIdx.x;
-    const int     group = (int)(block / 4 % l.groups), step = (int)(block / 4 / l.groups);
+    const int     lane = threadIdx.x % kWave, tile = threadIdx.x / kWave, r = lane & 15, q = lane >> 4;
+    const int     group = blockIdx.x % l.groups, block = blockIdx.x / l.groups;
     const bool    second = gated && tile >= 2;
     const int     row = gated ? group * 32 + (r >> 2) * 8 + (tile & 1) * 4 + (r & 3) : group * 64 + (r >> 2) * 16 + tile * 4 + (r & 3);
     const int8_t* src = second ? a.up + row * a.up_stride : a.w + row * a.w_stride;
-    uintx4        out = 0;
-    for (int b = 0; b < 16; ++b) {
-        const int k = step * 64 + q * 16 + b;
-        if (row < a.M && k < a.K)
-            out[b / 4] |= (unsigned)(uint8_t)src[k] << (8 * (b % 4));
+    uintx4*       to  = reinterpret_cast<uintx4*>(a.packed + (int64_t)blockIdx.x * kGroup8) + tile * 64 + lane;
+    for (int step = 0; step < 2; ++step) {
+        const int k   = block * 128 + step * 64 + q * 16;
+        uintx4    out = 0;
+        if (row < a.M && k + 16 <= a.K)
+            out = *reinterpret_cast<const loose_bytes16*>(src + k);
+        else if (row < a.M)
+            for (int b = 0; b < 16; ++b)
+                if (k + b < a.K)
+                    out[b / 4] |= (unsigned)(uint8_t)src[k + b] << (8 * (b % 4));
+        to[step * 256] = out;
     }
-    reinterpret_cast<uintx4*>(a.packed + ((int64_t)(step / 2) * l.groups + group) * kGroup8)[(step % 2 * 4 + tile) * 64 + lane] = out;
-    if (step == 0 && tile == 0) { // 64 scales: of the group's rows, or of 32 rows of the gate and of up
+    if (block == 0 && tile == 0) { // 64 scales: of the group's rows, or of 32 rows of the gate and of up
         const int  per = gated ? 32 : 64, m = group * per + lane % per;
         const bool u = gated && lane >= 32;
         reinterpret_cast<float*>(a.packed + l.scales)[(u ? (int64_t)l.groups * 32 : 0) + m] =
@@ -615,8 +619,8 @@ struct Tiles8 {
     int    rows, cols, resident;
     double tile, block, both;
 };
-constexpr Tiles8 kTiles[] = {{16, 16, 1, 2.6, 1.27, 0},    {8, 16, 1, 2.3, 0.73, 0},     {16, 8, 1, 2.2, 0.69, 0},
-                             {8, 8, 1, 1.6, 0.43, 0},      {8, 8, 2, 1.3, 0.57, 0.81},   {8, 4, 2, 1.2, 0.36, 0.58}};
+constexpr Tiles8 kTiles[] = {{16, 16, 1, 2.7, 1.34, 0},    {8, 16, 1, 2.4, 0.78, 0},     {16, 8, 1, 2.3, 0.73, 0},
+                             {8, 8, 1, 1.8, 0.46, 0},      {8, 8, 2, 1.5, 0.59, 0.84},   {8, 4, 2, 1.5, 0.365, 0.58}};
 constexpr int kShapes = sizeof kTiles / sizeof *kTiles;
 
 #ifdef SPMM_KEEP_VARIANTS
@@ -631,7 +635,7 @@ void share8(Plan8& p, int64_t blocks, int64_t shares)
     p.shares = (int)up8(blocks, p.per);
 }
 
-// The cheapest by a model of a call's time in microseconds, fitted to 2815 calls of 97 shapes, from 256x256 to 36864x9216 and from 1 to 6000
+// The cheapest by a model of a call's time in microseconds, fitted to 2912 calls of 110 shapes, from 256x256 to 36864x9216 and from 1 to 6000
 // columns, on which it is 2 % off the best on average and 32 % at worst (rows of an odd length with few columns of K).  Workgroups are
 // counted in rounds, one (or two) for every CU; W's and Y's bytes are added to them; K in shares costs a launch and the shares'
 // bytes.  Examples, us: 5120x5120, N = 37 10.2 narrow with two row and three column tiles, 12.9 in tiles of 128 x 64;
@@ -654,7 +658,7 @@ Plan8 plan8(int M, int N, int K, bool gated)
 #endif
     auto consider = [&](double us) {
         if (p.shares > 1)
-            us += 3.2 + p.shares * part_mb / 7.6;
+            us += 3.2 + p.shares * part_mb / 7.8;
         if (us < least)
             least = us, best = p;
     };
@@ -679,7 +683,7 @@ Plan8 plan8(int M, int N, int K, bool gated)
                 continue;
             share8(p, blocks, fill > 0 ? std::min<int64_t>(64, 256 * fill / groups) : 1);
             const int64_t slots = 256 * k.resident, full = groups * p.shares / slots, rest = groups * p.shares % slots;
-            double        us = 4.7 + w_mb / 16 + y_mb / 3.3;
+            double        us = 4.3 + w_mb / 17.3 + y_mb / 3.4;
             us += (double)full * (k.tile + p.per * (k.resident > 1 ? k.both : k.block));
             if (rest > 0)
                 us += k.tile + p.per * (rest > 256 ? k.both : k.block);
@@ -861,10 +865,7 @@ extern "C" int W8_Pack(hipStream_t stream, W8_Weights w, const W8_Weights* up, i
         a.up = up->codes, a.up_scales = up->scales, a.up_stride = up->w_stride;
     a.M = M, a.K = K, a.packed = static_cast<uint8_t*>(packed);
     const Layout8 l      = layout8(M, K, up != nullptr);
-    const int64_t blocks = (int64_t)l.groups * l.steps * 4;
-    if (blocks > 0x7fffffff)
-        return refuse("weights of %d rows and %d columns: more than 2^31 blocks", M, K);
-    return launch(w8_pack, dim3((unsigned)blocks, 1, 1), dim3(64, 1, 1), stream, a);
+    return launch(w8_pack, dim3((unsigned)(l.groups * (l.steps / 2)), 1, 1), dim3(256, 1, 1), stream, a);
 }
 
 extern "C" size_t W8_WorkspaceBytes(int M, int N, int K, int gated, int x16)
