@@ -7,6 +7,8 @@
 // Bound by memory: 2 bytes for x, 2 for the residual and 2 for h, 2 or 1 for the result of every element.
 #include "w8_common.hiph"
 
+#include <algorithm>
+
 namespace decode {
 namespace {
 
@@ -212,8 +214,22 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
 template <bool BF16, bool NORM, bool QUANT, int WAVES, int V>
 int start(hipStream_t stream, const NormArgs& a)
 {
-    const unsigned rows = WAVES == 1 ? (unsigned)(((int64_t)a.N + 3) / 4) : (unsigned)a.N;
-    return launch(rms_norm<BF16, NORM, QUANT, WAVES, V>, dim3(rows, 1, 1), dim3(WAVES == 1 ? 256 : WAVES * kWave, 1, 1), stream, a);
+    constexpr int kMost = 1 << 21; // rows of a launch: its threads are counted in 32 bits
+    NormArgs      b     = a;
+    for (int64_t first = 0; first < a.N; first += kMost) {
+        b.N = (int)std::min<int64_t>(kMost, a.N - first);
+        const int e = launch(rms_norm<BF16, NORM, QUANT, WAVES, V>, dim3((unsigned)(WAVES == 1 ? (b.N + 3) / 4 : b.N), 1, 1),
+                             dim3(WAVES == 1 ? 256 : WAVES * kWave, 1, 1), stream, b);
+        if (e != 0)
+            return e;
+        b.x += kMost * b.x_stride;
+        b.residual = b.residual != nullptr ? b.residual + kMost * b.r_stride : nullptr;
+        b.h        = b.h != nullptr ? b.h + kMost * b.h_stride : nullptr;
+        b.y        = b.y != nullptr ? b.y + kMost * b.y_stride : nullptr;
+        b.codes    = b.codes != nullptr ? b.codes + kMost * b.c_stride : nullptr;
+        b.scales   = b.scales != nullptr ? b.scales + kMost : nullptr;
+    }
+    return 0;
 }
 
 // Waves to a row and vectors to a lane.  Many rows: few waves, as many vectors as leave few lanes without one, since rows in flight

@@ -352,7 +352,7 @@ template <int OFFSET>
 __device__ __forceinline__ void to_lds(unsigned lds, const void* base, unsigned offset)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(lds), "v"(offset), "s"(base), "n"(OFFSET)
-                 : "memory");
+                 : "memory", "m0");
 }
 
 // The same of memory that is read once: the caches are kept for what is read again (36864x9216 with 64 columns 92 -> 87 us).
@@ -360,18 +360,18 @@ template <int OFFSET>
 __device__ __forceinline__ void to_lds_once(unsigned lds, const void* base, unsigned offset)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3 nt" ::"s"(lds), "v"(offset), "s"(base), "n"(OFFSET)
-                 : "memory");
+                 : "memory", "m0");
 }
 
 // The same of one word, or of 16 bits in a word, a lane.
 __device__ __forceinline__ void word_to_lds(unsigned lds, const void* address)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(address) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(address) : "memory", "m0");
 }
 
 __device__ __forceinline__ void short_to_lds(unsigned lds, const void* address)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, off" ::"s"(lds), "v"(address) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, off" ::"s"(lds), "v"(address) : "memory", "m0");
 }
 
 // Workgroups are dealt to the eight dies in turn, each with an L2 of its own: consecutive numbers on one die, and there a band of

@@ -15,7 +15,8 @@ other kernel launch.
 
 The decode operators (include/decode_api.h; spmspm_amd/decode.py is their direct form, with less host time a call) are
 registered beside it: `w4_linear` with its `W4LinearModule`, and `kv4_append`, `kv4_gather` and `kv4_attention` over the four
-arrays of a 4-bit cache, of which kv4_append is declared to mutate them.
+arrays of a 4-bit cache, of which kv4_append is declared to mutate them; and so are the 8-bit linears and the norm before them
+(include/w8_api.h, spmspm_amd/w8.py): `rms_norm`, `rms_norm_x8`, `quantize_x8`, `w8_linear` and `w8_gated` with `W8LinearModule`.
 """
 from typing import Optional
 
@@ -24,8 +25,10 @@ import torch
 
 from . import api as A
 from . import decode as D
+from . import w8 as W
 
-__all__ = ["sparse_linear", "SparseLinearModule", "w4_linear", "W4LinearModule", "kv4_append", "kv4_gather", "kv4_attention"]
+__all__ = ["sparse_linear", "SparseLinearModule", "w4_linear", "W4LinearModule", "kv4_append", "kv4_gather", "kv4_attention",
+           "rms_norm", "rms_norm_x8", "quantize_x8", "w8_linear", "w8_gated", "W8LinearModule"]
 
 
 @torch.library.custom_op("spmspm_amd::sparse_linear", mutates_args=(), device_types="cuda")
@@ -198,3 +201,93 @@ def kv4_attention(q: torch.Tensor, k_codes: torch.Tensor, k_words: torch.Tensor,
 @kv4_attention.register_fake
 def _(q, k_codes, k_words, v_codes, v_words, block_table, seq_lens, cu_tokens, scale, window, max_len):
     return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("spmspm_amd::rms_norm", mutates_args=(), device_types="cuda")
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float,
+             residual: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    """`spmspm_amd.rms_norm`: (y, h), h an empty tensor without a residual."""
+    y = W.rms_norm(x, weight, eps, residual)
+    return (y, x.new_empty(0)) if residual is None else y
+
+
+@rms_norm.register_fake
+def _(x, weight, eps, residual):
+    return x.new_empty(x.shape), x.new_empty(0 if residual is None else x.shape)
+
+
+@torch.library.custom_op("spmspm_amd::rms_norm_x8", mutates_args=(), device_types="cuda")
+def rms_norm_x8(x: torch.Tensor, weight: torch.Tensor, eps: float,
+                residual: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """`spmspm_amd.rms_norm_x8`: (codes, scales, h), h an empty tensor without a residual."""
+    out = W.rms_norm_x8(x, weight, eps, residual)
+    return (*out, x.new_empty(0)) if residual is None else out
+
+
+@rms_norm_x8.register_fake
+def _(x, weight, eps, residual):
+    codes, _, scales = W._new_codes(x, x.shape[0], x.shape[1])
+    return codes, scales, x.new_empty(0 if residual is None else x.shape)
+
+
+@torch.library.custom_op("spmspm_amd::quantize_x8", mutates_args=(), device_types="cuda")
+def quantize_x8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """`spmspm_amd.quantize_x8`."""
+    return W.quantize_x8(x)
+
+
+@quantize_x8.register_fake
+def _(x):
+    codes, _, scales = W._new_codes(x, x.shape[0], x.shape[1])
+    return codes, scales
+
+
+def _w8(packed, M, K, dtype, biases, activation, gated, x, scales):
+    layer = object.__new__(W.W8GatedLinear if gated else W.W8Linear)
+    layer._adopt(packed, int(M), K, dtype, biases, int(activation), gated)
+    return layer(x, scales)
+
+
+@torch.library.custom_op("spmspm_amd::w8_linear", mutates_args=(), device_types="cuda")
+def w8_linear(x: torch.Tensor, scales: Optional[torch.Tensor], packed: torch.Tensor, bias: Optional[torch.Tensor], M: int,
+              activation: int, dtype: torch.dtype) -> torch.Tensor:
+    """y[N][M] = act(W x + bias) in `dtype` for 8-bit weights laid out by `spmspm_amd.w8_pack`; x int8 with its scales, or 16-bit rows
+    of `dtype` without."""
+    return _w8(packed, M, x.shape[1] if x.dim() == 2 else 0, dtype, (bias,), activation, False, x, scales)
+
+
+@w8_linear.register_fake
+def _(x, scales, packed, bias, M, activation, dtype):
+    return x.new_empty((x.shape[0], M), dtype=dtype)
+
+
+@torch.library.custom_op("spmspm_amd::w8_gated", mutates_args=(), device_types="cuda")
+def w8_gated(x: torch.Tensor, scales: Optional[torch.Tensor], packed: torch.Tensor, gate_bias: Optional[torch.Tensor],
+             up_bias: Optional[torch.Tensor], M: int, activation: int, dtype: torch.dtype) -> torch.Tensor:
+    """y[N][M] = act(G x + gate_bias) * (U x + up_bias), x and weights as w8_linear's."""
+    return _w8(packed, M, x.shape[1] if x.dim() == 2 else 0, dtype, (gate_bias, up_bias), activation, True, x, scales)
+
+
+@w8_gated.register_fake
+def _(x, scales, packed, gate_bias, up_bias, M, activation, dtype):
+    return x.new_empty((x.shape[0], M), dtype=dtype)
+
+
+class W8LinearModule(torch.nn.Module):
+    """`nn.Module` around the registered operators, over the packed weights of a `spmspm_amd.W8Linear` or `W8GatedLinear` (shared)."""
+
+    def __init__(self, layer):
+        super().__init__()
+        self.M, self.K, self.activation, self.dtype, self.gated = layer.M, layer.K, layer.activation, layer.dtype, layer.gated
+        self.register_buffer("packed", layer.packed)
+        for name, b in zip(("gate_bias", "up_bias") if layer.gated else ("bias",), layer.biases):
+            self.register_buffer(name, b)
+
+    def forward(self, x, scales=None):
+        if self.gated:
+            return torch.ops.spmspm_amd.w8_gated(x, scales, self.packed, self.gate_bias, self.up_bias, self.M, self.activation,
+                                                 self.dtype)
+        return torch.ops.spmspm_amd.w8_linear(x, scales, self.packed, self.bias, self.M, self.activation, self.dtype)
+
+    def extra_repr(self):
+        return f"M={self.M}, K={self.K}, gated={self.gated}, activation={self.activation}"

@@ -91,12 +91,18 @@ def _out_rows(name, t, like, inputs, outputs=()):
 
 
 def _overlap(a, b):
-    """Whether the address ranges of two tensors meet (ranges that interlace without sharing an element count too)."""
+    """Whether two tensors of rows may share an element: their address ranges meet, and they are not slices side by side of rows of
+    one stride."""
     span = lambda t: (t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size())
     if a.numel() == 0 or b.numel() == 0:
         return False
     (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if a0 >= b1 or b0 >= a1:
+        return False
+    if a.dim() != 2 or b.dim() != 2 or a.dtype != b.dtype or a.stride() != b.stride() or a.stride(1) != 1 or a.stride(0) < 1:
+        return True
+    stride, apart = a.stride(0), (b0 - a0) // a.element_size()
+    return (b0 - a0) % a.element_size() != 0 or apart % stride < a.shape[1] or apart % stride + b.shape[1] > stride
 
 
 def _new_codes(x, N, K):
@@ -262,8 +268,9 @@ class _Product:
         return (2 if self.gated else 1) * self.M * (self.K + 4) + N * (self.K + 4 + 2 * self.M)
 
     def __call__(self, x, scales=None, out=None, stream=None):
-        """x int8 [N][K] with float32 scales [N] (of rms_norm_x8 or quantize_x8), or 16-bit [N][K] in the layer's type, which is rounded
-        to 8 bits first.  Returns [N][M] in the layer's type."""
+        """x int8 [N][K] with float32 scales [N] (of rms_norm_x8 or quantize_x8; codes whose rows are not aligned to 16 bytes, and readable
+        up to a multiple of 16, are copied first), or 16-bit [N][K] in the layer's type, which is rounded to 8 bits first.  Returns
+        [N][M] in the layer's type."""
         shape, K = x.shape, self.K
         if len(shape) != 2 or shape[1] != K or x.device != self.device:
             raise ValueError(f"x must be [N][{K}] on {self.device}")
@@ -283,8 +290,8 @@ class _Product:
             wide = (K + 15) // 16 * 16
             if N and (x.data_ptr() % 16 or (N > 1 and (stride % 16 or stride < wide or stride > 1 << 28))
                       or (wide != K and x.storage_offset() + (N - 1) * stride + wide > x.untyped_storage().nbytes())):
-                raise ValueError("rows of codes must be aligned to 16 bytes, at most 2^28 apart and readable up to a multiple of 16")
-            if N == 1:
+                stride = 0  # not as the kernels read rows: copied
+            elif N == 1:
                 stride = wide
         if out is not None:
             _check("out", out, self.device, self.dtype, (N, self.M))
@@ -294,11 +301,14 @@ class _Product:
         def call(handle):
             y = self.packed.new_empty((N, self.M), dtype=self.dtype) if out is None else out
             if N:
-                L, M, gated = _library(), self.M, self.gated
+                L, M, gated, codes, width = _library(), self.M, self.gated, x, stride
+                if scales is not None and not stride:
+                    codes, width, _ = _new_codes(x, N, K)
+                    codes.copy_(x)
                 need = L.W8_WorkspaceBytes(M, N, K, gated, scales is None)
                 ws = self.packed.new_empty(need) if need else None
                 err = (L.W8_Gated if gated else L.W8_Linear)(
-                    handle, self.packed.data_ptr(), _Codes(x.data_ptr(), stride, None if scales is None else scales.data_ptr()),
+                    handle, self.packed.data_ptr(), _Codes(codes.data_ptr(), width, None if scales is None else scales.data_ptr()),
                     y.data_ptr(), M, N, K, *[None if b is None else b.data_ptr() for b in self.biases], self.activation, None if ws is None else ws.data_ptr(), need,
                     self._kind)
                 if err:

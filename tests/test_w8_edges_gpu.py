@@ -1,0 +1,246 @@
+"""The 8-bit linears' kernels one by one (the tests' build of the library takes a plan), and calls that are easily got wrong:
+broadcast and interlaced rows, in-place outputs, refusals of the host layer, graphs that share nothing."""
+import ctypes as C
+import os
+
+import numpy as np
+import pytest
+
+import spmspm_amd as S
+from oracle import w8_oracle as O
+from spmspm_amd import api as A
+from spmspm_amd import w8 as M
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    return torch
+
+
+@pytest.fixture
+def set_plan(monkeypatch):
+    lib = C.CDLL(os.path.join(os.path.dirname(S.library_path()), "libSpMM_API_variants.so"))
+    monkeypatch.setattr(A, "library", lambda: lib)
+    monkeypatch.setattr(M, "_lib", None)
+    yield lib.W8_Debug_SetPlan
+    lib.W8_Debug_SetPlan(0, 0, 0, 0)
+
+
+def weights(torch, M_, K, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(-127, 128, (M_, K), generator=gen, dtype=torch.int8, device="cuda")
+    return codes, (0.5 + torch.rand(M_, generator=gen, device="cuda")) * (0.01 / K ** 0.5)
+
+
+def rows8(torch, N, K, seed):
+    x = torch.randn((N, K), generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").half()
+    return S.quantize_x8(x)
+
+
+def products(torch, gated, M_, K, N, seed=0, act=A.ACT_SILU):
+    """A layer, its input and its outputs in float64 with their bound."""
+    pairs = [weights(torch, M_, K, seed + i) for i in range(2 if gated else 1)]
+    b = [torch.randn(M_, generator=torch.Generator(device="cuda").manual_seed(seed + 5 + i), device="cuda").half()
+         for i in range(len(pairs))]
+    codes, scales = rows8(torch, N, K, seed + 9)
+    n = lambda t: t.cpu().numpy() if t.dtype != torch.float16 else t.double().cpu().numpy()
+    if gated:
+        layer = S.W8GatedLinear(*pairs[0], *pairs[1], gate_bias=b[0], up_bias=b[1], activation=act)
+        want, bound = O.gated(n(codes), n(scales), *[n(t) for p in pairs for t in p], *[n(t) for t in b], act)
+    else:
+        layer = S.W8Linear(*pairs[0], bias=b[0], activation=act)
+        want, bound = O.linear(n(codes), n(scales), *[n(t) for t in pairs[0]], n(b[0]), act)
+    return layer, codes, scales, want, bound
+
+
+def assert_close(got, want, bound):
+    off = np.abs(got.double().cpu().numpy() - want) - (2.0 ** -11 * np.abs(want) + 1.01 * bound + 2.0 ** -25)
+    assert (off <= 0).all(), off.max()
+
+
+# rows past and below a tile's end, one block of K and many, fewer columns than a tile and several tiles, an odd M
+SIZES = [(33, 100, 5), (300, 1100, 70), (129, 4100, 300), (520, 640, 17)]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("rows", [1, 2, 4])
+@pytest.mark.parametrize("cols", [1, 2, 3, 4])
+@pytest.mark.parametrize("shares", [1, 3])
+def test_narrow_kernels(torch, set_plan, gated, size, rows, cols, shares):
+    if gated and rows == 1:
+        pytest.skip("rows of the gate and of up come in pairs of tiles")
+    assert set_plan(0, rows, cols, shares) == 0
+    layer, codes, scales, want, bound = products(torch, gated, *size)
+    got = layer(codes, scales)
+    assert_close(got, want, bound)
+    assert torch.equal(got, layer(codes, scales))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("size", SIZES + [(1000, 257, 513)])
+@pytest.mark.parametrize("kind", [1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("shares", [1, 2, 7])
+def test_tile_kernels(torch, set_plan, gated, size, kind, shares):
+    assert set_plan(kind, 0, 0, shares) == 0
+    layer, codes, scales, want, bound = products(torch, gated, *size)
+    got = layer(codes, scales)
+    assert_close(got, want, bound)
+    assert torch.equal(got, layer(codes, scales))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kind,shares", [(1, 1), (2, 1), (3, 1), (4, 1), (5, 1), (6, 1), (6, 3)])
+def test_many_tiles_of_a_workgroup(torch, set_plan, gated, kind, shares):
+    """More tiles than workgroups run at once, of one block of K and of three: loads that are ahead of the products by whole tiles,
+    stores that the next tile does not wait for."""
+    for K in (40, 380):
+        size = (2100, K, 4100) if kind < 4 else (2100, K, 2100)
+        assert set_plan(0, 2, 4, 1) == 0
+        layer, codes, scales, want, bound = products(torch, gated, *size, act=A.ACT_NONE)
+        first = layer(codes, scales)
+        assert_close(first[:, :70], want[:, :70], bound[:, :70])
+        assert set_plan(kind, 0, 0, shares) == 0
+        for _ in range(3):
+            assert torch.equal(first, layer(codes, scales))
+
+
+def test_a_rows_result_does_not_depend_on_the_batch(torch):
+    """Sums are whole numbers: whatever kernel a batch takes, a row has the same bits."""
+    w, g, u = weights(torch, 700, 1000, 1), weights(torch, 700, 1000, 2), weights(torch, 700, 1000, 3)
+    codes, scales = rows8(torch, 700, 1000, 4)
+    for layer in (S.W8Linear(*w, activation=A.ACT_GELU), S.W8GatedLinear(*g, *u)):
+        whole = layer(codes, scales)
+        for n in (1, 2, 16, 17, 40, 64, 100, 256, 300):
+            assert torch.equal(layer(codes[:n], scales[:n]), whole[:n])
+            assert torch.equal(layer(codes[700 - n:], scales[700 - n:].contiguous()), whole[700 - n:])
+
+
+@pytest.mark.parametrize("K", [48, 777, 1024, 5000])
+def test_rows_that_are_one_row(torch, K):
+    """Inputs of stride 0: every row the same memory."""
+    one = torch.randn((1, K), device="cuda").half()
+    x, w = one.expand(5, K), torch.rand(K, device="cuda").half()
+    codes, scales = S.quantize_x8(x)
+    assert torch.equal(codes, S.quantize_x8(x.contiguous())[0]) and (scales == scales[0]).all()
+    y, h = S.rms_norm(x, w, residual=x)
+    y2, h2 = S.rms_norm(x.contiguous(), w, residual=x.contiguous())
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+
+
+def test_interlaced_rows_of_one_buffer(torch):
+    """x, the residual and both outputs as slices of wider rows, in types of two bytes at odd places."""
+    wide = torch.randn((6, 4 * 333 + 1), device="cuda").bfloat16()
+    x, r, a, b = (wide[:, 1 + 333 * i:1 + 333 * (i + 1)] for i in range(4))
+    w = torch.rand(333, device="cuda").bfloat16()
+    want = S.rms_norm(x.contiguous(), w, residual=r.contiguous())
+    before = wide.clone()
+    room = torch.zeros((6, 2 * 333 + 7), device="cuda").bfloat16()
+    y, h = S.rms_norm(x, w, residual=r, out=room[:, 3:336], residual_out=torch.empty((6, 333), device="cuda").bfloat16())
+    assert torch.equal(y, want[0]) and torch.equal(h, want[1]) and torch.equal(wide, before)
+    assert (room[:, :3] == 0).all() and (room[:, 336:] == 0).all()
+    S.rms_norm(x, w, residual=r, out=a, residual_out=b)  # side by side in the rows that x and the residual lie in
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1]) and torch.equal(wide[:, :667], before[:, :667])
+    with pytest.raises(ValueError):
+        S.rms_norm(x, w, residual=r, out=wide[:, 300:633], residual_out=b)
+
+
+def test_more_rows_than_a_launch_has_threads_for(torch):
+    """Three million rows of nine numbers, each as it is alone."""
+    x = torch.randn((3_000_001, 9), device="cuda").half()
+    r, w = x.flip(0), torch.rand(9, device="cuda").half()
+    y, h = S.rms_norm(x, w, residual=r)
+    codes, scales, h8 = S.rms_norm_x8(x, w, residual=r)
+    c, s = S.quantize_x8(x)
+    assert torch.equal(h, x + r) and torch.equal(h8, h)
+    for part in (slice(0, 5), slice((1 << 21) - 4, (1 << 21) + 5), slice(2_999_990, None)):
+        one = S.rms_norm(x[part], w, residual=r[part])
+        assert torch.equal(y[part], one[0])
+        one = S.rms_norm_x8(x[part], w, residual=r[part])
+        assert torch.equal(codes[part], one[0]) and torch.equal(scales[part], one[1])
+        one = S.quantize_x8(x[part])
+        assert torch.equal(c[part], one[0]) and torch.equal(s[part], one[1])
+
+
+def test_host_layer_refusals(torch):
+    x, w = torch.zeros((4, 64), device="cuda").half(), torch.ones(64, device="cuda").half()
+    c, s = S.quantize_x8(x)
+    big = torch.zeros((8, 64), device="cuda").half()
+    layer = S.W8Linear(*S.quantize_w8(torch.ones((32, 64), device="cuda")))
+    for call in (lambda: S.rms_norm(x, w[:32]), lambda: S.rms_norm(x, w.bfloat16()), lambda: S.rms_norm(x, w.cpu()),
+                 lambda: S.rms_norm(x, w, eps=0), lambda: S.rms_norm(x, w, eps=float("nan")), lambda: S.rms_norm(x[0], w),
+                 lambda: S.rms_norm(x, w, residual=x[:2]), lambda: S.rms_norm(x, w, residual=x.bfloat16()),
+                 lambda: S.rms_norm(x, w, residual_out=x), lambda: S.rms_norm(x.t().contiguous().t(), w),
+                 lambda: S.rms_norm(x, w, out=x[:2]), lambda: S.rms_norm(big[:4], w, out=big[1:5]),
+                 lambda: S.rms_norm(x, w, residual=big[:4], residual_out=big[4:], out=big[4:]),
+                 lambda: S.rms_norm(x, w, out=torch.empty((1, 64), device="cuda").half().expand(4, 64)),
+                 lambda: S.rms_norm(x, x[0], out=x), lambda: S.rms_norm_x8(x, x[0], residual=x, residual_out=x),
+                 lambda: S.rms_norm_x8(x, w, residual_out=x), lambda: S.quantize_x8(x.float()), lambda: S.quantize_x8(x[:, ::2]),
+                 lambda: S.quantize_x8(torch.zeros((1, M.MAX_K + 1), device="cuda").half()),
+                 lambda: layer(c), lambda: layer(c, s[:2]), lambda: layer(c, s.half()), lambda: layer(x, s), lambda: layer(x.bfloat16()),
+                 lambda: layer(c[:, :32], s), lambda: layer(c.cpu(), s), lambda: layer(c.t().contiguous().t(), s),
+                 lambda: layer(x, out=torch.empty((4, 31), device="cuda").half()), lambda: layer(x[:, :32], out=x[:, :32]),
+                 lambda: layer(x, out=x[:, :32]),
+                 lambda: S.W8Linear(c, s.half()), lambda: S.W8Linear(c, s[:2]), lambda: S.W8Linear(c.short(), s),
+                 lambda: S.W8Linear(c, s, bias=w), lambda: S.W8Linear(c, s, activation=4), lambda: S.W8Linear(c, s, dtype=torch.float32),
+                 lambda: S.W8GatedLinear(c, s, c[:2], s[:2]), lambda: S.w8_pack(c[:, :0], s)):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.parametrize("K", [50, 64, 1029])
+def test_codes_that_are_not_laid_out_for_the_kernels(torch, K):
+    """Rows at odd places, rows all the same, a last row that ends with its codes: copied, with the same result."""
+    layer = S.W8Linear(*weights(torch, 96, K, 1))
+    codes, scales = rows8(torch, 5, K, 2)
+    want = layer(codes, scales)
+    end = (K + 15) // 16 * 16
+    tight = torch.empty(4 * end + K, dtype=torch.int8, device="cuda").as_strided((5, K), (end, 1))
+    for c in (codes.contiguous(), torch.empty((5, K + 3), dtype=torch.int8, device="cuda")[:, 3:], tight):
+        c.copy_(codes)
+        assert torch.equal(layer(c, scales), want)
+    assert torch.equal(layer(codes[1:2].expand(5, K), scales), layer(codes[1:2].repeat(5, 1), scales))
+    far = torch.empty(4 * ((1 << 28) + 16) + end, dtype=torch.int8, device="cuda").as_strided((5, K), ((1 << 28) + 16, 1))
+    far.copy_(codes)
+    assert torch.equal(layer(far, scales), want)
+
+
+def test_two_graphs_and_an_eager_call_at_once(torch):
+    """Two recorded calls of one layer replayed on two streams beside eager calls: each has a workspace of its own."""
+    M_, K, N = 300, 8192, 90  # K in shares
+    layer = S.W8Linear(*weights(torch, M_, K, 1))
+    xs = [torch.randn((N, K), device="cuda").half() for _ in range(3)]
+    want = [layer(x) for x in xs]
+    graphs, outs = [], []
+    for x in xs[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(layer(x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = layer(xs[2])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
+
+
+def test_workspace_is_what_the_call_asks_for(torch):
+    """A call with one byte less than W8_WorkspaceBytes is refused before anything is launched, over sizes with and without shares."""
+    L, rng, seen = M._library(), np.random.default_rng(0), set()
+    for _ in range(200):
+        m, k, n = int(np.exp(rng.uniform(4, 9))), int(np.exp(rng.uniform(4, 11))), int(np.exp(rng.uniform(0, 7)))
+        gated, x16 = bool(rng.integers(2)), bool(rng.integers(2))
+        need = L.W8_WorkspaceBytes(m, n, k, gated, x16)
+        seen.add((need > 0, x16))
+        if need:
+            c = M._Codes(1 << 20, 1 << 20, None if x16 else 1 << 20)
+            f = L.W8_Gated if gated else L.W8_Linear
+            assert f(None, 1 << 20, c, 1 << 20, m, n, k, *((None, None) if gated else (None,)), 0, 1 << 20, need - 1, 0) == 1
+    assert (True, False) in seen and (False, False) in seen and (True, True) in seen
