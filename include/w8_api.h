@@ -24,56 +24,42 @@
 extern "C" {
 #endif
 
-/* Rows of N x K 16-bit numbers, `stride` elements apart; any alignment of the type. */
-typedef struct W8_Rows {
-    const void* data;
-    int64_t     stride;
-} W8_Rows;
-
-/* Rows in 8 bits as above; scales float32 [N]. */
-typedef struct W8_Codes {
-    int8_t* codes;
-    int64_t stride;
-    float*  scales;
-} W8_Codes;
-
-/* Root-mean-square norm.  h = x + residual, rounded to `dtype` (residual.data NULL: h = x), t = h * weight,
+/* Root-mean-square norm.  h = x + residual, rounded to `dtype` (residual NULL: h = x), t = h * weight,
  *   y = t / sqrt(mean(h^2) + eps)
- * rounded to `dtype` into y [N rows], or as 8-bit rows of t with scale m / 127 / sqrt(...) into `codes`; one of the two, the other NULL.
- * h_out (data NULL: not wanted) receives h; it and y may be x or the residual themselves (same address and stride), no output may
- * overlap an input or another output otherwise.  weight [K]; sums in float32; eps from 1e-20 up.  K from 1 to 2^24 (131071 for codes),
- * N below 2^31. */
-int RMS_Norm(hipStream_t stream, W8_Rows x, W8_Rows residual, const void* weight, float eps, int N, int K, W8_Rows h_out,
-             W8_Rows y, const W8_Codes* codes, int dtype);
+ * rounded to `dtype` into y (codes NULL), or as 8-bit rows of t with scale m / 127 / sqrt(...) into codes and scales (y NULL).
+ * h_out (NULL: not wanted) receives h; it and y may be x or the residual themselves (same address and stride), no output may overlap
+ * an input or another output otherwise.  Rows of x, residual, h_out and y lie x_stride ... elements apart, at any alignment of the
+ * type.  weight [K]; sums in float32; eps from 1e-20 up.  K from 1 to 2^24 (131071 for codes), N below 2^31. */
+int RMS_Norm(hipStream_t stream, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+             float eps, int N, int K, void* h_out, int64_t h_stride, void* y, int64_t y_stride, int8_t* codes,
+             int64_t codes_stride, float* scales, int dtype);
 
 /* 8-bit rows of x. */
-int W8_Quantize(hipStream_t stream, W8_Rows x, int N, int K, const W8_Codes* codes, int dtype);
+int W8_Quantize(hipStream_t stream, const void* x, int64_t x_stride, int N, int K, int8_t* codes, int64_t codes_stride,
+                float* scales, int dtype);
 
-/* Weights, laid out once: codes int8 [M][K] (rows w_stride bytes apart, no alignment) and scales float32 [M] into `packed`,
- * W8_PackedBytes(M, K, 0) bytes, 16-byte aligned.  A second pair, `up`, makes it the weights of a gated product: up not NULL,
+/* Weights, laid out once: codes int8 [M][K] (rows `stride` bytes apart, no alignment) and scales float32 [M] into `packed`,
+ * W8_PackedBytes(M, K, 0) bytes, 16-byte aligned.  A second pair, up_codes not NULL, makes it the weights of a gated product:
  * W8_PackedBytes(M, K, 1) bytes.  M from 1 to 2^24, K from 1 to 131071 (a sum of K products stays in 32 bits).  0 bytes: sizes
  * that are refused. */
-typedef struct W8_Weights {
-    const int8_t* codes;
-    int64_t       w_stride;
-    const float*  scales;
-} W8_Weights;
 size_t W8_PackedBytes(int M, int K, int gated);
-int    W8_Pack(hipStream_t stream, W8_Weights w, const W8_Weights* up, int M, int K, void* packed);
+int    W8_Pack(hipStream_t stream, const int8_t* codes, int64_t stride, const float* scales, const int8_t* up_codes,
+               int64_t up_stride, const float* up_scales, int M, int K, void* packed);
 
 /* Y[n][m] = act(sum_k value(x)[n][k] * scale[m] code[m][k] + bias[m]), Y [N][M] contiguous in `dtype`, rounded once.  Sums of codes'
  * products are exact; they are turned into float32 and multiplied by the weight's scale, then by the row's.
  * W8_Gated: Y[n][m] = act(gate) * up, gate and up each such a sum over the two halves of gated weights, with gate_bias and up_bias.
- * x.scales NULL: x.codes holds 16-bit rows (x.stride in elements, any alignment of the type) instead, which the call itself turns into
- * 8-bit rows in the workspace.  Biases NULL or [M] in `dtype`.  `activation`: 0 none, 1 ReLU, 2 GELU (tanh form), 3 SiLU (x / (1 + exp(-x))).
- * N from 0 to 2^24.  `workspace` must hold W8_WorkspaceBytes of the same sizes (NULL where that is 0), 16-byte aligned, contents
- * irrelevant; `x16` says that x holds 16-bit rows. */
+ * x_scales NULL: x holds 16-bit rows (x_stride in elements, any alignment of the type) instead of 8-bit rows, which the call itself
+ * turns into 8-bit rows in the workspace.  Biases NULL or [M] in `dtype`.  `activation`: 0 none, 1 ReLU, 2 GELU (tanh form), 3 SiLU
+ * (x / (1 + exp(-x))).  N from 0 to 16 * 65535.  `workspace` must hold W8_WorkspaceBytes of the same sizes (NULL where that is 0),
+ * 16-byte aligned, contents irrelevant; `x16` says that x holds 16-bit rows. */
 #define W8_ACT_SILU 3
 size_t W8_WorkspaceBytes(int M, int N, int K, int gated, int x16);
-int    W8_Linear(hipStream_t stream, const void* packed, W8_Codes x, void* Y, int M, int N, int K, const void* bias,
-                 int activation, void* workspace, size_t workspace_bytes, int dtype);
-int    W8_Gated(hipStream_t stream, const void* packed, W8_Codes x, void* Y, int M, int N, int K, const void* gate_bias,
-                const void* up_bias, int activation, void* workspace, size_t workspace_bytes, int dtype);
+int    W8_Linear(hipStream_t stream, const void* packed, const void* x, int64_t x_stride, const float* x_scales, void* Y, int M,
+                 int N, int K, const void* bias, int activation, void* workspace, size_t workspace_bytes, int dtype);
+int    W8_Gated(hipStream_t stream, const void* packed, const void* x, int64_t x_stride, const float* x_scales, void* Y, int M,
+                int N, int K, const void* gate_bias, const void* up_bias, int activation, void* workspace,
+                size_t workspace_bytes, int dtype);
 
 #ifdef __cplusplus
 }

@@ -311,45 +311,44 @@ int run_quantize(hipStream_t stream, const void* x, int64_t x_stride, int N, int
 
 using namespace decode;
 
-extern "C" int RMS_Norm(hipStream_t stream, W8_Rows x, W8_Rows residual, const void* weight, float eps, int N, int K,
-                        W8_Rows h_out, W8_Rows y, const W8_Codes* codes, int dtype)
+extern "C" int RMS_Norm(hipStream_t stream, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                        const void* weight, float eps, int N, int K, void* h_out, int64_t h_stride, void* y, int64_t y_stride,
+                        int8_t* codes, int64_t codes_stride, float* scales, int dtype)
 {
-    if (int e = check_sizes(N, K, codes != nullptr ? kMaxK8 : 1 << 24, dtype))
+    if (int e = check_sizes(N, K, codes != nullptr || scales != nullptr ? kMaxK8 : 1 << 24, dtype))
         return e;
     if (!(eps >= 1e-20f) || !(eps < INFINITY))
         return refuse("eps %g: 1e-20 or more", (double)eps);
-    if ((codes != nullptr) == (y.data != nullptr))
-        return refuse("a norm writes either 16-bit rows or codes");
     if (N == 0)
         return 0;
-    if (bad_rows16(x) || bad_pointer(weight, 2) || (residual.data != nullptr && bad_rows16(residual)) ||
-        (h_out.data != nullptr && bad_rows16(h_out)) || (y.data != nullptr && bad_rows16(y)))
+    if ((codes != nullptr) == (y != nullptr))
+        return refuse("a norm writes either 16-bit rows or codes");
+    if (bad_pointer(x, 2) || bad_pointer(weight, 2) || (residual != nullptr && bad_pointer(residual, 2)) ||
+        (h_out != nullptr && bad_pointer(h_out, 2)) || (y != nullptr && bad_pointer(y, 2)))
         return refuse("a null or misaligned x, residual, weight, h or y (2 bytes)");
-    if (codes != nullptr && (bad_codes(*codes, N, K) || bad_pointer(codes->scales, 4)))
+    if (codes != nullptr && bad_codes(codes, codes_stride, scales, N, K))
         return refuse("codes null or misaligned (16 bytes, rows too), or scales (4)");
-    if (N > 1 && ((h_out.data != nullptr && h_out.stride < K) || (y.data != nullptr && y.stride < K)))
+    if (N > 1 && ((h_out != nullptr && h_stride < K) || (y != nullptr && y_stride < K)))
         return refuse("rows of an output less than %d numbers apart", K);
     NormArgs a{};
-    a.x = static_cast<const uint16_t*>(x.data), a.x_stride = x.stride;
-    a.residual = static_cast<const uint16_t*>(residual.data), a.r_stride = residual.stride;
+    a.x = static_cast<const uint16_t*>(x), a.x_stride = x_stride;
+    a.residual = static_cast<const uint16_t*>(residual), a.r_stride = residual_stride;
     a.weight = static_cast<const uint16_t*>(weight);
-    a.h = static_cast<uint16_t*>(const_cast<void*>(h_out.data)), a.h_stride = h_out.stride;
-    a.y = static_cast<uint16_t*>(const_cast<void*>(y.data)), a.y_stride = y.stride;
-    if (codes != nullptr)
-        a.codes = codes->codes, a.c_stride = codes->stride, a.scales = codes->scales;
+    a.h = static_cast<uint16_t*>(h_out), a.h_stride = h_stride;
+    a.y = static_cast<uint16_t*>(y), a.y_stride = y_stride;
+    a.codes = codes, a.c_stride = codes_stride, a.scales = scales;
     a.N = N, a.K = K, a.eps = eps;
     return start(stream, a, dtype);
 }
 
-extern "C" int W8_Quantize(hipStream_t stream, W8_Rows x, int N, int K, const W8_Codes* codes, int dtype)
+extern "C" int W8_Quantize(hipStream_t stream, const void* x, int64_t x_stride, int N, int K, int8_t* codes, int64_t codes_stride,
+                           float* scales, int dtype)
 {
     if (int e = check_sizes(N, K, kMaxK8, dtype))
         return e;
-    if (codes == nullptr)
-        return refuse("no codes given");
     if (N == 0)
         return 0;
-    if (bad_rows16(x) || bad_codes(*codes, N, K) || bad_pointer(codes->scales, 4))
+    if (bad_pointer(x, 2) || bad_codes(codes, codes_stride, scales, N, K))
         return refuse("x null or misaligned (2 bytes), codes (16, rows too) or scales (4)");
-    return run_quantize(stream, x.data, x.stride, N, K, codes->codes, codes->stride, codes->scales, dtype);
+    return run_quantize(stream, x, x_stride, N, K, codes, codes_stride, scales, dtype);
 }

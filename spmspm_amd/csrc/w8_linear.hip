@@ -788,8 +788,9 @@ Space8 space8(int M, int N, int K, bool gated, bool x16, const Plan8& p)
     return s;
 }
 
-int run_product(hipStream_t stream, const void* packed, const W8_Codes& x, void* Y, int M, int N, int K, const void* bias,
-                const void* up_bias, int activation, void* workspace, size_t workspace_bytes, int dtype, bool gated)
+int run_product(hipStream_t stream, const void* packed, const void* x, int64_t x_stride, const float* x_scales, void* Y, int M, int N,
+                int K, const void* bias, const void* up_bias, int activation, void* workspace, size_t workspace_bytes, int dtype,
+                bool gated)
 {
     if (int e = check_sizes8(M, K))
         return e;
@@ -804,21 +805,21 @@ int run_product(hipStream_t stream, const void* packed, const W8_Codes& x, void*
     if (bad_pointer(packed, 16) || bad_pointer(Y, 2) || (bias != nullptr && bad_pointer(bias, 2)) ||
         (up_bias != nullptr && bad_pointer(up_bias, 2)))
         return refuse("a null or misaligned weight (16 bytes), Y or bias (2)");
-    const bool   x16 = x.scales == nullptr;
+    const bool   x16 = x_scales == nullptr;
     const Plan8  p   = plan8(M, N, K, gated);
     const Space8 s   = space8(M, N, K, gated, x16, p);
-    if (x16 ? bad_pointer(x.codes, 2) : bad_codes(x, N, K) || bad_pointer(x.scales, 4))
+    if (x16 ? bad_pointer(x, 2) : bad_codes(x, x_stride, x_scales, N, K))
         return refuse("X null or misaligned (16-bit rows: 2 bytes; codes: 16, rows too, scales 4)");
     const size_t need = (size_t)s.bytes;
     if (need > 0 && (bad_pointer(workspace, 16) || workspace_bytes < need))
         return refuse("workspace of %zu bytes (16-byte aligned), %zu needed", workspace == nullptr ? (size_t)0 : workspace_bytes, need);
     ProductArgs a{};
     a.packed = static_cast<const uint8_t*>(packed);
-    a.x = x.codes, a.x_scales = x.scales, a.x_stride = x.stride;
+    a.x = static_cast<const int8_t*>(x), a.x_scales = x_scales, a.x_stride = x_stride;
     if (x16) {
         int8_t* codes  = static_cast<int8_t*>(workspace) + s.codes;
         float*  scales = reinterpret_cast<float*>(static_cast<int8_t*>(workspace) + s.scales);
-        if (int e = run_quantize(stream, x.codes, x.stride, N, K, codes, s.stride, scales, dtype))
+        if (int e = run_quantize(stream, x, x_stride, N, K, codes, s.stride, scales, dtype))
             return e;
         a.x = codes, a.x_scales = scales, a.x_stride = s.stride;
     }
@@ -852,19 +853,20 @@ extern "C" size_t W8_PackedBytes(int M, int K, int gated)
     return (size_t)layout8(M, K, gated != 0).bytes;
 }
 
-extern "C" int W8_Pack(hipStream_t stream, W8_Weights w, const W8_Weights* up, int M, int K, void* packed)
+extern "C" int W8_Pack(hipStream_t stream, const int8_t* codes, int64_t stride, const float* scales, const int8_t* up_codes,
+                       int64_t up_stride, const float* up_scales, int M, int K, void* packed)
 {
     if (int e = check_sizes8(M, K))
         return e;
-    if (w.codes == nullptr || bad_pointer(w.scales, 4) || (up != nullptr && (up->codes == nullptr || bad_pointer(up->scales, 4))) ||
-        bad_pointer(packed, 16) || (M > 1 && (w.w_stride < K || (up != nullptr && up->w_stride < K))))
+    const bool gated = up_codes != nullptr;
+    if (codes == nullptr || bad_pointer(scales, 4) || (gated && bad_pointer(up_scales, 4)) || bad_pointer(packed, 16) ||
+        (M > 1 && (stride < K || (gated && up_stride < K))))
         return refuse("null or misaligned codes, scales (4 bytes) or packed weights (16), or rows less than %d codes apart", K);
     PackArgs a{};
-    a.w = w.codes, a.scales = w.scales, a.w_stride = w.w_stride;
-    if (up != nullptr)
-        a.up = up->codes, a.up_scales = up->scales, a.up_stride = up->w_stride;
+    a.w = codes, a.scales = scales, a.w_stride = stride;
+    a.up = up_codes, a.up_scales = up_scales, a.up_stride = up_stride;
     a.M = M, a.K = K, a.packed = static_cast<uint8_t*>(packed);
-    const Layout8 l      = layout8(M, K, up != nullptr);
+    const Layout8 l = layout8(M, K, gated);
     return launch(w8_pack, dim3((unsigned)(l.groups * (l.steps / 2)), 1, 1), dim3(256, 1, 1), stream, a);
 }
 
@@ -875,14 +877,17 @@ extern "C" size_t W8_WorkspaceBytes(int M, int N, int K, int gated, int x16)
     return (size_t)space8(M, N, K, gated != 0, x16 != 0, plan8(M, N, K, gated != 0)).bytes;
 }
 
-extern "C" int W8_Linear(hipStream_t stream, const void* packed, W8_Codes x, void* Y, int M, int N, int K, const void* bias,
-                         int activation, void* workspace, size_t workspace_bytes, int dtype)
+extern "C" int W8_Linear(hipStream_t stream, const void* packed, const void* x, int64_t x_stride, const float* x_scales, void* Y, int M,
+                         int N, int K, const void* bias, int activation, void* workspace, size_t workspace_bytes, int dtype)
 {
-    return run_product(stream, packed, x, Y, M, N, K, bias, nullptr, activation, workspace, workspace_bytes, dtype, false);
+    return run_product(stream, packed, x, x_stride, x_scales, Y, M, N, K, bias, nullptr, activation, workspace, workspace_bytes, dtype,
+                       false);
 }
 
-extern "C" int W8_Gated(hipStream_t stream, const void* packed, W8_Codes x, void* Y, int M, int N, int K, const void* gate_bias,
-                        const void* up_bias, int activation, void* workspace, size_t workspace_bytes, int dtype)
+extern "C" int W8_Gated(hipStream_t stream, const void* packed, const void* x, int64_t x_stride, const float* x_scales, void* Y, int M,
+                        int N, int K, const void* gate_bias, const void* up_bias, int activation, void* workspace,
+                        size_t workspace_bytes, int dtype)
 {
-    return run_product(stream, packed, x, Y, M, N, K, gate_bias, up_bias, activation, workspace, workspace_bytes, dtype, true);
+    return run_product(stream, packed, x, x_stride, x_scales, Y, M, N, K, gate_bias, up_bias, activation, workspace, workspace_bytes,
+                       dtype, true);
 }

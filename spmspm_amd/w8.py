@@ -24,18 +24,6 @@ __all__ = ["rms_norm", "rms_norm_x8", "quantize_x8", "quantize_w8", "w8_pack", "
 MAX_K = 131071  # sums of products of codes stay in 32 bits
 
 
-class _Rows(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("stride", C.c_int64)]
-
-
-class _Codes(C.Structure):
-    _fields_ = [("codes", C.c_void_p), ("stride", C.c_int64), ("scales", C.c_void_p)]
-
-
-class _Weights(C.Structure):
-    _fields_ = [("codes", C.c_void_p), ("w_stride", C.c_int64), ("scales", C.c_void_p)]
-
-
 _lib = None
 
 
@@ -43,42 +31,32 @@ def _library():
     global _lib
     if _lib is None:
         L = A.library()
-        codes, weights = C.POINTER(_Codes), C.POINTER(_Weights)
-        L.RMS_Norm.restype = C.c_int
-        L.RMS_Norm.argtypes = [C.c_void_p, _Rows, _Rows, C.c_void_p, C.c_float, C.c_int, C.c_int, _Rows, _Rows, codes, C.c_int]
-        L.W8_Quantize.restype = C.c_int
-        L.W8_Quantize.argtypes = [C.c_void_p, _Rows, C.c_int, C.c_int, codes, C.c_int]
-        L.W8_PackedBytes.restype = C.c_size_t
-        L.W8_PackedBytes.argtypes = [C.c_int] * 3
-        L.W8_Pack.restype = C.c_int
-        L.W8_Pack.argtypes = [C.c_void_p, _Weights, weights, C.c_int, C.c_int, C.c_void_p]
-        L.W8_WorkspaceBytes.restype = C.c_size_t
-        L.W8_WorkspaceBytes.argtypes = [C.c_int] * 5
-        L.W8_Linear.restype = C.c_int
-        L.W8_Linear.argtypes = [C.c_void_p, C.c_void_p, _Codes, C.c_void_p] + [C.c_int] * 3 + [
-            C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_int]
-        L.W8_Gated.restype = C.c_int
-        L.W8_Gated.argtypes = [C.c_void_p, C.c_void_p, _Codes, C.c_void_p] + [C.c_int] * 3 + [
-            C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_int]
+        p, n, s = C.c_void_p, C.c_int, C.c_int64
+        L.RMS_Norm.argtypes = [p, p, s, p, s, p, C.c_float, n, n, p, s, p, s, p, s, p, n]
+        L.W8_Quantize.argtypes = [p, p, s, n, n, p, s, p, n]
+        L.W8_Pack.argtypes = [p, p, s, p, p, s, p, n, n, p]
+        L.W8_Linear.argtypes = [p, p, p, s, p, p, n, n, n, p, n, p, C.c_size_t, n]
+        L.W8_Gated.argtypes = [p, p, p, s, p, p, n, n, n, p, p, n, p, C.c_size_t, n]
+        for f in (L.RMS_Norm, L.W8_Quantize, L.W8_Pack, L.W8_Linear, L.W8_Gated):
+            f.restype = n
+        L.W8_PackedBytes.restype, L.W8_PackedBytes.argtypes = C.c_size_t, [n] * 3
+        L.W8_WorkspaceBytes.restype, L.W8_WorkspaceBytes.argtypes = C.c_size_t, [n] * 5
         _lib = L
     return _lib
 
 
-_NONE = _Rows(None, 0)
-
-
 def _rows(name, t, dtype, shape, device):
-    """16-bit rows of any stride."""
+    """Stride of 16-bit rows."""
     strides = t.stride()
     if t.dtype != dtype or t.shape != shape or t.device != device or (strides[1] != 1 and shape[1] > 1):
         raise ValueError(f"{name} must be {dtype} {list(shape)} on {device} with contiguous rows")
-    return _Rows(t.data_ptr(), strides[0])
+    return strides[0]
 
 
 def _out_rows(name, t, like, inputs, outputs=()):
-    """Rows of an output, which may be an input itself but not a part of one, nor lap over another output."""
-    rows = _rows(name, t, like.dtype, like.shape, like.device)
-    if like.shape[0] > 1 and t.stride(0) < like.shape[1]:
+    """Stride of an output's rows; it may be an input itself but not a part of one, nor lap over another output."""
+    stride = _rows(name, t, like.dtype, like.shape, like.device)
+    if like.shape[0] > 1 and stride < like.shape[1]:
         raise ValueError(f"{name}: rows of an output must not overlap")
     for other in inputs:
         if other is not None and _overlap(t, other) and not (
@@ -87,7 +65,7 @@ def _out_rows(name, t, like, inputs, outputs=()):
     for other in outputs:
         if other is not None and _overlap(t, other):
             raise ValueError(f"{name} overlaps another output")
-    return rows
+    return stride
 
 
 def _overlap(a, b):
@@ -116,33 +94,53 @@ def _new_codes(x, N, K):
     return codes, width, x.new_empty(N, dtype=torch.float32)
 
 
-def _norm_args(x, weight, eps, residual, most):
-    """Checked rows of x and of the residual, the kind of their type, N and K."""
+def _norm(name, x, weight, eps, residual, residual_out, out, codes, stream):
+    """Both norms: checks, allocations and the call; `codes` says that the result is in 8 bits."""
     shape, dtype, device = x.shape, x.dtype, x.device
     kind = _type(dtype)
     if len(shape) != 2 or shape[1] == 0 or not x.is_cuda:
         raise ValueError("x must be [tokens][K] on the GPU")
     N, K = shape
+    most = MAX_K if codes else 1 << 24
     if N >= 1 << 31 or K > most:
         raise ValueError(f"{N} tokens of {K} numbers: 2^31 - 1 tokens and {most} numbers at most")
     if weight.shape != (K,) or weight.dtype != dtype or weight.device != device or not weight.is_contiguous():
         raise ValueError(f"weight must be {dtype} [{K}], contiguous, on {device}")
     if not 1e-20 <= eps < 3e38:
         raise ValueError(f"eps {eps}: from 1e-20 up")
-    xr = _rows("x", x, dtype, shape, device)
-    return xr, _NONE if residual is None else _rows("residual", residual, dtype, shape, device), kind, N, K
+    x_stride = _rows("x", x, dtype, shape, device)
+    added = residual is not None
+    r, r_stride = (residual.data_ptr(), _rows("residual", residual, dtype, shape, device)) if added else (None, 0)
+    h_stride = y_stride = K
+    if residual_out is not None:
+        if not added:
+            raise ValueError("residual_out without a residual: h is x itself")
+        h_stride = _out_rows("residual_out", residual_out, x, (x, residual))
+    if out is not None:
+        y_stride = _out_rows("out", out, x, (x, residual), (residual_out,))
+    if (out is not None and _overlap(out, weight)) or (residual_out is not None and _overlap(residual_out, weight)):
+        raise ValueError("an output overlaps the weight")
 
+    def call(handle):
+        y, h = out, residual_out
+        if codes:
+            y, width, scales = _new_codes(x, N, K)
+        elif y is None:
+            y = x.new_empty((N, K))
+        if added and h is None:
+            h = x.new_empty((N, K))
+        if N:
+            at = y.data_ptr()
+            err = _library().RMS_Norm(handle, x.data_ptr(), x_stride, r, r_stride, weight.data_ptr(), eps, N, K,
+                                      h.data_ptr() if added else None, h_stride, *((None, 0, at, width, scales.data_ptr()) if codes
+                                                                                  else (at, y_stride, None, 0, None)), kind)
+            if err:
+                _raise(err, name)
+        if codes:
+            return (y, scales, h) if added else (y, scales)
+        return (y, h) if added else y
 
-def _given(x, residual, weight, residual_out, out):
-    """Checked rows of outputs that a caller gives, None for those that are to be made."""
-    if residual is None and residual_out is not None:
-        raise ValueError("residual_out without a residual: h is x itself")
-    hr = None if residual_out is None else _out_rows("residual_out", residual_out, x, (x, residual))
-    yr = None if out is None else _out_rows("out", out, x, (x, residual), (residual_out,))
-    for name, t in (("out", out), ("residual_out", residual_out)):
-        if t is not None and _overlap(t, weight):
-            raise ValueError(f"{name} overlaps the weight")
-    return hr, yr
+    return _run(device, stream, call)
 
 
 def rms_norm(x, weight, eps=1e-5, residual=None, out=None, residual_out=None, stream=None):
@@ -150,24 +148,7 @@ def rms_norm(x, weight, eps=1e-5, residual=None, out=None, residual_out=None, st
 
     x, residual [tokens][K], fp16 or bf16, contiguous rows of any stride; weight [K] of that type.  Returns y, with a residual
     (y, h).  `out` and `residual_out` take y and h: new tensors by default; either may be x or the residual itself."""
-    xr, rr, kind, N, K = _norm_args(x, weight, eps, residual, 1 << 24)
-    hr, yr = (None, None) if residual_out is None and out is None else _given(x, residual, weight, residual_out, out)
-
-    def call(handle):
-        y, h, hrows, yrows = out, residual_out, hr or _NONE, yr
-        if y is None:
-            y = x.new_empty((N, K))
-            yrows = _Rows(y.data_ptr(), K)
-        if h is None and residual is not None:
-            h = x.new_empty((N, K))
-            hrows = _Rows(h.data_ptr(), K)
-        if N:
-            err = _library().RMS_Norm(handle, xr, rr, weight.data_ptr(), eps, N, K, hrows, yrows, None, kind)
-            if err:
-                _raise(err, "rms_norm")
-        return y if residual is None else (y, h)
-
-    return _run(x.device, stream, call)
+    return _norm("rms_norm", x, weight, eps, residual, residual_out, out, False, stream)
 
 
 def rms_norm_x8(x, weight, eps=1e-5, residual=None, residual_out=None, stream=None):
@@ -175,23 +156,7 @@ def rms_norm_x8(x, weight, eps=1e-5, residual=None, residual_out=None, stream=No
 
     codes int8 [tokens][K] (rows 16-byte aligned, in general a slice of wider ones), scales float32 [tokens];
     y ~ codes * scales.  What a W8Linear and a W8GatedLinear take."""
-    xr, rr, kind, N, K = _norm_args(x, weight, eps, residual, MAX_K)
-    hr = None if residual_out is None else _given(x, residual, weight, residual_out, None)[0]
-
-    def call(handle):
-        codes, width, scales = _new_codes(x, N, K)
-        h, hrows = residual_out, hr or _NONE
-        if h is None and residual is not None:
-            h = x.new_empty((N, K))
-            hrows = _Rows(h.data_ptr(), K)
-        if N:
-            err = _library().RMS_Norm(handle, xr, rr, weight.data_ptr(), eps, N, K, hrows, _NONE,
-                                      _Codes(codes.data_ptr(), width, scales.data_ptr()), kind)
-            if err:
-                _raise(err, "rms_norm_x8")
-        return (codes, scales) if residual is None else (codes, scales, h)
-
-    return _run(x.device, stream, call)
+    return _norm("rms_norm_x8", x, weight, eps, residual, residual_out, None, True, stream)
 
 
 def quantize_x8(x, stream=None):
@@ -199,13 +164,12 @@ def quantize_x8(x, stream=None):
     kind = _type(x.dtype)
     if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] > MAX_K or x.shape[0] >= 1 << 31 or x.device.type != "cuda":
         raise ValueError(f"x must be [tokens][K] on the GPU, K at most {MAX_K}")
-    xr = _rows("x", x, x.dtype, x.shape, x.device)
-    N, K = x.shape
+    stride, (N, K) = _rows("x", x, x.dtype, x.shape, x.device), x.shape
 
     def call(handle):
         codes, width, scales = _new_codes(x, N, K)
         if N:
-            err = _library().W8_Quantize(handle, xr, N, K, _Codes(codes.data_ptr(), width, scales.data_ptr()), kind)
+            err = _library().W8_Quantize(handle, x.data_ptr(), stride, N, K, codes.data_ptr(), width, scales.data_ptr(), kind)
             if err:
                 _raise(err, "quantize_x8")
         return codes, scales
@@ -238,8 +202,8 @@ def w8_pack(codes, scales, up_codes=None, up_scales=None, stream=None):
 
     def call(handle):
         packed = torch.empty(need, dtype=torch.uint8, device=device)
-        w = [_Weights(c.data_ptr(), K, s.data_ptr()) for c, s in pairs]
-        _raise(_library().W8_Pack(handle, w[0], w[1] if len(w) == 2 else None, M, K, packed.data_ptr()), "w8_pack")
+        w = [v for c, s in pairs for v in (c.data_ptr(), K, s.data_ptr())] + ([None, 0, None] if len(pairs) == 1 else [])
+        _raise(_library().W8_Pack(handle, *w, M, K, packed.data_ptr()), "w8_pack")
         return packed
 
     return _run(device, stream, call)
@@ -261,7 +225,7 @@ class _Product:
         for b in biases:
             if b is not None:
                 _check("bias", b, self.device, dtype, (M,))
-        self._kind = _TYPES[dtype]
+        self._kind, self._need = _TYPES[dtype], {}
 
     def bytes_per_call(self, N):
         """Bytes a call with N rows of 8-bit x must move: weights and scales, x and y."""
@@ -305,12 +269,16 @@ class _Product:
                 if scales is not None and not stride:
                     codes, width, _ = _new_codes(x, N, K)
                     codes.copy_(x)
-                need = L.W8_WorkspaceBytes(M, N, K, gated, scales is None)
+                need = self._need.get((N, scales is None))
+                if need is None:  # of the sizes alone: looked up once for each N that comes
+                    if len(self._need) >= 1024:
+                        self._need.clear()
+                    need = self._need[N, scales is None] = L.W8_WorkspaceBytes(M, N, K, gated, scales is None)
                 ws = self.packed.new_empty(need) if need else None
                 err = (L.W8_Gated if gated else L.W8_Linear)(
-                    handle, self.packed.data_ptr(), _Codes(codes.data_ptr(), width, None if scales is None else scales.data_ptr()),
-                    y.data_ptr(), M, N, K, *[None if b is None else b.data_ptr() for b in self.biases], self.activation, None if ws is None else ws.data_ptr(), need,
-                    self._kind)
+                    handle, self.packed.data_ptr(), codes.data_ptr(), width, None if scales is None else scales.data_ptr(),
+                    y.data_ptr(), M, N, K, *[None if b is None else b.data_ptr() for b in self.biases], self.activation,
+                    None if ws is None else ws.data_ptr(), need, self._kind)
                 if err:
                     _raise(err, type(self).__name__)
             return y

@@ -37,44 +37,40 @@ def test_no_kernel_spills(source):
         assert r["vgpr_spill"] == 0 and r["sgpr_spill"] == 0 and r["scratch_bytes"] == 0, (name, r)
 
 
-def rows(data=X, stride=64):
-    return M._Rows(data, stride)
+def norm(x=X, x_stride=64, residual=None, r_stride=64, weight=X, eps=1e-5, N=2, K=64, h=None, h_stride=64, y=X, y_stride=64, codes=None,
+         c_stride=64, scales=None, dtype=0):
+    return M._library().RMS_Norm(None, x, x_stride, residual, r_stride, weight, eps, N, K, h, h_stride, y, y_stride, codes, c_stride,
+                                 scales, dtype)
 
 
-def codes(data=X, stride=64, scales=X):
-    return M._Codes(data, stride, scales)
-
-
-def norm(x=rows(), residual=rows(None, 0), weight=X, eps=1e-5, N=2, K=64, h=rows(None, 0), y=rows(), c=None, dtype=0):
-    return M._library().RMS_Norm(None, x, residual, weight, eps, N, K, h, y, c, dtype)
+IN8 = dict(y=None, codes=X, scales=X)
 
 
 @pytest.mark.parametrize("kw", [
-    dict(x=rows(None)), dict(x=rows(X + 1)), dict(weight=None), dict(weight=X + 1), dict(residual=rows(X + 1)), dict(h=rows(X + 1)),
-    dict(y=rows(X + 1)), dict(h=rows(X, 63)), dict(y=rows(X, 63)), dict(eps=0.0), dict(eps=-1.0), dict(eps=float("nan")),
-    dict(eps=float("inf")), dict(eps=1e-21), dict(N=-1), dict(K=0), dict(K=(1 << 24) + 1), dict(dtype=2), dict(dtype=-1),
-    dict(y=rows(None, 0)), dict(c=codes()), dict(y=rows(None, 0), c=codes(X + 8)), dict(y=rows(None, 0), c=codes(stride=72)),
-    dict(y=rows(None, 0), c=codes(stride=48)), dict(y=rows(None, 0), c=codes(scales=X + 2)), dict(y=rows(None, 0), c=codes(scales=None)),
-    dict(y=rows(None, 0), c=codes(None)), dict(y=rows(None, 0), c=codes(), K=131072)])
+    dict(x=None), dict(x=X + 1), dict(weight=None), dict(weight=X + 1), dict(residual=X + 1), dict(h=X + 1), dict(y=X + 1),
+    dict(h=X, h_stride=63), dict(y_stride=63), dict(eps=0.0), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")),
+    dict(eps=1e-21), dict(N=-1), dict(K=0), dict(K=(1 << 24) + 1), dict(dtype=2), dict(dtype=-1), dict(y=None), dict(codes=X, scales=X),
+    dict(IN8, codes=X + 8), dict(IN8, c_stride=72), dict(IN8, c_stride=48), dict(IN8, scales=X + 2), dict(IN8, scales=None),
+    dict(IN8, codes=None), dict(IN8, K=131072), dict(IN8, c_stride=(1 << 28) + 16)])
 def test_norm_refuses(kw, capfd):
     assert norm(**kw) == BAD
     assert "Error" in capfd.readouterr().out
 
 
 def test_nothing_to_do_launches_nothing():
-    assert norm(N=0) == 0 and norm(N=0, x=rows(None), y=rows(None, 0), c=codes(None)) == 0
+    assert norm(N=0) == 0 and norm(N=0, x=None, y=None) == 0
     L = M._library()
-    assert L.W8_Quantize(None, rows(None), 0, 64, codes(None), 0) == 0
+    assert L.W8_Quantize(None, None, 64, 0, 64, None, 64, None, 0) == 0
     for f, b in ((L.W8_Linear, (None,)), (L.W8_Gated, (None, None))):
-        assert f(None, None, codes(None), None, 64, 0, 64, *b, 0, None, 0, 0) == 0
+        assert f(None, None, None, 64, None, None, 64, 0, 64, *b, 0, None, 0, 0) == 0
 
 
-@pytest.mark.parametrize("kw", [dict(x=rows(None)), dict(x=rows(X + 1)), dict(c=None), dict(c=codes(X + 8)), dict(c=codes(stride=40)),
-                                dict(c=codes(stride=32)), dict(c=codes(scales=None)), dict(N=-1), dict(K=0), dict(K=131072), dict(dtype=7)])
+@pytest.mark.parametrize("kw", [dict(x=None), dict(x=X + 1), dict(codes=None), dict(codes=X + 8), dict(c_stride=40), dict(c_stride=32),
+                                dict(scales=None), dict(scales=X + 1), dict(N=-1), dict(K=0), dict(K=131072), dict(dtype=7)])
 def test_quantize_refuses(kw, capfd):
-    a = dict(x=rows(), N=2, K=64, c=codes(), dtype=0)
+    a = dict(x=X, N=2, K=64, codes=X, c_stride=64, scales=X, dtype=0)
     a.update(kw)
-    assert M._library().W8_Quantize(None, a["x"], a["N"], a["K"], a["c"], a["dtype"]) == BAD
+    assert M._library().W8_Quantize(None, a["x"], 64, a["N"], a["K"], a["codes"], a["c_stride"], a["scales"], a["dtype"]) == BAD
     assert "Error" in capfd.readouterr().out
 
 
@@ -89,30 +85,29 @@ def test_sizes():
     assert L.W8_WorkspaceBytes(64, 3, 100, 0, 1) >= 3 * 112 + 12 and L.W8_WorkspaceBytes(64, 0, 100, 0, 1) == 0
 
 
-def product(gated=False, packed=X, x=codes(), Y=X, m=64, N=2, K=64, bias=None, act=0, ws=X, room=1 << 40, dtype=0):
+def product(gated=False, packed=X, x=X, stride=64, scales=X, Y=X, m=64, N=2, K=64, bias=None, act=0, ws=X, room=1 << 40, dtype=0):
     L = M._library()
     f = L.W8_Gated if gated else L.W8_Linear
-    return f(None, packed, x, Y, m, N, K, *((bias, None) if gated else (bias,)), act, ws, room, dtype)
+    return f(None, packed, x, stride, scales, Y, m, N, K, *((bias, None) if gated else (bias,)), act, ws, room, dtype)
 
 
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("kw", [
-    dict(packed=None), dict(packed=X + 8), dict(x=codes(None)), dict(x=codes(X + 8)), dict(x=codes(stride=40)), dict(x=codes(stride=48)),
-    dict(x=codes(scales=X + 2)), dict(Y=None), dict(Y=X + 1), dict(m=0), dict(m=(1 << 24) + 1), dict(K=0), dict(K=131072), dict(N=-1),
-    dict(N=16 * 65535 + 1), dict(bias=X + 1), dict(act=4), dict(act=-1), dict(dtype=2), dict(x=codes(X + 1, scales=None)),
-    dict(x=codes(scales=None), ws=None), dict(x=codes(scales=None), room=2 * 64), dict(x=codes(scales=None), ws=X + 8)])
+    dict(packed=None), dict(packed=X + 8), dict(x=None), dict(x=X + 8), dict(stride=40), dict(stride=48), dict(stride=(1 << 28) + 16),
+    dict(scales=X + 2), dict(Y=None), dict(Y=X + 1), dict(m=0), dict(m=(1 << 24) + 1), dict(K=0), dict(K=131072), dict(N=-1),
+    dict(N=16 * 65535 + 1), dict(bias=X + 1), dict(act=4), dict(act=-1), dict(dtype=2), dict(x=X + 1, scales=None),
+    dict(scales=None, ws=None), dict(scales=None, room=2 * 64), dict(scales=None, ws=X + 8)])
 def test_products_refuse(gated, kw, capfd):
     assert product(gated, **kw) == BAD
     assert "Error" in capfd.readouterr().out
 
 
 @pytest.mark.parametrize("kw", [dict(c=None), dict(s=X + 2), dict(s=None), dict(p=X + 8), dict(p=None), dict(stride=63), dict(m=0), dict(k=0),
-                                dict(k=131072), dict(up=(None, 64, X)), dict(up=(X, 63, X)), dict(up=(X, 64, X + 1))])
+                                dict(k=131072), dict(up=(X, 63, X)), dict(up=(X, 64, X + 1)), dict(up=(X, 64, None))])
 def test_pack_refuses(kw, capfd):
-    a = dict(c=X, s=X, p=X, stride=64, m=2, k=64, up=None)
+    a = dict(c=X, s=X, p=X, stride=64, m=2, k=64, up=(None, 0, None))
     a.update(kw)
-    up = None if a["up"] is None else M._Weights(*a["up"])
-    assert M._library().W8_Pack(None, M._Weights(a["c"], a["stride"], a["s"]), up, a["m"], a["k"], a["p"]) == BAD
+    assert M._library().W8_Pack(None, a["c"], a["stride"], a["s"], *a["up"], a["m"], a["k"], a["p"]) == BAD
     assert "Error" in capfd.readouterr().out
 
 

@@ -104,6 +104,7 @@ def test_many_tiles_of_a_workgroup(torch, set_plan, gated, kind, shares):
         first = layer(codes, scales)
         assert_close(first[:, :70], want[:, :70], bound[:, :70])
         assert set_plan(kind, 0, 0, shares) == 0
+        layer._need.clear()  # the workspace of another plan
         for _ in range(3):
             assert torch.equal(first, layer(codes, scales))
 
@@ -240,7 +241,6 @@ def test_workspace_is_what_the_call_asks_for(torch):
         need = L.W8_WorkspaceBytes(m, n, k, gated, x16)
         seen.add((need > 0, x16))
         if need:
-            c = M._Codes(1 << 20, 1 << 20, None if x16 else 1 << 20)
-            f = L.W8_Gated if gated else L.W8_Linear
-            assert f(None, 1 << 20, c, 1 << 20, m, n, k, *((None, None) if gated else (None,)), 0, 1 << 20, need - 1, 0) == 1
+            f, X = L.W8_Gated if gated else L.W8_Linear, 1 << 20
+            assert f(None, X, X, X, None if x16 else X, X, m, n, k, *((None, None) if gated else (None,)), 0, X, need - 1, 0) == 1
     assert (True, False) in seen and (False, False) in seen and (True, True) in seen
