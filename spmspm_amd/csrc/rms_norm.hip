@@ -22,36 +22,6 @@ struct NormArgs {
     float           eps;
 };
 
-// Eight elements of a row from e on; what lies behind its K is 0.  The row's end is taken by a whole vector too, the last one there
-// is, and moved down: no lane's loads wait for another's branch.
-__device__ __forceinline__ shortx8 load8(const uint16_t* row, int e, int K)
-{
-    if (K < 8) {
-        shortx8 v = 0;
-        for (int i = 0; i < 7; ++i)
-            if (e + i < K)
-                v[i] = row[e + i];
-        return v;
-    }
-    const int at = min(e, K - 8);
-    shortx8   v  = *reinterpret_cast<const loose8*>(row + at);
-    if (e > at) {
-        const int by = e - at;
-        uintx4    u  = __builtin_bit_cast(uintx4, v);
-        if (by & 2)
-            u = uintx4{u[1], u[2], u[3], 0};
-        if (by & 4)
-            u = uintx4{u[2], u[3], 0, 0};
-        if (by & 1)
-            for (int i = 0; i < 4; ++i)
-                u[i] = u[i] >> 16 | (i < 3 ? u[i + 1] << 16 : 0);
-        if (by >= 8)
-            u = 0;
-        v = __builtin_bit_cast(shortx8, u);
-    }
-    return v;
-}
-
 __device__ __forceinline__ void store8(uint16_t* p, shortx8 v, int left)
 {
     if (left >= 8) {
@@ -182,11 +152,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
         }
         inverse_rms = 1.f / sqrtf(mean + (unit == 1.f ? a.eps : 0.f)) * unit;
     }
-    const float m       = __uint_as_float(most);
-    const bool  bad     = QUANT && most >= 0x7f800000u, none = QUANT && (bad || m < kNoRow8);
-    const float inverse = none ? 0.f : 127.f / m;
+    const Row8 r8(most);
     if (QUANT && lane == 0)
-        a.scales[row] = bad ? NAN : (none ? 0.f : m / 127.f * inverse_rms);
+        a.scales[row] = r8.scale * inverse_rms;
 #pragma unroll kHeld
     for (int j = 0; j < n; ++j) {
         const int e = (j * kThreads + lane) * 8;
@@ -199,9 +167,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
         if constexpr (QUANT) {
             float t[8];
             for (int i = 0; i < 8; ++i)
-                t[i] = none ? 0.f : (NORM ? up<BF16>(v[i]) * up<BF16>(w[i]) : up<BF16>(v[i]));
+                t[i] = r8.none ? 0.f : (NORM ? up<BF16>(v[i]) * up<BF16>(w[i]) : up<BF16>(v[i]));
             // rows are readable, and here written, up to 16 bytes: the codes of the zeros behind the row are 0
-            *reinterpret_cast<uintx2*>(a.codes + row * a.c_stride + e) = codes8(t, m, inverse);
+            *reinterpret_cast<uintx2*>(a.codes + row * a.c_stride + e) = codes8(t, r8.m, r8.inverse);
         } else {
             shortx8 y;
             for (int i = 0; i < 8; ++i)

@@ -239,7 +239,10 @@ __global__ __launch_bounds__(256) void w8_join(ProductArgs a)
 // load and takes the operands' order in a corner of LDS that the wave has for itself (read in that order, 16 rows at once, a load
 // keeps the address unit four times as long: 2.3 us for every 16 columns of 5120).  A wave has D blocks of both in flight.  The
 // waves' sums meet in LDS.  A gated product has rows of the gate and of up in every workgroup: tiles t and t + 2 with R = 2.
+// X16: X holds 16-bit rows, eight at most, which every workgroup rounds to 8 bits for itself while its first blocks of W are on their
+// way: of few tokens that is less than a kernel before this one.
 constexpr int kNarrowWaves = 8;
+constexpr int kRows16      = 8;
 
 // What a wave wrote to LDS is there for its other lanes, and what they read may be written over: no instruction, the wave's
 // accesses keep their order.
@@ -250,10 +253,11 @@ __device__ __forceinline__ void wave_handoff8()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <bool GATED, int R, int NT, int D>
+template <bool GATED, int R, int NT, int D, bool X16>
 __global__ __launch_bounds__(64 * kNarrowWaves) void w8_narrow(ProductArgs a, int column_tiles)
 {
-    static_assert(!GATED || R >= 2);
+    static_assert((!GATED || R >= 2) && (!X16 || NT == 1));
+    __shared__ unsigned top[X16 ? kRows16 : 1][kNarrowWaves];
     __shared__ int   total[R * NT][kWave][4];
     __shared__ intx4 turned[kNarrowWaves][NT][2][kWave]; // X: 8 rows a KB, row r's chunk c at place 8 r + (c ^ r)
     const Layout8  l    = layout8(a.M, a.K, GATED);
@@ -264,19 +268,24 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void w8_narrow(ProductArgs a, in
     const int      last = (a.K - 1) / 16 * 16;
     for (int i = threadIdx.x; i < R * NT * kWave; i += 64 * kNarrowWaves)
         reinterpret_cast<intx4*>(total)[i] = 0;
-    __syncthreads();
+    if constexpr (!X16)
+        __syncthreads();
 
     const intx4*  w = reinterpret_cast<const intx4*>(a.packed + (int64_t)group * kGroup8) + first * 64 + lane;
     const int8_t* x[NT][2];
     for (int u = 0; u < NT; ++u) // rows behind the last are the last again
         for (int s = 0; s < 2; ++s)
-            x[u][s] = a.x + (int64_t)min(n0 + u * 16 + s * 8 + (lane >> 3), a.N - 1) * a.x_stride;
+            x[u][s] = a.x + (int64_t)min(n0 + u * 16 + s * 8 + (lane >> 3), a.N - 1) * a.x_stride * (X16 ? 2 : 1);
     struct Block {
-        intx4 w[2][R], x[NT][2];
+        intx4   w[2][R], x[X16 ? 1 : NT][2];
+        shortx8 x16[2];
     };
     Block held[D];
     auto  fetch = [&](Block& h, int block) {
-        for (int u = 0; u < NT; ++u) // behind the last 16 columns of X the weights are 0
+        if constexpr (X16)
+            for (int i = 0; i < 2; ++i)
+                h.x16[i] = load8(reinterpret_cast<const uint16_t*>(x[0][0]), block * 128 + 16 * (lane & 7) + 8 * i, a.K);
+        for (int u = 0; u < (X16 ? 0 : NT); ++u) // behind the last 16 columns of X the weights are 0
             for (int s = 0; s < 2; ++s)
                 h.x[u][s] = *reinterpret_cast<const intx4*>(x[u][s] + min(block * 128 + 16 * (lane & 7), last));
         for (int s = 0; s < 2; ++s)
@@ -290,12 +299,47 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void w8_narrow(ProductArgs a, in
     for (int d = 0; d < D; ++d)
         if (from + wave + d * kNarrowWaves < to)
             fetch(held[d], from + wave + d * kNarrowWaves);
+    Row8 mine{};
+    auto row8 = [&](int n) { // what the codes of row n are made with
+        unsigned bits = 0;
+        for (int w = 0; w < kNarrowWaves; ++w)
+            bits = max(bits, top[X16 ? n : 0][w]);
+        return Row8(bits);
+    };
+    if constexpr (X16) {
+        for (int n = 0; n < a.N; ++n) {
+            const uint16_t* row  = reinterpret_cast<const uint16_t*>(a.x) + n * a.x_stride;
+            unsigned        bits = 0; // of the largest magnitude: an infinity or a NaN is larger than every number
+            for (int e = threadIdx.x * 8; e < a.K; e += 512 * kNarrowWaves) {
+                const shortx8 v = load8(row, e, a.K);
+                for (int i = 0; i < 8; ++i)
+                    bits = max(bits, __float_as_uint(from16(v[i], a.bf16)) & 0x7fffffffu);
+            }
+            for (int d = 32; d > 0; d >>= 1)
+                bits = max(bits, (unsigned)__shfl_xor((int)bits, d));
+            if (lane == 0)
+                top[n][wave] = bits;
+        }
+        __syncthreads();
+        mine = row8(min(lane >> 3, a.N - 1));
+    }
     for (int block = from + wave; block < to;) {
 #pragma unroll
         for (int d = 0; d < D; ++d, block += kNarrowWaves) {
             if (block >= to)
                 break;
-            for (int u = 0; u < NT; ++u)
+            if constexpr (X16) { // columns past the eighth are not there: what they are multiplied by does not matter
+                uintx4 code;
+                for (int i = 0; i < 2; ++i) {
+                    float t[8];
+                    for (int j = 0; j < 8; ++j)
+                        t[j] = mine.none ? 0.f : from16(held[d].x16[i][j], a.bf16);
+                    const uintx2 c8 = codes8(t, mine.m, mine.inverse);
+                    code[2 * i] = c8[0], code[2 * i + 1] = c8[1];
+                }
+                turned[wave][0][0][(lane & 56) | ((lane & 7) ^ (lane >> 3))] = __builtin_bit_cast(intx4, code);
+            }
+            for (int u = 0; u < (X16 ? 0 : NT); ++u)
                 for (int s = 0; s < 2; ++s)
                     turned[wave][u][s][(lane & 56) | ((lane & 7) ^ (lane >> 3))] = held[d].x[u][s];
             wave_handoff8();
@@ -329,7 +373,7 @@ __global__ __launch_bounds__(64 * kNarrowWaves) void w8_narrow(ProductArgs a, in
     if (a.part != nullptr || n >= a.N)
         return;
     constexpr int W  = GATED ? 2 * R : (R == 1 ? 4 : 8); // consecutive outputs of a lane
-    const float   sx = a.x_scales[n];
+    const float   sx = X16 ? row8(n).scale : a.x_scales[n];
     const int     m  = GATED ? group * 32 + 8 * q + 4 * first : group * 64 + 16 * q + 4 * first;
     for (int i = 0; i < (GATED ? 1 : R * 4 / W); ++i)
         Tail8<GATED, W>(a, l, m + i * W).store(a, n, sx, v + i * W, v + 2 * R);
@@ -611,6 +655,7 @@ struct Plan8 {
     int kind;        // 0: w8_narrow, otherwise a w8_tiles of kTiles[kind - 1]
     int rows, cols;  // row and column tiles of 16 that a workgroup of w8_narrow takes
     int shares, per; // shares of K, blocks of 128 columns in each
+    bool x16;        // of w8_narrow: rows of 16 bits, which its workgroups round to 8 themselves
 };
 
 // What plan8 knows of the shapes of w8_tiles: a workgroup's row and column tiles, how many fit a CU, and in microseconds what a tile costs
@@ -624,7 +669,7 @@ constexpr Tiles8 kTiles[] = {{16, 16, 1, 2.7, 1.34, 0},    {8, 16, 1, 2.4, 0.78,
 constexpr int kShapes = sizeof kTiles / sizeof *kTiles;
 
 #ifdef SPMM_KEEP_VARIANTS
-Plan8 g_plan8{0, 0, 0, 0, 0};
+Plan8 g_plan8{};
 #endif
 
 int64_t up8(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -641,7 +686,7 @@ void share8(Plan8& p, int64_t blocks, int64_t shares)
 // bytes.  Examples, us: 5120x5120, N = 37 10.2 narrow with two row and three column tiles, 12.9 in tiles of 128 x 64;
 // 20480x5120, N = 64 25.6 in tiles of 128 x 64, 30.3 narrow; 9216x36864, N = 193 97 in tiles of 256 x 256 and seven shares of K,
 // 113 in tiles of 128 x 256 and three, 410 in one.
-Plan8 plan8(int M, int N, int K, bool gated)
+Plan8 choose8(int M, int N, int K, bool gated)
 {
     const Layout8 l      = layout8(M, K, gated);
     const int64_t blocks = l.steps / 2, tiles = (int64_t)l.groups * 4;
@@ -693,6 +738,20 @@ Plan8 plan8(int M, int N, int K, bool gated)
     return best;
 }
 
+// 16-bit rows are rounded within w8_narrow where few are read beside few weights: a call then is one launch and needs no workspace, 6.7
+// us of a Python caller's time instead of 10.7.  In a graph: 1024x1024, N = 1 4.1 us, 5.3 with a kernel before it; N = 8 7.3 and 6.7;
+// 5120x5120, N = 1 9.7 and 9.2, N = 4 12.0 and 10.0; 20480x5120, N = 1 27.7 and 21.5.  Not where K is in shares, whose sum another
+// kernel ends, with scales from memory.
+constexpr int64_t kMost16 = 8192, kMostWeights16 = 1 << 25;
+
+Plan8 plan8(int M, int N, int K, bool gated, bool x16)
+{
+    Plan8 p = choose8(M, N, K, gated);
+    p.x16   = x16 && p.kind == 0 && p.cols == 1 && p.shares == 1 && N <= kRows16 && (int64_t)N * K <= kMost16 &&
+            layout8(M, K, gated).scales <= kMostWeights16;
+    return p;
+}
+
 size_t part_bytes8(int M, int N, int K, bool gated, const Plan8& p)
 {
     return p.shares > 1 ? (size_t)p.shares * up8(N, 16) * layout8(M, K, gated).groups * 4096 : 0;
@@ -709,19 +768,21 @@ int run_tiles8(hipStream_t stream, ProductArgs a, int resident)
                   dim3(64 * WM * WN, 1, 1), stream, a);
 }
 
-template <bool GATED, int R, int NT, int D>
+template <bool GATED, int R, int NT, int D, bool X16 = false>
 int run_narrow8(hipStream_t stream, const ProductArgs& a)
 {
     const int     cols  = (int)up8(a.N, NT * 16);
     const int64_t units = (int64_t)layout8(a.M, a.K, GATED).groups * (4 / R) * cols;
     if (units > 0x7fffffff)
         return refuse("%lld tiles of outputs", (long long)units);
-    return launch(w8_narrow<GATED, R, NT, D>, dim3((unsigned)units, (unsigned)a.shares, 1), dim3(64 * kNarrowWaves, 1, 1), stream, a, cols);
+    return launch(w8_narrow<GATED, R, NT, D, X16>, dim3((unsigned)units, (unsigned)a.shares, 1), dim3(64 * kNarrowWaves, 1, 1), stream, a, cols);
 }
 
 template <bool GATED, int R>
 int run_narrow8(hipStream_t stream, const Plan8& p, const ProductArgs& a)
 {
+    if (p.x16)
+        return run_narrow8<GATED, R, 1, R == 4 ? 3 : 4, true>(stream, a);
     if (p.cols == 1)
         return run_narrow8<GATED, R, 1, R == 4 ? 3 : 4>(stream, a);
     if (p.cols == 2)
@@ -806,8 +867,8 @@ int run_product(hipStream_t stream, const void* packed, const void* x, int64_t x
         (up_bias != nullptr && bad_pointer(up_bias, 2)))
         return refuse("a null or misaligned weight (16 bytes), Y or bias (2)");
     const bool   x16 = x_scales == nullptr;
-    const Plan8  p   = plan8(M, N, K, gated);
-    const Space8 s   = space8(M, N, K, gated, x16, p);
+    const Plan8  p   = plan8(M, N, K, gated, x16);
+    const Space8 s   = space8(M, N, K, gated, x16 && !p.x16, p);
     if (x16 ? bad_pointer(x, 2) : bad_codes(x, x_stride, x_scales, N, K))
         return refuse("X null or misaligned (16-bit rows: 2 bytes; codes: 16, rows too, scales 4)");
     const size_t need = (size_t)s.bytes;
@@ -816,7 +877,7 @@ int run_product(hipStream_t stream, const void* packed, const void* x, int64_t x
     ProductArgs a{};
     a.packed = static_cast<const uint8_t*>(packed);
     a.x = static_cast<const int8_t*>(x), a.x_scales = x_scales, a.x_stride = x_stride;
-    if (x16) {
+    if (x16 && !p.x16) {
         int8_t* codes  = static_cast<int8_t*>(workspace) + s.codes;
         float*  scales = reinterpret_cast<float*>(static_cast<int8_t*>(workspace) + s.scales);
         if (int e = run_quantize(stream, x, x_stride, N, K, codes, s.stride, scales, dtype))
@@ -841,7 +902,7 @@ extern "C" int W8_Debug_SetPlan(int kind, int rows, int cols, int shares)
     if (kind < 0 || kind > kShapes || shares < 0 ||
         (kind == 0 && shares > 0 && ((rows != 1 && rows != 2 && rows != 4) || cols < 1 || cols > 4)))
         return 1;
-    g_plan8 = Plan8{kind, rows, cols, shares, 0};
+    g_plan8 = Plan8{kind, rows, cols, shares, 0, false};
     return 0;
 }
 #endif
@@ -874,7 +935,8 @@ extern "C" size_t W8_WorkspaceBytes(int M, int N, int K, int gated, int x16)
 {
     if (W8_PackedBytes(M, K, gated) == 0 || N < 1 || N > kMaxN8)
         return 0;
-    return (size_t)space8(M, N, K, gated != 0, x16 != 0, plan8(M, N, K, gated != 0)).bytes;
+    const Plan8 p = plan8(M, N, K, gated != 0, x16 != 0);
+    return (size_t)space8(M, N, K, gated != 0, x16 != 0 && !p.x16, p).bytes;
 }
 
 extern "C" int W8_Linear(hipStream_t stream, const void* packed, const void* x, int64_t x_stride, const float* x_scales, void* Y, int M,

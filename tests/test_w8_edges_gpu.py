@@ -244,3 +244,24 @@ def test_workspace_is_what_the_call_asks_for(torch):
             f, X = L.W8_Gated if gated else L.W8_Linear, 1 << 20
             assert f(None, X, X, X, None if x16 else X, X, m, n, k, *((None, None) if gated else (None,)), 0, X, need - 1, 0) == 1
     assert (True, False) in seen and (False, False) in seen and (True, True) in seen
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("K", [1, 7, 8, 9, 100, 127, 129, 1000, 2048, 5120, 13696])
+@pytest.mark.parametrize("N", [1, 2, 3, 8, 9])
+def test_16_bit_rows_are_rounded_alike_inside_and_outside(torch, dtype, K, N):
+    """Few rows are rounded by the product's own workgroups: the same bits as of codes made before, rows of every kind among them."""
+    kind = torch.float16 if dtype == "fp16" else torch.bfloat16
+    wide = torch.randn((N, K + 3), generator=torch.Generator(device="cuda").manual_seed(K), device="cuda").to(kind)
+    x = wide[:, 1:K + 1]  # rows at odd places
+    for turn in range(2):
+        if turn:
+            x[0, K - 1] = float("inf")
+            x[N - 1] = torch.finfo(kind).tiny
+            if N > 2:
+                x[1, 0], x[2] = float("nan"), 0
+        for M_ in (40, 700):
+            w, g, u = (weights(torch, M_, K, i) for i in range(3))
+            for layer in (S.W8Linear(*w, activation=A.ACT_GELU, dtype=kind), S.W8GatedLinear(*g, *u, dtype=kind)):
+                got, want = layer(x), layer(*S.quantize_x8(x))
+                assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(7), want.nan_to_num(7))
