@@ -178,12 +178,15 @@ def quantize_x8(x, stream=None):
 
 
 def quantize_w8(weight):
-    """Round a [M][K] weight to 8 bits: codes int8 [M][K] (-127..127), scales float32 [M], weight ~ scale * code.  Plain torch
-    operations, on any device."""
+    """Round a [M][K] weight to 8 bits: codes int8 [M][K] (-127..127), scales float32 [M], weight ~ scale * code.  A row with an
+    infinity or a NaN has codes 0 and scale NaN.  Plain torch operations, on any device."""
     w = weight.float()
     scales = w.abs().amax(-1) / 127
+    whole = torch.isfinite(scales)
     scales = torch.where(scales > 2.0 ** -100, scales, torch.ones_like(scales))  # a row of zeros
-    return torch.round(w / scales[:, None]).clamp(-127, 127).to(torch.int8), scales
+    codes = torch.round(w / scales[:, None]).clamp(-127, 127)
+    return (torch.where(whole[:, None], codes, torch.zeros_like(codes)).to(torch.int8),
+            torch.where(whole, scales, torch.full_like(scales, float("nan"))))
 
 
 def w8_pack(codes, scales, up_codes=None, up_scales=None, stream=None):

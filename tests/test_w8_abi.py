@@ -131,6 +131,18 @@ def test_quantize_w8_rounds_to_half_a_step():
     assert (off[:3] <= scales.double()[:3, None] * (0.5 + 127 * 2.0 ** -23)).all() and off[4].max() < 2e-38
 
 
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_quantize_w8_keeps_a_broken_row_broken(value, dtype):
+    w = torch.randn((4, 70), generator=torch.Generator().manual_seed(1)).to(dtype)
+    want, scales = S.quantize_w8(w)
+    w[2, 69] = value
+    codes8, got = S.quantize_w8(w)
+    assert (codes8[2] == 0).all() and got[2].isnan() and got.dtype == torch.float32
+    for m in (0, 1, 3):
+        assert torch.equal(codes8[m], want[m]) and got[m] == scales[m]
+
+
 def test_oracle_codes_are_the_nearest():
     rng = np.random.default_rng(0)
     t = rng.standard_normal((50, 400)).astype(np.float32)
