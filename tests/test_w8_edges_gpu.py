@@ -65,14 +65,11 @@ def assert_close(got, want, bound):
 SIZES = [(33, 100, 5), (300, 1100, 70), (129, 4100, 300), (520, 640, 17)]
 
 
-@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("gated,rows", [(False, 1), (False, 2), (False, 4), (True, 2), (True, 4)])
 @pytest.mark.parametrize("size", SIZES)
-@pytest.mark.parametrize("rows", [1, 2, 4])
 @pytest.mark.parametrize("cols", [1, 2, 3, 4])
 @pytest.mark.parametrize("shares", [1, 3])
 def test_narrow_kernels(torch, set_plan, gated, size, rows, cols, shares):
-    if gated and rows == 1:
-        pytest.skip("rows of the gate and of up come in pairs of tiles")
     assert set_plan(0, rows, cols, shares) == 0
     layer, codes, scales, want, bound = products(torch, gated, *size)
     got = layer(codes, scales)
