@@ -163,6 +163,31 @@ def test_more_rows_than_a_launch_has_threads_for(torch):
         assert torch.equal(c[part], one[0]) and torch.equal(s[part], one[1])
 
 
+@pytest.mark.parametrize("M_,K,N", [(1 << 24, 1, 1), (1 << 24, 2, 19), (1, M.MAX_K, 1), (5, M.MAX_K, 300), (1, 1, 16 * 65535), (33, 40, 16 * 65535)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_the_largest_sizes(torch, M_, K, N, gated):
+    """Against sums in float64, which are exact, on the GPU."""
+    pairs = [weights(torch, M_, K, i) for i in range(2 if gated else 1)]
+    codes, scales = rows8(torch, N, K, 3)
+    layer = S.W8GatedLinear(*pairs[0], *pairs[1], activation=A.ACT_NONE) if gated else S.W8Linear(*pairs[0])
+    y = layer(codes, scales)
+    assert y.shape == (N, M_)
+    for n in range(0, N, 1 << 16):
+        part = slice(n, min(N, n + (1 << 16)))
+        want = 1
+        for w, sw in pairs:
+            want = want * ((codes[part].double() @ w.double().t()) * sw.double()) * scales[part].double()[:, None]
+        # of a sum its conversion and two products, the gate's product, the rounding to 16 bits, there subnormal too
+        bound = (2.0 ** -11 + 7 * 2.0 ** -24) * want.abs() * (1 + 2.0 ** -11) + 2.0 ** -25
+        assert ((y[part].double() - want).abs() <= bound).all()
+    if N == 1:  # the norm's longest row
+        x = torch.randn((1, 1 << 24), device="cuda").bfloat16()
+        got = S.rms_norm(x, torch.ones_like(x[0]))
+        want = x.double() / (x.double().square().mean() + 1e-5).sqrt()
+        # 2^24 squares summed by 1024 lanes, 2^14 each: 2^14 + 16 roundings in the worst order, half of that behind the root
+        assert ((got.double() - want).abs() <= (2.0 ** -8 + (2 ** 13 + 20) * 2.0 ** -24) * want.abs()).all()
+
+
 def test_host_layer_refusals(torch):
     x, w = torch.zeros((4, 64), device="cuda").half(), torch.ones(64, device="cuda").half()
     c, s = S.quantize_x8(x)
