@@ -105,19 +105,21 @@ __device__ __forceinline__ ProductArgs late_args8()
 }
 
 // ReLU, GELU (tanh form) or SiLU of W sums.  The last two are y / (1 + exp(-z)), with z = 2 sqrt(2/pi) (y + 0.044715 y^3), since
-// (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), or z = y; far from 0 they end at 0 and y.  The reciprocal's last bit is far below 16 bits.
+// (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), or z = y; far from 0 they end at 0 and y.  The exponential is one of 2, with -log2(e) in z's
+// coefficients; the reciprocal's last bit is far below 16 bits.
 template <int W>
 __device__ __forceinline__ void activate8(float* y, int act)
 {
+    constexpr float kLog2e = 1.4426950408889634f, kOne = -kLog2e * 1.5957691216057308f, kCube = kOne * 0.044715f;
     if (act == 1) {
         for (int i = 0; i < W; ++i)
             y[i] = y[i] < 0.f ? 0.f : y[i]; // a NaN stays one
-    } else if (act > 1) {
-        const float cube = act == 2 ? 1.5957691216057308f * 0.044715f : 0.f, one = act == 2 ? 1.5957691216057308f : 1.f;
-        for (int i = 0; i < W; ++i) {
-            const float z = y[i] * (one + cube * y[i] * y[i]);
-            y[i]          = y[i] * __builtin_amdgcn_rcpf(1.f + __expf(-z));
-        }
+    } else if (act == 2) {
+        for (int i = 0; i < W; ++i)
+            y[i] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y[i] * (kOne + kCube * y[i] * y[i])));
+    } else if (act == 3) {
+        for (int i = 0; i < W; ++i)
+            y[i] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * y[i]));
     }
 }
 
@@ -171,18 +173,25 @@ struct Tail8 {
         }
     }
 
-    // The end of the sums of column n, of its row of X the scale sx; `up` is read by gated products only.
-    __device__ __forceinline__ void store(const ProductArgs& a, int n, float sx, const int* sum, const int* up) const
+    // What a column's sums, of the gate in a gated product, are ahead of the activation; sx is the scale of its row of X.
+    __device__ __forceinline__ void scale(float* y, const int* sum, float sx) const
+    {
+        for (int i = 0; i < W; ++i)
+            y[i] = (float)sum[i] * sw[i] * sx + b[i];
+    }
+
+    // The gate's times the sums of up.
+    __device__ __forceinline__ void times(float* y, const int* up, float sx) const
+    {
+        for (int i = 0; i < W; ++i)
+            y[i] *= (float)up[i] * su[i] * sx + bu[i];
+    }
+
+    // Into column n.
+    __device__ __forceinline__ void put(const ProductArgs& a, int n, const float* y) const
     {
         if (left <= 0)
             return;
-        float y[W];
-        for (int i = 0; i < W; ++i)
-            y[i] = (float)sum[i] * sw[i] * sx + b[i];
-        activate8<W>(y, a.act);
-        if constexpr (GATED)
-            for (int i = 0; i < W; ++i)
-                y[i] *= (float)up[i] * su[i] * sx + bu[i];
         typename Loose<W>::type out;
         if (a.bf16)
             for (int i = 0; i < W; ++i)
@@ -198,6 +207,19 @@ struct Tail8 {
         for (int i = 0; i < W - 1; ++i)
             if (i < left)
                 to[i] = out[i];
+    }
+
+    // The three of one column; `up` is read by gated products only.
+    __device__ __forceinline__ void store(const ProductArgs& a, int n, float sx, const int* sum, const int* up) const
+    {
+        if (left <= 0)
+            return;
+        float y[W];
+        scale(y, sum, sx);
+        activate8<W>(y, a.act);
+        if constexpr (GATED)
+            times(y, up, sx);
+        put(a, n, y);
     }
 };
 
@@ -445,7 +467,7 @@ __device__ __forceinline__ void place8(const ProductArgs& a, int id, int& row, i
 // loaded while the results of the last are written, and a tile costs its products alone.
 // Measured in tiles of 256 x 256: 8192 x 8192 x 8192 398 us, 2760 TOP/s, the matrix cores busy for 65 % of the cycles at 2.0 GHz; with
 // operands of zeros 337 us, 3260 TOP/s at a clock that is not throttled; products alone, from registers, reach 4000 TOP/s on random
-// codes.  20480 x 5120 with 4096 columns 354 us, 2430 TOP/s.  Lines that the next die-mates miss, brought ahead into L2, help
+// codes.  20480 x 5120 with 4096 columns 339 us, 2530 TOP/s.  Lines that the next die-mates miss, brought ahead into L2, help
 // operands of zeros (338 -> 312) and not others (400 -> 406).  Rings of steps of 64 436, four waves of 128 x 128 each 764 (the
 // accumulators are moved about).
 template <bool GATED, int MT, int NT, int WM, int WN, int S>
@@ -618,20 +640,37 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs args)
             place8(a, now, row, column, share);
             const Ends& e = ends[turn % kEnds];
             if (a.part == nullptr) {
+                constexpr int kEnd = 2;
+                // A group's rows at a time, whose scales and biases are read once, and two columns of tiles: their steps hide each other's latency
+                // (gated 24960x256, N = 4917 187 us one by one, 154 so).  For more there are not registers enough.
                 each<MT / 4>([&](auto g) {
                     const int group = wm * (MT / 4) + g;
                     each<GATED ? 1 : 2>([&](auto h) {
                         const int j = GATED ? group * 32 + 8 * q : group * 64 + 16 * q + 8 * h;
-                        each<NT>([&](auto u) {
-                            const int n = column * kN + (wn * NT + u) * 16 + c;
-                            if (n >= a.N)
-                                return;
-                            asm volatile("" ::: "memory"); // scales and biases once more, rather than in registers there are not enough of
-                            const Tail8<GATED, 8> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
-                            int v[16];
-                            for (int i = 0; i < 16; ++i)
-                                v[i] = sum[g * 4 + i / 4][u][i % 4];
-                            tail.store(a, n, e.sx[(wn * NT + u) * 16 + c], v + 8 * h, v + 8);
+                        asm volatile("" ::: "memory");
+                        const Tail8<GATED, 8> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
+                        each<NT / kEnd>([&](auto part) {
+                            float y[kEnd][8], sx[kEnd];
+                            int   v[8];
+                            auto  of = [&](auto first, auto u) { // eight sums, from row tile `first` of the group on
+                                for (int i = 0; i < 8; ++i)
+                                    v[i] = sum[g * 4 + first + i / 4][part * kEnd + u][i % 4];
+                            };
+                            each<kEnd>([&](auto u) {
+                                sx[u] = e.sx[(wn * NT + part * kEnd + u) * 16 + c];
+                                of(std::integral_constant<int, 2 * h>(), u);
+                                tail.scale(y[u], v, sx[u]);
+                            });
+                            activate8<8 * kEnd>(y[0], a.act);
+                            each<kEnd>([&](auto u) {
+                                if constexpr (GATED) {
+                                    of(std::integral_constant<int, 2>(), u);
+                                    tail.times(y[u], v, sx[u]);
+                                }
+                                const int n = column * kN + (wn * NT + part * kEnd + u) * 16 + c;
+                                if (n < a.N)
+                                    tail.put(a, n, y[u]);
+                            });
                         });
                     });
                 });
