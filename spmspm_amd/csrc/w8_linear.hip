@@ -650,7 +650,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs args)
                         asm volatile("" ::: "memory");
                         const Tail8<GATED, 8> tail(a, row * (GATED ? kM / 2 : kM) + j, e.sw + j, e.b + j, kM / 2);
                         each<NT / kEnd>([&](auto part) {
-                            float y[kEnd][8], sx[kEnd];
+                            float y[8 * kEnd], sx[kEnd];
                             int   v[8];
                             auto  of = [&](auto first, auto u) { // eight sums, from row tile `first` of the group on
                                 for (int i = 0; i < 8; ++i)
@@ -659,17 +659,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void w8_tiles(ProductArgs args)
                             each<kEnd>([&](auto u) {
                                 sx[u] = e.sx[(wn * NT + part * kEnd + u) * 16 + c];
                                 of(std::integral_constant<int, 2 * h>(), u);
-                                tail.scale(y[u], v, sx[u]);
+                                tail.scale(y + 8 * u, v, sx[u]);
                             });
-                            activate8<8 * kEnd>(y[0], a.act);
+                            activate8<8 * kEnd>(y, a.act);
                             each<kEnd>([&](auto u) {
                                 if constexpr (GATED) {
                                     of(std::integral_constant<int, 2>(), u);
-                                    tail.times(y[u], v, sx[u]);
+                                    tail.times(y + 8 * u, v, sx[u]);
                                 }
                                 const int n = column * kN + (wn * NT + part * kEnd + u) * 16 + c;
                                 if (n < a.N)
-                                    tail.put(a, n, y[u]);
+                                    tail.put(a, n, y + 8 * u);
                             });
                         });
                     });
