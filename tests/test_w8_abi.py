@@ -167,3 +167,18 @@ def test_oracle_rounds_once_to_16_bits():
     assert (np.abs(got - x) <= np.abs(want - x)).all() and (got == want).mean() > 0.999
     assert np.array_equal(O.round16(x, False), x.astype(np.float16).astype(np.float64))
     assert np.isnan(O.round16(np.array([np.nan]), True)[0]) and O.round16(np.array([np.inf]), True)[0] == np.inf
+
+
+@pytest.mark.parametrize("gated", [0, 1])
+def test_room_for_rounded_rows_beside_shares_of_k(gated):
+    """The kernel that adds up shares of K reads the rows' scales from memory: 16-bit rows then have codes and scales in the workspace,
+    however few they are."""
+    L, split = M._library(), 0
+    for m in (1, 40, 256, 576, 5120, 20480):
+        for n in (1, 2, 5, 8, 40, 193):
+            for k in list(range(128, 8193, 128)) + [16384, 36864]:
+                part = L.W8_WorkspaceBytes(m, n, k, gated, 0)
+                if part:
+                    split += n * k <= 8192
+                    assert L.W8_WorkspaceBytes(m, n, k, gated, 1) >= part + n * (k + 4)
+    assert split > 0 or not gated  # some of them few enough to be rounded where they are read

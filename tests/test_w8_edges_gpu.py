@@ -287,3 +287,38 @@ def test_16_bit_rows_are_rounded_alike_inside_and_outside(torch, dtype, K, N):
             for layer in (S.W8Linear(*w, activation=A.ACT_GELU, dtype=kind), S.W8GatedLinear(*g, *u, dtype=kind)):
                 got, want = layer(x), layer(*S.quantize_x8(x))
                 assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(7), want.nan_to_num(7))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("M_,K", [(1, 6208), (256, 7168), (576, 8192)])
+def test_one_16_bit_row_with_k_in_shares(torch, dtype, M_, K):
+    """Few enough to be rounded by the product's workgroups, but the kernel that adds up the shares reads the scale from memory: rounded
+    by a kernel before the product."""
+    kind = torch.float16 if dtype == "fp16" else torch.bfloat16
+    assert K <= 8192 and M._library().W8_WorkspaceBytes(M_, 1, K, 1, 0) > 0
+    g, u = weights(torch, M_, K, 1), weights(torch, M_, K, 2)
+    layer, x = S.W8GatedLinear(*g, *u, dtype=kind), torch.randn((1, K), device="cuda").to(kind)
+    codes, scales = S.quantize_x8(x)
+    got, n = layer(x), lambda t: t.cpu().numpy()
+    want, bound = O.gated(n(codes), n(scales), n(g[0]), n(g[1]), n(u[0]), n(u[1]))
+    half = 2.0 ** (-11 if dtype == "fp16" else -8)
+    assert (np.abs(got.double().cpu().numpy() - want) <= half * np.abs(want) + 1.01 * bound + 2.0 ** -25).all()
+    assert torch.equal(got, layer(codes, scales))
+
+
+@pytest.mark.parametrize("gated,rows", [(False, 1), (False, 2), (False, 4), (True, 2), (True, 4)])
+@pytest.mark.parametrize("N", [1, 3, 8])
+def test_few_16_bit_rows_with_k_in_shares(torch, set_plan, gated, rows, N):
+    """The same of every kernel that rounds rows itself where K is whole."""
+    assert set_plan(0, rows, 1, 3) == 0
+    M_, K = 150, 650
+    pairs = [weights(torch, M_, K, i) for i in range(2 if gated else 1)]
+    layer = S.W8GatedLinear(*pairs[0], *pairs[1]) if gated else S.W8Linear(*pairs[0], activation=A.ACT_GELU)
+    assert M._library().W8_WorkspaceBytes(M_, N, K, gated, 0) > 0
+    x = torch.randn((N, K), device="cuda").half()
+    codes, scales = S.quantize_x8(x)
+    n = lambda t: t.cpu().numpy()
+    want, bound = O.gated(n(codes), n(scales), *[n(t) for p in pairs for t in p]) if gated else \
+        O.linear(n(codes), n(scales), *[n(t) for t in pairs[0]], act=A.ACT_GELU)
+    assert_close(layer(x), want, bound)
+    assert torch.equal(layer(x), layer(codes, scales))
