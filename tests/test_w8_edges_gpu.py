@@ -322,3 +322,39 @@ def test_few_16_bit_rows_with_k_in_shares(torch, set_plan, gated, rows, N):
         O.linear(n(codes), n(scales), *[n(t) for t in pairs[0]], act=A.ACT_GELU)
     assert_close(layer(x), want, bound)
     assert torch.equal(layer(x), layer(codes, scales))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M_,N", [(300, 90), (700, 193), (40, 5)])
+def test_shares_of_k_in_two_graphs_and_an_eager_call_at_once(torch, gated, M_, N):
+    """Sums that go through memory to a second kernel: recorded calls of one layer, replayed on two streams beside eager calls on a
+    third, have a workspace each."""
+    K = 36864
+    assert M._library().W8_WorkspaceBytes(M_, N, K, gated, 0) > 0
+    pairs = [weights(torch, M_, K, i) for i in range(2 if gated else 1)]
+    layer = S.W8GatedLinear(*pairs[0], *pairs[1]) if gated else S.W8Linear(*pairs[0])
+    xs = [rows8(torch, N, K, 10 + i) for i in range(3)]
+    want = [layer(*x) for x in xs]
+    assert not torch.equal(want[0], want[1])
+    n = lambda t: t.cpu().numpy()
+    exact, bound = (O.gated if gated else O.linear)(n(xs[0][0]), n(xs[0][1]), *[n(t) for p in pairs for t in p])
+    assert_close(want[0], exact, bound)
+    graphs, outs = [], []
+    for x in xs[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(layer(*x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for turn in range(5):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for s, g in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+            with torch.cuda.stream(streams[2]):
+                eager = layer(*xs[2])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
