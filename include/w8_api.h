@@ -13,7 +13,7 @@
  *   scale = m / 127, or m / 127 / rms where the norm below writes it
  * m below 2^-100: a row of zeros, codes and scale 0.  A row with an infinity or a NaN has codes 0 and scale NaN, and so NaN in
  * all that is computed from it.  Rows lie `stride` bytes apart, a multiple of 16, at most 2^28, 16-byte aligned, each readable up to K rounded
- * up to 16 bytes; what the bytes behind K hold does not matter.
+ * up to 16 bytes where a product reads them; what the bytes behind K hold does not matter.  What writes rows writes K bytes of each.
  */
 #ifndef W8_API_H
 #define W8_API_H

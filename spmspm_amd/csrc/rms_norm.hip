@@ -157,6 +157,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
     const Row8 r8(most);
     if (QUANT && lane == 0)
         a.scales[row] = r8.scale * inverse_rms;
+    int8_t* codes = a.codes + row * a.c_stride;
+    uintx2  end   = 0; // codes of the vector that the row ends in
 #pragma unroll kHeld
     for (int j = 0; j < n; ++j) {
         const int e = (j * kThreads + lane) * 8;
@@ -170,8 +172,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
             float t[8];
             for (int i = 0; i < 8; ++i)
                 t[i] = r8.none ? 0.f : (NORM ? up<BF16>(v[i]) * up<BF16>(w[i]) : up<BF16>(v[i]));
-            // rows are readable, and here written, up to 16 bytes: the codes of the zeros behind the row are 0
-            *reinterpret_cast<uintx2*>(a.codes + row * a.c_stride + e) = codes8(t, r8.m, r8.inverse);
+            const uintx2 c = codes8(t, r8.m, r8.inverse);
+            if (e + 8 <= a.K)
+                *reinterpret_cast<uintx2*>(codes + e) = c;
+            else
+                end = c;
         } else {
             shortx8 y;
             for (int i = 0; i < 8; ++i)
@@ -179,6 +184,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
             store8(a.y + row * a.y_stride + e, y, a.K - e);
         }
     }
+    // What a caller keeps behind a row's codes stays.
+    if (QUANT && a.K % 8 != 0 && lane == a.K / 8 % kThreads)
+        for (int i = 0; i < 7; ++i)
+            if (i < a.K % 8)
+                codes[a.K / 8 * 8 + i] = (int8_t)(end[i / 4] >> (8 * (i % 4)));
 }
 
 template <bool BF16, bool NORM, bool QUANT, int WAVES, int V>

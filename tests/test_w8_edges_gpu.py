@@ -358,3 +358,28 @@ def test_shares_of_k_in_two_graphs_and_an_eager_call_at_once(torch, gated, M_, N
                 eager = layer(*xs[2])
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
+
+
+@pytest.mark.parametrize("K", [1, 7, 8, 9, 100, 520, 1027, 5121, 9210, 33001, 70001])
+@pytest.mark.parametrize("N", [1, 5, 300])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_bytes_behind_a_rows_codes_stay(torch, K, N, dtype):
+    """What a caller keeps between K and the stride, behind the last row too, is there afterwards."""
+    if N * K > 1 << 21:
+        N = 2
+    kind, L = (torch.float16, torch.bfloat16)[dtype], M._library()
+    x, w = torch.randn((N, K), device="cuda").to(kind), torch.rand(K, device="cuda").to(kind)
+    stride = (K + 15) // 16 * 16 + 16
+    scales, stream = torch.empty(N, device="cuda"), torch.cuda.current_stream().cuda_stream
+    for norm in (False, True):
+        room = torch.full((N + 1, stride), 77, dtype=torch.int8, device="cuda")
+        if norm:
+            err = L.RMS_Norm(stream, x.data_ptr(), K, None, 0, w.data_ptr(), 1e-5, N, K, None, 0, None, 0, room.data_ptr(), stride,
+                             scales.data_ptr(), dtype)
+        else:
+            err = L.W8_Quantize(stream, x.data_ptr(), K, N, K, room.data_ptr(), stride, scales.data_ptr(), dtype)
+        assert err == 0
+        t = x.double().cpu().numpy().astype(np.float32)
+        want, _ = O.encode(t * w.double().cpu().numpy().astype(np.float32) if norm else t)
+        assert np.array_equal(room[:N, :K].cpu().numpy(), want)
+        assert (room[:, K:] == 77).all() and (room[N] == 77).all()
