@@ -96,14 +96,22 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
     };
     float    squares = 0.f;
     unsigned most    = 0; // bits of max |t|: an infinity or a NaN is larger than every number
-    auto     take    = [&](shortx8 v, shortx8 w) {
+    auto     take    = [&](float& sum, shortx8 v, shortx8 w) {
         for (int i = 0; i < 8; ++i) {
             const float f = up<BF16>(v[i]), t = NORM ? f * up<BF16>(w[i]) : f;
             if (NORM)
-                squares = __builtin_fmaf(f, f, squares);
+                sum = __builtin_fmaf(f, f, sum);
             if (QUANT)
                 most = max(most, __float_as_uint(t) & 0x7fffffffu);
         }
+    };
+    // Rows that are read twice have up to 2048 vectors a lane: sums of vectors, of 32 of those, and of these, since in one sum the
+    // roundings of thousands of additions of like numbers go one way (2^24 of them: off by 2.4e-4).
+    float sums = 0.f;
+    auto  fold = [&](float& total, float sum, int j) {
+        sums += sum;
+        if (j % 32 == 31 || j == n - 1)
+            total += sums, sums = 0.f;
     };
 #pragma unroll kHeld
     for (int j = 0; j < n; ++j) {
@@ -116,13 +124,16 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
         }
         if (NORM && a.h != nullptr && e < a.K)
             store8(h + e, held[k], a.K - e);
-        if (V == 0)
-            take(held[0], gain[0]);
+        if (V == 0) {
+            float sum = 0.f;
+            take(sum, held[0], gain[0]);
+            fold(squares, sum, j);
+        }
     }
     if (V > 0) { // behind all loads: h may take x's place
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            take(held[j], gain[j]);
+            take(squares, held[j], gain[j]);
         }
     }
     // The row once more, for rows that are not held: h where it was written (it may have taken x's place), x and the residual otherwise.
@@ -140,14 +151,19 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void rms_norm(Nor
             float    small = 0.f;
             unsigned none  = 0;
             for (int j = 0; j < n; ++j) {
-                const int e = (j * kThreads + lane) * 8;
+                const int e   = (j * kThreads + lane) * 8;
+                float     sum = V > 0 ? small : 0.f;
                 if (e < a.K) {
                     const shortx8 v = again(j, e);
                     for (int i = 0; i < 8; ++i) {
                         const float f = up<BF16>(v[i]) * 0x1p-96f;
-                        small         = __builtin_fmaf(f, f, small);
+                        sum           = __builtin_fmaf(f, f, sum);
                     }
                 }
+                if (V > 0)
+                    small = sum;
+                else
+                    fold(small, sum, j);
             }
             reduce<WAVES>(small, none, sum, top, 1);
             mean = small / (float)a.K, unit = 0x1p-96f;

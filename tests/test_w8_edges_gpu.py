@@ -383,3 +383,28 @@ def test_bytes_behind_a_rows_codes_stay(torch, K, N, dtype):
         want, _ = O.encode(t * w.double().cpu().numpy().astype(np.float32) if norm else t)
         assert np.array_equal(room[:N, :K].cpu().numpy(), want)
         assert (room[:, K:] == 77).all() and (room[N] == 77).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("K", [32776, 131071, 1 << 20, 1 << 24])
+@pytest.mark.parametrize("factor", [1.0, 2.0 ** 70])
+def test_the_sum_of_squares_of_a_long_row(torch, dtype, K, factor):
+    """Rows of nearly equal numbers, whose roundings in a sum all go one way: seven of eight are 1.40625, the eighth is any.  Of a row that
+    is read twice a lane adds eight squares, 32 such sums and up to 64 of those, and 22 lanes and waves follow: 126 roundings of
+    2^-24, half of them behind the root, and six operations, below 2^-17.  2^70: squares that leave float32 and are summed again."""
+    if factor > 1 and dtype == "fp16":
+        factor = 2.0 ** 4
+    kind, half = (torch.float16, 2.0 ** -11) if dtype == "fp16" else (torch.bfloat16, 2.0 ** -8)
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.full((2, K), 1.40625 * factor, device="cuda")
+    x[:, ::8] = (1 + torch.rand((2, (K + 7) // 8), generator=gen, device="cuda")) * factor
+    x = x.to(kind)
+    w = torch.ones(K, device="cuda").to(kind)
+    rms = (x.double().square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    want = x.double() / rms
+    got = S.rms_norm(x, w)
+    assert ((got.double() - want).abs() <= (half + 2.0 ** -17) * want).all()
+    if K <= M.MAX_K:
+        codes, scales = S.rms_norm_x8(x, w)
+        want = x.double().amax(-1) / 127 / rms[:, 0]
+        assert ((scales.double() - want).abs() <= (2.0 ** -24 + 2.0 ** -17) * want).all()
