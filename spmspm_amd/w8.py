@@ -2,7 +2,7 @@
 
 Thin host layer over include/w8_api.h, in the manner of spmspm_amd/decode.py: every size, type and stride is checked here before a
 kernel sees a pointer (ValueError), an error of the library raises RuntimeError, calls run on torch's current stream unless
-`stream` names another.  There is no CPU fallback.
+`stream` names another.  There is no CPU fallback, and no backward pass: asking a result for a gradient raises RuntimeError.
 
     codes, scales, h = rms_norm_x8(x, norm_weight, residual=h)      # h + x, normed, in 8 bits with a scale per token
     gates = W8GatedLinear(*quantize_w8(w_gate), *quantize_w8(w_up))  # silu(gate) * up in one kernel
@@ -83,6 +83,27 @@ def _overlap(a, b):
     return (b0 - a0) % a.element_size() != 0 or apart % stride < a.shape[1] or apart % stride + b.shape[1] > stride
 
 
+class _NoBackward(torch.autograd.Function):
+    """Stands behind a result whose inputs require a gradient."""
+
+    @staticmethod
+    def forward(ctx, name, result, *inputs):
+        ctx.name = name
+        return result.detach()
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name}: no backward pass")
+
+
+def _without_backward(name, results, *inputs):
+    """The results of a call with an input that requires a gradient: asking them for one raises, as it does behind the registered
+    operators, where a result without a history would lose it.  Codes, as all whole numbers, carry none."""
+    if not isinstance(results, tuple):
+        return _NoBackward.apply(name, results, *inputs)
+    return tuple(t if t.dtype == torch.int8 else _NoBackward.apply(name, t, *inputs) for t in results)
+
+
 def _new_codes(x, N, K):
     """Room for N rows of K codes, 16-byte aligned, and their scales.  Long rows lie an odd multiple of 128 bytes apart: rows a power of
     two apart would meet on the same memory channels."""
@@ -140,7 +161,10 @@ def _norm(name, x, weight, eps, residual, residual_out, out, codes, stream):
             return (y, scales, h) if added else (y, scales)
         return (y, h) if added else y
 
-    return _run(device, stream, call)
+    results = _run(device, stream, call)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (added and residual.requires_grad)):
+        return _without_backward(name, results, x, weight, residual)
+    return results
 
 
 def rms_norm(x, weight, eps=1e-5, residual=None, out=None, residual_out=None, stream=None):
@@ -174,7 +198,8 @@ def quantize_x8(x, stream=None):
                 _raise(err, "quantize_x8")
         return codes, scales
 
-    return _run(x.device, stream, call)
+    results = _run(x.device, stream, call)
+    return _without_backward("quantize_x8", results, x) if x.requires_grad and torch.is_grad_enabled() else results
 
 
 def quantize_w8(weight):
@@ -286,7 +311,17 @@ class _Product:
                     _raise(err, type(self).__name__)
             return y
 
-        return _run(self.device, stream, call)
+        y = _run(self.device, stream, call)
+        if torch.is_grad_enabled() and (x.requires_grad or (scales is not None and scales.requires_grad) or self._learns()):
+            return _without_backward(type(self).__name__, y, x, scales, *self.biases)
+        return y
+
+    def _learns(self):
+        """Whether a bias requires a gradient."""
+        for b in self.biases:
+            if b is not None and b.requires_grad:
+                return True
+        return False
 
 
 class W8Linear(_Product):

@@ -408,3 +408,41 @@ def test_the_sum_of_squares_of_a_long_row(torch, dtype, K, factor):
         codes, scales = S.rms_norm_x8(x, w)
         want = x.double().amax(-1) / 127 / rms[:, 0]
         assert ((scales.double() - want).abs() <= (2.0 ** -24 + 2.0 ** -17) * want).all()
+
+
+def test_a_gradient_is_refused_and_not_lost(torch):
+    """There is no backward pass: results of tensors that require a gradient raise where one is asked for, as the registered operators'
+    do; without gradients, and for tensors that require none, nothing changes."""
+    x, r = (torch.randn((3, 64), device="cuda").half() for _ in range(2))
+    gain = torch.ones(64, device="cuda").half()
+    bias = torch.zeros(40, device="cuda").half()
+    w, u = weights(torch, 40, 64, 1), weights(torch, 40, 64, 2)
+
+    def calls(x, r, gain, bias, scale=None):
+        codes, scales = S.quantize_x8(x)
+        scales = scales if scale is None else scale
+        one, two = S.W8Linear(*w, bias=bias), S.W8GatedLinear(*w, *u, up_bias=bias)
+        return [(S.rms_norm(x, gain),), S.rms_norm(x, gain, residual=r), S.rms_norm_x8(x, gain)[1:], S.rms_norm_x8(x, gain, residual=r)[1:],
+                (scales,), (one(x),), (one(codes, scales),), (two(x),), (two(codes, scales),),
+                (S.rms_norm(x, gain, out=torch.empty_like(x)),)]
+
+    plain = calls(x, r, gain, bias)
+    assert not any(t.requires_grad for c in plain for t in c)
+    leaf = lambda t: t.clone().requires_grad_()
+    for args, touched in (((leaf(x), r, gain, bias), range(10)), ((x, leaf(r), gain, bias), (1, 3)), ((x, r, leaf(gain), bias), (0, 1, 2, 3, 9)),
+                          ((x, r, gain, leaf(bias)), (5, 6, 7, 8)), ((x, r, gain, bias, leaf(S.quantize_x8(x)[1])), (6, 8))):
+        for i, (got, want) in enumerate(zip(calls(*args), plain)):
+            for t, p in zip(got, want):
+                assert torch.equal(t, p)
+                if i in touched:
+                    with pytest.raises(RuntimeError, match="no backward"):
+                        t.float().sum().backward()
+                elif i != 4:  # the scales may be a leaf of the test
+                    assert not t.requires_grad
+        with torch.no_grad():
+            assert not any(t.requires_grad for i, c in enumerate(calls(*args)) for t in c if i != 4)
+    h = S.rms_norm(x, leaf(gain), residual=r)[1]
+    h += 1  # the stream is worked on in place
+    kept = r.clone()
+    y, h = S.rms_norm(x, leaf(gain), residual=kept, residual_out=kept)
+    assert h.data_ptr() == kept.data_ptr() and torch.equal(kept, plain[1][1]) and not kept.requires_grad
