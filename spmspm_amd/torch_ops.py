@@ -252,7 +252,7 @@ def _w8(packed, M, K, dtype, biases, activation, gated, x, scales):
 def w8_linear(x: torch.Tensor, scales: Optional[torch.Tensor], packed: torch.Tensor, bias: Optional[torch.Tensor], M: int,
               activation: int, dtype: torch.dtype) -> torch.Tensor:
     """y[N][M] = act(W x + bias) in `dtype` for 8-bit weights laid out by `spmspm_amd.w8_pack`; x int8 with its scales, or 16-bit rows
-    of `dtype` without."""
+    of `dtype` without.  x must have the weights' K, which their packed size tells up to the next multiple of 128 only."""
     return _w8(packed, M, x.shape[1] if x.dim() == 2 else 0, dtype, (bias,), activation, False, x, scales)
 
 
@@ -284,6 +284,8 @@ class W8LinearModule(torch.nn.Module):
             self.register_buffer(name, b)
 
     def forward(self, x, scales=None):
+        if x.dim() != 2 or x.shape[1] != self.K:
+            raise ValueError(f"x must be [N][{self.K}]")
         if self.gated:
             return torch.ops.spmspm_amd.w8_gated(x, scales, self.packed, self.gate_bias, self.up_bias, self.M, self.activation,
                                                  self.dtype)

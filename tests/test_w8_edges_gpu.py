@@ -446,3 +446,17 @@ def test_a_gradient_is_refused_and_not_lost(torch):
     kept = r.clone()
     y, h = S.rms_norm(x, leaf(gain), residual=kept, residual_out=kept)
     assert h.data_ptr() == kept.data_ptr() and torch.equal(kept, plain[1][1]) and not kept.requires_grad
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_a_module_takes_rows_of_its_own_length_only(torch, gated):
+    """Weights of 100 and of 128 columns are packed to the same size, which is all that the operator sees of them."""
+    w, u = weights(torch, 40, 100, 1), weights(torch, 40, 100, 2)
+    layer = S.W8GatedLinear(*w, *u) if gated else S.W8Linear(*w)
+    module = layer.module()
+    x = torch.randn((3, 128), device="cuda").half()
+    assert torch.equal(module(x[:, :100]), layer(x[:, :100]))
+    for bad in (x, x[:, :90], x[0, :100]):
+        for args in ((bad,), S.quantize_x8(bad) if bad.dim() == 2 else (bad, None)):
+            with pytest.raises(ValueError):
+                module(*args)
