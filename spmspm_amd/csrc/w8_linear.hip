@@ -262,8 +262,8 @@ __global__ __launch_bounds__(256) void w8_join(ProductArgs a)
 // load and takes the operands' order in a corner of LDS that the wave has for itself (read in that order, 16 rows at once, a load
 // keeps the address unit four times as long: 2.3 us for every 16 columns of 5120).  A wave has D blocks of both in flight.  The
 // waves' sums meet in LDS.  A gated product has rows of the gate and of up in every workgroup: tiles t and t + 2 with R = 2.
-// X16: X holds 16-bit rows, eight at most, which every workgroup rounds to 8 bits for itself while its first blocks of W are on their
-// way: of few tokens that is less than a kernel before this one.
+// X16: X holds 16-bit rows, eight at most, which every workgroup rounds to 8 bits for itself: a launch less.  Its first blocks of W are
+// asked for ahead of the rows, whose maxima therefore wait for them (5120x5120, N = 1 9.2 us of a Python caller, 7.5 on given codes).
 // Bound by memory: 28672x7168 with 16 columns 34 us, 6.0 TB/s of W; 13696x5120 gate and up of one token 25 us, 5.6 TB/s.
 constexpr int kNarrowWaves = 8;
 constexpr int kRows16      = 8;
@@ -786,9 +786,10 @@ Plan8 choose8(int M, int N, int K, bool gated)
 }
 
 // 16-bit rows are rounded within w8_narrow where few are read beside few weights: a call then is one launch and needs no workspace, 6.7
-// us of a Python caller's time instead of 10.7.  In a graph: 1024x1024, N = 1 4.1 us, 5.3 with a kernel before it; N = 8 7.3 and 6.7;
-// 5120x5120, N = 1 9.7 and 9.2, N = 4 12.0 and 10.0; 20480x5120, N = 1 27.7 and 21.5.  Not where K is in shares, whose sum another
-// kernel ends, with scales from memory.
+// us of a Python caller's time instead of 10.7, which is what a call takes that is not recorded.  The limits are for that; in a graph
+// they hold what is lost by it to 0.6 us.  There, within and with a kernel before it: 1024x1024, N = 1 4.1 us and 5.3, N = 8 7.3 and
+// 6.7; 5120x5120, N = 1 9.7 and 9.2; past the limits N = 4 12.0 and 10.0, 20480x5120, N = 1 27.7 and 21.5.  Not where K is in
+// shares: w8_join, which ends their sums, reads the rows' scales from memory, and w8_narrow writes none.
 constexpr int64_t kMost16 = 8192, kMostWeights16 = 1 << 25;
 
 Plan8 plan8(int M, int N, int K, bool gated, bool x16)
