@@ -785,18 +785,22 @@ Plan8 choose8(int M, int N, int K, bool gated)
     return best;
 }
 
-// 16-bit rows are rounded within w8_narrow where few are read beside few weights: a call then is one launch and needs no workspace, 6.7
-// us of a Python caller's time instead of 10.7, which is what a call takes that is not recorded.  The limits are for that; in a graph
-// they hold what is lost by it to 0.6 us.  There, within and with a kernel before it: 1024x1024, N = 1 4.1 us and 5.3, N = 8 7.3 and
-// 6.7; 5120x5120, N = 1 9.7 and 9.2; past the limits N = 4 12.0 and 10.0, 20480x5120, N = 1 27.7 and 21.5.  Not where K is in
-// shares: w8_join, which ends their sums, reads the rows' scales from memory, and w8_narrow writes none.
+// 16-bit rows are rounded within w8_narrow where few are read beside few weights: a call then is one launch and needs no workspace, 6.8
+// us of a Python caller's time instead of 10.7, which is what a call takes that is not recorded.  Every workgroup reads all the rows for
+// itself, one row after another, so that a second round of workgroups does it once more: several rows only where all workgroups run
+// at once, one row where there are two to a CU (65536x512, N = 8 28.4 us within, 10.8 with a kernel before it; 32768x1024, N = 4 12.8 and 10.6,
+// N = 1 10.0 and 10.6).  By the kernels' time, as in a graph, within and not: 1024x1024, N = 1 4.1 and 5.4, N = 4 5.3 and 5.4, N = 8
+// 7.3 and 5.7; 4096x2048, N = 4 6.4 and 5.7; 4096x8192, N = 1 10.3 and 8.4; gated 1024x4096, N = 2 10.3 and 7.9.  What a graph loses so, 2.4
+// us at most of 121 sizes, is the price of the shorter call.  Not where K is in shares: w8_join, which ends their sums, reads the rows'
+// scales from memory, and w8_narrow writes none.
 constexpr int64_t kMost16 = 8192, kMostWeights16 = 1 << 25;
 
 Plan8 plan8(int M, int N, int K, bool gated, bool x16)
 {
-    Plan8 p = choose8(M, N, K, gated);
-    p.x16   = x16 && p.kind == 0 && p.cols == 1 && p.shares == 1 && N <= kRows16 && (int64_t)N * K <= kMost16 &&
-            layout8(M, K, gated).scales <= kMostWeights16;
+    const Layout8 l = layout8(M, K, gated);
+    Plan8         p = choose8(M, N, K, gated);
+    p.x16 = x16 && p.kind == 0 && p.cols == 1 && p.shares == 1 && N <= kRows16 && (int64_t)N * K <= kMost16 && l.scales <= kMostWeights16 &&
+            (int64_t)l.groups * 4 / p.rows <= (N == 1 ? 512 : 256);
     return p;
 }
 

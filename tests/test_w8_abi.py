@@ -182,3 +182,12 @@ def test_room_for_rounded_rows_beside_shares_of_k(gated):
                     split += n * k <= 8192
                     assert L.W8_WorkspaceBytes(m, n, k, gated, 1) >= part + n * (k + 4)
     assert split > 0 or not gated  # some of them few enough to be rounded where they are read
+
+
+@pytest.mark.parametrize("m,k,n,gated", [(65536, 512, 8, 0), (32768, 1024, 8, 0), (32768, 1024, 2, 0), (32768, 512, 8, 1), (16384, 1024, 4, 1)])
+def test_rows_are_rounded_once_where_workgroups_come_in_rounds(m, k, n, gated):
+    """Each workgroup that rounds rows for itself reads all of them: several rows are rounded by a kernel before the product, into the
+    workspace, where there are more workgroups than run at once; one row, and the rows of fewer, need none."""
+    L = M._library()
+    assert L.W8_WorkspaceBytes(m, n, k, gated, 1) >= n * (k + 4)
+    assert L.W8_WorkspaceBytes(m // 4, n, k, gated, 1) == 0 == L.W8_WorkspaceBytes(min(m, 16384 if gated else 32768), 1, k, gated, 1)

@@ -460,3 +460,13 @@ def test_a_module_takes_rows_of_its_own_length_only(torch, gated):
         for args in ((bad,), S.quantize_x8(bad) if bad.dim() == 2 else (bad, None)):
             with pytest.raises(ValueError):
                 module(*args)
+
+
+@pytest.mark.parametrize("gated,M_,K,N", [(False, 16384, 1000, 8), (False, 32768, 1000, 1), (False, 32768, 1000, 8), (False, 65536, 500, 1),
+                                          (True, 8000, 1000, 8), (True, 16384, 1000, 1), (True, 16384, 1000, 2)])
+def test_16_bit_rows_of_many_weights(torch, gated, M_, K, N):
+    """On both sides of where rows are rounded by the product's workgroups: the same bits as of codes made before."""
+    pairs = [weights(torch, M_, K, i) for i in range(2 if gated else 1)]
+    layer = S.W8GatedLinear(*pairs[0], *pairs[1]) if gated else S.W8Linear(*pairs[0], activation=A.ACT_GELU)
+    x = torch.randn((N, K), device="cuda").half()
+    assert torch.equal(layer(x), layer(*S.quantize_x8(x)))
